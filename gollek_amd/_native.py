@@ -25,6 +25,9 @@ Q8_0 = 8
 Q4_K = 12
 Q5_K = 13
 Q6_K = 14
+F32 = 0
+F16 = 1
+BF16 = 30
 
 _c = ctypes
 _P = _c.c_void_p
@@ -54,6 +57,10 @@ SIGNATURES: dict[str, tuple[object, list[object]]] = {
     "gollek_hip_gemm_bf16": (_I32, [_P, _P, _I64, _I64, _P, _I64, _CHARP, _SZ]),
     "gollek_hip_gemm_bf16_device": (_I32, [_P, _P, _I64, _P, _P, _CHARP, _SZ]),
     "gollek_hip_gemm_bf16_device_noalloc": (_I32, [_P, _P, _I64, _P, _P, _CHARP, _SZ]),
+    "gollek_hip_linear": (_I32, [_P, _P, _I64, _I64, _P, _I32, _P, _P, _P, _I32, _I64, _CHARP, _SZ]),
+    "gollek_hip_linear_workspace_bytes": (_I64, [_P, _I64]),
+    "gollek_hip_linear_device": (_I32, [_P, _P, _I64, _P, _I32, _P, _I64, _P, _I64, _P, _I32, _I64, _P, _I64, _P,
+                                        _CHARP, _SZ]),
     "gollek_hip_moe_workspace_bytes": (_I64, [_I64, _I64, _I64, _I64, _I64]),
     "gollek_hip_moe_grouped": (_I32, [_P, _P, _P, _I64, _P, _I64, _P, _P, _I64, _P, _I64,
                                       _CHARP, _SZ]),
@@ -110,6 +117,18 @@ def load() -> ctypes.CDLL:
             fn.argtypes = argtypes
         _lib = lib
         return lib
+
+
+_thread = threading.local()
+
+
+def err_buf() -> "ErrBuf":
+    """This thread's error buffer, for the entry points a decode loop calls once
+    or more per token (a new one costs about 1 us)."""
+    buf = getattr(_thread, "err", None)
+    if buf is None:
+        buf = _thread.err = ErrBuf()
+    return buf
 
 
 class ErrBuf:

@@ -854,6 +854,175 @@ int32_t gollek_hip_gemm_bf16_device_noalloc(gollek_hip_weight *w, const uint16_t
     return GOLLEK_HIP_OK;
 }
 
+// ---- the linear layer: a product with its epilogue -----------------------
+
+namespace {
+
+// A device current for the calls inside, the caller's again afterwards.
+class DeviceGuard {
+public:
+    explicit DeviceGuard(int device) {
+        if (hipGetDevice(&before_) != hipSuccess || before_ == device) before_ = -1;
+        else if (hipSetDevice(device) != hipSuccess) before_ = -1;
+    }
+    ~DeviceGuard() {
+        if (before_ >= 0) (void)hipSetDevice(before_);
+    }
+    DeviceGuard(const DeviceGuard &) = delete;
+    DeviceGuard &operator=(const DeviceGuard &) = delete;
+
+private:
+    int before_ = -1;
+};
+
+int element_size(int32_t type) {
+    return type == GOLLEK_HIP_F32 ? 4 : type == GOLLEK_HIP_F16 || type == GOLLEK_HIP_BF16 ? 2 : 0;
+}
+
+// Whether writing matrix y (m rows of n elements, y_stride apart) changes an
+// element of matrix b other than the one at the same place: the same matrix
+// is fine, and so are two column ranges of one wider matrix.
+bool overlaps(const void *y, int64_t y_stride, const void *b, int64_t b_stride, int64_t m, int64_t n, int64_t size) {
+    const uintptr_t ya = reinterpret_cast<uintptr_t>(y), ba = reinterpret_cast<uintptr_t>(b);
+    const uintptr_t ye = ya + (uintptr_t)(((m - 1) * y_stride + n) * size);
+    const uintptr_t be = ba + (uintptr_t)(((m - 1) * b_stride + n) * size);
+    if (ye <= ba || be <= ya) return false;
+    if (m == 1) return ya != ba;
+    if (y_stride != b_stride) return true;
+    if (ya == ba) return false;
+    const uintptr_t row = (uintptr_t)(y_stride * size), width = (uintptr_t)(n * size);
+    const uintptr_t apart = (ya > ba ? ya - ba : ba - ya) % row;
+    return !(apart >= width && row - apart >= width);
+}
+
+// Checks a linear call's epilogue and fills `out`.  Strides of 0 are packed rows.
+int32_t make_epilogue(const gollek_hip_weight *w, int64_t m, const float *bias, int32_t activation, const void *mul,
+                      int64_t mul_stride, const void *residual, int64_t residual_stride, void *y, int32_t y_type,
+                      int64_t y_stride, gollek::Epilogue *out, char *err, size_t err_len) {
+    const int size = element_size(y_type);
+    if (size == 0)
+        return fail(GOLLEK_HIP_ERR_UNSUPPORTED, err, err_len, "Unsupported linear output type id: %d (F32, F16 or BF16)",
+                    y_type);
+    if (activation < GOLLEK_HIP_ACT_NONE || activation > GOLLEK_HIP_ACT_GELU_TANH)
+        return fail(GOLLEK_HIP_ERR_ARG, err, err_len, "Unknown activation %d", activation);
+    const int64_t n = w->rows;
+    struct {
+        const char *name;
+        const void *p;
+        int64_t *stride;
+    } each[] = {{"output", y, &y_stride}, {"mul", mul, &mul_stride}, {"residual", residual, &residual_stride}};
+    for (auto &b : each) {
+        if (*b.stride == 0) *b.stride = n;
+        if (b.p == nullptr) continue;
+        if (*b.stride < n || *b.stride > (int64_t)1 << 40)
+            return fail(GOLLEK_HIP_ERR_ARG, err, err_len, "The %s's row stride %lld is not at least %lld columns",
+                        b.name, (long long)*b.stride, (long long)n);
+        if (reinterpret_cast<uintptr_t>(b.p) % (uintptr_t)size != 0)
+            return fail(GOLLEK_HIP_ERR_ARG, err, err_len, "The %s is not aligned to its %d-byte elements", b.name, size);
+        if (b.p != y && m > 0 && n > 0 && overlaps(y, y_stride, b.p, *b.stride, m, n, size))
+            return fail(GOLLEK_HIP_ERR_ARG, err, err_len, "The output overlaps the %s other than element for element",
+                        b.name);
+        if (b.p == y && m > 1 && *b.stride != y_stride)
+            return fail(GOLLEK_HIP_ERR_ARG, err, err_len, "The output is the %s with another row stride", b.name);
+    }
+    if (reinterpret_cast<uintptr_t>(bias) % sizeof(float) != 0)
+        return fail(GOLLEK_HIP_ERR_ARG, err, err_len, "The bias is not aligned to its 4-byte elements");
+    *out = gollek::make_epilogue(y, bias, mul, residual, y_stride, mul_stride, residual_stride, activation, y_type);
+    return GOLLEK_HIP_OK;
+}
+
+}  // namespace
+
+int64_t gollek_hip_linear_workspace_bytes(const gollek_hip_weight *w, int64_t m) {
+    if (w == nullptr || m < 0 || m > (int64_t)0x7FFFFFFF || w->rows > 0x7FFFFFFF || w->cols > 0x7FFFFFFF) return -1;
+    if (m == 0 || w->rows == 0 || w->compact) return 0;
+    return (int64_t)align_up(gollek::linear_workspace_bytes(w->type_id, (int)m, (int)w->rows, (int)w->cols), 256);
+}
+
+int32_t gollek_hip_linear_device(gollek_hip_weight *w, const uint16_t *x, int64_t m, const float *bias,
+                                 int32_t activation, const void *mul, int64_t mul_stride, const void *residual,
+                                 int64_t residual_stride, void *y, int32_t y_type, int64_t y_stride, void *workspace,
+                                 int64_t workspace_bytes, void *stream, char *err, size_t err_len) {
+    int32_t rc = check_gemm(w, x, y, m, true, err, err_len);
+    if (rc != GOLLEK_HIP_OK) return rc;
+    gollek::Epilogue epi;
+    rc = make_epilogue(w, m, bias, activation, mul, mul_stride, residual, residual_stride, y, y_type, y_stride, &epi,
+                       err, err_len);
+    if (rc != GOLLEK_HIP_OK) return rc;
+    if (reinterpret_cast<uintptr_t>(x) % sizeof(uint16_t) != 0)
+        return fail(GOLLEK_HIP_ERR_ARG, err, err_len, "The input is not aligned to its 2-byte elements");
+    if (workspace_bytes < 0 || (reinterpret_cast<uintptr_t>(workspace) & 255u) != 0)
+        return fail(GOLLEK_HIP_ERR_ARG, err, err_len, "The workspace (%lld bytes) is not 256-byte aligned",
+                    (long long)workspace_bytes);
+    if (m == 0 || w->rows == 0) {
+        ok(err, err_len);
+        return GOLLEK_HIP_OK;
+    }
+    const uintptr_t ya = reinterpret_cast<uintptr_t>(y), xa = reinterpret_cast<uintptr_t>(x);
+    const uintptr_t ye = ya + (uintptr_t)(((m - 1) * epi.y_stride + w->rows) * element_size(y_type));
+    if (xa < ye && ya < xa + (uintptr_t)(2 * m * w->cols))
+        return fail(GOLLEK_HIP_ERR_ARG, err, err_len, "The output overlaps the input");
+    const DeviceGuard device(w->device);
+    const hipError_t e = gollek::launch_linear(w->type_id, w->data, w->row_bytes, x, epi, (int)m, (int)w->rows,
+                                               (int)w->cols, static_cast<hipStream_t>(stream),
+                                               static_cast<float *>(workspace),
+                                               workspace != nullptr ? (size_t)workspace_bytes : 0, w->prep,
+                                               w->prep_rows);
+    if (e != hipSuccess) return hip_fail(e, "linear launch", err, err_len);
+    ok(err, err_len);
+    return GOLLEK_HIP_OK;
+}
+
+int32_t gollek_hip_linear(gollek_hip_weight *w, const uint16_t *x, int64_t x_len, int64_t m, const float *bias,
+                          int32_t activation, const void *mul, const void *residual, void *y, int32_t y_type,
+                          int64_t y_len, char *err, size_t err_len) {
+    int32_t rc = check_gemm(w, x, y, m, false, err, err_len);
+    if (rc != GOLLEK_HIP_OK) return rc;
+    gollek::Epilogue epi;
+    rc = make_epilogue(w, m, bias, activation, mul, 0, residual, 0, y, y_type, 0, &epi, err, err_len);
+    if (rc != GOLLEK_HIP_OK) return rc;
+    if (x_len < m * w->cols)
+        return fail(GOLLEK_HIP_ERR_ARG, err, err_len, "Input length %lld is smaller than %lld x %lld",
+                    (long long)x_len, (long long)m, (long long)w->cols);
+    if (y_len < m * w->rows)
+        return fail(GOLLEK_HIP_ERR_ARG, err, err_len, "Output length %lld is smaller than %lld x %lld",
+                    (long long)y_len, (long long)m, (long long)w->rows);
+    if (m == 0 || w->rows == 0) {
+        ok(err, err_len);
+        return GOLLEK_HIP_OK;
+    }
+    std::lock_guard<std::mutex> lock(w->mu);
+    rc = use_device(w->device, err, err_len);
+    if (rc != GOLLEK_HIP_OK) return rc;
+    const size_t xn = (size_t)(m * w->cols) * sizeof(uint16_t), bn = (size_t)w->rows * sizeof(float);
+    const size_t yn = (size_t)(m * w->rows) * element_size(y_type);
+    const size_t ws_bytes = gollek::linear_workspace_bytes(w->type_id, (int)m, (int)w->rows, (int)w->cols);
+    const size_t b_off = align_up(xn, 256), m_off = b_off + (bias != nullptr ? align_up(bn, 256) : 0);
+    const size_t r_off = m_off + (mul != nullptr ? align_up(yn, 256) : 0);
+    const size_t y_off = r_off + (residual != nullptr ? align_up(yn, 256) : 0), ws_off = y_off + align_up(yn, 256);
+    rc = ensure_staging(w, ws_off + ws_bytes, err, err_len);
+    if (rc != GOLLEK_HIP_OK) return rc;
+    uint8_t *const d = w->staging;
+    hipError_t e = hipMemcpyAsync(d, x, xn, hipMemcpyHostToDevice, w->stream);
+    if (e == hipSuccess && bias != nullptr) e = hipMemcpyAsync(d + b_off, bias, bn, hipMemcpyHostToDevice, w->stream);
+    if (e == hipSuccess && mul != nullptr) e = hipMemcpyAsync(d + m_off, mul, yn, hipMemcpyHostToDevice, w->stream);
+    if (e == hipSuccess && residual != nullptr)
+        e = hipMemcpyAsync(d + r_off, residual, yn, hipMemcpyHostToDevice, w->stream);
+    epi = gollek::make_epilogue(d + y_off, bias != nullptr ? reinterpret_cast<const float *>(d + b_off) : nullptr,
+                                mul != nullptr ? d + m_off : nullptr, residual != nullptr ? d + r_off : nullptr,
+                                w->rows, w->rows, w->rows, activation, y_type);
+    if (e == hipSuccess)
+        e = gollek::launch_linear(w->type_id, w->data, w->row_bytes, reinterpret_cast<const uint16_t *>(d), epi,
+                                  (int)m, (int)w->rows, (int)w->cols, w->stream,
+                                  ws_bytes ? reinterpret_cast<float *>(d + ws_off) : nullptr, ws_bytes, w->prep,
+                                  w->prep_rows);
+    if (e == hipSuccess) e = hipMemcpyAsync(y, d + y_off, yn, hipMemcpyDeviceToHost, w->stream);
+    if (e == hipSuccess) e = hipStreamSynchronize(w->stream);
+    if (e != hipSuccess) return hip_fail(e, "linear", err, err_len);
+    ok(err, err_len);
+    return GOLLEK_HIP_OK;
+}
+
 struct MoeShape {
     int E, H, I;
     int down_type;

@@ -140,11 +140,11 @@ __device__ __forceinline__ void skinny_read(uint32_t wr0, uint32_t w10a, uint32_
 
 }  // namespace
 
-template <int TT, int NS>
+template <int TT, int NS, class OUT>
 __global__ __launch_bounds__(256) void gemm_q8_0_bf16_skinny_kernel(const uint8_t *__restrict__ W,
                                                                     int64_t row_bytes,
                                                                     const uint16_t *__restrict__ X,
-                                                                    float *__restrict__ Y, int M,
+                                                                    OUT Y, int M,
                                                                     int N, int K) {
     using G = SkGeom<TT>;
     __shared__ __attribute__((aligned(16))) uint8_t lds[skinny_lds_bytes<TT, NS>()];
@@ -254,16 +254,17 @@ __global__ __launch_bounds__(256) void gemm_q8_0_bf16_skinny_kernel(const uint8_
 #pragma unroll
         for (int r = 0; r < 4; r++) {
             const int m = 16 * t + 4 * kq + r;
-            if (m < M) Y[(int64_t)m * N + n0 + lr] = v[r];
+            if (m < M) put(Y, m, n0 + lr, N, v[r]);
         }
     }
 }
 
 // Any shape: one thread per output, fp32, exact per-block scaling.
+template <class OUT>
 __global__ __launch_bounds__(256) void gemm_q8_0_generic_kernel(const uint8_t *__restrict__ W,
                                                                 int64_t row_bytes,
                                                                 const uint16_t *__restrict__ X,
-                                                                float *__restrict__ Y, int M,
+                                                                OUT Y, int M,
                                                                 int N, int K) {
     const int64_t t = (int64_t)blockIdx.x * blockDim.x + threadIdx.x;
     if (t >= (int64_t)M * N) return;
@@ -279,15 +280,15 @@ __global__ __launch_bounds__(256) void gemm_q8_0_generic_kernel(const uint8_t *_
             s = fmaf((float)(int)(int8_t)blk[2 + i], __uint_as_float((uint32_t)xr[32 * b + i] << 16), s);
         acc = fmaf(d, s, acc);
     }
-    Y[(int64_t)m * N + n] = acc;
+    put(Y, m, n, N, acc);
 }
 
 // Any shape, Q4_0 or Q4_K: one thread per output, fp32, the reference's block
 // structure (Q4_0: d * sum((q - 8) x); Q4_K per sub-block: fl(d sc) sum(q x) -
 // fl(dmin m) sum(x), the min term skipped for a zero min code).
-template <int T>
+template <int T, class OUT>
 __global__ __launch_bounds__(256) void gemm_generic_kernel(const uint8_t *__restrict__ W, int64_t row_bytes,
-                                                           const uint16_t *__restrict__ X, float *__restrict__ Y,
+                                                           const uint16_t *__restrict__ X, OUT Y,
                                                            int M, int N, int K) {
     const int64_t t = (int64_t)blockIdx.x * blockDim.x + threadIdx.x;
     if (t >= (int64_t)M * N) return;
@@ -329,7 +330,7 @@ __global__ __launch_bounds__(256) void gemm_generic_kernel(const uint8_t *__rest
             }
         }
     }
-    Y[(int64_t)m * N + n] = acc;
+    put(Y, m, n, N, acc);
 }
 
 // Q5_K / Q6_K: 16 x 16 outputs per workgroup, one per thread.  Per
@@ -337,11 +338,11 @@ __global__ __launch_bounds__(256) void gemm_generic_kernel(const uint8_t *__rest
 // superblocks are staged in LDS, then each output adds its block's
 // generic_block_dot (the dequantizers' block formulas folded into a dot;
 // gguf_block_dot.hpp) in superblock order.
-template <int T>
+template <int T, class OUT>
 __global__ __launch_bounds__(256) void gemm_kquant_generic_kernel(const uint8_t *__restrict__ W,
                                                                   int64_t row_bytes,
                                                                   const uint16_t *__restrict__ X,
-                                                                  float *__restrict__ Y, int M, int N, int K) {
+                                                                  OUT Y, int M, int N, int K) {
     constexpr int PB = T == kQ6_K ? 210 : kQ5KBlockBytes;
     __shared__ float xs[16][kQK];
     __shared__ uint8_t ws[16][PB];
@@ -361,7 +362,7 @@ __global__ __launch_bounds__(256) void gemm_kquant_generic_kernel(const uint8_t 
         __syncthreads();
         acc += generic_block_dot(T, ws[n], xs[m]);
     }
-    if (m0 + m < M && n0 + n < N) Y[(int64_t)(m0 + m) * N + n0 + n] = acc;
+    if (m0 + m < M && n0 + n < N) put(Y, m0 + m, n0 + n, N, acc);
 }
 
 // Q6_K on the matrix cores in fp32: a workgroup owns 16 NT W rows and 16 MT
@@ -379,9 +380,9 @@ __global__ __launch_bounds__(256) void gemm_kquant_generic_kernel(const uint8_t 
 // wave order.  X rows must be 4-byte aligned and W 2-byte aligned
 // (launch_gemm_bf16 checks): W rows are read 2 bytes at a time (superblocks
 // start on even bytes).
-template <int MT, int NT>
+template <int MT, int NT, class OUT>
 __global__ __launch_bounds__(256) void gemm_q6k_f32_kernel(const uint8_t *__restrict__ W, int64_t row_bytes,
-                                                           const uint16_t *__restrict__ X, float *__restrict__ Y,
+                                                           const uint16_t *__restrict__ X, OUT Y,
                                                            int M, int N, int K) {
 #pragma clang fp contract(off)
     static_assert(NT == 1 || NT == 4, "one N tile split over the waves, or one per wave");
@@ -477,7 +478,7 @@ __global__ __launch_bounds__(256) void gemm_q6k_f32_kernel(const uint8_t *__rest
 #pragma unroll
             for (int r = 0; r < 4; r++) {
                 const int m = m0 + 16 * mt + 4 * (lane >> 4) + r;
-                if (m < M && n < N) Y[(int64_t)m * N + n] = acc[mt][r];
+                if (m < M && n < N) put(Y, m, n, N, acc[mt][r]);
             }
     } else {
 #pragma unroll
@@ -490,7 +491,7 @@ __global__ __launch_bounds__(256) void gemm_q6k_f32_kernel(const uint8_t *__rest
 #pragma unroll
             for (int r = 0; r < 4; r++) {
                 const int m = m0 + 16 * mt + 4 * (ln >> 4) + r;
-                if (m < M && n < N) Y[(int64_t)m * N + n] = v[r];
+                if (m < M && n < N) put(Y, m, n, N, v[r]);
             }
         }
     }
@@ -522,9 +523,12 @@ size_t gemm_workspace_max_bytes(int type_id, int N, int K) {
     return most;
 }
 
-hipError_t launch_gemm_bf16(int type_id, const uint8_t *w, int64_t row_bytes, const uint16_t *x, float *y,
-                            int M, int N, int K, hipStream_t stream, float *workspace, size_t workspace_bytes,
-                            const uint8_t *prep, int64_t prep_rows) {
+namespace {
+
+template <class OUT>
+hipError_t launch_gemm(int type_id, const uint8_t *w, int64_t row_bytes, const uint16_t *x, OUT y,
+                       int M, int N, int K, hipStream_t stream, float *workspace, size_t workspace_bytes,
+                       const uint8_t *prep, int64_t prep_rows) {
     if (M <= 0) return hipSuccess;
     const bool aligned = (reinterpret_cast<uintptr_t>(w) & 3u) == 0 && (row_bytes & 3) == 0 &&
                          (reinterpret_cast<uintptr_t>(x) & 15u) == 0;
@@ -537,10 +541,10 @@ hipError_t launch_gemm_bf16(int type_id, const uint8_t *w, int64_t row_bytes, co
     if (type_id == kQ8_0 && aligned && M <= 32 && N % 16 == 0 && K % 256 == 0 &&
         (int64_t)16 * row_bytes < ((int64_t)1 << 31) && (int64_t)M * K * 2 < ((int64_t)1 << 31)) {
         if (M <= 16)
-            hipLaunchKernelGGL((gemm_q8_0_bf16_skinny_kernel<1, 4>), dim3(N / 16), dim3(256), 0, stream, w,
+            hipLaunchKernelGGL((gemm_q8_0_bf16_skinny_kernel<1, 4, OUT>), dim3(N / 16), dim3(256), 0, stream, w,
                                row_bytes, x, y, M, N, K);
         else
-            hipLaunchKernelGGL((gemm_q8_0_bf16_skinny_kernel<2, 4>), dim3(N / 16), dim3(256), 0, stream, w,
+            hipLaunchKernelGGL((gemm_q8_0_bf16_skinny_kernel<2, 4, OUT>), dim3(N / 16), dim3(256), 0, stream, w,
                                row_bytes, x, y, M, N, K);
         return hipGetLastError();
     }
@@ -560,25 +564,25 @@ hipError_t launch_gemm_bf16(int type_id, const uint8_t *w, int64_t row_bytes, co
         const int64_t wide = (int64_t)((N + 63) / 64) * ((M + 63) / 64);
         if (mt == 4 && wide >= 2 * (int64_t)device_cus()) {
             const dim3 g6((unsigned)((N + 63) / 64), (unsigned)((M + 63) / 64));
-            hipLaunchKernelGGL((gemm_q6k_f32_kernel<4, 4>), g6, dim3(256), 0, stream, w, row_bytes, x, y, M, N, K);
+            hipLaunchKernelGGL((gemm_q6k_f32_kernel<4, 4, OUT>), g6, dim3(256), 0, stream, w, row_bytes, x, y, M, N, K);
         } else {
             const dim3 g6((unsigned)((N + 15) / 16), (unsigned)((M + 16 * mt - 1) / (16 * mt)));
             if (mt == 1)
-                hipLaunchKernelGGL((gemm_q6k_f32_kernel<1, 1>), g6, dim3(256), 0, stream, w, row_bytes, x, y, M, N, K);
+                hipLaunchKernelGGL((gemm_q6k_f32_kernel<1, 1, OUT>), g6, dim3(256), 0, stream, w, row_bytes, x, y, M, N, K);
             else if (mt == 2)
-                hipLaunchKernelGGL((gemm_q6k_f32_kernel<2, 1>), g6, dim3(256), 0, stream, w, row_bytes, x, y, M, N, K);
+                hipLaunchKernelGGL((gemm_q6k_f32_kernel<2, 1, OUT>), g6, dim3(256), 0, stream, w, row_bytes, x, y, M, N, K);
             else
-                hipLaunchKernelGGL((gemm_q6k_f32_kernel<4, 1>), g6, dim3(256), 0, stream, w, row_bytes, x, y, M, N, K);
+                hipLaunchKernelGGL((gemm_q6k_f32_kernel<4, 1, OUT>), g6, dim3(256), 0, stream, w, row_bytes, x, y, M, N, K);
         }
         return hipGetLastError();
     }
     if (type_id == kQ5_K || type_id == kQ6_K) {
         const dim3 g16((unsigned)((N + 15) / 16), (unsigned)((M + 15) / 16));
         if (type_id == kQ5_K)
-            hipLaunchKernelGGL(gemm_kquant_generic_kernel<kQ5_K>, g16, dim3(256), 0, stream, w, row_bytes, x, y, M,
+            hipLaunchKernelGGL((gemm_kquant_generic_kernel<kQ5_K, OUT>), g16, dim3(256), 0, stream, w, row_bytes, x, y, M,
                                N, K);
         else
-            hipLaunchKernelGGL(gemm_kquant_generic_kernel<kQ6_K>, g16, dim3(256), 0, stream, w, row_bytes, x, y, M,
+            hipLaunchKernelGGL((gemm_kquant_generic_kernel<kQ6_K, OUT>), g16, dim3(256), 0, stream, w, row_bytes, x, y, M,
                                N, K);
         return hipGetLastError();
     }
@@ -586,18 +590,39 @@ hipError_t launch_gemm_bf16(int type_id, const uint8_t *w, int64_t row_bytes, co
     const dim3 grid((unsigned)((total + 255) / 256)), block(256);
     switch (type_id) {
     case kQ8_0:
-        hipLaunchKernelGGL(gemm_q8_0_generic_kernel, grid, block, 0, stream, w, row_bytes, x, y, M, N, K);
+        hipLaunchKernelGGL(gemm_q8_0_generic_kernel<OUT>, grid, block, 0, stream, w, row_bytes, x, y, M, N, K);
         break;
     case kQ4_0:
-        hipLaunchKernelGGL(gemm_generic_kernel<kQ4_0>, grid, block, 0, stream, w, row_bytes, x, y, M, N, K);
+        hipLaunchKernelGGL((gemm_generic_kernel<kQ4_0, OUT>), grid, block, 0, stream, w, row_bytes, x, y, M, N, K);
         break;
     case kQ4_K:
-        hipLaunchKernelGGL(gemm_generic_kernel<kQ4_K>, grid, block, 0, stream, w, row_bytes, x, y, M, N, K);
+        hipLaunchKernelGGL((gemm_generic_kernel<kQ4_K, OUT>), grid, block, 0, stream, w, row_bytes, x, y, M, N, K);
         break;
     default:
         return hipErrorInvalidValue;
     }
     return hipGetLastError();
+}
+
+}  // namespace
+
+hipError_t launch_gemm_bf16(int type_id, const uint8_t *w, int64_t row_bytes, const uint16_t *x, float *y,
+                            int M, int N, int K, hipStream_t stream, float *workspace, size_t workspace_bytes,
+                            const uint8_t *prep, int64_t prep_rows) {
+    return launch_gemm<float *>(type_id, w, row_bytes, x, y, M, N, K, stream, workspace, workspace_bytes, prep,
+                                prep_rows);
+}
+
+size_t linear_workspace_bytes(int type_id, int M, int N, int K) {
+    const size_t most = gemm_workspace_bytes(type_id, M, N, K);
+    return most > 0 ? most + (size_t)M * N * sizeof(float) : 0;
+}
+
+hipError_t launch_linear(int type_id, const uint8_t *w, int64_t row_bytes, const uint16_t *x, const Epilogue &y,
+                         int M, int N, int K, hipStream_t stream, float *workspace, size_t workspace_bytes,
+                         const uint8_t *prep, int64_t prep_rows) {
+    return launch_gemm<Epilogue>(type_id, w, row_bytes, x, y, M, N, K, stream, workspace, workspace_bytes, prep,
+                                 prep_rows);
 }
 
 }  // namespace gollek

@@ -231,11 +231,11 @@ __device__ __forceinline__ void ops_wait_row(int i, Ops &o) {
 // One 16 MT x 128 tile of Y (or of split `split`'s partial sum) per workgroup.
 // RAGGED: K is any multiple of 32 and rows may start 2 bytes past a dword (kept
 // apart: the address masks and the skipped half stage cost whole-round K 1 to 2 %).
-template <int T, int MT, bool RAGGED>
+template <int T, int MT, bool RAGGED, class OUT>
 __global__ __launch_bounds__(kThreads) void gemm_tile_kernel(const uint8_t *__restrict__ W,
                                                             int64_t row_bytes,
                                                             const uint16_t *__restrict__ X,
-                                                            float *__restrict__ Y, int M, int N,
+                                                            OUT Y, int M, int N,
                                                             int K, int S, float *__restrict__ part) {
     using G = TileGeom<T, MT>;
     using R = RawW<T>;
@@ -456,11 +456,23 @@ __global__ __launch_bounds__(kThreads) void gemm_tile_kernel(const uint8_t *__re
                     stage[(16 * mt + 4 * lk + r) * kStagePitch + 32 * nq + 16 * nt + lr] = acc[mt][nt][r];
     }
     __syncthreads();
-    // Split 0 writes Y, split k > 0 workspace partial k - 1 for the
-    // reduction kernel.
-    float *const out = split == 0 ? Y : part + (int64_t)(split - 1) * M * N;
+    // A plain Y: split 0 writes it, split k > 0 workspace partial k - 1 for the
+    // reduction kernel.  An epilogue: with splits all of them are partials.
     const int col = 4 * (tid & 31);
     if (tid >= kCompute) return;
+    if constexpr (kHasEpilogue<OUT>) {
+        if (S == 1) {
+#pragma unroll
+            for (int pass = 0; pass < kTileM * 32 / kCompute; pass++) {
+                const int row = 16 * pass + (tid >> 5);
+                const int m = m0 + row, n = n0 + col;
+                if (m >= M || n >= N) continue;
+                put4(Y, m, n, N, *reinterpret_cast<const float4 *>(stage + row * kStagePitch + col));
+            }
+            return;
+        }
+    }
+    float *const out = split_output(Y, part, split, (int64_t)M * N);
 #pragma unroll
     for (int pass = 0; pass < kTileM * 32 / kCompute; pass++) {
         const int row = 16 * pass + (tid >> 5);
@@ -474,6 +486,39 @@ __global__ __launch_bounds__(kThreads) void gemm_tile_kernel(const uint8_t *__re
         } else {
             const float v4[4] = {val.x, val.y, val.z, val.w};
             for (int i = 0; i < 4 && n + i < N; i++) dst[i] = v4[i];
+        }
+    }
+}
+
+// A linear layer's split product: the partials in split order, then the
+// epilogue (4 elements of a row a thread).
+__global__ __launch_bounds__(256) void linear_reduce_kernel(const float *__restrict__ part, int S, int M, int N,
+                                                            Epilogue y) {
+    const int n = 4 * ((int)blockIdx.x * 256 + (int)threadIdx.x), m = (int)blockIdx.y;
+    if (n >= N) return;
+    const int64_t mn = (int64_t)M * N;
+    const float *const p = part + (int64_t)m * N + n;
+    if ((N & 3) == 0) {
+        float4 b[8];
+#pragma unroll
+        for (int k = 0; k < 8; k++)
+            if (k < S) b[k] = *reinterpret_cast<const float4 *>(p + k * mn);
+        float4 a = b[0];
+#pragma unroll
+        for (int k = 1; k < 8; k++) {
+            if (k < S) {
+                a.x += b[k].x;
+                a.y += b[k].y;
+                a.z += b[k].z;
+                a.w += b[k].w;
+            }
+        }
+        put4(y, m, n, N, a);
+    } else {
+        for (int i = 0; i < 4 && n + i < N; i++) {
+            float a = p[i];
+            for (int k = 1; k < S; k++) a += p[k * mn + i];
+            put(y, m, n + i, N, a);
         }
     }
 }
@@ -574,14 +619,13 @@ void gemm_tile_plan(int type_id, int M, int N, int K, int32_t (&plan)[4]) {
     plan[3] = ((int64_t)M * N) % 4 == 0 ? tile_splits(type_id, M, N, K, (size_t)-1) : 1;
 }
 
+template <class OUT>
 hipError_t launch_gemm_tile(int type_id, const uint8_t *w, int64_t row_bytes, const uint16_t *x,
-                            float *y, int M, int N, int K, hipStream_t stream, float *workspace,
+                            OUT y, int M, int N, int K, hipStream_t stream, float *workspace,
                             size_t workspace_bytes) {
     if (M <= 0) return hipSuccess;
-    int S = tile_splits(type_id, M, N, K, workspace != nullptr ? workspace_bytes : 0);
-    if (((int64_t)M * N) % 4 != 0 ||
-        ((reinterpret_cast<uintptr_t>(workspace) | reinterpret_cast<uintptr_t>(y)) & 15u) != 0)
-        S = 1;
+    int S = tile_splits(type_id, M, N, K, split_bytes<OUT>(workspace, workspace_bytes, M, N));
+    if (!splits_aligned(y, workspace, M, N)) S = 1;
     const int mt = tile_mt(type_id, M, N, K), tm = 16 * mt;
     const unsigned tiles = (unsigned)(((M + tm - 1) / tm) * ((N + kTileN - 1) / kTileN));
     const dim3 grid(tiles * (unsigned)S), block(kThreads);
@@ -592,10 +636,10 @@ hipError_t launch_gemm_tile(int type_id, const uint8_t *w, int64_t row_bytes, co
     };
 #define GOLLEK_TILE_LAUNCH(TY)                                                                              \
     do {                                                                                                    \
-        if (mt == 1) ragged ? run(&gemm_tile_kernel<TY, 1, true>) : run(&gemm_tile_kernel<TY, 1, false>);   \
-        else if (mt == 2) ragged ? run(&gemm_tile_kernel<TY, 2, true>) : run(&gemm_tile_kernel<TY, 2, false>); \
-        else if (mt == 4) ragged ? run(&gemm_tile_kernel<TY, 4, true>) : run(&gemm_tile_kernel<TY, 4, false>); \
-        else ragged ? run(&gemm_tile_kernel<TY, 8, true>) : run(&gemm_tile_kernel<TY, 8, false>);           \
+        if (mt == 1) ragged ? run(&gemm_tile_kernel<TY, 1, true, OUT>) : run(&gemm_tile_kernel<TY, 1, false, OUT>);   \
+        else if (mt == 2) ragged ? run(&gemm_tile_kernel<TY, 2, true, OUT>) : run(&gemm_tile_kernel<TY, 2, false, OUT>); \
+        else if (mt == 4) ragged ? run(&gemm_tile_kernel<TY, 4, true, OUT>) : run(&gemm_tile_kernel<TY, 4, false, OUT>); \
+        else ragged ? run(&gemm_tile_kernel<TY, 8, true, OUT>) : run(&gemm_tile_kernel<TY, 8, false, OUT>);           \
     } while (0)
     switch (type_id) {
     case kQ8_0:
@@ -608,12 +652,23 @@ hipError_t launch_gemm_tile(int type_id, const uint8_t *w, int64_t row_bytes, co
         return hipErrorInvalidValue;
     }
 #undef GOLLEK_TILE_LAUNCH
-    return S > 1 ? launch_gemm_reduce(part, S, (int64_t)M * N, y, stream) : hipGetLastError();
+    return S > 1 ? launch_gemm_reduce(part, S, M, N, y, stream) : hipGetLastError();
 }
+template hipError_t launch_gemm_tile<float *>(int, const uint8_t *, int64_t, const uint16_t *, float *, int, int, int,
+                                              hipStream_t, float *, size_t);
+template hipError_t launch_gemm_tile<Epilogue>(int, const uint8_t *, int64_t, const uint16_t *, Epilogue, int, int, int,
+                                               hipStream_t, float *, size_t);
 
-hipError_t launch_gemm_reduce(const float *part, int S, int64_t mn, float *y, hipStream_t stream) {
+hipError_t launch_gemm_reduce(const float *part, int S, int M, int N, float *y, hipStream_t stream) {
+    const int64_t mn = (int64_t)M * N;
     hipLaunchKernelGGL(gemm_tile_reduce_kernel, dim3((unsigned)((mn / 4 + 255) / 256)), dim3(256), 0, stream, part,
                        S - 1, mn, y);
+    return hipGetLastError();
+}
+
+hipError_t launch_gemm_reduce(const float *part, int S, int M, int N, const Epilogue &y, hipStream_t stream) {
+    hipLaunchKernelGGL(linear_reduce_kernel, dim3((unsigned)((N + 1023) / 1024), (unsigned)M), dim3(256), 0, stream,
+                       part, S, M, N, y);
     return hipGetLastError();
 }
 

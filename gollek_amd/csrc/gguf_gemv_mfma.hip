@@ -726,10 +726,10 @@ struct ColGeom {
 // take a second operand set (a second MFMA per chunk on the same B).
 // Vector v is x + v K, its results y + v rows.  XB: x holds bf16 bit
 // patterns (the GEMM's input), widened to fp32 exactly as they load.
-template <int TYPE, bool PREP, int NV = 1, bool XB = false>
+template <int TYPE, bool PREP, int NV = 1, bool XB = false, class OUT = float *__restrict__>
 __global__ __launch_bounds__(kColThreads) void gemv_mfma_col_kernel(
     const uint8_t *__restrict__ w, int64_t row_bytes64, int nsb, const float *__restrict__ x,
-    float *__restrict__ y, int64_t rows, int rows_per_wg) {
+    OUT y, int64_t rows, int rows_per_wg) {
     using G = ColGeom<TYPE>;
     constexpr int PB = G::PB;
     constexpr int TB = G::kTileBytes;
@@ -885,7 +885,7 @@ __global__ __launch_bounds__(kColThreads) void gemv_mfma_col_kernel(
         float s = 0.0f;
 #pragma unroll
         for (int k = 0; k < kColWaves; k++) s += p[k].x + p[k].y;
-        y[(int64_t)v * rows + r0 + r] = s;
+        put(y, v, r0 + r, rows, s);
     }
 }
 
@@ -906,10 +906,10 @@ constexpr int kWideMaxCols = 4;  // columns per wave (K <= 16384)
 // NV = 2, XB: as the column kernel's (the small-M GEMM's M = 2 on bf16 X):
 // the second vector's digits in A rows 8..15 of the same compact operands,
 // its sums in output lanes 32..63 and a second row-sum buffer.
-template <int TYPE, bool PREP, int NV = 1, bool XB = false>
+template <int TYPE, bool PREP, int NV = 1, bool XB = false, class OUT = float *__restrict__>
 __global__ __launch_bounds__(kColThreads) void gemv_mfma_wide_kernel(
     const uint8_t *__restrict__ w, int64_t row_bytes64, int nsb, const float *__restrict__ x,
-    float *__restrict__ y, int64_t rows, int rows_per_wg) {
+    OUT y, int64_t rows, int rows_per_wg) {
     using G = ColGeom<TYPE>;
     constexpr int PB = G::PB;
     constexpr int TB = G::kTileBytes;
@@ -1051,7 +1051,7 @@ __global__ __launch_bounds__(kColThreads) void gemv_mfma_wide_kernel(
         }
         float s = 0.0f;
         for (int k = 0; k < nw; k++) s += part[v][k][r][0] + part[v][k][r][1];
-        y[(int64_t)v * rows + r0 + r] = s;
+        put(y, v, r0 + r, rows, s);
     }
 }
 
@@ -1203,7 +1203,8 @@ bool gemm_col_supported(int type_id, int64_t row_bytes, int M, int N, int K, con
     return col_layout_rows(type_id, N, K) > 0;
 }
 
-hipError_t launch_gemm_col(int type_id, const uint8_t *w, int64_t row_bytes, const uint16_t *x, float *y, int M,
+template <class OUT>
+hipError_t launch_gemm_col(int type_id, const uint8_t *w, int64_t row_bytes, const uint16_t *x, OUT y, int M,
                            int N, int K, hipStream_t stream, const uint8_t *prep, int64_t prep_rows) {
     const int nsb = K / kQK;
     const int64_t col_rows = col_layout_rows(type_id, N, K);
@@ -1216,19 +1217,19 @@ hipError_t launch_gemm_col(int type_id, const uint8_t *w, int64_t row_bytes, con
 #define GOLLEK_GEMM_COL_NV(T, NV)                                                                              \
     do {                                                                                                       \
         if (use_prep)                                                                                          \
-            hipLaunchKernelGGL((gemv_mfma_col_kernel<T, true, NV, true>), grid, dim3(kColThreads), 0, stream,   \
+            hipLaunchKernelGGL((gemv_mfma_col_kernel<T, true, NV, true, OUT>), grid, dim3(kColThreads), 0, stream,   \
                                src, row_bytes, nsb, xf, y, (int64_t)N, (int)col_rows);                        \
         else                                                                                                   \
-            hipLaunchKernelGGL((gemv_mfma_col_kernel<T, false, NV, true>), grid, dim3(kColThreads), 0, stream,  \
+            hipLaunchKernelGGL((gemv_mfma_col_kernel<T, false, NV, true, OUT>), grid, dim3(kColThreads), 0, stream,  \
                                src, row_bytes, nsb, xf, y, (int64_t)N, (int)col_rows);                        \
     } while (0)
 #define GOLLEK_GEMM_WIDE_NV(T, NV)                                                                             \
     do {                                                                                                       \
         if (use_prep)                                                                                          \
-            hipLaunchKernelGGL((gemv_mfma_wide_kernel<T, true, NV, true>), grid, dim3(kColThreads), 0, stream,  \
+            hipLaunchKernelGGL((gemv_mfma_wide_kernel<T, true, NV, true, OUT>), grid, dim3(kColThreads), 0, stream,  \
                                src, row_bytes, nsb, xf, y, (int64_t)N, (int)col_rows);                        \
         else                                                                                                   \
-            hipLaunchKernelGGL((gemv_mfma_wide_kernel<T, false, NV, true>), grid, dim3(kColThreads), 0, stream, \
+            hipLaunchKernelGGL((gemv_mfma_wide_kernel<T, false, NV, true, OUT>), grid, dim3(kColThreads), 0, stream, \
                                src, row_bytes, nsb, xf, y, (int64_t)N, (int)col_rows);                        \
     } while (0)
 #define GOLLEK_GEMM_COL(T)                                                                                      \
@@ -1250,6 +1251,10 @@ hipError_t launch_gemm_col(int type_id, const uint8_t *w, int64_t row_bytes, con
 #undef GOLLEK_GEMM_COL_NV
     return hipGetLastError();
 }
+template hipError_t launch_gemm_col<float *>(int, const uint8_t *, int64_t, const uint16_t *, float *, int, int, int,
+                                             hipStream_t, const uint8_t *, int64_t);
+template hipError_t launch_gemm_col<Epilogue>(int, const uint8_t *, int64_t, const uint16_t *, Epilogue, int, int, int,
+                                              hipStream_t, const uint8_t *, int64_t);
 
 hipError_t launch_gemv_q32_mfma(int type_id, const uint8_t *w, int64_t row_bytes, int64_t cols,
                                 const float *x, float *y, int64_t rows, hipStream_t stream,

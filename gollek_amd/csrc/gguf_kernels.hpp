@@ -8,6 +8,8 @@
 #include <atomic>
 #include <stdint.h>
 
+#include "gguf_epilogue.hpp"
+
 namespace gollek {
 
 // Kernel selection read by the launchers (gollek_hip_testing_set_option).
@@ -114,7 +116,10 @@ hipError_t launch_gemm_bf16(int type_id, const uint8_t *w, int64_t row_bytes, co
 // M = 1 .. 4 on the GEMV's column kernel (gguf_gemv_mfma.hip): two vectors
 // in each MFMA over one stream of the weights.
 bool gemm_col_supported(int type_id, int64_t row_bytes, int M, int N, int K, const void *w, const void *x);
-hipError_t launch_gemm_col(int type_id, const uint8_t *w, int64_t row_bytes, const uint16_t *x, float *y, int M,
+// (The product launchers take their output as the kernels do: float *, the
+// plain fp32 matrix, or Epilogue, the linear layer's.)
+template <class OUT>
+hipError_t launch_gemm_col(int type_id, const uint8_t *w, int64_t row_bytes, const uint16_t *x, OUT y, int M,
                            int N, int K, hipStream_t stream, const uint8_t *prep = nullptr,
                            int64_t prep_rows = 0);
 // Whether a shape splits K: when tiles of at most 128 x 128 fill at most half
@@ -128,19 +133,31 @@ size_t kq_gemm_workspace_bytes(int type_id, int M, int N, int K);
 // The plan of a call whose buffers are aligned and whose workspace suffices, for
 // the tests: {row tiles, column waves, K waves, K splits}.
 void kq_gemm_plan(int type_id, int M, int N, int K, int32_t (&plan)[4]);
-hipError_t launch_kq_gemm(int type_id, const uint8_t *w, int64_t row_bytes, const uint16_t *x, float *y, int M, int N,
+template <class OUT>
+hipError_t launch_kq_gemm(int type_id, const uint8_t *w, int64_t row_bytes, const uint16_t *x, OUT y, int M, int N,
                           int K, hipStream_t stream, float *workspace, size_t workspace_bytes);
 // The 128 x 128 tile kernel of Q8_0 and Q4_0 (gguf_gemm_tile.hip): K a
 // multiple of 32, W 4-byte aligned with rows on even bytes, x 16-byte aligned.
 bool gemm_tile_supported(int type_id, int64_t row_bytes, int M, int N, int K, const void *w, const void *x);
 size_t gemm_tile_workspace_bytes(int type_id, int M, int N, int K);
 void gemm_tile_plan(int type_id, int M, int N, int K, int32_t (&plan)[4]);  // {row tiles, 0, 0, K splits}
+template <class OUT>
 hipError_t launch_gemm_tile(int type_id, const uint8_t *w, int64_t row_bytes, const uint16_t *x,
-                            float *y, int M, int N, int K, hipStream_t stream, float *workspace,
+                            OUT y, int M, int N, int K, hipStream_t stream, float *workspace,
                             size_t workspace_bytes);
 // y += the S - 1 partial tiles of mn floats in `part`, in split order (mn a
 // multiple of 4, both 16-byte aligned; S <= 8).
-hipError_t launch_gemm_reduce(const float *part, int S, int64_t mn, float *y, hipStream_t stream);
+hipError_t launch_gemm_reduce(const float *part, int S, int M, int N, float *y, hipStream_t stream);
+// The linear layer's: y is the epilogue of the sum of all S partials.
+hipError_t launch_gemm_reduce(const float *part, int S, int M, int N, const Epilogue &y, hipStream_t stream);
+
+// The linear layer (gguf_epilogue.hpp) on the kernels of launch_gemm_bf16, whose
+// sums it shares.  Splits keep all S partials in the workspace, so it takes
+// linear_workspace_bytes (0: never splits; with less it splits less).
+size_t linear_workspace_bytes(int type_id, int M, int N, int K);
+hipError_t launch_linear(int type_id, const uint8_t *w, int64_t row_bytes, const uint16_t *x, const Epilogue &y, int M,
+                         int N, int K, hipStream_t stream, float *workspace, size_t workspace_bytes,
+                         const uint8_t *prep, int64_t prep_rows);
 
 // Workspace layout of the grouped MoE FFN (byte offsets; gguf_moe.hip).
 struct MoeLayout {

@@ -83,9 +83,9 @@ struct XRows {
 // A workgroup owns 16 MT rows of X and 32 NW rows of W: NW KW waves as NW
 // column groups of 32 and KW slices of the stage's superblocks.  Each wave
 // converts its rows' share of the next stage's x between its MFMAs.
-template <int T, int MT, int NW, int KW>
+template <int T, int MT, int NW, int KW, class OUT>
 __global__ __launch_bounds__(64 * NW *KW, MT == 1 && NW == 2 ? 4 : 1) void gemm_kq_kernel(const uint8_t *__restrict__ W, int64_t row_bytes,
-                                                              const uint16_t *__restrict__ X, float *__restrict__ Y,
+                                                              const uint16_t *__restrict__ X, OUT Y,
                                                               int M, int N, int K, int S, float *__restrict__ part) {
     constexpr int kWaves = NW * KW, UN = MT * KW;
     constexpr int kTileM = 16 * MT, kTileN = 32 * NW;
@@ -232,7 +232,23 @@ __global__ __launch_bounds__(64 * NW *KW, MT == 1 && NW == 2 ? 4 : 1) void gemm_
 #pragma unroll
                 for (int nt = 0; nt < 2; nt++) acc[mt][nt] += red[(((k * NW + nw) * MT + mt) * 2 + nt) * 64 + lane];
     }
-    float *const out = split == 0 ? Y : part + (int64_t)(split - 1) * M * N;
+    if constexpr (kHasEpilogue<OUT>) {
+        if (S == 1) {
+#pragma unroll
+            for (int mt = 0; mt < MT; mt++)
+#pragma unroll
+                for (int r = 0; r < 4; r++) {
+                    const int m = m0 + 16 * mt + 4 * g + r;
+#pragma unroll
+                    for (int nt = 0; nt < 2; nt++) {
+                        const int c = col0 + 16 * nt + n;
+                        if (m < M && c < N) put(Y, m, c, N, acc[mt][nt][r]);
+                    }
+                }
+            return;
+        }
+    }
+    float *const out = split_output(Y, part, split, (int64_t)M * N);
 #pragma unroll
     for (int mt = 0; mt < MT; mt++)
 #pragma unroll
@@ -274,10 +290,10 @@ GemmPlan kq_plan(int type_id, int M, int N, int K, size_t ws_bytes) {
     return pick_gemm_plan(kQ6KPlans, kQ6KSplit, M, N, K, ws_bytes);
 }
 
-template <int T, int MT, int NW, int KW>
-void launch(unsigned grid, hipStream_t stream, const uint8_t *w, int64_t row_bytes, const uint16_t *x, float *y,
+template <int T, int MT, int NW, int KW, class OUT>
+void launch(unsigned grid, hipStream_t stream, const uint8_t *w, int64_t row_bytes, const uint16_t *x, OUT y,
             int M, int N, int K, int S, float *part) {
-    hipLaunchKernelGGL((gemm_kq_kernel<T, MT, NW, KW>), dim3(grid), dim3(64 * NW * KW), 0, stream, w, row_bytes, x, y,
+    hipLaunchKernelGGL((gemm_kq_kernel<T, MT, NW, KW, OUT>), dim3(grid), dim3(64 * NW * KW), 0, stream, w, row_bytes, x, y,
                        M, N, K, S, part);
 }
 
@@ -324,11 +340,11 @@ void kq_gemm_plan(int type_id, int M, int N, int K, int32_t (&plan)[4]) {
     plan[3] = p.splits;
 }
 
-hipError_t launch_kq_gemm(int type_id, const uint8_t *w, int64_t row_bytes, const uint16_t *x, float *y, int M, int N,
+template <class OUT>
+hipError_t launch_kq_gemm(int type_id, const uint8_t *w, int64_t row_bytes, const uint16_t *x, OUT y, int M, int N,
                           int K, hipStream_t stream, float *workspace, size_t workspace_bytes) {
-    const bool split = workspace != nullptr && gemm_may_split(type_id, M, N, K) && ((int64_t)M * N) % 4 == 0 &&
-                       ((reinterpret_cast<uintptr_t>(workspace) | reinterpret_cast<uintptr_t>(y)) & 15u) == 0;
-    const GemmPlan p = kq_plan(type_id, M, N, K, split ? workspace_bytes : 0);
+    const bool split = workspace != nullptr && gemm_may_split(type_id, M, N, K) && splits_aligned(y, workspace, M, N);
+    const GemmPlan p = kq_plan(type_id, M, N, K, split ? split_bytes<OUT>(workspace, workspace_bytes, M, N) : 0);
     const unsigned grid =
         (unsigned)(((M + 16 * p.mt - 1) / (16 * p.mt)) * ((N + 32 * p.nw - 1) / (32 * p.nw)) * p.splits);
     bool ok;
@@ -336,8 +352,12 @@ hipError_t launch_kq_gemm(int type_id, const uint8_t *w, int64_t row_bytes, cons
     else if (type_id == kQ5_K) ok = launch_plan<kQ5_K>(p, grid, stream, w, row_bytes, x, y, M, N, K, p.splits, workspace);
     else ok = launch_plan<kQ6_K>(p, grid, stream, w, row_bytes, x, y, M, N, K, p.splits, workspace);
     if (!ok) return hipErrorInvalidValue;
-    if (p.splits > 1) return launch_gemm_reduce(workspace, p.splits, (int64_t)M * N, y, stream);
+    if (p.splits > 1) return launch_gemm_reduce(workspace, p.splits, M, N, y, stream);
     return hipGetLastError();
 }
+template hipError_t launch_kq_gemm<float *>(int, const uint8_t *, int64_t, const uint16_t *, float *, int, int, int,
+                                            hipStream_t, float *, size_t);
+template hipError_t launch_kq_gemm<Epilogue>(int, const uint8_t *, int64_t, const uint16_t *, Epilogue, int, int, int,
+                                             hipStream_t, float *, size_t);
 
 }  // namespace gollek

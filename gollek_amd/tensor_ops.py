@@ -346,6 +346,13 @@ class GgufFile:
 
 # ---- device-pointer entry points (inputs already resident in HBM) ---------
 
+# activations of linear()
+ACT_NONE = 0
+ACT_RELU = 1
+ACT_SILU = 2
+ACT_GELU = 3
+ACT_GELU_TANH = 4
+
 class DeviceWeight:
     """A handle over GGUF bytes already in device memory (borrowed)."""
 
@@ -411,6 +418,61 @@ class DeviceWeight:
                                              ctypes.c_void_p(y_ptr), ctypes.c_void_p(stream),
                                              err.buf, err.size)
         check(rc, err)
+
+
+    def linear_workspace_bytes(self, m: int) -> int:
+        """Device workspace with which linear() of m rows splits K as far as it
+        pays (0: never)."""
+        return int(_native.load().gollek_hip_linear_workspace_bytes(self.handle, m))
+
+    def linear(self, x_ptr: int, m: int, y_ptr: int, y_type: int, *, y_stride: int = 0, bias_ptr: int = 0,
+               activation: int = ACT_NONE, mul_ptr: int = 0, mul_stride: int = 0, residual_ptr: int = 0,
+               residual_stride: int = 0, ws_ptr: int = 0, ws_bytes: int = 0, stream: int = 0) -> None:
+        """Y = act(X W^T + bias) * mul + residual (gollek_hip_linear_device): x
+        bf16 (m, cols), y / mul / residual of y_type with row strides (0:
+        packed), bias float32.  mul and residual may be y itself."""
+        err = _native.err_buf()
+        check(_native.load().gollek_hip_linear_device(self.handle, x_ptr, m, bias_ptr, activation, mul_ptr,
+                                                      mul_stride, residual_ptr, residual_stride, y_ptr, y_type,
+                                                      y_stride, ws_ptr, ws_bytes, stream, err.buf, err.size), err)
+
+
+_LINEAR_DTYPES = {_native.F32: np.float32, _native.F16: np.float16, _native.BF16: np.uint16}
+
+
+def linear(tensor: GgufTensor, x_bf16: np.ndarray, y_type: int = _native.F32, *, bias=None,
+           activation: int = ACT_NONE, mul=None, residual=None) -> np.ndarray:
+    """act(X W^T + bias) * mul + residual on host arrays: x_bf16 (m, columns)
+    uint16 bf16 bit patterns, bias (rows,) float32, mul and residual (m, rows) of
+    y_type (BF16 as uint16 bit patterns) -> (m, rows) of y_type."""
+    if tensor is None:
+        raise NullPointerError("tensor")
+    if x_bf16 is None:
+        raise NullPointerError("input")
+    if y_type not in _LINEAR_DTYPES:
+        raise UnsupportedOperationError(f"Unsupported linear output type id: {y_type} (F32, F16 or BF16)")
+    x = np.ascontiguousarray(x_bf16, dtype=np.uint16)
+    if x.ndim != 2 or x.shape[1] != tensor.columns:
+        raise IllegalArgumentError(f"input must be (m, {tensor.columns})")
+    m, dtype = x.shape[0], _LINEAR_DTYPES[y_type]
+
+    def operand(a, name, shape, dt):
+        if a is None:
+            return None
+        a = np.ascontiguousarray(a)
+        if a.shape != shape or a.dtype != dt:
+            raise IllegalArgumentError(f"{name} must be {shape} of {np.dtype(dt).name}")
+        return a
+
+    b = operand(bias, "bias", (tensor.rows,), np.float32)
+    mu = operand(mul, "mul", (m, tensor.rows), dtype)
+    re = operand(residual, "residual", (m, tensor.rows), dtype)
+    y = np.empty((m, tensor.rows), dtype)
+    at = [None if a is None else a.ctypes.data for a in (b, mu, re)]
+    err = _native.ErrBuf()
+    check(_native.load().gollek_hip_linear(tensor.handle(), x.ctypes.data, x.size, m, at[0], activation, at[1], at[2],
+                                           y.ctypes.data, y_type, y.size, err.buf, err.size), err)
+    return y
 
 
 def gemm_bf16(tensor: GgufTensor, x_bf16: np.ndarray, output: np.ndarray) -> None:

@@ -192,6 +192,59 @@ int32_t gollek_hip_matvec_rows(gollek_hip_weight *weight, const float *x, int64_
 int32_t gollek_hip_gemm_bf16(gollek_hip_weight *weight, const uint16_t *x_bf16, int64_t x_len,
                              int64_t m, float *y, int64_t y_len, char *err, size_t err_len);
 
+/* ---- the linear layer ---------------------------------------------------- */
+
+/* Element types of a linear layer's output and of logits (ggml type ids). */
+#define GOLLEK_HIP_F32 0
+#define GOLLEK_HIP_F16 1
+#define GOLLEK_HIP_BF16 30
+
+/* Activations: relu max(v, 0); silu v / (1 + exp(-v)); gelu v Phi(v) (by erf);
+ * gelu_tanh its tanh form 0.5 v (1 + tanh(sqrt(2 / pi) (v + 0.044715 v^3))). */
+#define GOLLEK_HIP_ACT_NONE 0
+#define GOLLEK_HIP_ACT_RELU 1
+#define GOLLEK_HIP_ACT_SILU 2
+#define GOLLEK_HIP_ACT_GELU 3
+#define GOLLEK_HIP_ACT_GELU_TANH 4
+
+/* The GEMM with what a model does with its result:
+ *   Y[m, n] = act(sum_k X[m, k] W[n, k] + bias[n]) * mul[m, n] + residual[m, n]
+ * in fp32, rounded once to y_type (F32, F16 or BF16; nearest, ties to even).
+ * bias (`rows` floats), mul and residual (m x rows of y_type) may each be NULL
+ * and are then left out.  The sums are gollek_hip_gemm_bf16's for the same
+ * weight, X and m (bit for bit where neither splits K, or both in as many parts).
+ * A gated FFN is two calls: the up product, then the gate's with
+ * activation SILU and mul = the up product's Y.  The reference adds biases and
+ * residuals in Java after its linear (AccelOps.java:370-376).
+ * The host form takes packed matrices; x_len < m * cols or y_len < m * rows ->
+ * ARG (mul and residual hold y_len elements too).  An unknown activation -> ARG,
+ * another y_type -> UNSUPPORTED; the checks of gollek_hip_gemm_bf16 apply.
+ * m == 0 is a no-op. */
+int32_t gollek_hip_linear(gollek_hip_weight *weight, const uint16_t *x_bf16, int64_t x_len, int64_t m,
+                          const float *bias, int32_t activation, const void *mul, const void *residual, void *y,
+                          int32_t y_type, int64_t y_len, char *err, size_t err_len);
+
+/* Device workspace bytes with which gollek_hip_linear_device splits K as far as
+ * it pays (0: a call of m rows never splits); -1 for a NULL weight or m out of
+ * range. */
+int64_t gollek_hip_linear_workspace_bytes(const gollek_hip_weight *weight, int64_t m);
+
+/* Device variant, asynchronous on `stream`, which belongs to the weight's
+ * device; allocates nothing, so it can be captured into a graph.  The strides
+ * are elements between rows, at least `rows` (0: packed).  Y may be mul or
+ * residual (the same address and stride), or another column range of one wider
+ * matrix; any other overlap of Y with mul, residual or X -> ARG, and Y must not
+ * overlap bias, workspace or the weight.  Elements of Y's rows past column
+ * `rows` are left as they are.  Pointers are aligned to their elements (else
+ * ARG).  workspace (256-byte aligned, else ARG) may be smaller than
+ * gollek_hip_linear_workspace_bytes, or NULL: the call splits less, which
+ * changes Y by the rounding of the sums' order alone.  Calls that share a
+ * workspace must not overlap. */
+int32_t gollek_hip_linear_device(gollek_hip_weight *weight, const uint16_t *x_bf16, int64_t m, const float *bias,
+                                 int32_t activation, const void *mul, int64_t mul_stride, const void *residual,
+                                 int64_t residual_stride, void *y, int32_t y_type, int64_t y_stride, void *workspace,
+                                 int64_t workspace_bytes, void *stream, char *err, size_t err_len);
+
 /* Grouped MoE expert FFN over expert weights of any type this library takes
  * (Q4_0, Q8_0, Q4_K, Q5_K, Q6_K; gate, up and down may differ, as in Q4_K_M
  * files whose ffn_down_exps are Q6_K in some layers), stacked as GGUF stores

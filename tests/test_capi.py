@@ -125,3 +125,16 @@ def test_python_mirror_null_checks():
         ops.mat_vec_rows(None, np.zeros(4, np.float32), np.zeros(4, np.float32), 1)
     with pytest.raises(ops.NullPointerError):
         ops.dot_row(None, 0, np.zeros(4, np.float32))
+
+
+def test_linear_refuses_a_null_weight():
+    lib = _native.load()
+    e = _err()
+    x, y = np.zeros(32, np.uint16), np.zeros(4, np.float32)
+    assert lib.gollek_hip_linear(None, x.ctypes.data, 32, 1, None, 0, None, None, y.ctypes.data, _native.F32, 4, e.buf,
+                                 e.size) == _native.ERR_NULL
+    assert lib.gollek_hip_linear_device(None, None, 1, None, 0, None, 0, None, 0, None, _native.F32, 0, None, 0, None,
+                                        e.buf, e.size) == _native.ERR_NULL
+    assert lib.gollek_hip_linear_workspace_bytes(None, 1) == -1
+    with pytest.raises(ops.NullPointerError):
+        ops.linear(None, np.zeros((1, 32), np.uint16))

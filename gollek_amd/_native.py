@@ -33,6 +33,7 @@ _c = ctypes
 _P = _c.c_void_p
 _I32 = _c.c_int32
 _I64 = _c.c_int64
+_F32 = _c.c_float
 _SZ = _c.c_size_t
 _CHARP = _c.c_char_p
 
@@ -73,6 +74,12 @@ SIGNATURES: dict[str, tuple[object, list[object]]] = {
                                     _SZ]),
     "gollek_hip_moe_block_device": (_I32, [_P, _P, _P, _I64, _P, _P, _I64, _I64, _I32, _P, _P, _P,
                                            _P, _I64, _P, _CHARP, _SZ]),
+    "gollek_hip_moe_route": (_I32, [_P, _I32, _I64, _I64, _P, _I32, _I64, _I64, _I32, _I64, _I32, _F32, _P, _P,
+                                    _CHARP, _SZ]),
+    "gollek_hip_moe_route_device": (_I32, [_P, _I32, _I64, _I64, _P, _I32, _I64, _I64, _I32, _I64, _I32, _F32, _P,
+                                           _P, _P, _CHARP, _SZ]),
+    "gollek_hip_moe_block_routed_device": (_I32, [_P, _P, _P, _I64, _P, _P, _I32, _I64, _P, _I32, _I64, _I64, _I32,
+                                                  _I64, _I32, _F32, _P, _P, _P, _P, _I64, _P, _CHARP, _SZ]),
     "gollek_hip_moe_shared_expert": (_I32, [_P, _P, _P, _P, _P, _I64, _P, _I64, _CHARP, _SZ]),
     "gollek_hip_moe_shared_workspace_bytes": (_I64, [_I64, _I64, _I64]),
     "gollek_hip_moe_shared_expert_device": (_I32, [_P, _P, _P, _P, _P, _I64, _P, _P, _I64, _P, _CHARP,

@@ -875,6 +875,23 @@ private:
     int before_ = -1;
 };
 
+// The device that holds device memory p (the current one where there is no
+// other, or p is not known).
+int pointer_device(const void *p) {
+    static const int devices = [] {
+        int n = 0;
+        return hipGetDeviceCount(&n) == hipSuccess ? n : 0;
+    }();
+    int device = 0;
+    if (devices > 1) {
+        hipPointerAttribute_t at;
+        if (hipPointerGetAttributes(&at, p) == hipSuccess && at.type == hipMemoryTypeDevice) return at.device;
+        (void)hipGetLastError();
+    }
+    (void)hipGetDevice(&device);
+    return device;
+}
+
 int element_size(int32_t type) {
     return type == GOLLEK_HIP_F32 ? 4 : type == GOLLEK_HIP_F16 || type == GOLLEK_HIP_BF16 ? 2 : 0;
 }
@@ -1317,6 +1334,127 @@ int32_t gollek_hip_moe_select_topk(const float *logits, int64_t tokens, int64_t 
     if (e == hipSuccess) e = hipMemcpy(weights, d_w, (size_t)(tokens * top_k) * 4, hipMemcpyDeviceToHost);
     (void)hipFree(buf);
     if (e != hipSuccess) return hip_fail(e, "router", err, err_len);
+    ok(err, err_len);
+    return GOLLEK_HIP_OK;
+}
+
+static int32_t check_route(int32_t logits_type, const void *logits, int64_t tokens, int64_t n_experts,
+                           const float *bias, int32_t scoring, int64_t n_groups, int64_t top_groups, int32_t group_top,
+                           int64_t top_k, float scale, char *err, size_t err_len) {
+    const int32_t rc = check_router(tokens, n_experts, top_k, scoring, err, err_len);
+    if (rc != GOLLEK_HIP_OK) return rc;
+    const int size = element_size(logits_type);
+    if (size == 0)
+        return fail(GOLLEK_HIP_ERR_UNSUPPORTED, err, err_len, "Unsupported logits type id: %d (F32, F16 or BF16)",
+                    logits_type);
+    if (n_groups < 1 || n_groups > 64 || n_experts % n_groups != 0)
+        return fail(GOLLEK_HIP_ERR_ARG, err, err_len, "%lld experts do not fall into %lld groups (1 to 64)",
+                    (long long)n_experts, (long long)n_groups);
+    if (top_groups < 1 || top_groups > n_groups || group_top < 1 || group_top > 2)
+        return fail(GOLLEK_HIP_ERR_ARG, err, err_len, "Invalid top_groups %lld of %lld / group_top %d",
+                    (long long)top_groups, (long long)n_groups, group_top);
+    if (top_k > top_groups * (n_experts / n_groups))
+        return fail(GOLLEK_HIP_ERR_ARG, err, err_len, "top_k %lld is more than the %lld experts of %lld groups",
+                    (long long)top_k, (long long)(top_groups * (n_experts / n_groups)), (long long)top_groups);
+    if (!(scale - scale == 0.0f)) return fail(GOLLEK_HIP_ERR_ARG, err, err_len, "The scale is not finite");
+    if (reinterpret_cast<uintptr_t>(logits) % (uintptr_t)size != 0 ||
+        reinterpret_cast<uintptr_t>(bias) % sizeof(float) != 0)
+        return fail(GOLLEK_HIP_ERR_ARG, err, err_len, "The logits or the bias are not aligned to their elements");
+    return GOLLEK_HIP_OK;
+}
+
+int32_t gollek_hip_moe_route_device(const void *logits, int32_t logits_type, int64_t tokens, int64_t n_experts,
+                                    const float *bias, int32_t scoring, int64_t n_groups, int64_t top_groups,
+                                    int32_t group_top, int64_t top_k, int32_t renormalize, float scale, int32_t *ids,
+                                    float *weights, void *stream, char *err, size_t err_len) {
+    const int32_t rc = check_route(logits_type, logits, tokens, n_experts, bias, scoring, n_groups, top_groups,
+                                   group_top, top_k, scale, err, err_len);
+    if (rc != GOLLEK_HIP_OK) return rc;
+    if (tokens == 0) {
+        ok(err, err_len);
+        return GOLLEK_HIP_OK;
+    }
+    if (logits == nullptr || ids == nullptr || weights == nullptr)
+        return fail(GOLLEK_HIP_ERR_NULL, err, err_len, "router buffers");
+    const DeviceGuard device(pointer_device(logits));
+    const hipError_t e = gollek::launch_moe_expert_route(
+        logits, logits_type, (int)tokens, (int)n_experts, bias, scoring == GOLLEK_HIP_ROUTER_SIGMOID, (int)n_groups,
+        (int)top_groups, group_top, (int)top_k, renormalize != 0, scale, ids, weights, static_cast<hipStream_t>(stream));
+    if (e != hipSuccess) return hip_fail(e, "route launch", err, err_len);
+    ok(err, err_len);
+    return GOLLEK_HIP_OK;
+}
+
+int32_t gollek_hip_moe_route(const void *logits, int32_t logits_type, int64_t tokens, int64_t n_experts,
+                             const float *bias, int32_t scoring, int64_t n_groups, int64_t top_groups,
+                             int32_t group_top, int64_t top_k, int32_t renormalize, float scale, int32_t *ids,
+                             float *weights, char *err, size_t err_len) {
+    int32_t rc = check_route(logits_type, logits, tokens, n_experts, bias, scoring, n_groups, top_groups, group_top,
+                             top_k, scale, err, err_len);
+    if (rc != GOLLEK_HIP_OK) return rc;
+    if (tokens == 0) {
+        ok(err, err_len);
+        return GOLLEK_HIP_OK;
+    }
+    if (logits == nullptr || ids == nullptr || weights == nullptr)
+        return fail(GOLLEK_HIP_ERR_NULL, err, err_len, "router buffers");
+    const size_t ln = (size_t)(tokens * n_experts) * element_size(logits_type), rn = (size_t)(tokens * top_k) * 4;
+    const size_t lb = align_up(ln, 256), rb = align_up(rn, 256), bn = (size_t)n_experts * 4;
+    uint8_t *buf = nullptr;
+    hipError_t e = hipMalloc(reinterpret_cast<void **>(&buf), lb + 2 * rb + bn);
+    if (e != hipSuccess) return hip_fail(e, "hipMalloc(router)", err, err_len);
+    int32_t *const d_ids = reinterpret_cast<int32_t *>(buf + lb);
+    float *const d_w = reinterpret_cast<float *>(buf + lb + rb), *d_b = nullptr;
+    e = hipMemcpy(buf, logits, ln, hipMemcpyHostToDevice);
+    if (e == hipSuccess && bias != nullptr) {
+        d_b = reinterpret_cast<float *>(buf + lb + 2 * rb);
+        e = hipMemcpy(d_b, bias, bn, hipMemcpyHostToDevice);
+    }
+    if (e == hipSuccess)
+        e = gollek::launch_moe_expert_route(buf, logits_type, (int)tokens, (int)n_experts, d_b,
+                                            scoring == GOLLEK_HIP_ROUTER_SIGMOID, (int)n_groups, (int)top_groups,
+                                            group_top, (int)top_k, renormalize != 0, scale, d_ids, d_w, nullptr);
+    if (e == hipSuccess) e = hipMemcpy(ids, d_ids, rn, hipMemcpyDeviceToHost);
+    if (e == hipSuccess) e = hipMemcpy(weights, d_w, rn, hipMemcpyDeviceToHost);
+    (void)hipFree(buf);
+    if (e != hipSuccess) return hip_fail(e, "route", err, err_len);
+    ok(err, err_len);
+    return GOLLEK_HIP_OK;
+}
+
+int32_t gollek_hip_moe_block_routed_device(gollek_hip_weight *gate, gollek_hip_weight *up, gollek_hip_weight *down,
+                                           int64_t n_experts, const float *x, const void *logits, int32_t logits_type,
+                                           int64_t tokens, const float *bias, int32_t scoring, int64_t n_groups,
+                                           int64_t top_groups, int32_t group_top, int64_t top_k, int32_t renormalize,
+                                           float scale, int32_t *ids, float *weights, float *out, void *workspace,
+                                           int64_t workspace_bytes, void *stream, char *err, size_t err_len) {
+    MoeShape sh;
+    int32_t rc = check_moe(gate, up, down, n_experts, tokens, top_k, &sh, err, err_len);
+    if (rc != GOLLEK_HIP_OK) return rc;
+    // every check before the first launch: a refused call leaves ids and weights alone
+    rc = check_route(logits_type, logits, tokens, n_experts, bias, scoring, n_groups, top_groups, group_top, top_k,
+                     scale, err, err_len);
+    if (rc != GOLLEK_HIP_OK) return rc;
+    if (tokens == 0) {
+        ok(err, err_len);
+        return GOLLEK_HIP_OK;
+    }
+    if (x == nullptr || logits == nullptr || ids == nullptr || weights == nullptr || out == nullptr ||
+        workspace == nullptr)
+        return fail(GOLLEK_HIP_ERR_NULL, err, err_len, "MoE block buffers");
+    const int64_t need = gollek_hip_moe_workspace_bytes(tokens, top_k, sh.H, sh.I, sh.E);
+    if (workspace_bytes < need || (reinterpret_cast<uintptr_t>(workspace) & 255u) != 0)
+        return fail(GOLLEK_HIP_ERR_ARG, err, err_len,
+                    "Workspace of %lld bytes (256-byte aligned) needed, got %lld",
+                    (long long)need, (long long)workspace_bytes);
+    const DeviceGuard device(gate->device);
+    const hipStream_t s = static_cast<hipStream_t>(stream);
+    hipError_t e = gollek::launch_moe_expert_route(
+        logits, logits_type, (int)tokens, sh.E, bias, scoring == GOLLEK_HIP_ROUTER_SIGMOID, (int)n_groups,
+        (int)top_groups, group_top, (int)top_k, renormalize != 0, scale, ids, weights, s);
+    if (e == hipSuccess)
+        e = moe_launch(sh, gate, up, down, x, ids, weights, tokens, top_k, out, static_cast<uint8_t *>(workspace), s);
+    if (e != hipSuccess) return hip_fail(e, "moe block launch", err, err_len);
     ok(err, err_len);
     return GOLLEK_HIP_OK;
 }

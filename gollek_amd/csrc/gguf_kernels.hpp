@@ -234,6 +234,12 @@ hipError_t launch_moe_combine(const int32_t *ids, const float *wts, const float 
 size_t moe_topk_lds_bytes(int E, int K);
 hipError_t launch_moe_topk(const float *logits, int T, int E, int K, int sigmoid, int32_t *ids,
                            float *wts, hipStream_t stream);
+// Routing with a balancing bias, groups and unnormalised or scaled weights
+// (gguf_moe_route.hip): E <= 4096, groups <= 64 dividing E, group_top 1 or 2,
+// top_k <= top_groups * E / groups.
+hipError_t launch_moe_expert_route(const void *logits, int logits_type, int T, int E, const float *bias, bool sigmoid,
+                                   int groups, int top_groups, int group_top, int top_k, bool renormalize, float scale,
+                                   int32_t *ids, float *weights, hipStream_t stream);
 
 }  // namespace gollek
 

@@ -598,6 +598,55 @@ def moe_block_device(gate: DeviceWeight, up: DeviceWeight, down: DeviceWeight, n
     check(rc, err)
 
 
+def moe_route(logits, top_k: int, scoring: int, *, bias=None, n_groups: int = 1, top_groups: int = 1,
+              group_top: int = 1, renormalize: bool = True, scale: float = 1.0):
+    """Routing with a balancing bias and groups (gollek_hip_moe_route) on host
+    arrays: logits (tokens, n_experts) float32 or float16 -> ids (tokens, top_k)
+    int32, weights (tokens, top_k) float32."""
+    if logits is None:
+        raise NullPointerError("logits")
+    lv = np.ascontiguousarray(logits)
+    if lv.dtype != np.float16:
+        lv = np.ascontiguousarray(lv, dtype=np.float32)
+    if lv.ndim != 2:
+        raise IllegalArgumentError("logits must be (tokens, n_experts)")
+    tokens, n_experts = lv.shape
+    bv = None if bias is None else np.ascontiguousarray(bias, dtype=np.float32)
+    if bv is not None and bv.shape != (n_experts,):
+        raise IllegalArgumentError(f"bias must be ({n_experts},)")
+    ids = np.zeros((tokens, max(top_k, 0)), np.int32)
+    w = np.zeros((tokens, max(top_k, 0)), np.float32)
+    err = _native.ErrBuf()
+    check(_native.load().gollek_hip_moe_route(lv.ctypes.data, _native.F16 if lv.dtype == np.float16 else _native.F32,
+                                              tokens, n_experts, None if bv is None else bv.ctypes.data, scoring,
+                                              n_groups, top_groups, group_top, top_k, int(renormalize), scale,
+                                              ids.ctypes.data, w.ctypes.data, err.buf, err.size), err)
+    return ids, w
+
+
+def moe_route_device(logits_ptr: int, logits_type: int, tokens: int, n_experts: int, top_k: int, scoring: int,
+                     ids_ptr: int, w_ptr: int, *, bias_ptr: int = 0, n_groups: int = 1, top_groups: int = 1,
+                     group_top: int = 1, renormalize: bool = True, scale: float = 1.0, stream: int = 0) -> None:
+    err = _native.err_buf()
+    check(_native.load().gollek_hip_moe_route_device(logits_ptr, logits_type, tokens, n_experts, bias_ptr, scoring,
+                                                     n_groups, top_groups, group_top, top_k, renormalize, scale,
+                                                     ids_ptr, w_ptr, stream, err.buf, err.size), err)
+
+
+def moe_block_routed_device(gate: DeviceWeight, up: DeviceWeight, down: DeviceWeight, n_experts: int, x_ptr: int,
+                            logits_ptr: int, logits_type: int, tokens: int, top_k: int, scoring: int, ids_ptr: int,
+                            w_ptr: int, out_ptr: int, ws_ptr: int, ws_bytes: int, *, bias_ptr: int = 0,
+                            n_groups: int = 1, top_groups: int = 1, group_top: int = 1, renormalize: bool = True,
+                            scale: float = 1.0, stream: int = 0) -> None:
+    """moe_route_device followed by moe_grouped_device on one stream
+    (gollek_hip_moe_block_routed_device)."""
+    err = _native.err_buf()
+    check(_native.load().gollek_hip_moe_block_routed_device(
+        gate.handle, up.handle, down.handle, n_experts, x_ptr, logits_ptr, logits_type, tokens, bias_ptr, scoring,
+        n_groups, top_groups, group_top, top_k, renormalize, scale, ids_ptr, w_ptr, out_ptr, ws_ptr, ws_bytes, stream,
+        err.buf, err.size), err)
+
+
 def moe_shared_expert(gate: GgufTensor, up: GgufTensor, down: GgufTensor, x, out,
                       gate_inp=None) -> np.ndarray:
     """The shared expert added to the routed output `out` (MoeForwardPass.java:

@@ -360,6 +360,40 @@ int32_t gollek_hip_moe_block_device(gollek_hip_weight *gate, gollek_hip_weight *
                                     void *workspace, int64_t workspace_bytes, void *stream,
                                     char *err, size_t err_len);
 
+/* Routing with what gollek_hip_moe_select_topk has not: logits of type F32, F16
+ * or BF16, a bias for balance, groups, and weights as they are.  Per token:
+ *   p = softmax(l) or 1 / (1 + exp(-l)) by `scoring`;  c = p + bias (n_experts
+ *   floats, NULL: none);
+ *   the n_experts / n_groups neighbours of a group make it worth the sum of
+ *   their group_top (1 or 2) largest c; the top_groups groups worth most stay;
+ *   of their experts the top_k with the largest c, in that order -> ids; ties
+ *   (of groups too) go to the lower index, NaN comes first;
+ *   weights = p of each (without the bias), divided by their sum if renormalize
+ *   and the sum is > 0, times scale.
+ * Computed in double and rounded once; ids and weights row-major tokens x
+ * top_k.  n_experts in [1, 4096]; n_groups in [1, 64] dividing it, top_groups in
+ * [1, n_groups]; top_k in [1, top_groups * n_experts / n_groups]; a finite scale;
+ * aligned logits: else ARG; another logits_type -> UNSUPPORTED.  No reference
+ * counterpart: MoeForwardPass.java:174-203 routes by plain scores alone. */
+int32_t gollek_hip_moe_route(const void *logits, int32_t logits_type, int64_t tokens, int64_t n_experts,
+                             const float *bias, int32_t scoring, int64_t n_groups, int64_t top_groups,
+                             int32_t group_top, int64_t top_k, int32_t renormalize, float scale, int32_t *ids,
+                             float *weights, char *err, size_t err_len);
+int32_t gollek_hip_moe_route_device(const void *logits, int32_t logits_type, int64_t tokens, int64_t n_experts,
+                                    const float *bias, int32_t scoring, int64_t n_groups, int64_t top_groups,
+                                    int32_t group_top, int64_t top_k, int32_t renormalize, float scale, int32_t *ids,
+                                    float *weights, void *stream, char *err, size_t err_len);
+
+/* The MoE block behind that routing: gollek_hip_moe_route_device, then
+ * gollek_hip_moe_grouped_device with the ids and weights it chose, on one
+ * stream (as gollek_hip_moe_block_device; the checks of both calls apply). */
+int32_t gollek_hip_moe_block_routed_device(gollek_hip_weight *gate, gollek_hip_weight *up, gollek_hip_weight *down,
+                                           int64_t n_experts, const float *x, const void *logits, int32_t logits_type,
+                                           int64_t tokens, const float *bias, int32_t scoring, int64_t n_groups,
+                                           int64_t top_groups, int32_t group_top, int64_t top_k, int32_t renormalize,
+                                           float scale, int32_t *ids, float *weights, float *out, void *workspace,
+                                           int64_t workspace_bytes, void *stream, char *err, size_t err_len);
+
 /* The shared expert, added to the routed output of the same tokens
  * (SFE/generation/moe/MoeForwardPass.java:240-247 with runSharedExpert
  * :418-426 and resolveSharedExpertGate :428-442): for each token t

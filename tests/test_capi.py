@@ -138,3 +138,32 @@ def test_linear_refuses_a_null_weight():
     assert lib.gollek_hip_linear_workspace_bytes(None, 1) == -1
     with pytest.raises(ops.NullPointerError):
         ops.linear(None, np.zeros((1, 32), np.uint16))
+
+
+@pytest.mark.parametrize("kw", [dict(n_groups=5), dict(n_groups=0), dict(n_groups=2, top_groups=3), dict(top_groups=0),
+                                dict(group_top=0), dict(group_top=3), dict(top_k=33), dict(top_k=0),
+                                dict(n_groups=4, top_groups=1, top_k=9), dict(scale=float("nan")),
+                                dict(scale=float("inf")), dict(scoring=2), dict(bias=np.zeros(31, np.float32))])
+def test_route_refuses(kw):
+    call = dict(top_k=4, scoring=0)
+    call.update(kw)
+    with pytest.raises(ops.IllegalArgumentError):
+        ops.moe_route(np.zeros((3, 32), np.float32), **call)
+
+
+def test_route_refuses_types_nulls_and_misaligned_logits():
+    lib, e = _native.load(), _err()
+
+    def rc(logits=4096, kind=0, tokens=1, experts=32, bias=0, ids=4096, w=4096):
+        return lib.gollek_hip_moe_route_device(logits, kind, tokens, experts, bias, 0, 1, 1, 1, 2, 1, 1.0, ids, w, None,
+                                               e.buf, e.size)
+
+    assert rc(kind=8) == _native.ERR_UNSUPPORTED
+    assert rc(logits=0) == rc(ids=0) == rc(w=0) == _native.ERR_NULL
+    assert rc(logits=4098) == rc(logits=4097, kind=30) == rc(bias=4098) == _native.ERR_ARG
+    assert rc(tokens=-1) == rc(experts=4097) == rc(experts=0) == _native.ERR_ARG
+    assert rc(tokens=0, logits=0) == _native.OK
+    with pytest.raises(ops.NullPointerError):
+        ops.moe_route(None, 2, 0)
+    with pytest.raises(ops.IllegalArgumentError):
+        ops.moe_route(np.zeros(32, np.float32), 2, 0)

@@ -84,6 +84,11 @@ SIGNATURES: dict[str, tuple[object, list[object]]] = {
     "gollek_hip_moe_shared_workspace_bytes": (_I64, [_I64, _I64, _I64]),
     "gollek_hip_moe_shared_expert_device": (_I32, [_P, _P, _P, _P, _P, _I64, _P, _P, _I64, _P, _CHARP,
                                                    _SZ]),
+    "gollek_hip_sample": (_I32, [_P, _I32, _I64, _I64, _P, _P, _P, _P, _P, _P, _P, _P, _CHARP, _SZ]),
+    "gollek_hip_sample_workspace_bytes": (_I64, [_I64, _I64]),
+    "gollek_hip_sample_device": (_I32, [_P, _I32, _I64, _I64, _I64, _P, _P, _P, _P, _P, _P, _P, _P, _P, _I64, _P,
+                                        _CHARP, _SZ]),
+    "gollek_hip_next_token": (_I32, [_P, _P, _I64, _F32, _I32, _F32, _F32, _F32, _P, _P, _P, _CHARP, _SZ]),
     "gollek_hip_gguf_open": (_P, [_CHARP, _CHARP, _SZ]),
     "gollek_hip_gguf_close": (None, [_P]),
     "gollek_hip_gguf_info": (_I32, [_P, _P, _P, _P, _P, _P, _P]),

@@ -1555,6 +1555,164 @@ int32_t gollek_hip_moe_block(gollek_hip_weight *gate, gollek_hip_weight *up,
     return GOLLEK_HIP_OK;
 }
 
+// ---- sampling -------------------------------------------------------------
+
+constexpr int64_t kSampleMaxVocab = (int64_t)1 << 22, kSampleMaxRows = 65535;
+
+static int32_t check_sample(const void *logits, int32_t logits_type, int64_t rows, int64_t vocab, int64_t stride,
+                            const float *temperature, const int32_t *top_k, const float *top_p, const float *min_p,
+                            const float *u, const int32_t *tokens, const float *probs, const int32_t *kept, char *err,
+                            size_t err_len) {
+    const int size = element_size(logits_type);
+    if (size == 0)
+        return fail(GOLLEK_HIP_ERR_UNSUPPORTED, err, err_len, "Unsupported logits type id: %d (F32, F16 or BF16)",
+                    logits_type);
+    if (rows < 0 || rows > kSampleMaxRows || vocab < 1 || vocab > kSampleMaxVocab)
+        return fail(GOLLEK_HIP_ERR_ARG, err, err_len, "Logits of %lld x %lld are out of range (at most %lld x %lld)",
+                    (long long)rows, (long long)vocab, (long long)kSampleMaxRows, (long long)kSampleMaxVocab);
+    if (stride < vocab || stride > (int64_t)1 << 40)
+        return fail(GOLLEK_HIP_ERR_ARG, err, err_len, "The logits' row stride %lld is not at least %lld",
+                    (long long)stride, (long long)vocab);
+    if (rows == 0) return GOLLEK_HIP_OK;
+    if (logits == nullptr || u == nullptr || tokens == nullptr)
+        return fail(GOLLEK_HIP_ERR_NULL, err, err_len, "sampling buffers");
+    const uintptr_t four = reinterpret_cast<uintptr_t>(temperature) | reinterpret_cast<uintptr_t>(top_k) |
+                           reinterpret_cast<uintptr_t>(top_p) | reinterpret_cast<uintptr_t>(min_p) |
+                           reinterpret_cast<uintptr_t>(u) | reinterpret_cast<uintptr_t>(tokens) |
+                           reinterpret_cast<uintptr_t>(probs) | reinterpret_cast<uintptr_t>(kept);
+    if (reinterpret_cast<uintptr_t>(logits) % (uintptr_t)size != 0 || (four & 3u) != 0)
+        return fail(GOLLEK_HIP_ERR_ARG, err, err_len, "The sampling buffers are not aligned to their elements");
+    return GOLLEK_HIP_OK;
+}
+
+int64_t gollek_hip_sample_workspace_bytes(int64_t rows, int64_t vocab) {
+    if (rows < 0 || rows > kSampleMaxRows || vocab < 1 || vocab > kSampleMaxVocab) return -1;
+    return (int64_t)align_up(gollek::sample_workspace_bytes((int)rows, (int)vocab), 256);
+}
+
+int32_t gollek_hip_sample_device(const void *logits, int32_t logits_type, int64_t rows, int64_t vocab,
+                                 int64_t logits_stride, const float *temperature, const int32_t *top_k,
+                                 const float *top_p, const float *min_p, const float *u, int32_t *tokens, float *probs,
+                                 int32_t *kept, void *workspace, int64_t workspace_bytes, void *stream, char *err,
+                                 size_t err_len) {
+    if (logits_stride == 0) logits_stride = vocab;
+    const int32_t rc = check_sample(logits, logits_type, rows, vocab, logits_stride, temperature, top_k, top_p, min_p,
+                                    u, tokens, probs, kept, err, err_len);
+    if (rc != GOLLEK_HIP_OK) return rc;
+    if (rows == 0) {
+        ok(err, err_len);
+        return GOLLEK_HIP_OK;
+    }
+    const int64_t need = gollek_hip_sample_workspace_bytes(rows, vocab);
+    if (need > 0 && workspace == nullptr) return fail(GOLLEK_HIP_ERR_NULL, err, err_len, "sampling workspace");
+    if (workspace_bytes < need || (reinterpret_cast<uintptr_t>(workspace) & 255u) != 0)
+        return fail(GOLLEK_HIP_ERR_ARG, err, err_len, "Workspace of %lld bytes (256-byte aligned) needed, got %lld",
+                    (long long)need, (long long)workspace_bytes);
+    const DeviceGuard device(pointer_device(logits));
+    const hipError_t e = gollek::launch_sample(logits, logits_type, (int)rows, (int)vocab, logits_stride, temperature,
+                                               top_k, top_p, min_p, u, tokens, probs, kept,
+                                               static_cast<uint8_t *>(workspace), static_cast<hipStream_t>(stream));
+    if (e != hipSuccess) return hip_fail(e, "sample launch", err, err_len);
+    ok(err, err_len);
+    return GOLLEK_HIP_OK;
+}
+
+int32_t gollek_hip_sample(const void *logits, int32_t logits_type, int64_t rows, int64_t vocab,
+                          const float *temperature, const int32_t *top_k, const float *top_p, const float *min_p,
+                          const float *u, int32_t *tokens, float *probs, int32_t *kept, char *err, size_t err_len) {
+    const int32_t rc = check_sample(logits, logits_type, rows, vocab, vocab, temperature, top_k, top_p, min_p, u,
+                                    tokens, probs, kept, err, err_len);
+    if (rc != GOLLEK_HIP_OK) return rc;
+    if (rows == 0) {
+        ok(err, err_len);
+        return GOLLEK_HIP_OK;
+    }
+    // one allocation: logits | temperature, top_k, top_p, min_p, u | tokens, probs, kept | workspace
+    const size_t ln = (size_t)(rows * vocab) * element_size(logits_type), rn = (size_t)rows * 4;
+    const size_t lb = align_up(ln, 256), rb = align_up(rn, 256);
+    const size_t ws = gollek::sample_workspace_bytes((int)rows, (int)vocab);
+    uint8_t *d = nullptr;
+    hipError_t e = hipMalloc(reinterpret_cast<void **>(&d), lb + 8 * rb + ws);
+    if (e != hipSuccess) return hip_fail(e, "hipMalloc(sampling)", err, err_len);
+    const void *const in[5] = {temperature, top_k, top_p, min_p, u};
+    uint8_t *at[8];
+    for (int i = 0; i < 8; i++) at[i] = d + lb + (size_t)i * rb;
+    e = hipMemcpy(d, logits, ln, hipMemcpyHostToDevice);
+    for (int i = 0; i < 5 && e == hipSuccess; i++)
+        if (in[i] != nullptr) e = hipMemcpy(at[i], in[i], rn, hipMemcpyHostToDevice);
+        else at[i] = nullptr;
+    if (e == hipSuccess)
+        e = gollek::launch_sample(d, logits_type, (int)rows, (int)vocab, vocab, reinterpret_cast<float *>(at[0]),
+                                  reinterpret_cast<int32_t *>(at[1]), reinterpret_cast<float *>(at[2]),
+                                  reinterpret_cast<float *>(at[3]), reinterpret_cast<float *>(at[4]),
+                                  reinterpret_cast<int32_t *>(at[5]), reinterpret_cast<float *>(at[6]),
+                                  reinterpret_cast<int32_t *>(at[7]), d + lb + 8 * rb, nullptr);
+    if (e == hipSuccess) e = hipMemcpy(tokens, at[5], rn, hipMemcpyDeviceToHost);
+    if (e == hipSuccess && probs != nullptr) e = hipMemcpy(probs, at[6], rn, hipMemcpyDeviceToHost);
+    if (e == hipSuccess && kept != nullptr) e = hipMemcpy(kept, at[7], rn, hipMemcpyDeviceToHost);
+    (void)hipFree(d);
+    if (e != hipSuccess) return hip_fail(e, "sample", err, err_len);
+    ok(err, err_len);
+    return GOLLEK_HIP_OK;
+}
+
+int32_t gollek_hip_next_token(gollek_hip_weight *w, const float *x, int64_t x_len, float temperature, int32_t top_k,
+                              float top_p, float min_p, float u, int32_t *token, float *prob, int32_t *kept, char *err,
+                              size_t err_len) {
+    if (w == nullptr) return fail(GOLLEK_HIP_ERR_NULL, err, err_len, "tensor");
+    if (x == nullptr) return fail(GOLLEK_HIP_ERR_NULL, err, err_len, "vector");
+    if (token == nullptr) return fail(GOLLEK_HIP_ERR_NULL, err, err_len, "token");
+    if (x_len < w->cols)
+        return fail(GOLLEK_HIP_ERR_ARG, err, err_len, "Vector length %lld is smaller than columns %lld",
+                    (long long)x_len, (long long)w->cols);
+    if (w->rows < 1 || w->rows > kSampleMaxVocab)
+        return fail(GOLLEK_HIP_ERR_ARG, err, err_len, "A vocabulary of %lld is out of range (at most %lld)",
+                    (long long)w->rows, (long long)kSampleMaxVocab);
+    std::lock_guard<std::mutex> lock(w->mu);
+    int32_t rc = use_device(w->device, err, err_len);
+    if (rc != GOLLEK_HIP_OK) return rc;
+    // staging: x | the settings and results | logits | workspace
+    struct Row {
+        float temperature, top_p, min_p, u, prob;
+        int32_t top_k, token, kept;
+    };
+    const size_t xn = (size_t)w->cols * sizeof(float), x_bytes = align_up(xn, 256);
+    const size_t y_off = x_bytes + 256, ws_off = align_up(y_off + (size_t)w->rows * sizeof(float), 256);
+    rc = ensure_staging(w, ws_off + gollek::sample_workspace_bytes(1, (int)w->rows), err, err_len);
+    if (rc != GOLLEK_HIP_OK) return rc;
+    uint8_t *const hs = host_staging(w, y_off);
+    if (hs == nullptr) return fail(GOLLEK_HIP_ERR_NOMEM, err, err_len, "page-locked staging of %lld bytes", (long long)y_off);
+    uint8_t *const d = w->staging;
+    Row row = {temperature, top_p, min_p, u, 0.0f, top_k, -1, 0};
+    std::memcpy(hs, x, xn);
+    std::memcpy(hs + x_bytes, &row, sizeof(row));
+    hipError_t e = pull_staging(d, hs, x_bytes + 256, w->stream);
+    const float *const d_x = reinterpret_cast<float *>(d);
+    float *const d_y = reinterpret_cast<float *>(d + y_off);
+    if (e == hipSuccess && w->compact) {
+        e = gollek::launch_gemv_prepared(w->type_id, w->prep, w->row_bytes, w->cols, d_x, d_y, w->rows, w->prep_rows,
+                                         w->stream);
+        if (e == hipErrorInvalidValue)
+            return fail(GOLLEK_HIP_ERR_UNSUPPORTED, err, err_len,
+                        "compacted handle: the column kernel's partition is no longer its layout's");
+    } else if (e == hipSuccess) {
+        e = gollek::launch_gemv(w->type_id, w->data, w->row_bytes, w->cols, d_x, d_y, w->rows, w->stream, w->prep,
+                                w->prep_rows);
+    }
+    Row *const dr = reinterpret_cast<Row *>(d + x_bytes), *const hr = reinterpret_cast<Row *>(hs + x_bytes);
+    if (e == hipSuccess)  // (the results go to the page-locked staging, which is mapped for the device)
+        e = gollek::launch_sample(d_y, gollek::kF32, 1, (int)w->rows, w->rows, &dr->temperature, &dr->top_k, &dr->top_p,
+                                  &dr->min_p, &dr->u, &hr->token, &hr->prob, &hr->kept, d + ws_off, w->stream);
+    if (e == hipSuccess) e = hipStreamSynchronize(w->stream);
+    if (e != hipSuccess) return hip_fail(e, "next token", err, err_len);
+    std::memcpy(&row, hs + x_bytes, sizeof(row));
+    *token = row.token;
+    if (prob != nullptr) *prob = row.prob;
+    if (kept != nullptr) *kept = row.kept;
+    ok(err, err_len);
+    return GOLLEK_HIP_OK;
+}
+
 }  // extern "C"
 
 namespace gollek {

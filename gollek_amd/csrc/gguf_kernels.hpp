@@ -240,6 +240,13 @@ hipError_t launch_moe_topk(const float *logits, int T, int E, int K, int sigmoid
 hipError_t launch_moe_expert_route(const void *logits, int logits_type, int T, int E, const float *bias, bool sigmoid,
                                    int groups, int top_groups, int group_top, int top_k, bool renormalize, float scale,
                                    int32_t *ids, float *weights, hipStream_t stream);
+// One token per row of logits (gguf_sample.hip); the parameter arrays but u may
+// be nullptr, as may probs and kept.  vocab <= 2^22.
+size_t sample_workspace_bytes(int rows, int vocab);
+hipError_t launch_sample(const void *logits, int logits_type, int rows, int vocab, int64_t stride,
+                         const float *temperature, const int32_t *top_k, const float *top_p, const float *min_p,
+                         const float *u, int32_t *tokens, float *probs, int32_t *kept, uint8_t *workspace,
+                         hipStream_t stream);
 
 }  // namespace gollek
 

@@ -685,3 +685,73 @@ def moe_shared_expert_device(gate: DeviceWeight, up: DeviceWeight, down: DeviceW
                                                  V(out_ptr), V(ws_ptr), ws_bytes, V(stream),
                                                  err.buf, err.size)
     check(rc, err)
+
+
+# ---- sampling ------------------------------------------------------------------
+
+def sample(logits, u, *, temperature=None, top_k=None, top_p=None, min_p=None):
+    """One token per row of logits (gollek_hip_sample) on host arrays: logits
+    (rows, vocab) float32 or float16, u (rows,) the random numbers, settings
+    scalars or (rows,) arrays (None: off, temperature 1) -> tokens int32, probs
+    float32, kept int32, each (rows,)."""
+    if logits is None:
+        raise NullPointerError("logits")
+    if u is None:
+        raise NullPointerError("u")
+    lv = np.ascontiguousarray(logits)
+    if lv.dtype != np.float16:
+        lv = np.ascontiguousarray(lv, dtype=np.float32)
+    if lv.ndim != 2:
+        raise IllegalArgumentError("logits must be (rows, vocab)")
+    rows, vocab = lv.shape
+
+    def per_row(v, name, dtype):
+        if v is None:
+            return None
+        a = np.asarray(v, dtype=dtype)
+        if a.ndim == 0:
+            a = np.full(rows, a, dtype)
+        if a.shape != (rows,):
+            raise IllegalArgumentError(f"{name} must be a number or ({rows},)")
+        return np.ascontiguousarray(a)
+
+    args = [per_row(v, n, t) for v, n, t in ((temperature, "temperature", np.float32), (top_k, "top_k", np.int32),
+                                             (top_p, "top_p", np.float32), (min_p, "min_p", np.float32),
+                                             (u, "u", np.float32))]
+    tokens, probs, kept = np.empty(rows, np.int32), np.empty(rows, np.float32), np.empty(rows, np.int32)
+    err = _native.ErrBuf()
+    check(_native.load().gollek_hip_sample(lv.ctypes.data, _native.F16 if lv.dtype == np.float16 else _native.F32,
+                                           rows, vocab, *(None if a is None else a.ctypes.data for a in args),
+                                           tokens.ctypes.data, probs.ctypes.data, kept.ctypes.data, err.buf,
+                                           err.size), err)
+    return tokens, probs, kept
+
+
+def sample_workspace_bytes(rows: int, vocab: int) -> int:
+    return int(_native.load().gollek_hip_sample_workspace_bytes(rows, vocab))
+
+
+def sample_device(logits_ptr: int, logits_type: int, rows: int, vocab: int, u_ptr: int, tokens_ptr: int, *,
+                  logits_stride: int = 0, temperature_ptr: int = 0, top_k_ptr: int = 0, top_p_ptr: int = 0,
+                  min_p_ptr: int = 0, probs_ptr: int = 0, kept_ptr: int = 0, ws_ptr: int = 0, ws_bytes: int = 0,
+                  stream: int = 0) -> None:
+    err = _native.err_buf()
+    check(_native.load().gollek_hip_sample_device(logits_ptr, logits_type, rows, vocab, logits_stride,
+                                                  temperature_ptr, top_k_ptr, top_p_ptr, min_p_ptr, u_ptr, tokens_ptr,
+                                                  probs_ptr, kept_ptr, ws_ptr, ws_bytes, stream, err.buf, err.size),
+          err)
+
+
+def next_token(lm_head: GgufTensor, vector, u: float, *, temperature: float = 1.0, top_k: int = 0, top_p: float = 1.0,
+               min_p: float = 0.0):
+    """The lm_head's mat-vec of `vector` and a token sampled from it
+    (gollek_hip_next_token; the logits stay on the device) -> token, prob, kept."""
+    if lm_head is None:
+        raise NullPointerError("tensor")
+    x = _f32_in(vector, "vector")
+    token, prob, kept = ctypes.c_int32(), ctypes.c_float(), ctypes.c_int32()
+    err = _native.err_buf()
+    check(_native.load().gollek_hip_next_token(lm_head.handle(), x.ctypes.data, x.size, temperature, top_k, top_p,
+                                               min_p, u, ctypes.byref(token), ctypes.byref(prob), ctypes.byref(kept),
+                                               err.buf, err.size), err)
+    return token.value, prob.value, kept.value

@@ -419,6 +419,53 @@ int32_t gollek_hip_moe_shared_expert_device(gollek_hip_weight *gate, gollek_hip_
                                             int64_t workspace_bytes, void *stream, char *err,
                                             size_t err_len);
 
+/* ---- sampling -------------------------------------------------------------- */
+
+/* One token per row of logits (rows x vocab of type F32, F16 or BF16, rows
+ * `logits_stride` elements apart, 0: packed), as the lm_head's product leaves
+ * them, with settings per row.  Tokens are ordered by logit, equal ones by
+ * index; -inf and NaN logits are no tokens (a grammar's mask).  Per row:
+ *   w_i = exp((l_i - max l) / temperature);  temperature <= 0 or NaN keeps the
+ *   first token alone;
+ *   top_k > 0 keeps the first top_k tokens;  top_p < 1 keeps of these the
+ *   shortest prefix whose w add up to at least top_p of theirs (one token at
+ *   least);  min_p > 0 keeps of these the ones with w_i >= min(min_p, 1);
+ *   the token is the first, in the order of the vocabulary, at which the kept w
+ *   add up to more than u times all kept w (u the caller's random number in
+ *   [0, 1); below 0 or NaN it counts as 0, from 1 as the last fp32 below it).
+ * -> tokens[row] (-1 where a row has no token), probs[row] = its share of the
+ * kept w (0 without a token), kept[row] = how many were kept.  temperature (1),
+ * top_k, top_p and min_p (off), probs and kept may be NULL.  An infinite logit
+ * leaves only the infinite ones with weight.  Weights are summed exactly as
+ * multiples of 2^-S, vocab 2^S < 2^62, so a row's token does not depend on
+ * the batch around it.
+ * rows in [0, 65535], vocab in [1, 4194304], a stride of at least vocab, aligned
+ * pointers: else ARG; another logits_type -> UNSUPPORTED.  The host form takes
+ * packed logits and copies them up.  No counterpart on the reference's GGUF path
+ * (its sampling runs on the logits in host memory). */
+int32_t gollek_hip_sample(const void *logits, int32_t logits_type, int64_t rows, int64_t vocab,
+                          const float *temperature, const int32_t *top_k, const float *top_p, const float *min_p,
+                          const float *u, int32_t *tokens, float *probs, int32_t *kept, char *err, size_t err_len);
+/* Device workspace bytes gollek_hip_sample_device needs (-1: out of range). */
+int64_t gollek_hip_sample_workspace_bytes(int64_t rows, int64_t vocab);
+/* Device variant (every pointer on the device; `workspace` 256-byte aligned and
+ * of at least gollek_hip_sample_workspace_bytes, else ARG; calls sharing it must
+ * not overlap).  Allocates nothing: it can be captured into a graph. */
+int32_t gollek_hip_sample_device(const void *logits, int32_t logits_type, int64_t rows, int64_t vocab,
+                                 int64_t logits_stride, const float *temperature, const int32_t *top_k,
+                                 const float *top_p, const float *min_p, const float *u, int32_t *tokens, float *probs,
+                                 int32_t *kept, void *workspace, int64_t workspace_bytes, void *stream, char *err,
+                                 size_t err_len);
+
+/* The next token of one sequence: the lm_head's mat-vec (gollek_hip_matvec_rows
+ * of all rows) and gollek_hip_sample on its result, which stays on the device
+ * (a 128k vocabulary's logits are 0.5 MB).  x: x_len >= cols floats in host
+ * memory; token, prob, kept: one each, the last two may be NULL.  The checks of
+ * both calls apply; a weight of 0 rows or more than 4194304 -> ARG. */
+int32_t gollek_hip_next_token(gollek_hip_weight *lm_head, const float *x, int64_t x_len, float temperature,
+                              int32_t top_k, float top_p, float min_p, float u, int32_t *token, float *prob,
+                              int32_t *kept, char *err, size_t err_len);
+
 /* ---- GGUF files --------------------------------------------------------- */
 /* GC/ = runner/gguf/gollek-gguf-core/src/main/java/tech/kayys/gollek/gguf/. */
 

@@ -167,3 +167,37 @@ def test_route_refuses_types_nulls_and_misaligned_logits():
         ops.moe_route(None, 2, 0)
     with pytest.raises(ops.IllegalArgumentError):
         ops.moe_route(np.zeros(32, np.float32), 2, 0)
+
+
+def test_sample_refuses():
+    lib, e = _native.load(), _err()
+
+    def rc(logits=4096, kind=0, rows=1, vocab=100, stride=0, t=0, k=0, p=0, mp=0, u=4096, tok=4096, prob=0, kept=0,
+           ws=256, ws_bytes=1 << 40):
+        return lib.gollek_hip_sample_device(logits, kind, rows, vocab, stride, t, k, p, mp, u, tok, prob, kept, ws,
+                                            ws_bytes, None, e.buf, e.size)
+
+    assert rc(kind=8) == _native.ERR_UNSUPPORTED
+    assert rc(logits=0) == rc(u=0) == rc(tok=0) == _native.ERR_NULL
+    for bad in (dict(rows=-1), dict(rows=65536), dict(vocab=0), dict(vocab=(1 << 22) + 1), dict(stride=99),
+                dict(stride=-1), dict(logits=4098), dict(logits=4097, kind=1), dict(t=4098), dict(k=4097), dict(p=4098),
+                dict(mp=4098), dict(u=4098), dict(tok=4098), dict(prob=4098), dict(kept=4098), dict(ws=128)):
+        assert rc(**bad) == _native.ERR_ARG, bad
+    assert rc(rows=0, logits=0, u=0, tok=0) == _native.OK
+    assert lib.gollek_hip_sample_workspace_bytes(1, 0) == lib.gollek_hip_sample_workspace_bytes(-1, 10) == -1
+    need = lib.gollek_hip_sample_workspace_bytes(1, 100)
+    if need > 0:
+        assert rc(ws=0) == _native.ERR_NULL and rc(ws_bytes=need - 1) == _native.ERR_ARG
+    l, u = np.zeros((2, 8), np.float32), np.zeros(2, np.float32)
+    for kw in (dict(top_k=[1, 2, 3]), dict(temperature=np.zeros((2, 1)))):
+        with pytest.raises(ops.IllegalArgumentError):
+            ops.sample(l, u, **kw)
+    with pytest.raises(ops.IllegalArgumentError):
+        ops.sample(l[0], u)
+    for a in ((None, u), (l, None)):
+        with pytest.raises(ops.NullPointerError):
+            ops.sample(*a)
+    with pytest.raises(ops.NullPointerError):
+        ops.next_token(None, u, 0.5)
+    assert lib.gollek_hip_next_token(None, u.ctypes.data, 2, 1.0, 0, 1.0, 0.0, 0.5, u.ctypes.data, None, None, e.buf,
+                                     e.size) == _native.ERR_NULL

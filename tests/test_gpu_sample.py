@@ -1,0 +1,258 @@
+"""Sampling against its definition in float64, row by row.
+
+Tokens and kept counts are compared exactly: the kernel sums weights as
+multiples of 2^-S (V 2^S < 2^62), so its masses are off by at most V 2^-(S + 1)
+of the largest weight (4e-9 at 128k), and the settings and random numbers of
+these cases lie further than that from a border.  A probability is
+a quotient of a weight in double and such a mass, rounded once to fp32: 2^-24
+and V 2^-(S + 1) relative.
+"""
+import numpy as np
+import pytest
+import torch
+
+from gollek_amd import _native
+from gollek_amd import synthetic as syn
+from gollek_amd import tensor_ops as ops
+
+pytestmark = pytest.mark.gpu
+DTYPE = {_native.F32: torch.float32, _native.F16: torch.float16, _native.BF16: torch.bfloat16}
+KIND = {v: k for k, v in DTYPE.items()}
+
+
+@pytest.fixture(scope="module", autouse=True)
+def _init():
+    ops.init(0)
+
+
+def reference(l, u, t=1.0, k=0, p=1.0, mp=0.0):
+    """token, prob, kept of one row of float64 logits."""
+    at = np.flatnonzero(l > -np.inf)  # (NaN compares false)
+    if not at.size:
+        return -1, 0.0, 0
+    at = at[np.lexsort((at, -l[at]))]
+    if not t > 0:
+        at, t = at[:1], 1.0
+    if k > 0:
+        at = at[:k]
+    if np.isinf(l[at[0]]):
+        w = (l[at] == np.inf).astype(np.float64)
+    else:
+        w = np.exp((l[at] - l[at[0]]) / t)
+    if p < 1:
+        mass = np.cumsum(w)
+        n = 1 if not p > 0 else int((mass < p * mass[-1]).sum()) + 1
+        at, w = at[:n], w[:n]
+    if mp > 0:
+        keep = w >= min(mp, 1.0)
+        at, w = at[keep], w[keep]
+    order = np.argsort(at)
+    at, w = at[order], w[order]
+    mass = np.cumsum(w)
+    u = min(max(0.0 if np.isnan(u) else u, 0.0), 1 - 2.0**-24)
+    i = int((mass <= u * mass[-1]).sum())
+    return int(at[i]), w[i] / mass[-1], at.size
+
+
+def sample(logits, u, t=None, k=None, p=None, mp=None, vocab=None, stream=None):
+    """The device entry on a CUDA tensor of logits (rows may be longer than vocab)."""
+    rows, stride = logits.shape
+    vocab = stride if vocab is None else vocab
+
+    def dev(v, dtype):
+        return None if v is None else torch.as_tensor(np.broadcast_to(np.asarray(v, dtype), (rows,)).copy()).cuda()
+
+    t, k, p, mp, u = dev(t, np.float32), dev(k, np.int32), dev(p, np.float32), dev(mp, np.float32), dev(u, np.float32)
+    tok = torch.full((rows,), -9, device="cuda", dtype=torch.int32)
+    kept = torch.full((rows,), -9, device="cuda", dtype=torch.int32)
+    prob = torch.full((rows,), float("nan"), device="cuda")
+    ws = torch.full((max(ops.sample_workspace_bytes(rows, vocab), 256),), 255, device="cuda", dtype=torch.uint8)
+    at = [0 if v is None else v.data_ptr() for v in (t, k, p, mp)]
+    ops.sample_device(logits.data_ptr(), KIND[logits.dtype], rows, vocab, u.data_ptr(), tok.data_ptr(),
+                      logits_stride=stride, temperature_ptr=at[0], top_k_ptr=at[1], top_p_ptr=at[2], min_p_ptr=at[3],
+                      probs_ptr=prob.data_ptr(), kept_ptr=kept.data_ptr(), ws_ptr=ws.data_ptr(), ws_bytes=ws.numel(),
+                      stream=torch.cuda.current_stream().cuda_stream if stream is None else stream)
+    torch.cuda.synchronize()
+    return tok.cpu().numpy(), prob.cpu().numpy(), kept.cpu().numpy()
+
+
+def compare(got, l, u, what, t=1.0, k=0, p=1.0, mp=0.0):
+    l = l.double().cpu().numpy() if torch.is_tensor(l) else np.asarray(l, np.float64)
+    rows, v = l.shape
+    f32 = lambda x: np.broadcast_to(np.asarray(x, np.float32).astype(np.float64), (rows,))  # noqa: E731
+    u, t, p, mp, k = f32(u), f32(t), f32(p), f32(mp), np.broadcast_to(np.asarray(k), (rows,))
+    tol = 2.0**-24 * 1.01 + v * 2.0 ** -(62 - v.bit_length() + 1)
+    for r in range(rows):
+        token, prob, kept = reference(l[r], u[r], t[r], int(k[r]), p[r], mp[r])
+        have = (int(got[0][r]), float(got[1][r]), int(got[2][r]))
+        print(f"[gpu] {what} row {r}: {have} want {(token, prob, kept)}", flush=True)
+        assert have[0] == token and have[2] == kept, (what, r)
+        assert abs(have[1] - prob) <= tol * prob + 2.0**-150, (what, r)
+
+
+def logits_of(rows, vocab, seed, dtype=torch.float32, sigma=2.5):
+    rng = np.random.default_rng(seed)
+    l = rng.normal(size=(rows, vocab)) * sigma
+    for r in range(rows):
+        l[r, rng.integers(0, vocab, 12)] = rng.uniform(6, 14, 12)
+    return torch.from_numpy(l.astype(np.float32)).to(dtype).cuda()
+
+
+SETTINGS = [dict(), dict(t=0.7), dict(t=1.4, k=40), dict(p=0.9), dict(t=0.8, k=40, p=0.95), dict(mp=0.05),
+            dict(t=1.3, k=300, p=0.8, mp=0.01), dict(t=0.0), dict(k=1), dict(t=0.01, p=0.99), dict(t=30.0, p=0.5),
+            dict(t=100.0, k=5000, p=0.9), dict(t=3.0, p=0.97, mp=1e-4), dict(t=50.0, mp=0.7)]
+
+
+@pytest.mark.parametrize("i", range(len(SETTINGS)))
+@pytest.mark.parametrize("vocab,rows", [(1, 2), (2, 5), (63, 9), (1000, 6), (1025, 4), (4097, 3), (32000, 3),
+                                        (128256, 2)])
+def test_sample_matches_float64(vocab, rows, i):
+    dtype = (torch.float32, torch.bfloat16, torch.float16)[(i + vocab) % 3]
+    l = logits_of(rows, vocab, 10 * i + vocab, dtype)
+    u = np.random.default_rng(i).random(rows).astype(np.float32)
+    compare(sample(l, u, **SETTINGS[i]), l, u, f"{vocab} {SETTINGS[i]} {dtype}", **SETTINGS[i])
+
+
+def test_a_batch_with_settings_of_its_own_and_a_stride():
+    rows, vocab, stride = 70, 5001, 5056
+    wide = logits_of(rows, stride, 3)
+    wide[:, vocab:] = 1e4  # behind the vocabulary: never read as a token
+    rng = np.random.default_rng(4)
+    kw = dict(t=rng.choice([0.0, 0.6, 1.0, 1.7], rows), k=rng.choice([0, -3, 1, 7, 50, 900, 10**6], rows),
+              p=rng.choice([0.5, 0.9, 0.99, 1.0, 1.5], rows), mp=rng.choice([0.0, -1.0, 0.02, 0.3], rows))
+    u = rng.random(rows).astype(np.float32)
+    compare(sample(wide, u, vocab=vocab, **kw), wide[:, :vocab], u, "batch", **kw)
+
+
+def test_the_random_number_runs_through_the_distribution():
+    l = logits_of(1, 300, 5, sigma=1.0)
+    u = np.concatenate([[0.0, 1 - 2.0**-24, 1.0, 2.0, -1.0, np.nan], np.linspace(0.001, 0.999, 500)]).astype(np.float32)
+    many = l.expand(u.size, -1).contiguous()
+    got = sample(many, u, k=60, p=0.9)
+    compare(got, many, u, "u", k=60, p=0.9)
+    kept = got[2][0]
+    assert (got[2] == kept).all() and len(set(got[0].tolist())) > kept // 2
+
+
+@pytest.mark.parametrize("vocab", [500, 40000])
+def test_equal_logits(vocab):
+    """Ties are kept by index, in every filter."""
+    u = np.array([0.0, 0.3, 0.77, 0.999], np.float32)
+    flat = torch.zeros((4, vocab), device="cuda")
+    for kw in (dict(), dict(k=37), dict(p=0.301), dict(k=200, p=0.503), dict(mp=0.9), dict(p=0.999, t=2.0)):
+        compare(sample(flat, u, **kw), flat, u, f"flat {kw}", **kw)
+    steps = (torch.arange(vocab, device="cuda") * 7919 % 5).float().expand(4, -1).contiguous()  # five values
+    steps[:, 1::2] *= -0.0  # and zeros of both signs
+    for kw in (dict(k=vocab // 3), dict(p=0.6003), dict(k=vocab // 2 + 1, p=0.8501, t=0.9), dict(mp=0.03)):
+        compare(sample(steps, u, **kw), steps, u, f"steps {kw}", **kw)
+
+
+def test_masked_empty_nan_and_infinite_rows():
+    inf, nan = float("inf"), float("nan")
+    vocab = 2050
+    l = logits_of(8, vocab, 6)
+    l[0] = -inf                                # nothing left
+    l[1, 1:] = -inf                            # one token
+    l[2] = nan
+    l[3, ::2] = nan                            # NaN is no token, wherever it stands
+    l[4, 100] = l[4, 2000] = inf               # two infinite ones share the weight
+    l[5, torch.arange(vocab) % 50 != 7] = -inf
+    l[6] = -3.0e38
+    l[7, :3] = torch.tensor([3.3e38, 3.4e38, -3.4e38])
+    u = np.full(8, 0.6, np.float32)
+    for kw in (dict(), dict(k=5), dict(p=0.7), dict(t=0.9, k=30, p=0.9, mp=0.02), dict(t=0.0), dict(t=nan),
+               dict(t=inf, k=100, p=0.33), dict(t=1e-44), dict(p=0.0), dict(p=-1.0), dict(p=nan, mp=nan), dict(mp=5.0)):
+        ref = dict(kw)
+        if kw.get("p") is not None and np.isnan(kw.get("p")):
+            ref.pop("p"), ref.pop("mp")  # neither is below 1 nor above 0: off
+        compare(sample(l, u, **kw), l, u, f"{kw}", **ref)
+
+
+def test_a_rows_token_does_not_depend_on_its_batch():
+    vocab = 33000
+    l = logits_of(130, vocab, 7)
+    u = np.random.default_rng(8).random(130).astype(np.float32)
+    for kw in (dict(t=1.1), dict(p=0.95), dict(k=80, p=0.9)):
+        all_rows = sample(l, u, **kw)
+        for r in (0, 64, 129):
+            one = sample(l[r:r + 1].contiguous(), u[r:r + 1], **kw)
+            assert [a[0] for a in one] == [a[r] for a in all_rows]
+        again = sample(l, u, **kw)
+        assert all(np.array_equal(a, b) for a, b in zip(all_rows, again))
+
+
+def test_captured_calls_replay():
+    rows, vocab = 3, 40000
+    kw = dict(t=0.9, k=50, p=0.9)
+    l = torch.zeros((rows, vocab), device="cuda")
+    u = torch.zeros(rows, device="cuda")
+    par = [torch.full((rows,), v, device="cuda", dtype=d) for v, d in ((0.9, torch.float32), (50, torch.int32),
+                                                                      (0.9, torch.float32))]
+    tok = torch.zeros(rows, device="cuda", dtype=torch.int32)
+    kept, prob = torch.zeros_like(tok), torch.zeros(rows, device="cuda")
+    ws = torch.zeros(max(ops.sample_workspace_bytes(rows, vocab), 256), device="cuda", dtype=torch.uint8)
+    s = torch.cuda.Stream()
+
+    def go(stream):
+        ops.sample_device(l.data_ptr(), _native.F32, rows, vocab, u.data_ptr(), tok.data_ptr(),
+                          temperature_ptr=par[0].data_ptr(), top_k_ptr=par[1].data_ptr(), top_p_ptr=par[2].data_ptr(),
+                          probs_ptr=prob.data_ptr(), kept_ptr=kept.data_ptr(), ws_ptr=ws.data_ptr(),
+                          ws_bytes=ws.numel(), stream=stream)
+
+    with torch.cuda.stream(s):
+        go(s.cuda_stream)
+    torch.cuda.synchronize()
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g, stream=s):
+        go(s.cuda_stream)
+    for turn in range(4):
+        new = logits_of(rows, vocab, 50 + turn)
+        nu = np.random.default_rng(turn).random(rows).astype(np.float32)
+        l.copy_(new)
+        u.copy_(torch.from_numpy(nu))
+        torch.cuda.synchronize()
+        g.replay()
+        torch.cuda.synchronize()
+        compare((tok.cpu().numpy(), prob.cpu().numpy(), kept.cpu().numpy()), new, nu, f"replay {turn}", **kw)
+        ref = sample(new, nu, **kw)  # eager work between the replays
+        assert np.array_equal(ref[0], tok.cpu().numpy())
+
+
+def test_optional_outputs_and_host_form():
+    rng = np.random.default_rng(9)
+    l = (rng.normal(size=(5, 3000)) * 3).astype(np.float32)
+    u = rng.random(5).astype(np.float32)
+    got = ops.sample(l, u, temperature=0.8, top_k=[40, 0, 3, 100, 1], top_p=0.9, min_p=0.01)
+    compare(got, l, u, "host", t=0.8, k=np.array([40, 0, 3, 100, 1]), p=0.9, mp=0.01)
+    h = l.astype(np.float16)
+    compare(ops.sample(h, u), h, u, "host fp16")
+    assert all(a.shape == (0,) for a in ops.sample(l[:0], u[:0]))
+    dl, du = torch.from_numpy(l).cuda(), torch.from_numpy(u).cuda()
+    tok = torch.zeros(5, device="cuda", dtype=torch.int32)
+    ws = torch.zeros(max(ops.sample_workspace_bytes(5, 3000), 256), device="cuda", dtype=torch.uint8)
+    ops.sample_device(dl.data_ptr(), _native.F32, 5, 3000, du.data_ptr(), tok.data_ptr(), ws_ptr=ws.data_ptr(),
+                      ws_bytes=ws.numel(), stream=torch.cuda.current_stream().cuda_stream)
+    torch.cuda.synchronize()
+    assert np.array_equal(tok.cpu().numpy(), ops.sample(l, u)[0])
+
+
+@pytest.mark.parametrize("compact", [False, True])
+def test_next_token_is_the_mat_vec_and_the_sample(compact):
+    rows, cols = 4096, 1024
+    data = syn.matrix(syn.Q4_K, rows, cols, seed=10)
+    t = ops.GgufTensor("output.weight", (cols, rows), syn.Q4_K, data.reshape(-1))
+    if compact:
+        t.prepare()
+        t.compact()
+    rng = np.random.default_rng(11)
+    for i in range(6):
+        x = rng.normal(size=cols).astype(np.float32)
+        y = np.zeros(rows, np.float32)
+        ops.mat_vec(t, x, y)
+        kw = dict(temperature=(0.0, 5.0, 20.0)[i % 3], top_k=(0, 50)[i % 2], top_p=(1.0, 0.9)[i // 3], min_p=0.0)
+        got = ops.next_token(t, x, float(np.float32(0.1 + 0.13 * i)), **kw)
+        want = ops.sample(y[None], [np.float32(0.1 + 0.13 * i)], **kw)
+        assert got == (want[0][0], want[1][0], want[2][0])
+    with pytest.raises(ops.IllegalArgumentError):
+        ops.next_token(t, x[:-1], 0.5)
+    t.close()

@@ -14,6 +14,22 @@
 // additions, so neither the split of a row over workgroups nor atomics change a
 // token, and their rounding (2^-45 a token) is far below what fp32 sums would
 // lose at the borders of top_p and u.
+//
+// A row is cut into chunks of 4096 tokens and the chunks dealt to workgroups;
+// four launches, each reading the row at most once:
+//   1 the chunks' largest and least logits;
+//   2 rows with top_k or top_p: a histogram (tokens and mass) over 512 bins of
+//     l, linear from the largest logit down to where weights round to 0 (or to
+//     the least logit); other rows: every chunk's kept mass;
+//   3 the bin in which a filter's border falls, from the histogram; its
+//     tokens are collected, or, where that makes at most 4096, those of every bin
+//     down to it; the chunks' mass above it;
+//   4 one workgroup per row: the collected tokens sorted, the border in them, the
+//     draw: among the collected ones, or in the chunk that the random number
+//     falls into.
+// Rows whose border bin holds more than 4096 tokens (equal logits, a
+// temperature of 30), or whose top_k and top_p together reach further, are
+// computed by the last workgroup alone, digit by digit over the whole row.
 #include <hip/hip_runtime.h>
 
 #include "gguf_kernels.hpp"
@@ -49,13 +65,16 @@ struct SampleArgs {
     const void *logits;
     int64_t stride;
     int type, vocab, shift;
+    bool vec4;  // rows allow loads of four logits
     const float *temperature, *top_p, *min_p, *u;
     const int32_t *top_k;
     int32_t *tokens, *kept;
     float *probs;
 };
 
-constexpr int kThreads = 1024, kWaves = kThreads / 64;
+constexpr int kThreads = 1024, kWaves = kThreads / 64;  // of the last launch
+constexpr int kScan = 256;                              // of the others
+constexpr int kChunk = 4096, kBins = 512, kList = 4096;
 
 struct Border {  // kept: key > this one, or the same key at an index up to this one
     uint32_t key;
@@ -198,28 +217,10 @@ __device__ Border select(const SampleArgs &a, int64_t base, const Scale &sc, Bor
     return Border{prefix, s.found};
 }
 
-// One workgroup per row.
-__global__ __launch_bounds__(kThreads) void sample_row_kernel(SampleArgs a) {
-    __shared__ RowLds s;
-    __shared__ float wave_max[kWaves];
-    const int row = (int)blockIdx.x, tid = (int)threadIdx.x;
+// A row by one workgroup, whatever it holds.
+__device__ void whole_row(const SampleArgs &a, int row, const Wish &wish, float m, RowLds &s) {
+    const int tid = (int)threadIdx.x;
     const int64_t base = (int64_t)row * a.stride;
-    const Wish wish = row_wish(a, row);
-
-    float m = -__builtin_inff();
-    for (int i = tid; i < a.vocab; i += kThreads) m = fmaxf(m, load_element(a.logits, a.type, base + i));
-    for (int d = 1; d < 64; d <<= 1) m = fmaxf(m, __shfl_xor(m, d));
-    if ((tid & 63) == 0) wave_max[tid >> 6] = m;
-    __syncthreads();
-    for (int w = 0; w < kWaves; w++) m = fmaxf(m, wave_max[w]);
-    if (!(m > -__builtin_inff())) {  // no token at all
-        if (tid == 0) {
-            a.tokens[row] = -1;
-            if (a.probs != nullptr) a.probs[row] = 0.0f;
-            if (a.kept != nullptr) a.kept[row] = 0;
-        }
-        return;
-    }
     const Scale sc = {m, wish.inv_t, a.shift};
 
     // Mass and number of the tokens within a border that min_p keeps.
@@ -290,25 +291,655 @@ __global__ __launch_bounds__(kThreads) void sample_row_kernel(SampleArgs a) {
     }
 }
 
+// ---- the four launches --------------------------------------------------------
+
+struct Plan {
+    int mode;          // see kWhole ..
+    int bin;           // the border's bin
+    uint32_t before;   // tokens in the bins above it
+    uint32_t tokens;   // of the row that top_k leaves
+    u64 before_mass;   // mass in the bins above it
+    double target;     // mass that top_p wants
+};
+enum : int {
+    kWhole,   // the last workgroup alone
+    kFree,    // no border with weight below it: every token, by chunks
+    kBorder,  // the collected tokens are the border's bin
+    kAll,     // the collected tokens are all that top_k keeps, and some more
+};
+
+struct SampleWs {
+    float2 *range;        // [rows][chunks] largest, least logit
+    u64 *mass;            // [rows][parts][kBins]
+    u64 *chunk_mass;      // [rows][chunks]
+    u64 *list;            // [rows][kList]
+    Plan *plan;           // [rows]
+    uint32_t *count;      // [rows][parts][kBins]
+    uint32_t *chunk_kept; // [rows][chunks]
+    uint32_t *listed;     // [rows]
+    int chunks, parts;
+    // chunks of a part
+    __device__ __forceinline__ int first(int part) const { return (int)((int64_t)part * chunks / parts); }
+};
+
+// Logits i .. i + 3 of a row, -inf behind the vocabulary.
+__device__ __forceinline__ void load4(const SampleArgs &a, int64_t base, int i, float (&l)[4]) {
+    if (a.vec4 && i + 4 <= a.vocab) {
+        if (a.type == kF32) {
+            const float4 v = *reinterpret_cast<const float4 *>(static_cast<const float *>(a.logits) + base + i);
+            l[0] = v.x, l[1] = v.y, l[2] = v.z, l[3] = v.w;
+        } else {
+            const uint2 v = *reinterpret_cast<const uint2 *>(static_cast<const uint16_t *>(a.logits) + base + i);
+            const uint32_t h[4] = {v.x & 0xFFFFu, v.x >> 16, v.y & 0xFFFFu, v.y >> 16};
+#pragma unroll
+            for (int j = 0; j < 4; j++)
+                l[j] = a.type == kBF16 ? __uint_as_float(h[j] << 16) : (float)__builtin_bit_cast(_Float16, (uint16_t)h[j]);
+        }
+    } else {
+#pragma unroll
+        for (int j = 0; j < 4; j++) l[j] = i + j < a.vocab ? load_element(a.logits, a.type, base + i + j) : -__builtin_inff();
+    }
+}
+
+// The largest and least logit of the row's tokens.
+__device__ __forceinline__ float2 row_range(const SampleWs &ws, int row) {
+    float2 r = {-__builtin_inff(), __builtin_inff()};
+    for (int c = (int)threadIdx.x & 63; c < ws.chunks; c += 64) {
+        const float2 v = ws.range[(int64_t)row * ws.chunks + c];
+        r = {fmaxf(r.x, v.x), fminf(r.y, v.y)};
+    }
+    for (int d = 1; d < 64; d <<= 1) r = {fmaxf(r.x, __shfl_xor(r.x, d)), fminf(r.y, __shfl_xor(r.y, d))};
+    return r;
+}
+
+// Bins of a row: 0 at the largest logit.  far: the last bin is open, and what
+// falls into it has weight 0 (below 2^-(S + 1)).
+struct Bins {
+    float m, inv;
+    bool far;
+    __device__ __forceinline__ int of(float l) const {
+        return l == m || inv == 0.0f ? 0 : (int)fminf((m - l) * inv, (float)(kBins - 1));  // (m infinite: the last)
+    }
+};
+__device__ __forceinline__ Bins row_bins(const SampleArgs &a, const Wish &w, float2 r) {
+    const float reach = (float)((double)(a.shift + 2) * 0.69314718055994531 / w.inv_t);  // (infinite at T = inf)
+    const float span = r.x - r.y;                                                        // (or at huge logits)
+    const bool far = !(span < reach);
+    const float range = far ? reach : span;
+    // A range of 0, or of infinity, leaves one bin.
+    return {r.x, range > 0.0f ? fminf((float)(kBins - 1) / range, 0x1p100f) : 0.0f, far};
+}
+// Whether a row has a border to look for.
+__device__ __forceinline__ bool has_border(const SampleArgs &a, const Wish &w) { return w.has_p || w.top_k < a.vocab; }
+// A border is looked for in bins unless min_p reaches into the weights that are 0.
+__device__ __forceinline__ bool by_bins(const SampleArgs &a, const Wish &w) {
+    return !(w.min_p > 0.0 && w.min_p < __builtin_ldexp(1.0, 2 - a.shift));
+}
+
+__global__ __launch_bounds__(kScan) void sample_range_kernel(SampleArgs a, SampleWs ws) {
+    __shared__ float2 part[kScan / 64];
+    const int row = (int)blockIdx.y, tid = (int)threadIdx.x;
+    const int64_t base = (int64_t)row * a.stride;
+    if (blockIdx.x == 0 && tid == 0) ws.listed[row] = 0;
+    for (int c = ws.first((int)blockIdx.x); c < ws.first((int)blockIdx.x + 1); c++) {
+        float l[4][4];
+#pragma unroll
+        for (int j = 0; j < 4; j++) load4(a, base, c * kChunk + j * 1024 + 4 * tid, l[j]);
+        float2 r = {-__builtin_inff(), __builtin_inff()};
+#pragma unroll
+        for (int j = 0; j < 16; j++) {
+            const float v = l[j >> 2][j & 3];
+            r.x = fmaxf(r.x, v);
+            if (v > -__builtin_inff()) r.y = fminf(r.y, v);
+        }
+        for (int d = 1; d < 64; d <<= 1) r = {fmaxf(r.x, __shfl_xor(r.x, d)), fminf(r.y, __shfl_xor(r.y, d))};
+        __syncthreads();
+        if ((tid & 63) == 0) part[tid >> 6] = r;
+        __syncthreads();
+        if (tid == 0) {
+            for (int w = 1; w < kScan / 64; w++) r = {fmaxf(r.x, part[w].x), fminf(r.y, part[w].y)};
+            ws.range[(int64_t)row * ws.chunks + c] = r;
+        }
+    }
+}
+
+// Sums over the workgroup of kScan threads, in thread 0.
+__device__ __forceinline__ void scan_sum(u64 &mass, uint32_t &n, u64 *pm, uint32_t *pn) {
+    for (int d = 1; d < 64; d <<= 1) {
+        mass += __shfl_xor(mass, d);
+        n += __shfl_xor(n, d);
+    }
+    __syncthreads();
+    if ((threadIdx.x & 63) == 0) {
+        pm[threadIdx.x >> 6] = mass;
+        pn[threadIdx.x >> 6] = n;
+    }
+    __syncthreads();
+    mass = 0;
+    n = 0;
+    for (int w = 0; w < kScan / 64; w++) {
+        mass += pm[w];
+        n += pn[w];
+    }
+}
+
+__global__ __launch_bounds__(kScan) void sample_bins_kernel(SampleArgs a, SampleWs ws) {
+    __shared__ u64 mass[kBins];
+    __shared__ uint32_t count[kBins];
+    __shared__ u64 pm[kScan / 64];
+    __shared__ uint32_t pn[kScan / 64];
+    const int row = (int)blockIdx.y, part = (int)blockIdx.x, tid = (int)threadIdx.x;
+    const int64_t base = (int64_t)row * a.stride;
+    const Wish wish = row_wish(a, row);
+    const float2 r = row_range(ws, row);
+    if (!(r.x > -__builtin_inff())) return;  // no token
+    const Scale sc = {r.x, wish.inv_t, a.shift};
+    const Bins bins = row_bins(a, wish, r);
+    const bool border = has_border(a, wish);
+    if (border && !by_bins(a, wish)) return;
+    if (border) {
+        for (int b = tid; b < kBins; b += kScan) {
+            mass[b] = 0;
+            count[b] = 0;
+        }
+        __syncthreads();
+    }
+    for (int c = ws.first(part); c < ws.first(part + 1); c++) {
+        float l[4][4];
+#pragma unroll
+        for (int j = 0; j < 4; j++) load4(a, base, c * kChunk + j * 1024 + 4 * tid, l[j]);
+        if (border) {
+#pragma unroll
+            for (int j = 0; j < 16; j++) {
+                const float v = l[j >> 2][j & 3];
+                if (!(v > -__builtin_inff())) continue;
+                const int b = bins.of(v);
+                atomicAdd(&count[b], 1u);  // LDS
+                if (wish.has_p && !(bins.far && b == kBins - 1)) atomicAdd(&mass[b], sc.fixed(sc.weight(v)));
+            }
+        } else {
+            u64 t = 0;
+            uint32_t n = 0;
+#pragma unroll
+            for (int j = 0; j < 16; j++) {
+                const float v = l[j >> 2][j & 3];
+                if (!(v > -__builtin_inff())) continue;
+                const double w = sc.weight(v);
+                if (!(w >= wish.min_p)) continue;
+                t += sc.fixed(w);
+                n++;
+            }
+            scan_sum(t, n, pm, pn);
+            if (tid == 0) {
+                ws.chunk_mass[(int64_t)row * ws.chunks + c] = t;
+                ws.chunk_kept[(int64_t)row * ws.chunks + c] = n;
+            }
+        }
+    }
+    if (!border) return;
+    __syncthreads();
+    const int64_t at = ((int64_t)row * ws.parts + part) * kBins;
+    for (int b = tid; b < kBins; b += kScan) {
+        ws.count[at + b] = count[b];
+        if (wish.has_p) ws.mass[at + b] = mass[b];
+    }
+}
+
+__global__ __launch_bounds__(kScan) void sample_border_kernel(SampleArgs a, SampleWs ws) {
+    __shared__ u64 pm[kScan / 64], cm[kScan / 64];
+    __shared__ uint32_t pn[kScan / 64], cn[kScan / 64];
+    __shared__ int cut_k, cut_p;
+    __shared__ uint32_t before_k, in_k, before_p, in_p;
+    __shared__ u64 before_mass;
+    __shared__ uint32_t place;
+    const int row = (int)blockIdx.y, part = (int)blockIdx.x, tid = (int)threadIdx.x, lane = tid & 63, wave = tid >> 6;
+    const int64_t base = (int64_t)row * a.stride;
+    const Wish wish = row_wish(a, row);
+    const float2 r = row_range(ws, row);
+    if (!(r.x > -__builtin_inff())) return;
+    Plan plan = {kFree, kBins, 0, 0x7FFFFFFF, 0, 0.0};
+    const bool border = has_border(a, wish);
+    if (!border || !by_bins(a, wish)) {
+        if (border) plan.mode = kWhole;
+        if (part == 0 && tid == 0) ws.plan[row] = plan;
+        return;
+    }
+    const Scale sc = {r.x, wish.inv_t, a.shift};
+    const Bins bins = row_bins(a, wish, r);
+
+    // The row's histogram: bins 2 tid, 2 tid + 1, summed over the parts, and its scan.
+    uint2 n = {0, 0};
+    u64 w0 = 0, w1 = 0;
+    const int64_t at = (int64_t)row * ws.parts * kBins + 2 * tid;
+#pragma unroll 8
+    for (int p = 0; p < ws.parts; p++) {
+        const uint2 v = *reinterpret_cast<const uint2 *>(ws.count + at + p * kBins);
+        n.x += v.x;
+        n.y += v.y;
+    }
+    if (wish.has_p) {
+#pragma unroll 8
+        for (int p = 0; p < ws.parts; p++) {
+            const ulonglong2 v = *reinterpret_cast<const ulonglong2 *>(ws.mass + at + p * kBins);
+            w0 += v.x;
+            w1 += v.y;
+        }
+    }
+    uint32_t cum = n.x + n.y;  // inclusive
+    u64 cmass = w0 + w1;
+    for (int d = 1; d < 64; d <<= 1) {
+        const uint32_t o = __shfl_up(cum, d);
+        const u64 q = __shfl_up(cmass, d);
+        if (lane >= d) {
+            cum += o;
+            cmass += q;
+        }
+    }
+    if (lane == 63) {
+        cn[wave] = cum;
+        cm[wave] = cmass;
+    }
+    if (tid == 0) {
+        cut_k = cut_p = kBins;
+        in_k = in_p = before_k = before_p = 0;
+        before_mass = 0;
+    }
+    __syncthreads();
+    uint32_t all = 0;
+    u64 total = 0;
+    for (int w = 0; w < kScan / 64; w++) {
+        if (w < wave) {
+            cum += cn[w];
+            cmass += cm[w];
+        }
+        all += cn[w];
+        total += cm[w];
+    }
+    const double target = wish.top_p * (double)total;  // (of the whole row; used where top_k drops no weight)
+    const uint32_t k = (uint32_t)wish.top_k;
+    {
+        const uint32_t c[3] = {cum - n.x - n.y, cum - n.y, cum};
+        const u64 q[3] = {cmass - w0 - w1, cmass - w1, cmass};
+#pragma unroll
+        for (int j = 0; j < 2; j++) {
+            if (k < all && c[j] < k && c[j + 1] >= k) {
+                cut_k = 2 * tid + j;
+                before_k = c[j];
+                in_k = c[j + 1] - c[j];
+            }
+            if (wish.has_p && (double)q[j] < target && !((double)q[j + 1] < target)) {
+                cut_p = 2 * tid + j;
+                before_p = c[j];
+                in_p = c[j + 1] - c[j];
+                before_mass = q[j];
+            }
+        }
+    }
+    __syncthreads();
+    const bool k_cuts = cut_k < kBins && !(bins.far && cut_k == kBins - 1);  // drops weight
+    plan.tokens = k < all ? k : all;
+    int last;  // bins up to this one are collected, from `from`
+    int from;
+    if (k_cuts && before_k + in_k <= (uint32_t)kList) {
+        plan.mode = kAll;
+        from = 0;
+        last = cut_k;
+    } else if (k_cuts) {
+        plan.mode = wish.has_p || in_k > (uint32_t)kList ? kWhole : kBorder;
+        plan.bin = from = last = cut_k;
+        plan.before = before_k;
+    } else if (wish.has_p) {
+        plan.mode = in_p > (uint32_t)kList ? kWhole : kBorder;
+        plan.bin = from = last = cut_p;
+        plan.before = before_p;
+        plan.before_mass = before_mass;
+        plan.target = target;
+    } else {
+        plan.mode = kFree;
+        from = kBins;
+        last = -1;
+    }
+    if (part == 0 && tid == 0) ws.plan[row] = plan;
+    if (plan.mode == kWhole) return;
+
+    for (int c = ws.first(part); c < ws.first(part + 1); c++) {
+        float l[4][4];
+        const int i0 = c * kChunk + 4 * tid;
+#pragma unroll
+        for (int j = 0; j < 4; j++) load4(a, base, i0 + j * 1024, l[j]);
+        u64 t = 0;
+        uint32_t kept = 0, mine = 0, listed = 0;  // listed: bit j: token j is collected
+#pragma unroll
+        for (int j = 0; j < 16; j++) {
+            const float v = l[j >> 2][j & 3];
+            if (!(v > -__builtin_inff())) continue;
+            const int b = bins.of(v);
+            if (b >= from && b <= last) {
+                listed |= 1u << j;
+                mine++;
+            } else if (plan.mode != kAll && b < plan.bin) {
+                const double w = sc.weight(v);
+                if (w >= wish.min_p) {
+                    t += sc.fixed(w);
+                    kept++;
+                }
+            }
+        }
+        if (plan.mode != kAll) {
+            scan_sum(t, kept, pm, pn);
+            if (tid == 0) {
+                ws.chunk_mass[(int64_t)row * ws.chunks + c] = t;
+                ws.chunk_kept[(int64_t)row * ws.chunks + c] = kept;
+            }
+        }
+        // places in the list: this thread's after those of the threads before
+        uint32_t upto = mine;
+        for (int d = 1; d < 64; d <<= 1) {
+            const uint32_t o = __shfl_up(upto, d);
+            if (lane >= d) upto += o;
+        }
+        __syncthreads();
+        if (lane == 63) cn[wave] = upto;
+        __syncthreads();
+        uint32_t sum = 0;
+        for (int w = 0; w < kScan / 64; w++) {
+            if (w < wave) upto += cn[w];
+            sum += cn[w];
+        }
+        if (sum == 0) continue;  // (the same in every thread)
+        if (tid == 0) place = atomicAdd(ws.listed + row, sum);
+        __syncthreads();
+        uint32_t p = place + upto - mine;
+#pragma unroll
+        for (int j = 0; j < 16; j++) {
+            if ((listed >> j) & 1u) {
+                // (the histogram counted them: at most kList)
+                if (p < (uint32_t)kList)
+                    ws.list[(int64_t)row * kList + p] = ((u64)(0xFFFFFFFFu - logit_key(l[j >> 2][j & 3])) << 32) |
+                                                        (uint32_t)(i0 + (j >> 2) * 1024 + (j & 3));
+                p++;
+            }
+        }
+    }
+}
+
+// Inclusive scan of a value per thread over the workgroup; `total` its end.
+__device__ __forceinline__ u64 block_scan(u64 v, u64 &total, RowLds &s) {
+    const int lane = (int)threadIdx.x & 63, wave = (int)threadIdx.x >> 6;
+    for (int d = 1; d < 64; d <<= 1) {
+        const u64 o = __shfl_up(v, d);
+        if (lane >= d) v += o;
+    }
+    __syncthreads();
+    if (lane == 63) s.part[wave] = v;
+    __syncthreads();
+    total = 0;
+    for (int w = 0; w < kWaves; w++) {
+        if (w < wave) v += s.part[w];
+        total += s.part[w];
+    }
+    return v;
+}
+
+// Sorts the first n (up to kList) of `list`, whose values differ, upwards.
+__device__ void sort_list(u64 *list, int n) {
+    const int tid = (int)threadIdx.x;
+    if (n <= 256) {  // each value's place: the values below it, four threads a value
+        const int e = tid >> 2, q = tid & 3;
+        const u64 v = e < n ? list[e] : 0;
+        int below = 0;
+        if (e < n)
+            for (int j = q; j < n; j += 4) below += list[j] < v ? 1 : 0;
+        below += __shfl_xor(below, 1);
+        below += __shfl_xor(below, 2);
+        __syncthreads();
+        if (e < n && q == 0) list[below] = v;
+        __syncthreads();
+        return;
+    }
+    int size = 512;
+    while (size < n) size <<= 1;
+    for (int i = n + tid; i < size; i += kThreads) list[i] = ~0ull;
+    __syncthreads();
+    for (int k = 2; k <= size; k <<= 1)
+        for (int j = k >> 1; j > 0; j >>= 1) {
+            for (int t = tid; t < size / 2; t += kThreads) {
+                const int i = 2 * t - (t & (j - 1)), o = i + j;
+                const u64 x = list[i], y = list[o];
+                if ((x > y) == ((i & k) == 0)) {
+                    list[i] = y;
+                    list[o] = x;
+                }
+            }
+            __syncthreads();
+        }
+}
+
+// One workgroup per row.
+__global__ __launch_bounds__(kThreads) void sample_draw_kernel(SampleArgs a, SampleWs ws) {
+    __shared__ RowLds s;
+    __shared__ u64 list[kList];
+    __shared__ u64 chunk[1024];
+    __shared__ int which;
+    __shared__ u64 before_chunk;
+    const int row = (int)blockIdx.x, tid = (int)threadIdx.x;
+    const int64_t base = (int64_t)row * a.stride;
+    const Wish wish = row_wish(a, row);
+    const float2 range = row_range(ws, row);
+    if (!(range.x > -__builtin_inff())) {  // no token at all
+        if (tid == 0) {
+            a.tokens[row] = -1;
+            if (a.probs != nullptr) a.probs[row] = 0.0f;
+            if (a.kept != nullptr) a.kept[row] = 0;
+        }
+        return;
+    }
+    const Plan plan = ws.plan[row];
+    if (plan.mode == kWhole) {
+        whole_row(a, row, wish, range.x, s);
+        return;
+    }
+    const Scale sc = {range.x, wish.inv_t, a.shift};
+    auto write = [&](int token, double w, u64 total, uint32_t kept) {
+        a.tokens[row] = token;
+        if (a.probs != nullptr) a.probs[row] = (float)(__builtin_ldexp(w, a.shift) / (double)total);
+        if (a.kept != nullptr) a.kept[row] = (int32_t)kept;
+    };
+
+    // The collected tokens in order: upper half the inverted key, lower half the index.
+    int n = 0;
+    if (plan.mode != kFree) {
+        n = (int)ws.listed[row];
+        for (int i = tid; i < n; i += kThreads) list[i] = ws.list[(int64_t)row * kList + i];
+        __syncthreads();
+        sort_list(list, n);
+    }
+    auto logit_at = [&](int i) { return key_logit(0xFFFFFFFFu - (uint32_t)(list[i] >> 32)); };
+
+    if (plan.mode == kAll) {
+        const int k = (int)plan.tokens;  // <= n
+        constexpr int kPer = kList / kThreads;
+        u64 f[kPer], sum = 0, total;
+        double w[kPer];
+#pragma unroll
+        for (int j = 0; j < kPer; j++) {
+            const int i = kPer * tid + j;
+            w[j] = i < k ? sc.weight(logit_at(i)) : 0.0;
+            f[j] = i < k ? sc.fixed(w[j]) : 0;
+            sum += f[j];
+        }
+        u64 before = block_scan(sum, total, s) - sum;
+        const double target = wish.top_p * (double)total;
+        uint32_t keep = 0;
+#pragma unroll
+        for (int j = 0; j < kPer; j++) {
+            const int i = kPer * tid + j;
+            if (i < k && (!wish.has_p || (double)before < target) && w[j] >= wish.min_p) keep++;
+            before += f[j];
+        }
+        keep = block_sum(keep, s);  // (a prefix)
+        // The kept ones by index: upper half the index, lower half the key.
+        __syncthreads();
+        for (int i = tid; i < (int)keep; i += kThreads) {
+            const u64 v = list[i];
+            list[i] = (v << 32) | (0xFFFFFFFFu - (uint32_t)(v >> 32));
+        }
+        __syncthreads();
+        sort_list(list, (int)keep);
+        sum = 0;
+#pragma unroll
+        for (int j = 0; j < kPer; j++) {
+            const int i = kPer * tid + j;
+            w[j] = i < (int)keep ? sc.weight(key_logit((uint32_t)list[i])) : 0.0;
+            f[j] = i < (int)keep ? sc.fixed(w[j]) : 0;
+            sum += f[j];
+        }
+        u64 cum = block_scan(sum, total, s) - sum;
+        const double point = wish.u * (double)total;
+#pragma unroll
+        for (int j = 0; j < kPer; j++) {
+            if (f[j] > 0 && !((double)cum > point) && (double)(cum + f[j]) > point)  // one thread, once
+                write((int)(list[kPer * tid + j] >> 32), w[j], total, keep);
+            cum += f[j];
+        }
+        return;
+    }
+
+    // By chunks: their mass above the border's bin, and the border's own tokens.
+    Border border = {0, 0x7FFFFFFF};
+    uint32_t kept = 0;
+    if (tid < ws.chunks) {
+        chunk[tid] = ws.chunk_mass[(int64_t)row * ws.chunks + tid];
+        kept = ws.chunk_kept[(int64_t)row * ws.chunks + tid];
+    }
+    __syncthreads();
+    if (plan.mode == kBorder) {
+        constexpr int kPer = kList / kThreads;
+        u64 f[kPer], sum = 0, total;
+        double w[kPer];
+#pragma unroll
+        for (int j = 0; j < kPer; j++) {
+            const int i = kPer * tid + j;
+            w[j] = i < n ? sc.weight(logit_at(i)) : 0.0;
+            f[j] = i < n ? sc.fixed(w[j]) : 0;
+            sum += f[j];
+        }
+        u64 before = plan.before_mass + block_scan(sum, total, s) - sum;
+        const bool by_mass = plan.target > 0.0;
+        uint32_t in = 0;
+#pragma unroll
+        for (int j = 0; j < kPer; j++) {
+            const int i = kPer * tid + j;
+            if (i < n && (by_mass ? (double)before < plan.target : plan.before + (uint32_t)i < plan.tokens)) {
+                in++;
+                if (w[j] >= wish.min_p) {
+                    kept++;
+                    if (f[j] > 0) atomicAdd(&chunk[(uint32_t)list[i] / kChunk], f[j]);  // LDS
+                }
+            }
+            before += f[j];
+        }
+        in = block_sum(in, s);
+        border = {0xFFFFFFFFu - (uint32_t)(list[in - 1] >> 32), (int)(uint32_t)list[in - 1]};
+    }
+    kept = block_sum(kept, s);
+    if (plan.mode == kFree && wish.min_p == 0.0 && plan.tokens < kept) kept = plan.tokens;  // top_k drops weights of 0
+    const u64 mine = tid < ws.chunks ? chunk[tid] : 0;
+    u64 total;
+    const u64 upto = block_scan(mine, total, s);
+    const double point = wish.u * (double)total;
+    if (mine > 0 && !((double)(upto - mine) > point) && (double)upto > point) {  // one thread
+        which = tid;
+        before_chunk = upto - mine;
+    }
+    __syncthreads();
+    const int i0 = which * kChunk + 4 * tid;
+    float l[4];
+    load4(a, base, i0, l);
+    double w[4];
+    u64 f[4], sum = 0;
+#pragma unroll
+    for (int j = 0; j < 4; j++) {
+        const uint32_t k = logit_key(l[j]);
+        f[j] = 0;
+        w[j] = 0.0;
+        if (k != 0 && border.keeps(k, i0 + j)) {
+            w[j] = sc.weight(l[j]);
+            if (w[j] >= wish.min_p) f[j] = sc.fixed(w[j]);
+        }
+        sum += f[j];
+    }
+    u64 in_chunk;
+    u64 cum = before_chunk + block_scan(sum, in_chunk, s) - sum;
+#pragma unroll
+    for (int j = 0; j < 4; j++) {
+        if (f[j] > 0 && !((double)cum > point) && (double)(cum + f[j]) > point) write(i0 + j, w[j], total, kept);
+        cum += f[j];
+    }
+}
+
+// Workgroups a row is dealt to: all rows' together about two a CU.
+int row_parts(int rows, int chunks) {
+    const int want = (2 * device_cus() + rows - 1) / rows;
+    return want < chunks ? want : chunks;
+}
+
+struct SampleLayout {
+    size_t range, mass, chunk_mass, list, plan, count, chunk_kept, listed, total;
+    int chunks, parts;
+};
+SampleLayout sample_layout(int rows, int vocab) {
+    SampleLayout o = {};
+    o.chunks = (vocab + kChunk - 1) / kChunk;
+    o.parts = row_parts(rows > 0 ? rows : 1, o.chunks);
+    auto take = [&](size_t bytes) {
+        const size_t at = o.total;
+        o.total += (bytes + 255) / 256 * 256;
+        return at;
+    };
+    const size_t r = (size_t)rows, rc = r * o.chunks, rb = r * o.parts * kBins;
+    o.range = take(rc * sizeof(float2));
+    o.mass = take(rb * sizeof(u64));
+    o.chunk_mass = take(rc * sizeof(u64));
+    o.list = take(r * kList * sizeof(u64));
+    o.plan = take(r * sizeof(Plan));
+    o.count = take(rb * sizeof(uint32_t));
+    o.chunk_kept = take(rc * sizeof(uint32_t));
+    o.listed = take(r * sizeof(uint32_t));
+    return o;
+}
+
 }  // namespace
 
-size_t sample_workspace_bytes(int rows, int vocab) {
-    (void)rows;
-    (void)vocab;
-    return 0;
-}
+size_t sample_workspace_bytes(int rows, int vocab) { return sample_layout(rows, vocab).total; }
 
 hipError_t launch_sample(const void *logits, int logits_type, int rows, int vocab, int64_t stride,
                          const float *temperature, const int32_t *top_k, const float *top_p, const float *min_p,
                          const float *u, int32_t *tokens, float *probs, int32_t *kept, uint8_t *workspace,
                          hipStream_t stream) {
-    (void)workspace;
     if (rows <= 0) return hipSuccess;
     int bits = 1;
     while ((1ll << bits) <= vocab) bits++;
-    const SampleArgs a = {logits, stride, logits_type, vocab,  62 - bits, temperature,
-                          top_p,  min_p,  u,           top_k,  tokens,    kept,        probs};
-    hipLaunchKernelGGL(sample_row_kernel, dim3((unsigned)rows), dim3(kThreads), 0, stream, a);
+    const uintptr_t size = logits_type == kF32 ? 4 : 2;
+    const bool vec4 = ((reinterpret_cast<uintptr_t>(logits) | (uintptr_t)stride * size) & (4 * size - 1)) == 0;
+    const SampleArgs a = {logits, stride, logits_type, vocab,  62 - bits, vec4, temperature,
+                          top_p,  min_p,  u,           top_k,  tokens,    kept, probs};
+    const SampleLayout o = sample_layout(rows, vocab);
+    const SampleWs ws = {reinterpret_cast<float2 *>(workspace + o.range),
+                         reinterpret_cast<u64 *>(workspace + o.mass),
+                         reinterpret_cast<u64 *>(workspace + o.chunk_mass),
+                         reinterpret_cast<u64 *>(workspace + o.list),
+                         reinterpret_cast<Plan *>(workspace + o.plan),
+                         reinterpret_cast<uint32_t *>(workspace + o.count),
+                         reinterpret_cast<uint32_t *>(workspace + o.chunk_kept),
+                         reinterpret_cast<uint32_t *>(workspace + o.listed),
+                         o.chunks,
+                         o.parts};
+    const dim3 grid((unsigned)o.parts, (unsigned)rows);
+    hipLaunchKernelGGL(sample_range_kernel, grid, dim3(kScan), 0, stream, a, ws);
+    hipLaunchKernelGGL(sample_bins_kernel, grid, dim3(kScan), 0, stream, a, ws);
+    hipLaunchKernelGGL(sample_border_kernel, grid, dim3(kScan), 0, stream, a, ws);
+    hipLaunchKernelGGL(sample_draw_kernel, dim3((unsigned)rows), dim3(kThreads), 0, stream, a, ws);
     return hipGetLastError();
 }
 

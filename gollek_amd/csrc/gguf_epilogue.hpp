@@ -29,7 +29,7 @@ struct Epilogue {
     const void *residual;  // or nullptr
     int64_t y_stride, mul_stride, residual_stride;  // elements between rows
     int act, type;
-    bool vec4;  // every matrix's rows allow loads and stores of four elements
+    bool vec;  // every matrix's rows start on 16-byte boundaries
 };
 
 inline Epilogue make_epilogue(void *y, const float *bias, const void *mul, const void *residual, int64_t y_stride,
@@ -39,7 +39,7 @@ inline Epilogue make_epilogue(void *y, const float *bias, const void *mul, const
     if (mul != nullptr) low |= reinterpret_cast<uintptr_t>(mul) | (uintptr_t)mul_stride * size;
     if (residual != nullptr) low |= reinterpret_cast<uintptr_t>(residual) | (uintptr_t)residual_stride * size;
     return {y,        bias, mul,  residual, y_stride, mul_stride, residual_stride,
-            act,      type, (low & (4 * size - 1)) == 0};
+            act,      type, (low & 15u) == 0};
 }
 
 // v / (1 + exp(-s v)) at s v: exp overflows to infinity past 88, which leaves -0.
@@ -77,10 +77,139 @@ __device__ __forceinline__ void put(const Epilogue &e, int64_t m, int64_t n, int
     store_element(e.y, e.type, m * e.y_stride + n, v);
 }
 
-// Elements (m, n .. n + 3), those past column N - 1 left out.
-__device__ __forceinline__ void put4(const Epilogue &e, int64_t m, int64_t n, int64_t N, float4 v) {
-    const float a[4] = {v.x, v.y, v.z, v.w};
-    for (int i = 0; i < 4 && n + i < N; i++) put(e, m, n + i, N, a[i]);
+// 16 bytes of elements: 4 floats, 8 halves.
+template <int TYPE>
+struct Elements {
+    static constexpr int kSize = TYPE == kF32 ? 4 : 2, kCount = 16 / kSize;
+    typedef uint32_t v4 __attribute__((ext_vector_type(4)));
+    v4 bits;
+    __device__ __forceinline__ void load(const void *p, int64_t i) {
+        bits = *reinterpret_cast<const v4 *>(static_cast<const uint8_t *>(p) + i * kSize);
+    }
+    __device__ __forceinline__ void store(void *p, int64_t i) const {
+        *reinterpret_cast<v4 *>(static_cast<uint8_t *>(p) + i * kSize) = bits;
+    }
+    __device__ __forceinline__ float get(int j) const {
+        if constexpr (TYPE == kF32) return __uint_as_float(bits[j]);
+        const uint32_t w = bits[j >> 1];
+        if constexpr (TYPE == kBF16) return __uint_as_float((j & 1) ? w & 0xFFFF0000u : w << 16);
+        return (float)__builtin_bit_cast(_Float16, (uint16_t)((j & 1) ? w >> 16 : w & 0xFFFFu));
+    }
+    __device__ __forceinline__ void set(const float *v) {
+#pragma unroll
+        for (int j = 0; j < 4; j++) {
+            if constexpr (TYPE == kF32) {
+                bits[j] = __float_as_uint(v[j]);
+            } else if constexpr (TYPE == kBF16) {
+                typedef __bf16 b2 __attribute__((ext_vector_type(2)));
+                bits[j] = __builtin_bit_cast(uint32_t, b2{(__bf16)v[2 * j], (__bf16)v[2 * j + 1]});
+            } else {
+                typedef _Float16 h2 __attribute__((ext_vector_type(2)));
+                bits[j] = __builtin_bit_cast(uint32_t, h2{(_Float16)v[2 * j], (_Float16)v[2 * j + 1]});
+            }
+        }
+    }
+};
+
+// The activations of n values (one uniform branch for all of them).
+template <int C>
+__device__ __forceinline__ void activate_all(int act, float (&v)[C]) {
+    switch (act) {
+#define GOLLEK_ACT(A)                                        \
+    case A:                                                  \
+        _Pragma("unroll") for (int j = 0; j < C; j++) v[j] = activate(A, v[j]); \
+        break
+        GOLLEK_ACT(kActRelu);
+        GOLLEK_ACT(kActSilu);
+        GOLLEK_ACT(kActGelu);
+        GOLLEK_ACT(kActGeluTanh);
+#undef GOLLEK_ACT
+    default: break;
+    }
+}
+
+// A ROWS x COLS tile of fp32 sums, row-major in LDS with rows kTilePitch<COLS>
+// floats apart, through the epilogue: a thread takes 16 bytes of a row at a
+// time, kBatch of them together, whose mul and residual are loaded before the
+// first is used (and the first batch's before fill(), which writes the tile).
+// Element by element instead, straight from the accumulators, every load waited
+// behind the store before it: Q4_K M = 2048, 14336 x 4096 with SiLU and mul 483
+// against TILE_US us.
+// Every thread of the workgroup calls this; fill() may hold barriers.
+template <int COLS>
+constexpr int kTilePitch = COLS + 4;
+
+template <int ROWS, int COLS, int THREADS, int TYPE, class FILL>
+__device__ __forceinline__ void put_tile_as(const Epilogue &e, const float *tile, int m0, int n0, int M, int N, int tid,
+                                            FILL &&fill) {
+    using V = Elements<TYPE>;
+    constexpr int C = V::kCount, kAcross = COLS / C, kStep = THREADS / kAcross;  // vectors of a row, rows of a round
+    static_assert(THREADS % kAcross == 0, "whole rows a round");
+    constexpr int kRounds = (ROWS + kStep - 1) / kStep, kBatch = kRounds < 4 ? kRounds : 4;
+    const int col = C * (tid % kAcross), row = tid / kAcross, n = n0 + col;
+    const bool whole = e.vec && n + C <= N;
+    float bias[C];
+    if (whole && e.bias != nullptr) {
+#pragma unroll
+        for (int j = 0; j < C; j++) bias[j] = e.bias[n + j];
+    }
+    V mul[kBatch], residual[kBatch];
+    auto fetch = [&](int i0) {
+#pragma unroll
+        for (int i = 0; i < kBatch; i++) {
+            const int r = row + (i0 + i) * kStep;
+            const bool in = whole && r < ROWS && m0 + r < M;
+            if (in && e.mul != nullptr) mul[i].load(e.mul, (int64_t)(m0 + r) * e.mul_stride + n);
+            if (in && e.residual != nullptr) residual[i].load(e.residual, (int64_t)(m0 + r) * e.residual_stride + n);
+        }
+    };
+    fetch(0);
+    fill();
+    __syncthreads();
+#pragma unroll
+    for (int i0 = 0; i0 < kRounds; i0 += kBatch) {
+        if (i0 > 0) fetch(i0);
+#pragma unroll
+        for (int i = 0; i < kBatch; i++) {
+            const int r = row + (i0 + i) * kStep;
+            if (r >= ROWS || m0 + r >= M) continue;
+            const float *const from = tile + r * kTilePitch<COLS> + col;
+            float v[C];
+#pragma unroll
+            for (int j = 0; j < C; j += 4) {
+                const float4 f = *reinterpret_cast<const float4 *>(from + j);
+                v[j] = f.x, v[j + 1] = f.y, v[j + 2] = f.z, v[j + 3] = f.w;
+            }
+            if (whole) {
+                if (e.bias != nullptr) {
+#pragma unroll
+                    for (int j = 0; j < C; j++) v[j] += bias[j];
+                }
+                activate_all(e.act, v);
+                if (e.mul != nullptr) {
+#pragma unroll
+                    for (int j = 0; j < C; j++) v[j] *= mul[i].get(j);
+                }
+                if (e.residual != nullptr) {
+#pragma unroll
+                    for (int j = 0; j < C; j++) v[j] += residual[i].get(j);
+                }
+                V out;
+                out.set(v);
+                out.store(e.y, (int64_t)(m0 + r) * e.y_stride + n);
+            } else {
+                for (int j = 0; j < C && n + j < N; j++) put(e, m0 + r, n + j, N, from[j]);
+            }
+        }
+    }
+}
+
+template <int ROWS, int COLS, int THREADS, class FILL>
+__device__ __forceinline__ void put_tile(const Epilogue &e, const float *tile, int m0, int n0, int M, int N, int tid,
+                                         FILL &&fill) {
+    if (e.type == kF32) put_tile_as<ROWS, COLS, THREADS, kF32>(e, tile, m0, n0, M, N, tid, fill);
+    else if (e.type == kF16) put_tile_as<ROWS, COLS, THREADS, kF16>(e, tile, m0, n0, M, N, tid, fill);
+    else put_tile_as<ROWS, COLS, THREADS, kBF16>(e, tile, m0, n0, M, N, tid, fill);
 }
 
 // Where split `split` of a product with `mn` outputs leaves its sums: a plain

@@ -445,33 +445,32 @@ __global__ __launch_bounds__(kThreads) void gemm_tile_kernel(const uint8_t *__re
     }
     __syncthreads();
     float *const stage = reinterpret_cast<float *>(ring);
-    if (wave < 8 && kg == 0) {
-        // D layout of a 16 x 16 tile: lane holds column lane & 15, rows 4 (lane >> 4) + r.
+    auto fill = [&] {
+        if (wave < 8 && kg == 0) {
+            // D layout of a 16 x 16 tile: lane holds column lane & 15, rows 4 (lane >> 4) + r.
 #pragma unroll
-        for (int mt = 0; mt < MT; mt++)
+            for (int mt = 0; mt < MT; mt++)
 #pragma unroll
-            for (int nt = 0; nt < 2; nt++)
+                for (int nt = 0; nt < 2; nt++)
 #pragma unroll
-                for (int r = 0; r < 4; r++)
-                    stage[(16 * mt + 4 * lk + r) * kStagePitch + 32 * nq + 16 * nt + lr] = acc[mt][nt][r];
+                    for (int r = 0; r < 4; r++)
+                        stage[(16 * mt + 4 * lk + r) * kStagePitch + 32 * nq + 16 * nt + lr] = acc[mt][nt][r];
+        }
+    };
+    if constexpr (kHasEpilogue<OUT>) {
+        if (S == 1) {
+            static_assert(kStagePitch == kTilePitch<kTileN>, "put_tile's layout");
+            if (wave < 8) put_tile<kTileM, kTileN, kCompute>(Y, stage, m0, n0, M, N, tid, fill);
+            else __syncthreads();  // put_tile's
+            return;
+        }
     }
+    fill();
     __syncthreads();
     // A plain Y: split 0 writes it, split k > 0 workspace partial k - 1 for the
     // reduction kernel.  An epilogue: with splits all of them are partials.
     const int col = 4 * (tid & 31);
     if (tid >= kCompute) return;
-    if constexpr (kHasEpilogue<OUT>) {
-        if (S == 1) {
-#pragma unroll
-            for (int pass = 0; pass < kTileM * 32 / kCompute; pass++) {
-                const int row = 16 * pass + (tid >> 5);
-                const int m = m0 + row, n = n0 + col;
-                if (m >= M || n >= N) continue;
-                put4(Y, m, n, N, *reinterpret_cast<const float4 *>(stage + row * kStagePitch + col));
-            }
-            return;
-        }
-    }
     float *const out = split_output(Y, part, split, (int64_t)M * N);
 #pragma unroll
     for (int pass = 0; pass < kTileM * 32 / kCompute; pass++) {
@@ -513,7 +512,8 @@ __global__ __launch_bounds__(256) void linear_reduce_kernel(const float *__restr
                 a.w += b[k].w;
             }
         }
-        put4(y, m, n, N, a);
+        const float v[4] = {a.x, a.y, a.z, a.w};
+        for (int i = 0; i < 4; i++) put(y, m, n + i, N, v[i]);
     } else {
         for (int i = 0; i < 4 && n + i < N; i++) {
             float a = p[i];

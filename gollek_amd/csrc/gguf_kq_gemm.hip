@@ -224,29 +224,36 @@ __global__ __launch_bounds__(64 * NW *KW, MT == 1 && NW == 2 ? 4 : 1) void gemm_
                 for (int nt = 0; nt < 2; nt++) red[((wave * MT + mt) * 2 + nt) * 64 + lane] = acc[mt][nt];
         }
         __syncthreads();
-        if (kw > 0) return;
+        if (!kHasEpilogue<OUT> && kw > 0) return;
+        if (!kHasEpilogue<OUT> || kw == 0) {
 #pragma unroll
-        for (int k = 1; k < KW; k++)
+            for (int k = 1; k < KW; k++)
 #pragma unroll
-            for (int mt = 0; mt < MT; mt++)
+                for (int mt = 0; mt < MT; mt++)
 #pragma unroll
-                for (int nt = 0; nt < 2; nt++) acc[mt][nt] += red[(((k * NW + nw) * MT + mt) * 2 + nt) * 64 + lane];
+                    for (int nt = 0; nt < 2; nt++) acc[mt][nt] += red[(((k * NW + nw) * MT + mt) * 2 + nt) * 64 + lane];
+        }
     }
     if constexpr (kHasEpilogue<OUT>) {
         if (S == 1) {
+            // the tile through LDS, over the stages' x
+            constexpr int kPitch = kTilePitch<kTileN>;
+            static_assert(sizeof(lds) >= sizeof(float) * kTileM * kPitch, "the tile's LDS");
+            float *const tile = reinterpret_cast<float *>(lds[0]);
+            put_tile<kTileM, kTileN, 64 * kWaves>(Y, tile, m0, n0, M, N, (int)threadIdx.x, [&] {
+                __syncthreads();  // the last stage's reads and the sums' are done
+                if (kw > 0) return;
 #pragma unroll
-            for (int mt = 0; mt < MT; mt++)
+                for (int mt = 0; mt < MT; mt++)
 #pragma unroll
-                for (int r = 0; r < 4; r++) {
-                    const int m = m0 + 16 * mt + 4 * g + r;
+                    for (int nt = 0; nt < 2; nt++)
 #pragma unroll
-                    for (int nt = 0; nt < 2; nt++) {
-                        const int c = col0 + 16 * nt + n;
-                        if (m < M && c < N) put(Y, m, c, N, acc[mt][nt][r]);
-                    }
-                }
+                        for (int r = 0; r < 4; r++)
+                            tile[(16 * mt + 4 * g + r) * kPitch + 32 * nw + 16 * nt + n] = acc[mt][nt][r];
+            });
             return;
         }
+        if (kw > 0) return;
     }
     float *const out = split_output(Y, part, split, (int64_t)M * N);
 #pragma unroll

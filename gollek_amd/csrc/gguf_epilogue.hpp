@@ -42,16 +42,27 @@ inline Epilogue make_epilogue(void *y, const float *bias, const void *mul, const
             act,      type, (low & 15u) == 0};
 }
 
-// v / (1 + exp(-s v)) at s v: exp overflows to infinity past 88, which leaves -0.
-__device__ __forceinline__ float gated(float v, float s) { return v / (1.0f + expf(-s)); }
+// v / (1 + exp(-s)); past 88 exp(-s) overflows to infinity, which leaves -0.
+// FAST, for results that are rounded to 16 bits: exp as 2^(s log2 e) by the
+// hardware's instruction, whose argument's rounding makes it 2^-24 |s| off,
+// and a reciprocal good to 2^-23: a tenth of fp16's half step up to |s| = 400
+// (beyond it the result is below fp16's range).  A quarter of the exact form's
+// instructions, which cost a 96 x 256 tile 4 us.
+template <bool FAST>
+__device__ __forceinline__ float gated(float v, float s) {
+    if constexpr (FAST)
+        return v * __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(-1.4426950408889634f * s));
+    return v / (1.0f + expf(-s));
+}
 
+template <bool FAST>
 __device__ __forceinline__ float activate(int act, float v) {
     switch (act) {
     case kActRelu: return v < 0.0f ? 0.0f : v;  // (NaN stays)
-    case kActSilu: return gated(v, v);
+    case kActSilu: return gated<FAST>(v, v);
     case kActGelu: return 0.5f * v * (1.0f + erff(v * 0.70710678118654752f));
     // 0.5 (1 + tanh(z)) is 1 / (1 + exp(-2 z))
-    case kActGeluTanh: return gated(v, 1.5957691216057308f * (v + 0.044715f * v * v * v));
+    case kActGeluTanh: return gated<FAST>(v, 1.5957691216057308f * (v + 0.044715f * v * v * v));
     default: return v;
     }
 }
@@ -71,9 +82,32 @@ __device__ __forceinline__ void store_element(void *p, int type, int64_t i, floa
 __device__ __forceinline__ void put(float *y, int64_t m, int64_t n, int64_t N, float v) { y[m * N + n] = v; }
 __device__ __forceinline__ void put(const Epilogue &e, int64_t m, int64_t n, int64_t, float v) {
     if (e.bias != nullptr) v += e.bias[n];
-    v = activate(e.act, v);
+    v = e.type == kF32 ? activate<false>(e.act, v) : activate<true>(e.act, v);
     if (e.mul != nullptr) v *= load_element(e.mul, e.type, m * e.mul_stride + n);
     if (e.residual != nullptr) v += load_element(e.residual, e.type, m * e.residual_stride + n);
+    store_element(e.y, e.type, m * e.y_stride + n, v);
+}
+
+// The same in two steps: what an element needs beside its sum, loaded while the
+// product still runs (a load behind it costs the small products 1 us), and the rest.
+struct Ahead {
+    float bias, mul, residual;
+};
+struct NoAhead {};
+__device__ __forceinline__ NoAhead load_ahead(float *, bool, int64_t, int64_t) { return {}; }
+__device__ __forceinline__ Ahead load_ahead(const Epilogue &e, bool in, int64_t m, int64_t n) {
+    Ahead a = {0.0f, 1.0f, 0.0f};
+    if (in && e.bias != nullptr) a.bias = e.bias[n];
+    if (in && e.mul != nullptr) a.mul = load_element(e.mul, e.type, m * e.mul_stride + n);
+    if (in && e.residual != nullptr) a.residual = load_element(e.residual, e.type, m * e.residual_stride + n);
+    return a;
+}
+__device__ __forceinline__ void put(float *y, int64_t m, int64_t n, int64_t N, float v, NoAhead) { y[m * N + n] = v; }
+__device__ __forceinline__ void put(const Epilogue &e, int64_t m, int64_t n, int64_t, float v, const Ahead &a) {
+    if (e.bias != nullptr) v += a.bias;
+    v = e.type == kF32 ? activate<false>(e.act, v) : activate<true>(e.act, v);
+    if (e.mul != nullptr) v *= a.mul;
+    if (e.residual != nullptr) v += a.residual;
     store_element(e.y, e.type, m * e.y_stride + n, v);
 }
 
@@ -111,13 +145,13 @@ struct Elements {
     }
 };
 
-// The activations of n values (one uniform branch for all of them).
-template <int C>
+// The activations of C values (one uniform branch for all of them).
+template <bool FAST, int C>
 __device__ __forceinline__ void activate_all(int act, float (&v)[C]) {
     switch (act) {
-#define GOLLEK_ACT(A)                                        \
-    case A:                                                  \
-        _Pragma("unroll") for (int j = 0; j < C; j++) v[j] = activate(A, v[j]); \
+#define GOLLEK_ACT(A)                                                                 \
+    case A:                                                                           \
+        _Pragma("unroll") for (int j = 0; j < C; j++) v[j] = activate<FAST>(A, v[j]); \
         break
         GOLLEK_ACT(kActRelu);
         GOLLEK_ACT(kActSilu);
@@ -129,49 +163,82 @@ __device__ __forceinline__ void activate_all(int act, float (&v)[C]) {
 }
 
 // A ROWS x COLS tile of fp32 sums, row-major in LDS with rows kTilePitch<COLS>
-// floats apart, through the epilogue: a thread takes 16 bytes of a row at a
-// time, kBatch of them together, whose mul and residual are loaded before the
-// first is used (and the first batch's before fill(), which writes the tile).
-// Element by element instead, straight from the accumulators, every load waited
-// behind the store before it: Q4_K M = 2048, 14336 x 4096 with SiLU and mul 483
-// against TILE_US us.
-// Every thread of the workgroup calls this; fill() may hold barriers.
+// floats apart, through the epilogue.  A thread takes 16 bytes of a row at a
+// time, in rounds of THREADS of them; the mul and residual of up to four rounds
+// (a batch) are loaded together, a batch before it is used: the first by
+// tile_ahead, which may stand anywhere before, the next while one is computed.
+// (Element by element, straight from the accumulators, every load waited behind
+// the store before it: Q4_K M = 2048, 14336 x 4096 with SiLU and mul 464 against
+// 378 us.)
 template <int COLS>
 constexpr int kTilePitch = COLS + 4;
 
-template <int ROWS, int COLS, int THREADS, int TYPE, class FILL>
-__device__ __forceinline__ void put_tile_as(const Epilogue &e, const float *tile, int m0, int n0, int M, int N, int tid,
-                                            FILL &&fill) {
-    using V = Elements<TYPE>;
-    constexpr int C = V::kCount, kAcross = COLS / C, kStep = THREADS / kAcross;  // vectors of a row, rows of a round
+template <int ROWS, int COLS, int THREADS, int TYPE>
+struct TileRounds {
+    static constexpr int kCount = Elements<TYPE>::kCount, kAcross = COLS / kCount;  // vectors of a row
+    static constexpr int kStep = THREADS / kAcross;                                 // rows of a round
+    static constexpr int kRounds = (ROWS + kStep - 1) / kStep;
+    static constexpr int kBatch = kRounds < 4 ? kRounds : 4;
     static_assert(THREADS % kAcross == 0, "whole rows a round");
-    constexpr int kRounds = (ROWS + kStep - 1) / kStep, kBatch = kRounds < 4 ? kRounds : 4;
-    const int col = C * (tid % kAcross), row = tid / kAcross, n = n0 + col;
+};
+
+template <int ROWS, int COLS, int THREADS>
+struct TileAhead {
+    static constexpr int kBatch = TileRounds<ROWS, COLS, THREADS, kF32>::kBatch;  // (F32 has the most rounds)
+    Elements<kF32> mul[kBatch], residual[kBatch];
+};
+
+// Rounds i0 .. i0 + kBatch - 1 of a thread.
+template <int ROWS, int COLS, int THREADS, int TYPE, class V, int B>
+__device__ __forceinline__ void tile_fetch(const Epilogue &e, int m0, int n0, int M, int N, int tid, int i0, V (&mul)[B],
+                                           V (&residual)[B]) {
+    using R = TileRounds<ROWS, COLS, THREADS, TYPE>;
+    constexpr int size = Elements<TYPE>::kSize;
+    const int n = n0 + R::kCount * (tid % R::kAcross), row = tid / R::kAcross;
+#pragma unroll
+    for (int i = 0; i < R::kBatch; i++) {
+        const int r = row + (i0 + i) * R::kStep;
+        if (r >= ROWS || m0 + r >= M || !e.vec || n + R::kCount > N) continue;
+        if (e.mul != nullptr) mul[i].load(e.mul, ((int64_t)(m0 + r) * e.mul_stride + n) * size / V::kSize);
+        if (e.residual != nullptr)
+            residual[i].load(e.residual, ((int64_t)(m0 + r) * e.residual_stride + n) * size / V::kSize);
+    }
+}
+
+template <int ROWS, int COLS, int THREADS>
+__device__ __forceinline__ void tile_ahead(const Epilogue &e, int m0, int n0, int M, int N, int tid,
+                                           TileAhead<ROWS, COLS, THREADS> &a) {
+    if (e.type == kF32) tile_fetch<ROWS, COLS, THREADS, kF32>(e, m0, n0, M, N, tid, 0, a.mul, a.residual);
+    else tile_fetch<ROWS, COLS, THREADS, kF16>(e, m0, n0, M, N, tid, 0, a.mul, a.residual);  // (as BF16)
+}
+
+template <int ROWS, int COLS, int THREADS, int TYPE>
+__device__ __forceinline__ void put_tile_as(const Epilogue &e, const float *tile, int m0, int n0, int M, int N, int tid,
+                                            const TileAhead<ROWS, COLS, THREADS> &first) {
+    using V = Elements<TYPE>;
+    using R = TileRounds<ROWS, COLS, THREADS, TYPE>;
+    constexpr int C = R::kCount, B = R::kBatch;
+    const int col = C * (tid % R::kAcross), row = tid / R::kAcross, n = n0 + col;
     const bool whole = e.vec && n + C <= N;
     float bias[C];
     if (whole && e.bias != nullptr) {
 #pragma unroll
         for (int j = 0; j < C; j++) bias[j] = e.bias[n + j];
     }
-    V mul[kBatch], residual[kBatch];
-    auto fetch = [&](int i0) {
+    V mul[2][B], residual[2][B];
 #pragma unroll
-        for (int i = 0; i < kBatch; i++) {
-            const int r = row + (i0 + i) * kStep;
-            const bool in = whole && r < ROWS && m0 + r < M;
-            if (in && e.mul != nullptr) mul[i].load(e.mul, (int64_t)(m0 + r) * e.mul_stride + n);
-            if (in && e.residual != nullptr) residual[i].load(e.residual, (int64_t)(m0 + r) * e.residual_stride + n);
-        }
-    };
-    fetch(0);
-    fill();
-    __syncthreads();
+    for (int i = 0; i < B; i++) {
+        mul[0][i].bits = first.mul[i].bits;
+        residual[0][i].bits = first.residual[i].bits;
+    }
 #pragma unroll
-    for (int i0 = 0; i0 < kRounds; i0 += kBatch) {
-        if (i0 > 0) fetch(i0);
+    for (int b = 0; b * B < R::kRounds; b++) {
+        if ((b + 1) * B < R::kRounds)
+            tile_fetch<ROWS, COLS, THREADS, TYPE>(e, m0, n0, M, N, tid, (b + 1) * B, mul[(b + 1) & 1],
+                                                  residual[(b + 1) & 1]);
 #pragma unroll
-        for (int i = 0; i < kBatch; i++) {
-            const int r = row + (i0 + i) * kStep;
+        for (int i = 0; i < B; i++) {
+            const int r = row + (b * B + i) * R::kStep;
             if (r >= ROWS || m0 + r >= M) continue;
             const float *const from = tile + r * kTilePitch<COLS> + col;
             float v[C];
@@ -185,14 +252,14 @@ __device__ __forceinline__ void put_tile_as(const Epilogue &e, const float *tile
 #pragma unroll
                     for (int j = 0; j < C; j++) v[j] += bias[j];
                 }
-                activate_all(e.act, v);
+                activate_all<TYPE != kF32>(e.act, v);
                 if (e.mul != nullptr) {
 #pragma unroll
-                    for (int j = 0; j < C; j++) v[j] *= mul[i].get(j);
+                    for (int j = 0; j < C; j++) v[j] *= mul[b & 1][i].get(j);
                 }
                 if (e.residual != nullptr) {
 #pragma unroll
-                    for (int j = 0; j < C; j++) v[j] += residual[i].get(j);
+                    for (int j = 0; j < C; j++) v[j] += residual[b & 1][i].get(j);
                 }
                 V out;
                 out.set(v);
@@ -204,12 +271,13 @@ __device__ __forceinline__ void put_tile_as(const Epilogue &e, const float *tile
     }
 }
 
-template <int ROWS, int COLS, int THREADS, class FILL>
+// The tile stands in LDS (a barrier after its writes); `first` from tile_ahead.
+template <int ROWS, int COLS, int THREADS>
 __device__ __forceinline__ void put_tile(const Epilogue &e, const float *tile, int m0, int n0, int M, int N, int tid,
-                                         FILL &&fill) {
-    if (e.type == kF32) put_tile_as<ROWS, COLS, THREADS, kF32>(e, tile, m0, n0, M, N, tid, fill);
-    else if (e.type == kF16) put_tile_as<ROWS, COLS, THREADS, kF16>(e, tile, m0, n0, M, N, tid, fill);
-    else put_tile_as<ROWS, COLS, THREADS, kBF16>(e, tile, m0, n0, M, N, tid, fill);
+                                         const TileAhead<ROWS, COLS, THREADS> &first) {
+    if (e.type == kF32) put_tile_as<ROWS, COLS, THREADS, kF32>(e, tile, m0, n0, M, N, tid, first);
+    else if (e.type == kF16) put_tile_as<ROWS, COLS, THREADS, kF16>(e, tile, m0, n0, M, N, tid, first);
+    else put_tile_as<ROWS, COLS, THREADS, kBF16>(e, tile, m0, n0, M, N, tid, first);
 }
 
 // Where split `split` of a product with `mn` outputs leaves its sums: a plain

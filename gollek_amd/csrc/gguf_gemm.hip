@@ -199,6 +199,16 @@ __global__ __launch_bounds__(256) void gemm_q8_0_bf16_skinny_kernel(const uint8_
     const uint32_t wrs = (uint32_t)(G::kWQ + 64 * lr);
     const uint32_t ring_base = (uint32_t)(uintptr_t)(lds_ptr)ring;
 
+    // an epilogue's operands of the outputs that wave 0 stores
+    decltype(load_ahead(Y, false, 0, 0)) ahead[TT][4];
+#pragma unroll
+    for (int t = 0; t < TT; t++)
+#pragma unroll
+        for (int r = 0; r < 4; r++) {
+            const int m = 16 * t + 4 * kq + r;
+            ahead[t][r] = load_ahead(Y, wave == 0 && m < M, m, n0 + lr);
+        }
+
     f32x4 acc[TT];
 #pragma unroll
     for (int t = 0; t < TT; t++) acc[t] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
@@ -254,7 +264,7 @@ __global__ __launch_bounds__(256) void gemm_q8_0_bf16_skinny_kernel(const uint8_
 #pragma unroll
         for (int r = 0; r < 4; r++) {
             const int m = 16 * t + 4 * kq + r;
-            if (m < M) put(Y, m, n0 + lr, N, v[r]);
+            if (m < M) put(Y, m, n0 + lr, N, v[r], ahead[t][r]);
         }
     }
 }

@@ -335,6 +335,14 @@ __global__ __launch_bounds__(kThreads) void gemm_tile_kernel(const uint8_t *__re
     const uint32_t soff = at & ~3u, nsh = 8u * (at & 3u);  // the scale's dword and half
     const int nib = 4 * (lk >> 1);  // nibble shift (Q4_0)
 
+    // An epilogue's operands: the compute waves load nothing else, and up to 64
+    // rows they have the registers to do it now.
+    constexpr bool kEarly = kHasEpilogue<OUT> && MT <= 4;
+    TileAhead<kTileM, kTileN, kCompute> ahead;
+    if constexpr (kEarly) {
+        if (S == 1 && wave < 8) tile_ahead(Y, m0, n0, M, N, tid, ahead);
+    }
+
     f32x4 acc[MT][2];
 #pragma unroll
     for (int a = 0; a < MT; a++)
@@ -460,8 +468,12 @@ __global__ __launch_bounds__(kThreads) void gemm_tile_kernel(const uint8_t *__re
     if constexpr (kHasEpilogue<OUT>) {
         if (S == 1) {
             static_assert(kStagePitch == kTilePitch<kTileN>, "put_tile's layout");
-            if (wave < 8) put_tile<kTileM, kTileN, kCompute>(Y, stage, m0, n0, M, N, tid, fill);
-            else __syncthreads();  // put_tile's
+            if constexpr (!kEarly) {
+                if (wave < 8) tile_ahead(Y, m0, n0, M, N, tid, ahead);
+            }
+            fill();
+            __syncthreads();
+            if (wave < 8) put_tile(Y, stage, m0, n0, M, N, tid, ahead);
             return;
         }
     }

@@ -744,6 +744,9 @@ __global__ __launch_bounds__(kColThreads) void gemv_mfma_col_kernel(
     const uint32_t row_bytes = (uint32_t)row_bytes64;
     const int tiles = (nr + kTileRows - 1) / kTileRows;
     const uint32_t lds0 = (uint32_t)(uintptr_t)(lds_ptr)lds;
+    static_assert(NV * G::kMaxRows <= kColThreads, "one output a thread");
+    const int out_v = NV > 1 ? (int)threadIdx.x / nr : 0;
+    const auto ahead = load_ahead(y, (int)threadIdx.x < NV * nr, out_v, r0 + (int)threadIdx.x - out_v * nr);
 
     if (wv < nsb) {  // wave-uniform; waves past nsb own no column
         // The column's rows: nr PB-byte pieces (PREP: contiguous from
@@ -885,7 +888,7 @@ __global__ __launch_bounds__(kColThreads) void gemv_mfma_col_kernel(
         float s = 0.0f;
 #pragma unroll
         for (int k = 0; k < kColWaves; k++) s += p[k].x + p[k].y;
-        put(y, v, r0 + r, rows, s);
+        put(y, v, r0 + r, rows, s, ahead);
     }
 }
 
@@ -923,6 +926,9 @@ __global__ __launch_bounds__(kColThreads) void gemv_mfma_wide_kernel(
     const int wv = __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
     const int64_t r0 = (int64_t)blockIdx.x * rows_per_wg;
     const int nr = (int)(rows - r0 < rows_per_wg ? rows - r0 : rows_per_wg);  // 1..kMaxRows
+    static_assert(NV * G::kMaxRows <= kColThreads, "one output a thread");
+    const int out_v = NV > 1 ? (int)threadIdx.x / nr : 0;
+    const auto ahead = load_ahead(y, (int)threadIdx.x < NV * nr, out_v, r0 + (int)threadIdx.x - out_v * nr);
     const uint32_t row_bytes = (uint32_t)row_bytes64;
     const int tiles = (nr + kTileRows - 1) / kTileRows;
     const int ncol = wv < nsb ? (nsb - wv + kColWaves - 1) / kColWaves : 0;  // wave-uniform
@@ -1051,7 +1057,7 @@ __global__ __launch_bounds__(kColThreads) void gemv_mfma_wide_kernel(
         }
         float s = 0.0f;
         for (int k = 0; k < nw; k++) s += part[v][k][r][0] + part[v][k][r][1];
-        put(y, v, r0 + r, rows, s);
+        put(y, v, r0 + r, rows, s, ahead);
     }
 }
 

@@ -112,6 +112,14 @@ __global__ __launch_bounds__(64 * NW *KW, MT == 1 && NW == 2 ? 4 : 1) void gemm_
     const int nsb = K / kQK, nst = (nsb + KW - 1) / KW;
     const int st0 = split * nst / S, st1 = (split + 1) * nst / S;
 
+    // An epilogue's operands: small tiles have the registers to load them now
+    // (but Q5_K's and Q6_K's at four waves a SIMD, which would spill).
+    constexpr bool kEarly = kHasEpilogue<OUT> && MT <= 2 && !(MT == 1 && NW == 2 && T != kQ4_K);
+    TileAhead<kTileM, kTileN, 64 * kWaves> ahead;
+    if constexpr (kEarly) {
+        if (S == 1) tile_ahead(Y, m0, n0, M, N, (int)threadIdx.x, ahead);
+    }
+
     const int col0 = n0 + 32 * nw;
     const uint8_t *wp[2];
 #pragma unroll
@@ -240,9 +248,9 @@ __global__ __launch_bounds__(64 * NW *KW, MT == 1 && NW == 2 ? 4 : 1) void gemm_
             constexpr int kPitch = kTilePitch<kTileN>;
             static_assert(sizeof(lds) >= sizeof(float) * kTileM * kPitch, "the tile's LDS");
             float *const tile = reinterpret_cast<float *>(lds[0]);
-            put_tile<kTileM, kTileN, 64 * kWaves>(Y, tile, m0, n0, M, N, (int)threadIdx.x, [&] {
-                __syncthreads();  // the last stage's reads and the sums' are done
-                if (kw > 0) return;
+            if constexpr (!kEarly) tile_ahead(Y, m0, n0, M, N, (int)threadIdx.x, ahead);
+            __syncthreads();  // the last stage's reads and the sums' are done
+            if (kw == 0) {
 #pragma unroll
                 for (int mt = 0; mt < MT; mt++)
 #pragma unroll
@@ -250,7 +258,9 @@ __global__ __launch_bounds__(64 * NW *KW, MT == 1 && NW == 2 ? 4 : 1) void gemm_
 #pragma unroll
                         for (int r = 0; r < 4; r++)
                             tile[(16 * mt + 4 * g + r) * kPitch + 32 * nw + 16 * nt + n] = acc[mt][nt][r];
-            });
+            }
+            __syncthreads();
+            put_tile(Y, tile, m0, n0, M, N, (int)threadIdx.x, ahead);
             return;
         }
         if (kw > 0) return;

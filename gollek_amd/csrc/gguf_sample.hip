@@ -15,21 +15,24 @@
 // token, and their rounding (2^-45 a token) is far below what fp32 sums would
 // lose at the borders of top_p and u.
 //
-// A row is cut into chunks of 4096 tokens and the chunks dealt to workgroups;
-// four launches, each reading the row at most once:
-//   1 the chunks' largest and least logits;
-//   2 rows with top_k or top_p: a histogram (tokens and mass) over 512 bins of
-//     l, linear from the largest logit down to where weights round to 0 (or to
-//     the least logit); other rows: every chunk's kept mass;
-//   3 the bin in which a filter's border falls, from the histogram; its
-//     tokens are collected, or, where that makes at most 4096, those of every bin
-//     down to it; the chunks' mass above it;
+// A row is cut into slabs of 256 tokens, sixteen of them a chunk, and the chunks
+// dealt to workgroups; four launches:
+//   1 the largest logit of every slab (reads the row);
+//   2 a top_k of up to as many as the slabs that hold a token, and 2048: the
+//     top_k-th largest slab maximum, below which no kept token lies (reads no
+//     logits); other rows with a filter: a histogram (tokens, and mass for
+//     top_p) over 512 bins of l, linear from the largest logit down to where
+//     weights round to 0 (or to the least logit); rows without: every chunk's
+//     kept mass;
+//   3 the tokens that may be kept are collected, from the slabs that hold any:
+//     those above the slab bound, or those down to the bin in which the filter's
+//     border falls; where that is more than 4096, the border's bin alone and the
+//     chunks' mass above it;
 //   4 one workgroup per row: the collected tokens sorted, the border in them, the
-//     draw: among the collected ones, or in the chunk that the random number
-//     falls into.
-// Rows whose border bin holds more than 4096 tokens (equal logits, a
-// temperature of 30), or whose top_k and top_p together reach further, are
-// computed by the last workgroup alone, digit by digit over the whole row.
+//     draw: the chunk that the random number falls into, then the token.
+// A row whose border bin holds more than 4096 tokens (equal logits, a
+// temperature of 30), or whose top_p border depends on a top_k border that far
+// down, is computed by the last workgroup alone, digit by digit over the row.
 #include <hip/hip_runtime.h>
 
 #include "gguf_kernels.hpp"
@@ -75,6 +78,8 @@ struct SampleArgs {
 constexpr int kThreads = 1024, kWaves = kThreads / 64;  // of the last launch
 constexpr int kScan = 256;                              // of the others
 constexpr int kChunk = 4096, kBins = 512, kList = 4096;
+constexpr int kSlabs = 16;  // of a chunk
+constexpr int kSlabTopK = 2048, kSlabsMax = 1024;  // of the slab bound
 
 struct Border {  // kept: key > this one, or the same key at an index up to this one
     uint32_t key;
@@ -296,20 +301,22 @@ __device__ void whole_row(const SampleArgs &a, int row, const Wish &wish, float 
 struct Plan {
     int mode;          // see kWhole ..
     int bin;           // the border's bin
-    uint32_t before;   // tokens in the bins above it
+    uint32_t floor;    // kSlabs: keys from here on are collected
+    uint32_t before;   // tokens in the bins above the border's
     uint32_t tokens;   // of the row that top_k leaves
     u64 before_mass;   // mass in the bins above it
-    double target;     // mass that top_p wants
+    double target;     // mass that top_p wants (0: its share of the collected tokens' first top_k)
 };
 enum : int {
     kWhole,   // the last workgroup alone
     kFree,    // no border with weight below it: every token, by chunks
     kBorder,  // the collected tokens are the border's bin
-    kAll,     // the collected tokens are all that top_k keeps, and some more
+    kAll,     // every token that may be kept is collected
 };
 
 struct SampleWs {
-    float2 *range;        // [rows][chunks] largest, least logit
+    float *tops;          // [rows][chunks * 16] slabs' largest logits
+    float *least;         // [rows][chunks * 4] least finite logits
     u64 *mass;            // [rows][parts][kBins]
     u64 *chunk_mass;      // [rows][chunks]
     u64 *list;            // [rows][kList]
@@ -340,15 +347,75 @@ __device__ __forceinline__ void load4(const SampleArgs &a, int64_t base, int i, 
         for (int j = 0; j < 4; j++) l[j] = i + j < a.vocab ? load_element(a.logits, a.type, base + i + j) : -__builtin_inff();
     }
 }
+// A thread's tokens of a chunk: the slabs are waves' quarters of 1024.
+__device__ __forceinline__ void load_chunk(const SampleArgs &a, int64_t base, int c, float (&l)[4][4]) {
+#pragma unroll
+    for (int j = 0; j < 4; j++) load4(a, base, c * kChunk + j * 1024 + 4 * (int)threadIdx.x, l[j]);
+}
 
-// The largest and least logit of the row's tokens.
-__device__ __forceinline__ float2 row_range(const SampleWs &ws, int row) {
-    float2 r = {-__builtin_inff(), __builtin_inff()};
-    for (int c = (int)threadIdx.x & 63; c < ws.chunks; c += 64) {
-        const float2 v = ws.range[(int64_t)row * ws.chunks + c];
-        r = {fmaxf(r.x, v.x), fminf(r.y, v.y)};
+template <int CTRL, int ROWS>
+__device__ __forceinline__ float dpp_max(float v) {
+    const int low = __float_as_int(-__builtin_inff());
+    return fmaxf(v, __int_as_float(__builtin_amdgcn_update_dpp(low, __float_as_int(v), CTRL, ROWS, 0xF, false)));
+}
+// The largest of the wave's values, in lane 63.
+__device__ __forceinline__ float wave_top(float v) {
+    v = dpp_max<0x111, 0xF>(v);  // row_shr 1, 2, 4, 8
+    v = dpp_max<0x112, 0xF>(v);
+    v = dpp_max<0x114, 0xF>(v);
+    v = dpp_max<0x118, 0xF>(v);
+    v = dpp_max<0x142, 0xA>(v);  // row_bcast 15, 31
+    return dpp_max<0x143, 0xC>(v);
+}
+
+__global__ __launch_bounds__(kScan) void sample_range_kernel(SampleArgs a, SampleWs ws) {
+    const int row = (int)blockIdx.y, tid = (int)threadIdx.x, lane = tid & 63, wave = tid >> 6;
+    const int64_t base = (int64_t)row * a.stride;
+    if (blockIdx.x == 0 && tid == 0) ws.listed[row] = 0;
+    for (int c = ws.first((int)blockIdx.x); c < ws.first((int)blockIdx.x + 1); c++) {
+        float l[4][4];
+        load_chunk(a, base, c, l);
+        const int64_t at = (int64_t)row * ws.chunks + c;
+        float low = -__builtin_inff();  // the largest of the negated tokens
+#pragma unroll
+        for (int j = 0; j < 4; j++) {
+            const float top = wave_top(fmaxf(fmaxf(l[j][0], l[j][1]), fmaxf(l[j][2], l[j][3])));
+            if (lane == 63) ws.tops[kSlabs * at + 4 * j + wave] = top;
+#pragma unroll
+            for (int i = 0; i < 4; i++)
+                if (l[j][i] > -__builtin_inff()) low = fmaxf(low, -l[j][i]);
+        }
+        low = wave_top(low);
+        if (lane == 63) ws.least[4 * at + wave] = -low;
     }
-    for (int d = 1; d < 64; d <<= 1) r = {fmaxf(r.x, __shfl_xor(r.x, d)), fminf(r.y, __shfl_xor(r.y, d))};
+}
+
+struct Range {
+    float top, least;
+    int slabs;  // that hold a token
+};
+// The row's largest and least logit, for a workgroup of THREADS.
+template <int THREADS>
+__device__ __forceinline__ Range row_range(const SampleWs &ws, int row) {
+    __shared__ Range part[THREADS / 64];
+    Range r = {-__builtin_inff(), __builtin_inff(), 0};
+    for (int i = (int)threadIdx.x; i < kSlabs * ws.chunks; i += THREADS) {
+        const float t = ws.tops[(int64_t)row * kSlabs * ws.chunks + i];
+        r.top = fmaxf(r.top, t);
+        r.slabs += t > -__builtin_inff() ? 1 : 0;
+    }
+    for (int i = (int)threadIdx.x; i < 4 * ws.chunks; i += THREADS)
+        r.least = fminf(r.least, ws.least[(int64_t)row * 4 * ws.chunks + i]);
+    for (int d = 1; d < 64; d <<= 1) {
+        r.top = fmaxf(r.top, __shfl_xor(r.top, d));
+        r.least = fminf(r.least, __shfl_xor(r.least, d));
+        r.slabs += __shfl_xor(r.slabs, d);
+    }
+    if ((threadIdx.x & 63) == 0) part[threadIdx.x >> 6] = r;
+    __syncthreads();
+    r = part[0];
+    for (int w = 1; w < THREADS / 64; w++)
+        r = {fmaxf(r.top, part[w].top), fminf(r.least, part[w].least), r.slabs + part[w].slabs};
     return r;
 }
 
@@ -361,49 +428,25 @@ struct Bins {
         return l == m || inv == 0.0f ? 0 : (int)fminf((m - l) * inv, (float)(kBins - 1));  // (m infinite: the last)
     }
 };
-__device__ __forceinline__ Bins row_bins(const SampleArgs &a, const Wish &w, float2 r) {
+__device__ __forceinline__ Bins row_bins(const SampleArgs &a, const Wish &w, const Range &r) {
     const float reach = (float)((double)(a.shift + 2) * 0.69314718055994531 / w.inv_t);  // (infinite at T = inf)
-    const float span = r.x - r.y;                                                        // (or at huge logits)
+    const float span = r.top - r.least;                                                  // (or at huge logits)
     const bool far = !(span < reach);
     const float range = far ? reach : span;
     // A range of 0, or of infinity, leaves one bin.
-    return {r.x, range > 0.0f ? fminf((float)(kBins - 1) / range, 0x1p100f) : 0.0f, far};
-}
-// Whether a row has a border to look for.
-__device__ __forceinline__ bool has_border(const SampleArgs &a, const Wish &w) { return w.has_p || w.top_k < a.vocab; }
-// A border is looked for in bins unless min_p reaches into the weights that are 0.
-__device__ __forceinline__ bool by_bins(const SampleArgs &a, const Wish &w) {
-    return !(w.min_p > 0.0 && w.min_p < __builtin_ldexp(1.0, 2 - a.shift));
+    return {r.top, range > 0.0f ? fminf((float)(kBins - 1) / range, 0x1p100f) : 0.0f, far};
 }
 
-__global__ __launch_bounds__(kScan) void sample_range_kernel(SampleArgs a, SampleWs ws) {
-    __shared__ float2 part[kScan / 64];
-    const int row = (int)blockIdx.y, tid = (int)threadIdx.x;
-    const int64_t base = (int64_t)row * a.stride;
-    if (blockIdx.x == 0 && tid == 0) ws.listed[row] = 0;
-    for (int c = ws.first((int)blockIdx.x); c < ws.first((int)blockIdx.x + 1); c++) {
-        float l[4][4];
-#pragma unroll
-        for (int j = 0; j < 4; j++) load4(a, base, c * kChunk + j * 1024 + 4 * tid, l[j]);
-        float2 r = {-__builtin_inff(), __builtin_inff()};
-#pragma unroll
-        for (int j = 0; j < 16; j++) {
-            const float v = l[j >> 2][j & 3];
-            r.x = fmaxf(r.x, v);
-            if (v > -__builtin_inff()) r.y = fminf(r.y, v);
-        }
-        for (int d = 1; d < 64; d <<= 1) r = {fmaxf(r.x, __shfl_xor(r.x, d)), fminf(r.y, __shfl_xor(r.y, d))};
-        __syncthreads();
-        if ((tid & 63) == 0) part[tid >> 6] = r;
-        __syncthreads();
-        if (tid == 0) {
-            for (int w = 1; w < kScan / 64; w++) r = {fmaxf(r.x, part[w].x), fminf(r.y, part[w].y)};
-            ws.range[(int64_t)row * ws.chunks + c] = r;
-        }
-    }
+// How a row's border is looked for.
+enum : int { kNoBorder, kBySlabs, kByBins, kBySearch };
+__device__ __forceinline__ int border_way(const SampleArgs &a, const SampleWs &ws, const Wish &w, const Range &r) {
+    if (!w.has_p && w.top_k >= a.vocab) return kNoBorder;
+    if (w.top_k <= r.slabs && w.top_k <= kSlabTopK && kSlabs * ws.chunks <= kSlabsMax) return kBySlabs;
+    // bins do not count tokens of weight 0 that a tiny min_p keeps
+    return w.min_p > 0.0 && w.min_p < __builtin_ldexp(1.0, 2 - a.shift) ? kBySearch : kByBins;
 }
 
-// Sums over the workgroup of kScan threads, in thread 0.
+// Sums over the workgroup of kScan threads, in every thread.
 __device__ __forceinline__ void scan_sum(u64 &mass, uint32_t &n, u64 *pm, uint32_t *pn) {
     for (int d = 1; d < 64; d <<= 1) {
         mass += __shfl_xor(mass, d);
@@ -423,6 +466,28 @@ __device__ __forceinline__ void scan_sum(u64 &mass, uint32_t &n, u64 *pm, uint32
     }
 }
 
+// The upper half of the k-th largest slab maximum's key (k slabs at least hold a
+// token that large): its bits one by one, by one wave.
+__device__ __forceinline__ uint32_t slab_floor(const SampleWs &ws, int row, int k) {
+    constexpr int kPer = kSlabsMax / 64;
+    const int lane = (int)threadIdx.x & 63, slabs = kSlabs * ws.chunks;
+    uint32_t key[kPer];
+#pragma unroll
+    for (int j = 0; j < kPer; j++)
+        key[j] = lane + 64 * j < slabs ? logit_key(ws.tops[(int64_t)row * slabs + lane + 64 * j]) : 0u;
+    uint32_t floor = 0;
+    for (int bit = 31; bit >= 16; bit--) {
+        const uint32_t next = floor | (1u << bit);
+        int n = 0;
+#pragma unroll
+        for (int j = 0; j < kPer; j++) {
+            if (64 * j < slabs) n += __builtin_popcountll(__ballot(key[j] >= next));
+        }
+        if (n >= k) floor = next;
+    }
+    return floor > 0u ? floor : 1u;  // (0 is no token)
+}
+
 __global__ __launch_bounds__(kScan) void sample_bins_kernel(SampleArgs a, SampleWs ws) {
     __shared__ u64 mass[kBins];
     __shared__ uint32_t count[kBins];
@@ -431,12 +496,23 @@ __global__ __launch_bounds__(kScan) void sample_bins_kernel(SampleArgs a, Sample
     const int row = (int)blockIdx.y, part = (int)blockIdx.x, tid = (int)threadIdx.x;
     const int64_t base = (int64_t)row * a.stride;
     const Wish wish = row_wish(a, row);
-    const float2 r = row_range(ws, row);
-    if (!(r.x > -__builtin_inff())) return;  // no token
-    const Scale sc = {r.x, wish.inv_t, a.shift};
+    const Range r = row_range<kScan>(ws, row);
+    if (!(r.top > -__builtin_inff())) return;  // no token
+    const int way = border_way(a, ws, wish, r);
+    if (way == kBySlabs || way == kBySearch) {
+        if (part != 0 || tid >= 64) return;
+        Plan plan = {kWhole, kBins, 0, 0, 0, 0, 0.0};
+        if (way == kBySlabs) {
+            plan.mode = kAll;
+            plan.floor = slab_floor(ws, row, wish.top_k);
+            plan.tokens = (uint32_t)wish.top_k;
+        }
+        if (tid == 0) ws.plan[row] = plan;
+        return;
+    }
+    const Scale sc = {r.top, wish.inv_t, a.shift};
     const Bins bins = row_bins(a, wish, r);
-    const bool border = has_border(a, wish);
-    if (border && !by_bins(a, wish)) return;
+    const bool border = way == kByBins;
     if (border) {
         for (int b = tid; b < kBins; b += kScan) {
             mass[b] = 0;
@@ -446,8 +522,7 @@ __global__ __launch_bounds__(kScan) void sample_bins_kernel(SampleArgs a, Sample
     }
     for (int c = ws.first(part); c < ws.first(part + 1); c++) {
         float l[4][4];
-#pragma unroll
-        for (int j = 0; j < 4; j++) load4(a, base, c * kChunk + j * 1024 + 4 * tid, l[j]);
+        load_chunk(a, base, c, l);
         if (border) {
 #pragma unroll
             for (int j = 0; j < 16; j++) {
@@ -476,12 +551,49 @@ __global__ __launch_bounds__(kScan) void sample_bins_kernel(SampleArgs a, Sample
             }
         }
     }
-    if (!border) return;
+    if (!border) {
+        if (part == 0 && tid == 0) ws.plan[row] = Plan{kFree, kBins, 0, 0, 0x7FFFFFFF, 0, 0.0};
+        return;
+    }
     __syncthreads();
     const int64_t at = ((int64_t)row * ws.parts + part) * kBins;
     for (int b = tid; b < kBins; b += kScan) {
         ws.count[at + b] = count[b];
         if (wish.has_p) ws.mass[at + b] = mass[b];
+    }
+}
+
+// Adds the tokens of a chunk that bit j of `listed` names (l[j / 4][j % 4]) to
+// the row's list; `counts`: a word per wave.
+__device__ __forceinline__ void collect(const SampleWs &ws, int row, int c, const float (&l)[4][4], uint32_t listed,
+                                        uint32_t *counts, uint32_t *place) {
+    const int tid = (int)threadIdx.x, lane = tid & 63, wave = tid >> 6;
+    const uint32_t mine = (uint32_t)__builtin_popcount(listed);
+    uint32_t upto = mine;  // places: this thread's after those of the threads before
+    for (int d = 1; d < 64; d <<= 1) {
+        const uint32_t o = __shfl_up(upto, d);
+        if (lane >= d) upto += o;
+    }
+    __syncthreads();
+    if (lane == 63) counts[wave] = upto;
+    __syncthreads();
+    uint32_t sum = 0;
+    for (int w = 0; w < kScan / 64; w++) {
+        if (w < wave) upto += counts[w];
+        sum += counts[w];
+    }
+    if (sum == 0) return;  // (the same in every thread)
+    if (tid == 0) *place = atomicAdd(ws.listed + row, sum);
+    __syncthreads();
+    uint32_t p = *place + upto - mine;
+#pragma unroll
+    for (int j = 0; j < 16; j++) {
+        if ((listed >> j) & 1u) {
+            if (p < (uint32_t)kList)  // (more: the last launch sees it by the count)
+                ws.list[(int64_t)row * kList + p] = ((u64)(0xFFFFFFFFu - logit_key(l[j >> 2][j & 3])) << 32) |
+                                                    (uint32_t)(c * kChunk + (j >> 2) * 1024 + 4 * tid + (j & 3));
+            p++;
+        }
     }
 }
 
@@ -495,16 +607,43 @@ __global__ __launch_bounds__(kScan) void sample_border_kernel(SampleArgs a, Samp
     const int row = (int)blockIdx.y, part = (int)blockIdx.x, tid = (int)threadIdx.x, lane = tid & 63, wave = tid >> 6;
     const int64_t base = (int64_t)row * a.stride;
     const Wish wish = row_wish(a, row);
-    const float2 r = row_range(ws, row);
-    if (!(r.x > -__builtin_inff())) return;
-    Plan plan = {kFree, kBins, 0, 0x7FFFFFFF, 0, 0.0};
-    const bool border = has_border(a, wish);
-    if (!border || !by_bins(a, wish)) {
-        if (border) plan.mode = kWhole;
-        if (part == 0 && tid == 0) ws.plan[row] = plan;
+    const Range r = row_range<kScan>(ws, row);
+    if (!(r.top > -__builtin_inff())) return;
+    const int way = border_way(a, ws, wish, r);
+    if (way == kNoBorder || way == kBySearch) return;
+    const float *const tops = ws.tops + (int64_t)row * kSlabs * ws.chunks;
+    // whether any slab of a chunk reaches a key, and whether this wave's slab j does
+    auto load_from = [&](int c, float least, float (&l)[4][4]) {
+        bool any = false;
+#pragma unroll
+        for (int j = 0; j < kSlabs; j++) any |= tops[kSlabs * c + j] >= least;
+        if (!any) return false;
+#pragma unroll
+        for (int j = 0; j < 4; j++) {
+            if (tops[kSlabs * c + 4 * j + wave] >= least) {
+                load4(a, base, c * kChunk + j * 1024 + 4 * tid, l[j]);
+            } else {
+#pragma unroll
+                for (int i = 0; i < 4; i++) l[j][i] = -__builtin_inff();
+            }
+        }
+        return true;
+    };
+    if (way == kBySlabs) {
+        const uint32_t floor = ws.plan[row].floor;
+        const float least = floor <= 0x007FFFFFu ? -3.402823466e38f : key_logit(floor);  // (no key lies below -max's)
+        for (int c = ws.first(part); c < ws.first(part + 1); c++) {
+            float l[4][4];
+            if (!load_from(c, least, l)) continue;
+            uint32_t listed = 0;
+#pragma unroll
+            for (int j = 0; j < 16; j++) listed |= logit_key(l[j >> 2][j & 3]) >= floor ? 1u << j : 0u;
+            collect(ws, row, c, l, listed, cn, &place);
+        }
         return;
     }
-    const Scale sc = {r.x, wish.inv_t, a.shift};
+    Plan plan = {kFree, kBins, 0, 0, 0, 0, 0.0};
+    const Scale sc = {r.top, wish.inv_t, a.shift};
     const Bins bins = row_bins(a, wish, r);
 
     // The row's histogram: bins 2 tid, 2 tid + 1, summed over the parts, and its scan.
@@ -579,15 +718,19 @@ __global__ __launch_bounds__(kScan) void sample_border_kernel(SampleArgs a, Samp
     const bool k_cuts = cut_k < kBins && !(bins.far && cut_k == kBins - 1);  // drops weight
     plan.tokens = k < all ? k : all;
     int last;  // bins up to this one are collected, from `from`
-    int from;
+    int from = 0;
     if (k_cuts && before_k + in_k <= (uint32_t)kList) {
         plan.mode = kAll;
-        from = 0;
         last = cut_k;
     } else if (k_cuts) {
         plan.mode = wish.has_p || in_k > (uint32_t)kList ? kWhole : kBorder;
         plan.bin = from = last = cut_k;
         plan.before = before_k;
+    } else if (wish.has_p && before_p + in_p <= (uint32_t)kList) {
+        plan.mode = kAll;
+        last = cut_p;
+        plan.tokens = before_p + in_p;
+        plan.target = target;
     } else if (wish.has_p) {
         plan.mode = in_p > (uint32_t)kList ? kWhole : kBorder;
         plan.bin = from = last = cut_p;
@@ -604,11 +747,9 @@ __global__ __launch_bounds__(kScan) void sample_border_kernel(SampleArgs a, Samp
 
     for (int c = ws.first(part); c < ws.first(part + 1); c++) {
         float l[4][4];
-        const int i0 = c * kChunk + 4 * tid;
-#pragma unroll
-        for (int j = 0; j < 4; j++) load4(a, base, i0 + j * 1024, l[j]);
+        load_chunk(a, base, c, l);
         u64 t = 0;
-        uint32_t kept = 0, mine = 0, listed = 0;  // listed: bit j: token j is collected
+        uint32_t kept = 0, listed = 0;  // listed: bit j: token j is collected
 #pragma unroll
         for (int j = 0; j < 16; j++) {
             const float v = l[j >> 2][j & 3];
@@ -616,7 +757,6 @@ __global__ __launch_bounds__(kScan) void sample_border_kernel(SampleArgs a, Samp
             const int b = bins.of(v);
             if (b >= from && b <= last) {
                 listed |= 1u << j;
-                mine++;
             } else if (plan.mode != kAll && b < plan.bin) {
                 const double w = sc.weight(v);
                 if (w >= wish.min_p) {
@@ -632,34 +772,7 @@ __global__ __launch_bounds__(kScan) void sample_border_kernel(SampleArgs a, Samp
                 ws.chunk_kept[(int64_t)row * ws.chunks + c] = kept;
             }
         }
-        // places in the list: this thread's after those of the threads before
-        uint32_t upto = mine;
-        for (int d = 1; d < 64; d <<= 1) {
-            const uint32_t o = __shfl_up(upto, d);
-            if (lane >= d) upto += o;
-        }
-        __syncthreads();
-        if (lane == 63) cn[wave] = upto;
-        __syncthreads();
-        uint32_t sum = 0;
-        for (int w = 0; w < kScan / 64; w++) {
-            if (w < wave) upto += cn[w];
-            sum += cn[w];
-        }
-        if (sum == 0) continue;  // (the same in every thread)
-        if (tid == 0) place = atomicAdd(ws.listed + row, sum);
-        __syncthreads();
-        uint32_t p = place + upto - mine;
-#pragma unroll
-        for (int j = 0; j < 16; j++) {
-            if ((listed >> j) & 1u) {
-                // (the histogram counted them: at most kList)
-                if (p < (uint32_t)kList)
-                    ws.list[(int64_t)row * kList + p] = ((u64)(0xFFFFFFFFu - logit_key(l[j >> 2][j & 3])) << 32) |
-                                                        (uint32_t)(i0 + (j >> 2) * 1024 + (j & 3));
-                p++;
-            }
-        }
+        collect(ws, row, c, l, listed, cn, &place);
     }
 }
 
@@ -681,34 +794,82 @@ __device__ __forceinline__ u64 block_scan(u64 v, u64 &total, RowLds &s) {
     return v;
 }
 
-// Sorts the first n (up to kList) of `list`, whose values differ, upwards.
-__device__ void sort_list(u64 *list, int n) {
+struct SortLds {
+    u64 list[kList], spare[kList];
+    uint32_t slot[kThreads];
+    uint32_t most;
+};
+
+// Sorts the first n (up to kList) of s.list, whose values differ, upwards.
+// bucket(v): a number in [0, kThreads) that does not fall as v rises.  Every
+// value goes to its bucket and finds its place there by counting the smaller
+// ones; with more than 64 values in a bucket (equal logits) a bitonic sort.
+template <class BUCKET>
+__device__ void sort_list(SortLds &s, RowLds &rl, int n, BUCKET &&bucket) {
     const int tid = (int)threadIdx.x;
-    if (n <= 256) {  // each value's place: the values below it, four threads a value
-        const int e = tid >> 2, q = tid & 3;
-        const u64 v = e < n ? list[e] : 0;
-        int below = 0;
-        if (e < n)
-            for (int j = q; j < n; j += 4) below += list[j] < v ? 1 : 0;
-        below += __shfl_xor(below, 1);
-        below += __shfl_xor(below, 2);
-        __syncthreads();
-        if (e < n && q == 0) list[below] = v;
+    if (n <= 64) {
+        if (tid < 64) {
+            const u64 v = tid < n ? s.list[tid] : 0;
+            int below = 0;
+            for (int j = 0; j < n; j++) below += s.list[j] < v ? 1 : 0;
+            __builtin_amdgcn_wave_barrier();  // (a wave's LDS accesses complete in order)
+            if (tid < n) s.list[below] = v;
+        }
         __syncthreads();
         return;
     }
-    int size = 512;
+    s.slot[tid] = 0;
+    if (tid == 0) s.most = 0;
+    __syncthreads();
+    constexpr int kPer = kList / kThreads;
+    u64 v[kPer];
+    int b[kPer];
+#pragma unroll
+    for (int j = 0; j < kPer; j++) {
+        const int i = tid + j * kThreads;
+        v[j] = i < n ? s.list[i] : 0;
+        b[j] = i < n ? bucket(v[j]) : 0;
+        if (i < n) atomicAdd(&s.slot[b[j]], 1u);  // LDS
+    }
+    __syncthreads();
+    const uint32_t mine = s.slot[tid];
+    uint32_t most = mine;
+    for (int d = 1; d < 64; d <<= 1) most = max(most, (uint32_t)__shfl_xor((int)most, d));
+    if ((tid & 63) == 0) atomicMax(&s.most, most);  // LDS
+    u64 total;
+    const uint32_t end = (uint32_t)block_scan(mine, total, rl);
+    if (s.most <= 64) {  // (block_scan's barriers stand between)
+        __syncthreads();
+        s.slot[tid] = end - mine;
+        __syncthreads();
+#pragma unroll
+        for (int j = 0; j < kPer; j++)
+            if (tid + j * kThreads < n) s.spare[atomicAdd(&s.slot[b[j]], 1u)] = v[j];
+        __syncthreads();
+        // s.slot[b] is the bucket's end now, s.slot[b - 1] its start
+#pragma unroll
+        for (int j = 0; j < kPer; j++) {
+            if (tid + j * kThreads >= n) continue;
+            const uint32_t from = b[j] > 0 ? s.slot[b[j] - 1] : 0u, to = s.slot[b[j]];
+            uint32_t place = from;
+            for (uint32_t i = from; i < to; i++) place += s.spare[i] < v[j] ? 1u : 0u;
+            s.list[place] = v[j];
+        }
+        __syncthreads();
+        return;
+    }
+    int size = 128;
     while (size < n) size <<= 1;
-    for (int i = n + tid; i < size; i += kThreads) list[i] = ~0ull;
+    for (int i = n + tid; i < size; i += kThreads) s.list[i] = ~0ull;
     __syncthreads();
     for (int k = 2; k <= size; k <<= 1)
         for (int j = k >> 1; j > 0; j >>= 1) {
             for (int t = tid; t < size / 2; t += kThreads) {
                 const int i = 2 * t - (t & (j - 1)), o = i + j;
-                const u64 x = list[i], y = list[o];
+                const u64 x = s.list[i], y = s.list[o];
                 if ((x > y) == ((i & k) == 0)) {
-                    list[i] = y;
-                    list[o] = x;
+                    s.list[i] = y;
+                    s.list[o] = x;
                 }
             }
             __syncthreads();
@@ -718,15 +879,18 @@ __device__ void sort_list(u64 *list, int n) {
 // One workgroup per row.
 __global__ __launch_bounds__(kThreads) void sample_draw_kernel(SampleArgs a, SampleWs ws) {
     __shared__ RowLds s;
-    __shared__ u64 list[kList];
-    __shared__ u64 chunk[1024];
+    __shared__ SortLds so;
+    __shared__ u64 chunk[kThreads];
     __shared__ int which;
     __shared__ u64 before_chunk;
+    __shared__ uint32_t in_chunk;
+    __shared__ float span[2 * kWaves];
+    constexpr int kPer = kList / kThreads;
     const int row = (int)blockIdx.x, tid = (int)threadIdx.x;
     const int64_t base = (int64_t)row * a.stride;
     const Wish wish = row_wish(a, row);
-    const float2 range = row_range(ws, row);
-    if (!(range.x > -__builtin_inff())) {  // no token at all
+    const Range range = row_range<kThreads>(ws, row);
+    if (!(range.top > -__builtin_inff())) {  // no token at all
         if (tid == 0) {
             a.tokens[row] = -1;
             if (a.probs != nullptr) a.probs[row] = 0.0f;
@@ -735,142 +899,153 @@ __global__ __launch_bounds__(kThreads) void sample_draw_kernel(SampleArgs a, Sam
         return;
     }
     const Plan plan = ws.plan[row];
-    if (plan.mode == kWhole) {
-        whole_row(a, row, wish, range.x, s);
+    const int n = plan.mode == kAll || plan.mode == kBorder ? (int)ws.listed[row] : 0;
+    if (plan.mode == kWhole || n > kList) {
+        whole_row(a, row, wish, range.top, s);
         return;
     }
-    const Scale sc = {range.x, wish.inv_t, a.shift};
+    const Scale sc = {range.top, wish.inv_t, a.shift};
     auto write = [&](int token, double w, u64 total, uint32_t kept) {
         a.tokens[row] = token;
         if (a.probs != nullptr) a.probs[row] = (float)(__builtin_ldexp(w, a.shift) / (double)total);
         if (a.kept != nullptr) a.kept[row] = (int32_t)kept;
     };
+    auto logit_of = [](u64 v) { return key_logit(0xFFFFFFFFu - (uint32_t)(v >> 32)); };
 
-    // The collected tokens in order: upper half the inverted key, lower half the index.
-    int n = 0;
-    if (plan.mode != kFree) {
-        n = (int)ws.listed[row];
-        for (int i = tid; i < n; i += kThreads) list[i] = ws.list[(int64_t)row * kList + i];
+    // The collected tokens in order (upper half the inverted key, lower half the
+    // index), their weights, and the border among them.
+    Border border = {0, 0x7FFFFFFF};
+    uint32_t kept = 0;
+    u64 f[kPer];
+    bool keep[kPer];
+    chunk[tid] = 0;
+    if (n > 0) {
+        float low = __builtin_inff(), high = -__builtin_inff();
+        for (int i = tid; i < n; i += kThreads) {
+            const u64 v = ws.list[(int64_t)row * kList + i];
+            so.list[i] = v;
+            low = fminf(low, logit_of(v));
+            high = fmaxf(high, logit_of(v));
+        }
+        for (int d = 1; d < 64; d <<= 1) {
+            low = fminf(low, __shfl_xor(low, d));
+            high = fmaxf(high, __shfl_xor(high, d));
+        }
+        if ((tid & 63) == 0) {
+            span[tid >> 6] = low;
+            span[kWaves + (tid >> 6)] = high;
+        }
         __syncthreads();
-        sort_list(list, n);
-    }
-    auto logit_at = [&](int i) { return key_logit(0xFFFFFFFFu - (uint32_t)(list[i] >> 32)); };
-
-    if (plan.mode == kAll) {
-        const int k = (int)plan.tokens;  // <= n
-        constexpr int kPer = kList / kThreads;
-        u64 f[kPer], sum = 0, total;
+        for (int w = 0; w < kWaves; w++) {
+            low = fminf(low, span[w]);
+            high = fmaxf(high, span[kWaves + w]);
+        }
+        const float wide = high - low;  // (infinite or 0: one bucket)
+        const float inv = wide > 0.0f && wide < 0x1p126f ? fminf((float)(kThreads - 1) / wide, 0x1p100f) : 0.0f;
+        sort_list(so, s, n, [&](u64 v) {
+            return inv > 0.0f ? (int)fminf((high - logit_of(v)) * inv, (float)(kThreads - 1)) : 0;
+        });
+        const int k = plan.mode == kAll && plan.tokens < (uint32_t)n ? (int)plan.tokens : n;
+        u64 sum = 0, total;
         double w[kPer];
 #pragma unroll
         for (int j = 0; j < kPer; j++) {
             const int i = kPer * tid + j;
-            w[j] = i < k ? sc.weight(logit_at(i)) : 0.0;
+            w[j] = i < k ? sc.weight(logit_of(so.list[i])) : 0.0;
             f[j] = i < k ? sc.fixed(w[j]) : 0;
             sum += f[j];
         }
-        u64 before = block_scan(sum, total, s) - sum;
-        const double target = wish.top_p * (double)total;
-        uint32_t keep = 0;
-#pragma unroll
-        for (int j = 0; j < kPer; j++) {
-            const int i = kPer * tid + j;
-            if (i < k && (!wish.has_p || (double)before < target) && w[j] >= wish.min_p) keep++;
-            before += f[j];
-        }
-        keep = block_sum(keep, s);  // (a prefix)
-        // The kept ones by index: upper half the index, lower half the key.
-        __syncthreads();
-        for (int i = tid; i < (int)keep; i += kThreads) {
-            const u64 v = list[i];
-            list[i] = (v << 32) | (0xFFFFFFFFu - (uint32_t)(v >> 32));
-        }
-        __syncthreads();
-        sort_list(list, (int)keep);
-        sum = 0;
-#pragma unroll
-        for (int j = 0; j < kPer; j++) {
-            const int i = kPer * tid + j;
-            w[j] = i < (int)keep ? sc.weight(key_logit((uint32_t)list[i])) : 0.0;
-            f[j] = i < (int)keep ? sc.fixed(w[j]) : 0;
-            sum += f[j];
-        }
-        u64 cum = block_scan(sum, total, s) - sum;
-        const double point = wish.u * (double)total;
-#pragma unroll
-        for (int j = 0; j < kPer; j++) {
-            if (f[j] > 0 && !((double)cum > point) && (double)(cum + f[j]) > point)  // one thread, once
-                write((int)(list[kPer * tid + j] >> 32), w[j], total, keep);
-            cum += f[j];
-        }
-        return;
-    }
-
-    // By chunks: their mass above the border's bin, and the border's own tokens.
-    Border border = {0, 0x7FFFFFFF};
-    uint32_t kept = 0;
-    if (tid < ws.chunks) {
-        chunk[tid] = ws.chunk_mass[(int64_t)row * ws.chunks + tid];
-        kept = ws.chunk_kept[(int64_t)row * ws.chunks + tid];
-    }
-    __syncthreads();
-    if (plan.mode == kBorder) {
-        constexpr int kPer = kList / kThreads;
-        u64 f[kPer], sum = 0, total;
-        double w[kPer];
-#pragma unroll
-        for (int j = 0; j < kPer; j++) {
-            const int i = kPer * tid + j;
-            w[j] = i < n ? sc.weight(logit_at(i)) : 0.0;
-            f[j] = i < n ? sc.fixed(w[j]) : 0;
-            sum += f[j];
-        }
         u64 before = plan.before_mass + block_scan(sum, total, s) - sum;
-        const bool by_mass = plan.target > 0.0;
+        const double target = plan.target > 0.0 ? plan.target : wish.top_p * (double)total;
         uint32_t in = 0;
 #pragma unroll
         for (int j = 0; j < kPer; j++) {
             const int i = kPer * tid + j;
-            if (i < n && (by_mass ? (double)before < plan.target : plan.before + (uint32_t)i < plan.tokens)) {
-                in++;
-                if (w[j] >= wish.min_p) {
-                    kept++;
-                    if (f[j] > 0) atomicAdd(&chunk[(uint32_t)list[i] / kChunk], f[j]);  // LDS
-                }
-            }
+            // (kBorder without a target: top_k's border)
+            const bool inside = i < k && (plan.mode == kBorder && !(plan.target > 0.0) ? plan.before + (uint32_t)i < plan.tokens
+                                                                                       : !wish.has_p || (double)before < target);
             before += f[j];
+            in += inside ? 1u : 0u;
+            keep[j] = inside && w[j] >= wish.min_p;
+            if (!keep[j]) continue;
+            kept++;
+            if (f[j] > 0) atomicAdd(&chunk[(uint32_t)so.list[i] / kChunk], f[j]);  // LDS
         }
-        in = block_sum(in, s);
-        border = {0xFFFFFFFFu - (uint32_t)(list[in - 1] >> 32), (int)(uint32_t)list[in - 1]};
+        if (plan.mode == kBorder) {
+            in = block_sum(in, s);
+            border = {0xFFFFFFFFu - (uint32_t)(so.list[in - 1] >> 32), (int)(uint32_t)so.list[in - 1]};
+        }
+    }
+    __syncthreads();
+    // The chunks' kept mass, and the one that the random number falls into.
+    u64 mine = tid < ws.chunks ? chunk[tid] : 0;
+    if (plan.mode != kAll && tid < ws.chunks) {
+        mine += ws.chunk_mass[(int64_t)row * ws.chunks + tid];
+        kept += ws.chunk_kept[(int64_t)row * ws.chunks + tid];
     }
     kept = block_sum(kept, s);
     if (plan.mode == kFree && wish.min_p == 0.0 && plan.tokens < kept) kept = plan.tokens;  // top_k drops weights of 0
-    const u64 mine = tid < ws.chunks ? chunk[tid] : 0;
     u64 total;
     const u64 upto = block_scan(mine, total, s);
     const double point = wish.u * (double)total;
+    if (tid == 0) in_chunk = 0;
     if (mine > 0 && !((double)(upto - mine) > point) && (double)upto > point) {  // one thread
         which = tid;
         before_chunk = upto - mine;
     }
     __syncthreads();
+    u64 cum = before_chunk;
+    if (plan.mode == kAll) {
+        // the chunk's kept tokens by index: upper half the index, lower half the key
+        u64 v[kPer];
+#pragma unroll
+        for (int j = 0; j < kPer; j++) {
+            const int i = kPer * tid + j;
+            v[j] = i < n ? so.list[i] : 0;
+        }
+        __syncthreads();
+#pragma unroll
+        for (int j = 0; j < kPer; j++)
+            if (kPer * tid + j < n && keep[j] && (int)((uint32_t)v[j] / kChunk) == which)
+                so.list[atomicAdd(&in_chunk, 1u)] = (v[j] << 32) | (0xFFFFFFFFu - (uint32_t)(v[j] >> 32));  // LDS
+        __syncthreads();
+        const int m = (int)in_chunk;
+        sort_list(so, s, m, [](u64 e) { return (int)((uint32_t)(e >> 32) % kChunk / (kChunk / kThreads)); });
+        u64 sum = 0, end;
+        double w[kPer];
+#pragma unroll
+        for (int j = 0; j < kPer; j++) {
+            const int i = kPer * tid + j;
+            w[j] = i < m ? sc.weight(key_logit((uint32_t)so.list[i])) : 0.0;
+            f[j] = i < m ? sc.fixed(w[j]) : 0;
+            sum += f[j];
+        }
+        cum += block_scan(sum, end, s) - sum;
+#pragma unroll
+        for (int j = 0; j < kPer; j++) {
+            if (f[j] > 0 && !((double)cum > point) && (double)(cum + f[j]) > point)  // one thread, once
+                write((int)(so.list[kPer * tid + j] >> 32), w[j], total, kept);
+            cum += f[j];
+        }
+        return;
+    }
     const int i0 = which * kChunk + 4 * tid;
     float l[4];
     load4(a, base, i0, l);
     double w[4];
-    u64 f[4], sum = 0;
+    u64 sum = 0, end;
 #pragma unroll
     for (int j = 0; j < 4; j++) {
-        const uint32_t k = logit_key(l[j]);
+        const uint32_t key = logit_key(l[j]);
         f[j] = 0;
         w[j] = 0.0;
-        if (k != 0 && border.keeps(k, i0 + j)) {
+        if (key != 0 && border.keeps(key, i0 + j)) {
             w[j] = sc.weight(l[j]);
             if (w[j] >= wish.min_p) f[j] = sc.fixed(w[j]);
         }
         sum += f[j];
     }
-    u64 in_chunk;
-    u64 cum = before_chunk + block_scan(sum, in_chunk, s) - sum;
+    cum += block_scan(sum, end, s) - sum;
 #pragma unroll
     for (int j = 0; j < 4; j++) {
         if (f[j] > 0 && !((double)cum > point) && (double)(cum + f[j]) > point) write(i0 + j, w[j], total, kept);
@@ -885,7 +1060,7 @@ int row_parts(int rows, int chunks) {
 }
 
 struct SampleLayout {
-    size_t range, mass, chunk_mass, list, plan, count, chunk_kept, listed, total;
+    size_t tops, least, mass, chunk_mass, list, plan, count, chunk_kept, listed, total;
     int chunks, parts;
 };
 SampleLayout sample_layout(int rows, int vocab) {
@@ -898,7 +1073,8 @@ SampleLayout sample_layout(int rows, int vocab) {
         return at;
     };
     const size_t r = (size_t)rows, rc = r * o.chunks, rb = r * o.parts * kBins;
-    o.range = take(rc * sizeof(float2));
+    o.tops = take(rc * kSlabs * sizeof(float));
+    o.least = take(rc * 4 * sizeof(float));
     o.mass = take(rb * sizeof(u64));
     o.chunk_mass = take(rc * sizeof(u64));
     o.list = take(r * kList * sizeof(u64));
@@ -925,7 +1101,8 @@ hipError_t launch_sample(const void *logits, int logits_type, int rows, int voca
     const SampleArgs a = {logits, stride, logits_type, vocab,  62 - bits, vec4, temperature,
                           top_p,  min_p,  u,           top_k,  tokens,    kept, probs};
     const SampleLayout o = sample_layout(rows, vocab);
-    const SampleWs ws = {reinterpret_cast<float2 *>(workspace + o.range),
+    const SampleWs ws = {reinterpret_cast<float *>(workspace + o.tops),
+                         reinterpret_cast<float *>(workspace + o.least),
                          reinterpret_cast<u64 *>(workspace + o.mass),
                          reinterpret_cast<u64 *>(workspace + o.chunk_mass),
                          reinterpret_cast<u64 *>(workspace + o.list),

@@ -298,16 +298,27 @@ __device__ void whole_row(const SampleArgs &a, int row, const Wish &wish, float 
 
 // ---- the four launches --------------------------------------------------------
 
+struct Bins {
+    float m, inv;
+    bool far;
+    __device__ __forceinline__ int of(float l) const {
+        return l == m || inv == 0.0f ? 0 : (int)fminf((m - l) * inv, (float)(kBins - 1));  // (m infinite: the last)
+    }
+};
 struct Plan {
-    int mode;          // see kWhole ..
-    int bin;           // the border's bin
-    uint32_t floor;    // kSlabs: keys from here on are collected
+    int mode;          // see kNone ..
+    int from, last;    // bins that are collected (none: 0, -1)
+    int bin;           // the border's bin, kBins: none
+    uint32_t floor;    // not 0: keys from here on are collected instead
     uint32_t before;   // tokens in the bins above the border's
     uint32_t tokens;   // of the row that top_k leaves
-    u64 before_mass;   // mass in the bins above it
+    float top;         // the row's largest logit
+    Bins bins;
+    u64 before_mass;   // mass in the bins above the border's
     double target;     // mass that top_p wants (0: its share of the collected tokens' first top_k)
 };
 enum : int {
+    kNone,    // no token
     kWhole,   // the last workgroup alone
     kFree,    // no border with weight below it: every token, by chunks
     kBorder,  // the collected tokens are the border's bin
@@ -421,13 +432,6 @@ __device__ __forceinline__ Range row_range(const SampleWs &ws, int row) {
 
 // Bins of a row: 0 at the largest logit.  far: the last bin is open, and what
 // falls into it has weight 0 (below 2^-(S + 1)).
-struct Bins {
-    float m, inv;
-    bool far;
-    __device__ __forceinline__ int of(float l) const {
-        return l == m || inv == 0.0f ? 0 : (int)fminf((m - l) * inv, (float)(kBins - 1));  // (m infinite: the last)
-    }
-};
 __device__ __forceinline__ Bins row_bins(const SampleArgs &a, const Wish &w, const Range &r) {
     const float reach = (float)((double)(a.shift + 2) * 0.69314718055994531 / w.inv_t);  // (infinite at T = inf)
     const float span = r.top - r.least;                                                  // (or at huge logits)
@@ -438,8 +442,9 @@ __device__ __forceinline__ Bins row_bins(const SampleArgs &a, const Wish &w, con
 }
 
 // How a row's border is looked for.
-enum : int { kNoBorder, kBySlabs, kByBins, kBySearch };
+enum : int { kEmpty, kNoBorder, kBySlabs, kByBins, kBySearch };
 __device__ __forceinline__ int border_way(const SampleArgs &a, const SampleWs &ws, const Wish &w, const Range &r) {
+    if (!(r.top > -__builtin_inff())) return kEmpty;
     if (!w.has_p && w.top_k >= a.vocab) return kNoBorder;
     if (w.top_k <= r.slabs && w.top_k <= kSlabTopK && kSlabs * ws.chunks <= kSlabsMax) return kBySlabs;
     // bins do not count tokens of weight 0 that a tiny min_p keeps
@@ -466,6 +471,21 @@ __device__ __forceinline__ void scan_sum(u64 &mass, uint32_t &n, u64 *pm, uint32
     }
 }
 
+template <int CTRL, int ROWS>
+__device__ __forceinline__ int dpp_add(int v) {
+    return v + __builtin_amdgcn_update_dpp(0, v, CTRL, ROWS, 0xF, false);
+}
+// The wave's sum, in every lane.
+__device__ __forceinline__ int wave_total(int v) {
+    v = dpp_add<0x111, 0xF>(v);
+    v = dpp_add<0x112, 0xF>(v);
+    v = dpp_add<0x114, 0xF>(v);
+    v = dpp_add<0x118, 0xF>(v);
+    v = dpp_add<0x142, 0xA>(v);
+    v = dpp_add<0x143, 0xC>(v);
+    return __builtin_amdgcn_readlane(v, 63);
+}
+
 // The upper half of the k-th largest slab maximum's key (k slabs at least hold a
 // token that large): its bits one by one, by one wave.
 __device__ __forceinline__ uint32_t slab_floor(const SampleWs &ws, int row, int k) {
@@ -480,10 +500,8 @@ __device__ __forceinline__ uint32_t slab_floor(const SampleWs &ws, int row, int 
         const uint32_t next = floor | (1u << bit);
         int n = 0;
 #pragma unroll
-        for (int j = 0; j < kPer; j++) {
-            if (64 * j < slabs) n += __builtin_popcountll(__ballot(key[j] >= next));
-        }
-        if (n >= k) floor = next;
+        for (int j = 0; j < kPer; j++) n += key[j] >= next ? 1 : 0;
+        if (wave_total(n) >= k) floor = next;
     }
     return floor > 0u ? floor : 1u;  // (0 is no token)
 }
@@ -497,19 +515,8 @@ __global__ __launch_bounds__(kScan) void sample_bins_kernel(SampleArgs a, Sample
     const int64_t base = (int64_t)row * a.stride;
     const Wish wish = row_wish(a, row);
     const Range r = row_range<kScan>(ws, row);
-    if (!(r.top > -__builtin_inff())) return;  // no token
     const int way = border_way(a, ws, wish, r);
-    if (way == kBySlabs || way == kBySearch) {
-        if (part != 0 || tid >= 64) return;
-        Plan plan = {kWhole, kBins, 0, 0, 0, 0, 0.0};
-        if (way == kBySlabs) {
-            plan.mode = kAll;
-            plan.floor = slab_floor(ws, row, wish.top_k);
-            plan.tokens = (uint32_t)wish.top_k;
-        }
-        if (tid == 0) ws.plan[row] = plan;
-        return;
-    }
+    if (way == kBySlabs || way == kBySearch || way == kEmpty) return;  // (nothing to count)
     const Scale sc = {r.top, wish.inv_t, a.shift};
     const Bins bins = row_bins(a, wish, r);
     const bool border = way == kByBins;
@@ -551,10 +558,7 @@ __global__ __launch_bounds__(kScan) void sample_bins_kernel(SampleArgs a, Sample
             }
         }
     }
-    if (!border) {
-        if (part == 0 && tid == 0) ws.plan[row] = Plan{kFree, kBins, 0, 0, 0x7FFFFFFF, 0, 0.0};
-        return;
-    }
+    if (!border) return;
     __syncthreads();
     const int64_t at = ((int64_t)row * ws.parts + part) * kBins;
     for (int b = tid; b < kBins; b += kScan) {
@@ -597,55 +601,33 @@ __device__ __forceinline__ void collect(const SampleWs &ws, int row, int c, cons
     }
 }
 
-__global__ __launch_bounds__(kScan) void sample_border_kernel(SampleArgs a, SampleWs ws) {
-    __shared__ u64 pm[kScan / 64], cm[kScan / 64];
-    __shared__ uint32_t pn[kScan / 64], cn[kScan / 64];
+// A row's plan, by a workgroup of kScan threads (the same in every thread).
+__device__ __forceinline__ Plan make_plan(const SampleArgs &a, const SampleWs &ws, int row) {
+    __shared__ u64 cm[kScan / 64];
+    __shared__ uint32_t cn[kScan / 64];
     __shared__ int cut_k, cut_p;
-    __shared__ uint32_t before_k, in_k, before_p, in_p;
+    __shared__ uint32_t before_k, in_k, before_p, in_p, slab_key;
     __shared__ u64 before_mass;
-    __shared__ uint32_t place;
-    const int row = (int)blockIdx.y, part = (int)blockIdx.x, tid = (int)threadIdx.x, lane = tid & 63, wave = tid >> 6;
-    const int64_t base = (int64_t)row * a.stride;
+    const int tid = (int)threadIdx.x, lane = tid & 63, wave = tid >> 6;
     const Wish wish = row_wish(a, row);
     const Range r = row_range<kScan>(ws, row);
-    if (!(r.top > -__builtin_inff())) return;
     const int way = border_way(a, ws, wish, r);
-    if (way == kNoBorder || way == kBySearch) return;
-    const float *const tops = ws.tops + (int64_t)row * kSlabs * ws.chunks;
-    // whether any slab of a chunk reaches a key, and whether this wave's slab j does
-    auto load_from = [&](int c, float least, float (&l)[4][4]) {
-        bool any = false;
-#pragma unroll
-        for (int j = 0; j < kSlabs; j++) any |= tops[kSlabs * c + j] >= least;
-        if (!any) return false;
-#pragma unroll
-        for (int j = 0; j < 4; j++) {
-            if (tops[kSlabs * c + 4 * j + wave] >= least) {
-                load4(a, base, c * kChunk + j * 1024 + 4 * tid, l[j]);
-            } else {
-#pragma unroll
-                for (int i = 0; i < 4; i++) l[j][i] = -__builtin_inff();
-            }
-        }
-        return true;
-    };
-    if (way == kBySlabs) {
-        const uint32_t floor = ws.plan[row].floor;
-        const float least = floor <= 0x007FFFFFu ? -3.402823466e38f : key_logit(floor);  // (no key lies below -max's)
-        for (int c = ws.first(part); c < ws.first(part + 1); c++) {
-            float l[4][4];
-            if (!load_from(c, least, l)) continue;
-            uint32_t listed = 0;
-#pragma unroll
-            for (int j = 0; j < 16; j++) listed |= logit_key(l[j >> 2][j & 3]) >= floor ? 1u << j : 0u;
-            collect(ws, row, c, l, listed, cn, &place);
-        }
-        return;
+    Plan plan = {kFree, 0, -1, kBins, 0, 0, 0x7FFFFFFF, r.top, row_bins(a, wish, r), 0, 0.0};
+    if (way == kEmpty || way == kBySearch || way == kNoBorder) {
+        plan.mode = way == kEmpty ? kNone : way == kBySearch ? kWhole : kFree;
+        return plan;
     }
-    Plan plan = {kFree, kBins, 0, 0, 0, 0, 0.0};
-    const Scale sc = {r.top, wish.inv_t, a.shift};
-    const Bins bins = row_bins(a, wish, r);
-
+    if (way == kBySlabs) {
+        if (wave == 0) {
+            const uint32_t floor = slab_floor(ws, row, wish.top_k);
+            if (tid == 0) slab_key = floor;
+        }
+        __syncthreads();
+        plan.mode = kAll;
+        plan.floor = slab_key;
+        plan.tokens = (uint32_t)wish.top_k;
+        return plan;
+    }
     // The row's histogram: bins 2 tid, 2 tid + 1, summed over the parts, and its scan.
     uint2 n = {0, 0};
     u64 w0 = 0, w1 = 0;
@@ -715,61 +697,106 @@ __global__ __launch_bounds__(kScan) void sample_border_kernel(SampleArgs a, Samp
         }
     }
     __syncthreads();
-    const bool k_cuts = cut_k < kBins && !(bins.far && cut_k == kBins - 1);  // drops weight
+    const bool k_cuts = cut_k < kBins && !(plan.bins.far && cut_k == kBins - 1);  // drops weight
     plan.tokens = k < all ? k : all;
-    int last;  // bins up to this one are collected, from `from`
-    int from = 0;
     if (k_cuts && before_k + in_k <= (uint32_t)kList) {
         plan.mode = kAll;
-        last = cut_k;
+        plan.last = cut_k;
     } else if (k_cuts) {
         plan.mode = wish.has_p || in_k > (uint32_t)kList ? kWhole : kBorder;
-        plan.bin = from = last = cut_k;
+        plan.bin = plan.from = plan.last = cut_k;
         plan.before = before_k;
     } else if (wish.has_p && before_p + in_p <= (uint32_t)kList) {
         plan.mode = kAll;
-        last = cut_p;
+        plan.last = cut_p;
         plan.tokens = before_p + in_p;
         plan.target = target;
     } else if (wish.has_p) {
         plan.mode = in_p > (uint32_t)kList ? kWhole : kBorder;
-        plan.bin = from = last = cut_p;
+        plan.bin = plan.from = plan.last = cut_p;
         plan.before = before_p;
         plan.before_mass = before_mass;
         plan.target = target;
-    } else {
-        plan.mode = kFree;
-        from = kBins;
-        last = -1;
     }
-    if (part == 0 && tid == 0) ws.plan[row] = plan;
-    if (plan.mode == kWhole) return;
+    return plan;
+}
 
+__global__ __launch_bounds__(kScan) void sample_plan_kernel(SampleArgs a, SampleWs ws) {
+    const int row = (int)blockIdx.x;
+    const Plan plan = make_plan(a, ws, row);
+    if (threadIdx.x == 0) ws.plan[row] = plan;
+}
+
+// PLAN: every workgroup makes its row's plan (part 0 leaves it for the last launch).
+template <bool PLAN>
+__global__ __launch_bounds__(kScan) void sample_collect_kernel(SampleArgs a, SampleWs ws) {
+    __shared__ u64 pm[kScan / 64];
+    __shared__ uint32_t pn[kScan / 64], cn[kScan / 64];
+    __shared__ uint32_t place;
+    const int row = (int)blockIdx.y, part = (int)blockIdx.x, tid = (int)threadIdx.x, wave = tid >> 6;
+    const int64_t base = (int64_t)row * a.stride;
+    Plan plan;
+    if constexpr (PLAN) {
+        plan = make_plan(a, ws, row);
+        if (part == 0 && tid == 0) ws.plan[row] = plan;
+    } else {
+        plan = ws.plan[row];
+    }
+    const Wish wish = row_wish(a, row);
+    if (plan.mode == kNone || plan.mode == kWhole) return;
+    if (plan.mode == kFree && !wish.has_p && wish.top_k >= a.vocab) return;  // (the second launch has its masses)
+    const Scale sc = {plan.top, wish.inv_t, a.shift};
+    const float *const tops = ws.tops + (int64_t)row * kSlabs * ws.chunks;
+    // Tokens that are collected, and others whose mass counts.
+    const bool by_key = plan.floor > 0;
+    const int deepest = plan.last > plan.bin - 1 ? plan.last : plan.mode == kAll ? plan.last : plan.bin - 1;
+    auto concerns = [&](float top) {
+        if (!(top > -__builtin_inff())) return false;
+        return by_key ? logit_key(top) >= plan.floor : plan.bins.of(top) <= deepest;
+    };
     for (int c = ws.first(part); c < ws.first(part + 1); c++) {
-        float l[4][4];
-        load_chunk(a, base, c, l);
-        u64 t = 0;
-        uint32_t kept = 0, listed = 0;  // listed: bit j: token j is collected
+        bool any = plan.mode != kAll;  // (then the chunk's mass is written, if it is 0)
 #pragma unroll
-        for (int j = 0; j < 16; j++) {
-            const float v = l[j >> 2][j & 3];
-            if (!(v > -__builtin_inff())) continue;
-            const int b = bins.of(v);
-            if (b >= from && b <= last) {
-                listed |= 1u << j;
-            } else if (plan.mode != kAll && b < plan.bin) {
-                const double w = sc.weight(v);
-                if (w >= wish.min_p) {
-                    t += sc.fixed(w);
-                    kept++;
-                }
+        for (int j = 0; j < kSlabs; j++) any |= concerns(tops[kSlabs * c + j]);
+        if (!any) continue;
+        float l[4][4];
+#pragma unroll
+        for (int j = 0; j < 4; j++) {
+            if (concerns(tops[kSlabs * c + 4 * j + wave])) {
+                load4(a, base, c * kChunk + j * 1024 + 4 * tid, l[j]);
+            } else {
+#pragma unroll
+                for (int i = 0; i < 4; i++) l[j][i] = -__builtin_inff();
             }
         }
-        if (plan.mode != kAll) {
-            scan_sum(t, kept, pm, pn);
-            if (tid == 0) {
-                ws.chunk_mass[(int64_t)row * ws.chunks + c] = t;
-                ws.chunk_kept[(int64_t)row * ws.chunks + c] = kept;
+        uint32_t listed = 0;  // bit j: token j is collected
+        if (by_key) {
+#pragma unroll
+            for (int j = 0; j < 16; j++) listed |= logit_key(l[j >> 2][j & 3]) >= plan.floor ? 1u << j : 0u;
+        } else {
+            u64 t = 0;
+            uint32_t kept = 0;
+#pragma unroll
+            for (int j = 0; j < 16; j++) {
+                const float v = l[j >> 2][j & 3];
+                if (!(v > -__builtin_inff())) continue;
+                const int b = plan.bins.of(v);
+                if (b >= plan.from && b <= plan.last) {
+                    listed |= 1u << j;
+                } else if (plan.mode != kAll && b < plan.bin) {
+                    const double w = sc.weight(v);
+                    if (w >= wish.min_p) {
+                        t += sc.fixed(w);
+                        kept++;
+                    }
+                }
+            }
+            if (plan.mode != kAll) {
+                scan_sum(t, kept, pm, pn);
+                if (tid == 0) {
+                    ws.chunk_mass[(int64_t)row * ws.chunks + c] = t;
+                    ws.chunk_kept[(int64_t)row * ws.chunks + c] = kept;
+                }
             }
         }
         collect(ws, row, c, l, listed, cn, &place);
@@ -889,8 +916,8 @@ __global__ __launch_bounds__(kThreads) void sample_draw_kernel(SampleArgs a, Sam
     const int row = (int)blockIdx.x, tid = (int)threadIdx.x;
     const int64_t base = (int64_t)row * a.stride;
     const Wish wish = row_wish(a, row);
-    const Range range = row_range<kThreads>(ws, row);
-    if (!(range.top > -__builtin_inff())) {  // no token at all
+    const Plan plan = ws.plan[row];
+    if (plan.mode == kNone) {
         if (tid == 0) {
             a.tokens[row] = -1;
             if (a.probs != nullptr) a.probs[row] = 0.0f;
@@ -898,19 +925,97 @@ __global__ __launch_bounds__(kThreads) void sample_draw_kernel(SampleArgs a, Sam
         }
         return;
     }
-    const Plan plan = ws.plan[row];
     const int n = plan.mode == kAll || plan.mode == kBorder ? (int)ws.listed[row] : 0;
     if (plan.mode == kWhole || n > kList) {
-        whole_row(a, row, wish, range.top, s);
+        whole_row(a, row, wish, plan.top, s);
         return;
     }
-    const Scale sc = {range.top, wish.inv_t, a.shift};
+    const Scale sc = {plan.top, wish.inv_t, a.shift};
     auto write = [&](int token, double w, u64 total, uint32_t kept) {
         a.tokens[row] = token;
         if (a.probs != nullptr) a.probs[row] = (float)(__builtin_ldexp(w, a.shift) / (double)total);
         if (a.kept != nullptr) a.kept[row] = (int32_t)kept;
     };
     auto logit_of = [](u64 v) { return key_logit(0xFFFFFFFFu - (uint32_t)(v >> 32)); };
+
+    if (plan.mode == kAll && n <= 128) {
+        // Few tokens, two a lane of one wave, without a barrier: places by
+        // counting, by key and then by index.
+        if (tid >= 64) return;
+        u64 v[2] = {~0ull, ~0ull};
+#pragma unroll
+        for (int j = 0; j < 2; j++) {
+            if (tid + 64 * j < n) v[j] = ws.list[(int64_t)row * kList + tid + 64 * j];
+            so.list[tid + 64 * j] = v[j];
+        }
+        auto place = [&](int count, bool (&in)[2]) {  // those of `in` below each value, of the first `count`
+            __builtin_amdgcn_wave_barrier();          // (a wave's LDS accesses complete in order)
+            int below[2] = {0, 0};
+            for (int i = 0; i < count; i++) {
+                const u64 o = so.list[i];
+                below[0] += o < v[0] ? 1 : 0;
+                below[1] += o < v[1] ? 1 : 0;
+            }
+            __builtin_amdgcn_wave_barrier();
+#pragma unroll
+            for (int j = 0; j < 2; j++)
+                if (in[j]) so.list[below[j]] = v[j];
+            __builtin_amdgcn_wave_barrier();
+        };
+        // Inclusive sums along 2 lane, 2 lane + 1, and the whole.
+        auto sums = [&](const u64 (&f)[2], u64 (&upto)[2]) {
+            u64 t = f[0] + f[1];
+            for (int d = 1; d < 64; d <<= 1) {
+                const u64 o = __shfl_up(t, d);
+                if (tid >= d) t += o;
+            }
+            upto[0] = t - f[1];
+            upto[1] = t;
+            return (u64)__shfl(t, 63);
+        };
+        bool in[2] = {tid < n, tid + 64 < n};
+        place(n, in);
+        const int k = plan.tokens < (uint32_t)n ? (int)plan.tokens : n;
+        double w[2];
+        u64 f[2], upto[2];
+#pragma unroll
+        for (int j = 0; j < 2; j++) {
+            const int i = 2 * tid + j;
+            v[j] = so.list[i];
+            in[j] = i < k;
+            w[j] = in[j] ? sc.weight(logit_of(v[j])) : 0.0;
+            f[j] = in[j] ? sc.fixed(w[j]) : 0;
+        }
+        u64 total = sums(f, upto);
+        const double target = plan.target > 0.0 ? plan.target : wish.top_p * (double)total;
+        int kept = 0;
+#pragma unroll
+        for (int j = 0; j < 2; j++) {
+            in[j] = in[j] && (!wish.has_p || (double)(upto[j] - f[j]) < target) && w[j] >= wish.min_p;
+            kept += __builtin_popcountll(__ballot(in[j]));
+        }
+        // by index: the kept ones are the first `kept` of the order
+#pragma unroll
+        for (int j = 0; j < 2; j++) {
+            v[j] = (v[j] << 32) | (0xFFFFFFFFu - (uint32_t)(v[j] >> 32));
+            so.list[2 * tid + j] = v[j];
+        }
+        place(kept, in);
+#pragma unroll
+        for (int j = 0; j < 2; j++) {
+            const int i = 2 * tid + j;
+            v[j] = so.list[i];
+            w[j] = i < kept ? sc.weight(key_logit((uint32_t)v[j])) : 0.0;
+            f[j] = i < kept ? sc.fixed(w[j]) : 0;
+        }
+        total = sums(f, upto);
+        const double point = wish.u * (double)total;
+#pragma unroll
+        for (int j = 0; j < 2; j++)
+            if (f[j] > 0 && (double)upto[j] > point && !((double)(upto[j] - f[j]) > point))  // one lane, once
+                write((int)(v[j] >> 32), w[j], total, (uint32_t)kept);
+        return;
+    }
 
     // The collected tokens in order (upper half the inverted key, lower half the
     // index), their weights, and the border among them.
@@ -1053,10 +1158,13 @@ __global__ __launch_bounds__(kThreads) void sample_draw_kernel(SampleArgs a, Sam
     }
 }
 
-// Workgroups a row is dealt to: all rows' together about two a CU.
+// Workgroups a row is dealt to: one a chunk, so that rows whose weights are
+// summed do not wait behind others, up to the 64 whose histograms are read back.
 int row_parts(int rows, int chunks) {
-    const int want = (2 * device_cus() + rows - 1) / rows;
-    return want < chunks ? want : chunks;
+    int want = 2048 / rows;
+    if (want > 64) want = 64;
+    if (want > chunks) want = chunks;
+    return want > 1 ? want : 1;
 }
 
 struct SampleLayout {
@@ -1115,7 +1223,14 @@ hipError_t launch_sample(const void *logits, int logits_type, int rows, int voca
     const dim3 grid((unsigned)o.parts, (unsigned)rows);
     hipLaunchKernelGGL(sample_range_kernel, grid, dim3(kScan), 0, stream, a, ws);
     hipLaunchKernelGGL(sample_bins_kernel, grid, dim3(kScan), 0, stream, a, ws);
-    hipLaunchKernelGGL(sample_border_kernel, grid, dim3(kScan), 0, stream, a, ws);
+    // The plans: few workgroups make their row's each, many read it (a histogram
+    // is up to 0.4 MB to sum, a launch 2 us).
+    if ((int64_t)o.parts * rows <= 128) {
+        hipLaunchKernelGGL(sample_collect_kernel<true>, grid, dim3(kScan), 0, stream, a, ws);
+    } else {
+        hipLaunchKernelGGL(sample_plan_kernel, dim3((unsigned)rows), dim3(kScan), 0, stream, a, ws);
+        hipLaunchKernelGGL(sample_collect_kernel<false>, grid, dim3(kScan), 0, stream, a, ws);
+    }
     hipLaunchKernelGGL(sample_draw_kernel, dim3((unsigned)rows), dim3(kThreads), 0, stream, a, ws);
     return hipGetLastError();
 }

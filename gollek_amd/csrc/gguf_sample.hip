@@ -9,7 +9,7 @@
 // -inf and NaN logits are no tokens.  Every filter keeps a prefix of the order,
 // so the kept set is a threshold (key, index).
 //
-// Masses are 64-bit integers, w in units of 2^-S with V 2^S < 2^62 (2^-44 for a
+// Masses are 64-bit integers, w in units of 2^-S with S <= 50 and V 2^S < 2^62 (2^-44 for a
 // vocabulary of 128k to 256k): integer sums do not depend on the order of the
 // additions, so neither the split of a row over workgroups nor atomics change a
 // token, and their rounding (2^-45 a token) is far below what fp32 sums would
@@ -52,16 +52,43 @@ __device__ __forceinline__ float key_logit(uint32_t k) {
     return __uint_as_float((k >> 31) ? k ^ 0x80000000u : ~k);
 }
 
-// Weights of a row.
+// Weights of a row: w = 2^t, t = (l - m) log2(e) / T, as 2^f of t's fraction by
+// its Taylor series (|f| <= 1/2: the term left out is below 2^-52) times 2^n.
+// (20 instructions in double; the library's exp and its conversion to an integer
+// cost 64 rows of 128256 3 us more.)
 struct Scale {
     float m;       // the largest logit
-    double inv_t;  // 1 / T
-    int shift;     // S
+    double rate;   // log2(e) / T
+    double unit;   // 2^S
+    __device__ __forceinline__ Scale(float top, double inv_t, int shift)
+        : m(top), rate(inv_t * 1.4426950408889634), unit(__builtin_ldexp(1.0, shift)) {}
     __device__ __forceinline__ double weight(float l) const {
         if (m == __builtin_inff()) return l == m ? 1.0 : 0.0;
-        return exp(((double)l - (double)m) * inv_t);
+        const double t = __builtin_fmax(((double)l - (double)m) * rate, -2000.0);
+        const double n = __builtin_rint(t), f = t - n;
+        // ln(2)^k / k!
+        constexpr double kTerm[13] = {1.0,
+                                      6.9314718055994531e-01,
+                                      2.4022650695910072e-01,
+                                      5.5504108664821580e-02,
+                                      9.6181291076284772e-03,
+                                      1.3333558146428443e-03,
+                                      1.5403530393381609e-04,
+                                      1.5252733804059841e-05,
+                                      1.3215486790144309e-06,
+                                      1.0178086009239699e-07,
+                                      7.0549116208011233e-09,
+                                      4.4455382718708114e-10,
+                                      2.5678435993488202e-11};
+        double p = kTerm[12];
+#pragma unroll
+        for (int k = 11; k >= 0; k--) p = __builtin_fma(p, f, kTerm[k]);
+        return __builtin_ldexp(p, (int)n);
     }
-    __device__ __forceinline__ u64 fixed(double w) const { return (u64)(__builtin_ldexp(w, shift) + 0.5); }
+    // w in units of 2^-S, rounded: w 2^S <= 2^50 stands in the low bits of 2^52 more.
+    __device__ __forceinline__ u64 fixed(double w) const {
+        return __builtin_bit_cast(u64, __builtin_fma(w, unit, 0x1p52)) & ((1ull << 52) - 1);
+    }
 };
 
 struct SampleArgs {
@@ -124,12 +151,52 @@ struct RowLds {
     int found;
 };
 
+// Lane operations along a wave by DPP: 1, 2, 4 and 8 lanes up within a row of 16,
+// then the last lanes of rows 0, 2 and of row 1 to the rows behind them.
+template <int CTRL, int ROWS>
+__device__ __forceinline__ uint32_t dpp(uint32_t v, uint32_t other) {
+    return (uint32_t)__builtin_amdgcn_update_dpp((int)other, (int)v, CTRL, ROWS, 0xF, false);
+}
+#define GOLLEK_ALONG(STEP) \
+    STEP(0x111, 0xF) STEP(0x112, 0xF) STEP(0x114, 0xF) STEP(0x118, 0xF) STEP(0x142, 0xA) STEP(0x143, 0xC)
+// Inclusive sums up to each lane.
+__device__ __forceinline__ uint32_t wave_scan(uint32_t v) {
+#define GOLLEK_STEP(C, R) v += dpp<C, R>(v, 0u);
+    GOLLEK_ALONG(GOLLEK_STEP)
+#undef GOLLEK_STEP
+    return v;
+}
+__device__ __forceinline__ u64 wave_scan(u64 v) {
+#define GOLLEK_STEP(C, R) v += ((u64)dpp<C, R>((uint32_t)(v >> 32), 0u) << 32) | dpp<C, R>((uint32_t)v, 0u);
+    GOLLEK_ALONG(GOLLEK_STEP)
+#undef GOLLEK_STEP
+    return v;
+}
+// The largest of the wave's values, in lane 63.
+__device__ __forceinline__ float wave_top(float v) {
+#define GOLLEK_STEP(C, R) v = fmaxf(v, __uint_as_float(dpp<C, R>(__float_as_uint(v), 0xFF800000u)));
+    GOLLEK_ALONG(GOLLEK_STEP)
+#undef GOLLEK_STEP
+    return v;
+}
+#undef GOLLEK_ALONG
+template <class V>
+__device__ __forceinline__ V last_lane(V v) {
+    if constexpr (sizeof(V) == 8) {
+        const u64 b = __builtin_bit_cast(u64, v);
+        return __builtin_bit_cast(V, ((u64)(uint32_t)__builtin_amdgcn_readlane((int)(b >> 32), 63) << 32) |
+                                         (uint32_t)__builtin_amdgcn_readlane((int)(uint32_t)b, 63));
+    } else {
+        return __builtin_bit_cast(V, __builtin_amdgcn_readlane(__builtin_bit_cast(int, v), 63));
+    }
+}
+
 // The sum over the workgroup, in every thread.
 template <class V>
 __device__ V block_sum(V v, RowLds &s) {
-    for (int m = 1; m < 64; m <<= 1) v += __shfl_xor(v, m);
+    v = wave_scan(v);
     __syncthreads();
-    if ((threadIdx.x & 63) == 0) s.part[threadIdx.x >> 6] = (u64)v;
+    if ((threadIdx.x & 63) == 63) s.part[threadIdx.x >> 6] = (u64)v;
     __syncthreads();
     V t = 0;
     for (int w = 0; w < kWaves; w++) t += (V)s.part[w];
@@ -226,7 +293,7 @@ __device__ Border select(const SampleArgs &a, int64_t base, const Scale &sc, Bor
 __device__ void whole_row(const SampleArgs &a, int row, const Wish &wish, float m, RowLds &s) {
     const int tid = (int)threadIdx.x;
     const int64_t base = (int64_t)row * a.stride;
-    const Scale sc = {m, wish.inv_t, a.shift};
+    const Scale sc(m, wish.inv_t, a.shift);
 
     // Mass and number of the tokens within a border that min_p keeps.
     auto sum = [&](Border in, double min_p, u64 &mass, uint32_t &n) {
@@ -272,11 +339,7 @@ __device__ void whole_row(const SampleArgs &a, int row, const Wish &wish, float 
                 if (w >= wish.min_p) f = sc.fixed(w);
             }
         }
-        u64 cum = f;  // inclusive over the wave
-        for (int d = 1; d < 64; d <<= 1) {
-            const u64 o = __shfl_up(cum, d);
-            if ((tid & 63) >= d) cum += o;
-        }
+        u64 cum = wave_scan(f);
         __syncthreads();
         if ((tid & 63) == 63) s.part[tid >> 6] = cum;
         __syncthreads();
@@ -364,21 +427,6 @@ __device__ __forceinline__ void load_chunk(const SampleArgs &a, int64_t base, in
     for (int j = 0; j < 4; j++) load4(a, base, c * kChunk + j * 1024 + 4 * (int)threadIdx.x, l[j]);
 }
 
-template <int CTRL, int ROWS>
-__device__ __forceinline__ float dpp_max(float v) {
-    const int low = __float_as_int(-__builtin_inff());
-    return fmaxf(v, __int_as_float(__builtin_amdgcn_update_dpp(low, __float_as_int(v), CTRL, ROWS, 0xF, false)));
-}
-// The largest of the wave's values, in lane 63.
-__device__ __forceinline__ float wave_top(float v) {
-    v = dpp_max<0x111, 0xF>(v);  // row_shr 1, 2, 4, 8
-    v = dpp_max<0x112, 0xF>(v);
-    v = dpp_max<0x114, 0xF>(v);
-    v = dpp_max<0x118, 0xF>(v);
-    v = dpp_max<0x142, 0xA>(v);  // row_bcast 15, 31
-    return dpp_max<0x143, 0xC>(v);
-}
-
 __global__ __launch_bounds__(kScan) void sample_range_kernel(SampleArgs a, SampleWs ws) {
     const int row = (int)blockIdx.y, tid = (int)threadIdx.x, lane = tid & 63, wave = tid >> 6;
     const int64_t base = (int64_t)row * a.stride;
@@ -417,12 +465,8 @@ __device__ __forceinline__ Range row_range(const SampleWs &ws, int row) {
     }
     for (int i = (int)threadIdx.x; i < 4 * ws.chunks; i += THREADS)
         r.least = fminf(r.least, ws.least[(int64_t)row * 4 * ws.chunks + i]);
-    for (int d = 1; d < 64; d <<= 1) {
-        r.top = fmaxf(r.top, __shfl_xor(r.top, d));
-        r.least = fminf(r.least, __shfl_xor(r.least, d));
-        r.slabs += __shfl_xor(r.slabs, d);
-    }
-    if ((threadIdx.x & 63) == 0) part[threadIdx.x >> 6] = r;
+    r = {wave_top(r.top), -wave_top(-r.least), (int)wave_scan((uint32_t)r.slabs)};
+    if ((threadIdx.x & 63) == 63) part[threadIdx.x >> 6] = r;
     __syncthreads();
     r = part[0];
     for (int w = 1; w < THREADS / 64; w++)
@@ -453,12 +497,10 @@ __device__ __forceinline__ int border_way(const SampleArgs &a, const SampleWs &w
 
 // Sums over the workgroup of kScan threads, in every thread.
 __device__ __forceinline__ void scan_sum(u64 &mass, uint32_t &n, u64 *pm, uint32_t *pn) {
-    for (int d = 1; d < 64; d <<= 1) {
-        mass += __shfl_xor(mass, d);
-        n += __shfl_xor(n, d);
-    }
+    mass = wave_scan(mass);
+    n = wave_scan(n);
     __syncthreads();
-    if ((threadIdx.x & 63) == 0) {
+    if ((threadIdx.x & 63) == 63) {
         pm[threadIdx.x >> 6] = mass;
         pn[threadIdx.x >> 6] = n;
     }
@@ -471,37 +513,40 @@ __device__ __forceinline__ void scan_sum(u64 &mass, uint32_t &n, u64 *pm, uint32
     }
 }
 
-template <int CTRL, int ROWS>
-__device__ __forceinline__ int dpp_add(int v) {
-    return v + __builtin_amdgcn_update_dpp(0, v, CTRL, ROWS, 0xF, false);
-}
-// The wave's sum, in every lane.
-__device__ __forceinline__ int wave_total(int v) {
-    v = dpp_add<0x111, 0xF>(v);
-    v = dpp_add<0x112, 0xF>(v);
-    v = dpp_add<0x114, 0xF>(v);
-    v = dpp_add<0x118, 0xF>(v);
-    v = dpp_add<0x142, 0xA>(v);
-    v = dpp_add<0x143, 0xC>(v);
-    return __builtin_amdgcn_readlane(v, 63);
-}
-
 // The upper half of the k-th largest slab maximum's key (k slabs at least hold a
-// token that large): its bits one by one, by one wave.
-__device__ __forceinline__ uint32_t slab_floor(const SampleWs &ws, int row, int k) {
-    constexpr int kPer = kSlabsMax / 64;
-    const int lane = (int)threadIdx.x & 63, slabs = kSlabs * ws.chunks;
+// token that large), by a workgroup of kScan threads: the bin of its first byte,
+// then of its second (bit by bit, in one wave, it took 2 us).
+__device__ __forceinline__ uint32_t slab_floor(const SampleWs &ws, int row, uint32_t k) {
+    static_assert(kScan == 256, "a thread a bin");
+    __shared__ uint32_t count[256], upto[kScan / 64], digit, before;
+    constexpr int kPer = kSlabsMax / kScan;
+    const int tid = (int)threadIdx.x, lane = tid & 63, wave = tid >> 6, slabs = kSlabs * ws.chunks;
     uint32_t key[kPer];
 #pragma unroll
     for (int j = 0; j < kPer; j++)
-        key[j] = lane + 64 * j < slabs ? logit_key(ws.tops[(int64_t)row * slabs + lane + 64 * j]) : 0u;
+        key[j] = tid + kScan * j < slabs ? logit_key(ws.tops[(int64_t)row * slabs + tid + kScan * j]) : 0u;
     uint32_t floor = 0;
-    for (int bit = 31; bit >= 16; bit--) {
-        const uint32_t next = floor | (1u << bit);
-        int n = 0;
 #pragma unroll
-        for (int j = 0; j < kPer; j++) n += key[j] >= next ? 1 : 0;
-        if (wave_total(n) >= k) floor = next;
+    for (int at = 24; at >= 16; at -= 8) {
+        __syncthreads();
+        count[tid] = 0;
+        __syncthreads();
+#pragma unroll
+        for (int j = 0; j < kPer; j++)
+            if (key[j] > 0 && (at == 24 || key[j] >> 24 == floor >> 24)) atomicAdd(&count[(key[j] >> at) & 255u], 1u);  // LDS
+        __syncthreads();
+        const uint32_t mine = count[255 - tid];  // from the top
+        uint32_t end = wave_scan(mine);
+        if (lane == 63) upto[wave] = end;
+        __syncthreads();
+        for (int w = 0; w < wave; w++) end += upto[w];
+        if (end >= k && end - mine < k) {  // one thread
+            digit = (uint32_t)(255 - tid);
+            before = end - mine;
+        }
+        __syncthreads();
+        floor |= digit << at;
+        k -= before;
     }
     return floor > 0u ? floor : 1u;  // (0 is no token)
 }
@@ -517,7 +562,7 @@ __global__ __launch_bounds__(kScan) void sample_bins_kernel(SampleArgs a, Sample
     const Range r = row_range<kScan>(ws, row);
     const int way = border_way(a, ws, wish, r);
     if (way == kBySlabs || way == kBySearch || way == kEmpty) return;  // (nothing to count)
-    const Scale sc = {r.top, wish.inv_t, a.shift};
+    const Scale sc(r.top, wish.inv_t, a.shift);
     const Bins bins = row_bins(a, wish, r);
     const bool border = way == kByBins;
     if (border) {
@@ -573,11 +618,7 @@ __device__ __forceinline__ void collect(const SampleWs &ws, int row, int c, cons
                                         uint32_t *counts, uint32_t *place) {
     const int tid = (int)threadIdx.x, lane = tid & 63, wave = tid >> 6;
     const uint32_t mine = (uint32_t)__builtin_popcount(listed);
-    uint32_t upto = mine;  // places: this thread's after those of the threads before
-    for (int d = 1; d < 64; d <<= 1) {
-        const uint32_t o = __shfl_up(upto, d);
-        if (lane >= d) upto += o;
-    }
+    uint32_t upto = wave_scan(mine);  // places: this thread's after those of the threads before
     __syncthreads();
     if (lane == 63) counts[wave] = upto;
     __syncthreads();
@@ -606,7 +647,7 @@ __device__ __forceinline__ Plan make_plan(const SampleArgs &a, const SampleWs &w
     __shared__ u64 cm[kScan / 64];
     __shared__ uint32_t cn[kScan / 64];
     __shared__ int cut_k, cut_p;
-    __shared__ uint32_t before_k, in_k, before_p, in_p, slab_key;
+    __shared__ uint32_t before_k, in_k, before_p, in_p;
     __shared__ u64 before_mass;
     const int tid = (int)threadIdx.x, lane = tid & 63, wave = tid >> 6;
     const Wish wish = row_wish(a, row);
@@ -618,13 +659,8 @@ __device__ __forceinline__ Plan make_plan(const SampleArgs &a, const SampleWs &w
         return plan;
     }
     if (way == kBySlabs) {
-        if (wave == 0) {
-            const uint32_t floor = slab_floor(ws, row, wish.top_k);
-            if (tid == 0) slab_key = floor;
-        }
-        __syncthreads();
         plan.mode = kAll;
-        plan.floor = slab_key;
+        plan.floor = slab_floor(ws, row, (uint32_t)wish.top_k);
         plan.tokens = (uint32_t)wish.top_k;
         return plan;
     }
@@ -646,16 +682,8 @@ __device__ __forceinline__ Plan make_plan(const SampleArgs &a, const SampleWs &w
             w1 += v.y;
         }
     }
-    uint32_t cum = n.x + n.y;  // inclusive
-    u64 cmass = w0 + w1;
-    for (int d = 1; d < 64; d <<= 1) {
-        const uint32_t o = __shfl_up(cum, d);
-        const u64 q = __shfl_up(cmass, d);
-        if (lane >= d) {
-            cum += o;
-            cmass += q;
-        }
-    }
+    uint32_t cum = wave_scan(n.x + n.y);  // inclusive
+    u64 cmass = wave_scan(w0 + w1);
     if (lane == 63) {
         cn[wave] = cum;
         cm[wave] = cmass;
@@ -745,7 +773,7 @@ __global__ __launch_bounds__(kScan) void sample_collect_kernel(SampleArgs a, Sam
     const Wish wish = row_wish(a, row);
     if (plan.mode == kNone || plan.mode == kWhole) return;
     if (plan.mode == kFree && !wish.has_p && wish.top_k >= a.vocab) return;  // (the second launch has its masses)
-    const Scale sc = {plan.top, wish.inv_t, a.shift};
+    const Scale sc(plan.top, wish.inv_t, a.shift);
     const float *const tops = ws.tops + (int64_t)row * kSlabs * ws.chunks;
     // Tokens that are collected, and others whose mass counts.
     const bool by_key = plan.floor > 0;
@@ -806,10 +834,7 @@ __global__ __launch_bounds__(kScan) void sample_collect_kernel(SampleArgs a, Sam
 // Inclusive scan of a value per thread over the workgroup; `total` its end.
 __device__ __forceinline__ u64 block_scan(u64 v, u64 &total, RowLds &s) {
     const int lane = (int)threadIdx.x & 63, wave = (int)threadIdx.x >> 6;
-    for (int d = 1; d < 64; d <<= 1) {
-        const u64 o = __shfl_up(v, d);
-        if (lane >= d) v += o;
-    }
+    v = wave_scan(v);
     __syncthreads();
     if (lane == 63) s.part[wave] = v;
     __syncthreads();
@@ -830,7 +855,7 @@ struct SortLds {
 // Sorts the first n (up to kList) of s.list, whose values differ, upwards.
 // bucket(v): a number in [0, kThreads) that does not fall as v rises.  Every
 // value goes to its bucket and finds its place there by counting the smaller
-// ones; with more than 64 values in a bucket (equal logits) a bitonic sort.
+// ones; with more than 128 values in a bucket (equal logits) a bitonic sort.
 template <class BUCKET>
 __device__ void sort_list(SortLds &s, RowLds &rl, int n, BUCKET &&bucket) {
     const int tid = (int)threadIdx.x;
@@ -865,7 +890,7 @@ __device__ void sort_list(SortLds &s, RowLds &rl, int n, BUCKET &&bucket) {
     if ((tid & 63) == 0) atomicMax(&s.most, most);  // LDS
     u64 total;
     const uint32_t end = (uint32_t)block_scan(mine, total, rl);
-    if (s.most <= 64) {  // (block_scan's barriers stand between)
+    if (s.most <= 128) {  // (block_scan's barriers stand between)
         __syncthreads();
         s.slot[tid] = end - mine;
         __syncthreads();
@@ -930,7 +955,7 @@ __global__ __launch_bounds__(kThreads) void sample_draw_kernel(SampleArgs a, Sam
         whole_row(a, row, wish, plan.top, s);
         return;
     }
-    const Scale sc = {plan.top, wish.inv_t, a.shift};
+    const Scale sc(plan.top, wish.inv_t, a.shift);
     auto write = [&](int token, double w, u64 total, uint32_t kept) {
         a.tokens[row] = token;
         if (a.probs != nullptr) a.probs[row] = (float)(__builtin_ldexp(w, a.shift) / (double)total);
@@ -964,14 +989,10 @@ __global__ __launch_bounds__(kThreads) void sample_draw_kernel(SampleArgs a, Sam
         };
         // Inclusive sums along 2 lane, 2 lane + 1, and the whole.
         auto sums = [&](const u64 (&f)[2], u64 (&upto)[2]) {
-            u64 t = f[0] + f[1];
-            for (int d = 1; d < 64; d <<= 1) {
-                const u64 o = __shfl_up(t, d);
-                if (tid >= d) t += o;
-            }
+            const u64 t = wave_scan(f[0] + f[1]);
             upto[0] = t - f[1];
             upto[1] = t;
-            return (u64)__shfl(t, 63);
+            return last_lane(t);
         };
         bool in[2] = {tid < n, tid + 64 < n};
         place(n, in);
@@ -1046,9 +1067,10 @@ __global__ __launch_bounds__(kThreads) void sample_draw_kernel(SampleArgs a, Sam
             high = fmaxf(high, span[kWaves + w]);
         }
         const float wide = high - low;  // (infinite or 0: one bucket)
-        const float inv = wide > 0.0f && wide < 0x1p126f ? fminf((float)(kThreads - 1) / wide, 0x1p100f) : 0.0f;
-        sort_list(so, s, n, [&](u64 v) {
-            return inv > 0.0f ? (int)fminf((high - logit_of(v)) * inv, (float)(kThreads - 1)) : 0;
+        const float inv = wide > 0.0f && wide < 0x1p126f ? fminf(1.0f / wide, 0x1p100f) : 0.0f;
+        sort_list(so, s, n, [&](u64 v) {  // (finer at the lower end, where tokens are denser)
+            const float x = inv > 0.0f ? fminf((high - logit_of(v)) * inv, 1.0f) : 0.0f;
+            return (int)(x * (0.4f + 0.6f * x) * (float)(kThreads - 1));
         });
         const int k = plan.mode == kAll && plan.tokens < (uint32_t)n ? (int)plan.tokens : n;
         u64 sum = 0, total;
@@ -1206,7 +1228,8 @@ hipError_t launch_sample(const void *logits, int logits_type, int rows, int voca
     while ((1ll << bits) <= vocab) bits++;
     const uintptr_t size = logits_type == kF32 ? 4 : 2;
     const bool vec4 = ((reinterpret_cast<uintptr_t>(logits) | (uintptr_t)stride * size) & (4 * size - 1)) == 0;
-    const SampleArgs a = {logits, stride, logits_type, vocab,  62 - bits, vec4, temperature,
+    const int shift = 62 - bits < 50 ? 62 - bits : 50;
+    const SampleArgs a = {logits, stride, logits_type, vocab,  shift, vec4, temperature,
                           top_p,  min_p,  u,           top_k,  tokens,    kept, probs};
     const SampleLayout o = sample_layout(rows, vocab);
     const SampleWs ws = {reinterpret_cast<float *>(workspace + o.tops),

@@ -106,6 +106,7 @@ constexpr int kThreads = 1024, kWaves = kThreads / 64;  // of the last launch
 constexpr int kScan = 256;                              // of the others
 constexpr int kChunk = 4096, kBins = 512, kList = 4096;
 constexpr int kSlabs = 16;  // of a chunk
+constexpr int kLine = 32;   // words between rows' counters
 constexpr int kSlabTopK = 2048, kSlabsMax = 1024;  // of the slab bound
 
 struct Border {  // kept: key > this one, or the same key at an index up to this one
@@ -397,7 +398,7 @@ struct SampleWs {
     Plan *plan;           // [rows]
     uint32_t *count;      // [rows][parts][kBins]
     uint32_t *chunk_kept; // [rows][chunks]
-    uint32_t *listed;     // [rows]
+    uint32_t *listed;     // [rows] kLine apart: rows' counters share no cache line
     int chunks, parts;
     // chunks of a part
     __device__ __forceinline__ int first(int part) const { return (int)((int64_t)part * chunks / parts); }
@@ -430,7 +431,7 @@ __device__ __forceinline__ void load_chunk(const SampleArgs &a, int64_t base, in
 __global__ __launch_bounds__(kScan) void sample_range_kernel(SampleArgs a, SampleWs ws) {
     const int row = (int)blockIdx.y, tid = (int)threadIdx.x, lane = tid & 63, wave = tid >> 6;
     const int64_t base = (int64_t)row * a.stride;
-    if (blockIdx.x == 0 && tid == 0) ws.listed[row] = 0;
+    if (blockIdx.x == 0 && tid == 0) ws.listed[kLine * row] = 0;
     for (int c = ws.first((int)blockIdx.x); c < ws.first((int)blockIdx.x + 1); c++) {
         float l[4][4];
         load_chunk(a, base, c, l);
@@ -559,6 +560,10 @@ __global__ __launch_bounds__(kScan) void sample_bins_kernel(SampleArgs a, Sample
     const int row = (int)blockIdx.y, part = (int)blockIdx.x, tid = (int)threadIdx.x;
     const int64_t base = (int64_t)row * a.stride;
     const Wish wish = row_wish(a, row);
+    // Rows that cannot go by slabs have their first chunk on the way meanwhile.
+    const bool early = wish.top_k > kSlabTopK;
+    float l[4][4];
+    if (early) load_chunk(a, base, ws.first(part), l);
     const Range r = row_range<kScan>(ws, row);
     const int way = border_way(a, ws, wish, r);
     if (way == kBySlabs || way == kBySearch || way == kEmpty) return;  // (nothing to count)
@@ -573,8 +578,7 @@ __global__ __launch_bounds__(kScan) void sample_bins_kernel(SampleArgs a, Sample
         __syncthreads();
     }
     for (int c = ws.first(part); c < ws.first(part + 1); c++) {
-        float l[4][4];
-        load_chunk(a, base, c, l);
+        if (!early || c > ws.first(part)) load_chunk(a, base, c, l);
         if (border) {
 #pragma unroll
             for (int j = 0; j < 16; j++) {
@@ -628,7 +632,7 @@ __device__ __forceinline__ void collect(const SampleWs &ws, int row, int c, cons
         sum += counts[w];
     }
     if (sum == 0) return;  // (the same in every thread)
-    if (tid == 0) *place = atomicAdd(ws.listed + row, sum);
+    if (tid == 0) *place = atomicAdd(ws.listed + kLine * row, sum);
     __syncthreads();
     uint32_t p = *place + upto - mine;
 #pragma unroll
@@ -668,14 +672,14 @@ __device__ __forceinline__ Plan make_plan(const SampleArgs &a, const SampleWs &w
     uint2 n = {0, 0};
     u64 w0 = 0, w1 = 0;
     const int64_t at = (int64_t)row * ws.parts * kBins + 2 * tid;
-#pragma unroll 8
+#pragma unroll 16
     for (int p = 0; p < ws.parts; p++) {
         const uint2 v = *reinterpret_cast<const uint2 *>(ws.count + at + p * kBins);
         n.x += v.x;
         n.y += v.y;
     }
     if (wish.has_p) {
-#pragma unroll 8
+#pragma unroll 16
         for (int p = 0; p < ws.parts; p++) {
             const ulonglong2 v = *reinterpret_cast<const ulonglong2 *>(ws.mass + at + p * kBins);
             w0 += v.x;
@@ -950,7 +954,7 @@ __global__ __launch_bounds__(kThreads) void sample_draw_kernel(SampleArgs a, Sam
         }
         return;
     }
-    const int n = plan.mode == kAll || plan.mode == kBorder ? (int)ws.listed[row] : 0;
+    const int n = plan.mode == kAll || plan.mode == kBorder ? (int)ws.listed[kLine * row] : 0;
     if (plan.mode == kWhole || n > kList) {
         whole_row(a, row, wish, plan.top, s);
         return;
@@ -1211,7 +1215,7 @@ SampleLayout sample_layout(int rows, int vocab) {
     o.plan = take(r * sizeof(Plan));
     o.count = take(rb * sizeof(uint32_t));
     o.chunk_kept = take(rc * sizeof(uint32_t));
-    o.listed = take(r * sizeof(uint32_t));
+    o.listed = take(r * kLine * sizeof(uint32_t));
     return o;
 }
 

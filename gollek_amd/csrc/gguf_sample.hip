@@ -18,18 +18,18 @@
 // A row is cut into slabs of 256 tokens, sixteen of them a chunk, and the chunks
 // dealt to workgroups; four launches:
 //   1 the largest logit of every slab (reads the row);
-//   2 a top_k of up to as many as the slabs that hold a token, and 2048: the
-//     top_k-th largest slab maximum, below which no kept token lies (reads no
-//     logits); other rows with a filter: a histogram (tokens, and mass for
-//     top_p) over 512 bins of l, linear from the largest logit down to where
-//     weights round to 0 (or to the least logit); rows without: every chunk's
-//     kept mass;
-//   3 the tokens that may be kept are collected, from the slabs that hold any:
-//     those above the slab bound, or those down to the bin in which the filter's
-//     border falls; where that is more than 4096, the border's bin alone and the
-//     chunks' mass above it;
+//   2 rows with a filter: a histogram (tokens, and mass for top_p) over 512 bins
+//     of l, linear from the largest logit down to where weights round to 0 (or to
+//     the least logit); rows without: every chunk's kept mass;
+//   3 from the histogram, the bin in which the filter's border falls; the tokens
+//     of the bins down to it are collected, or, where that is more than 4096,
+//     those of the border's bin alone and the chunks' mass above it;
 //   4 one workgroup per row: the collected tokens sorted, the border in them, the
 //     draw: the chunk that the random number falls into, then the token.
+// A top_k of up to 64, and to as many as the slabs that hold a token, goes without 2 and 3:
+// its tokens lie above the top_k-th largest slab maximum, in those slabs alone,
+// which the last launch reads itself.  (Every row passes every launch, since the
+// settings are on the device; with many rows 3 is two, a plan and the collection.)
 // A row whose border bin holds more than 4096 tokens (equal logits, a
 // temperature of 30), or whose top_p border depends on a top_k border that far
 // down, is computed by the last workgroup alone, digit by digit over the row.
@@ -105,9 +105,12 @@ struct SampleArgs {
 constexpr int kThreads = 1024, kWaves = kThreads / 64;  // of the last launch
 constexpr int kScan = 256;                              // of the others
 constexpr int kChunk = 4096, kBins = 512, kList = 4096;
-constexpr int kSlabs = 16;  // of a chunk
+constexpr int kChunkSlabs = 16;
 constexpr int kLine = 32;   // words between rows' counters
-constexpr int kSlabTopK = 2048, kSlabsMax = 1024;  // of the slab bound
+// The largest top_k that goes by slabs, in one workgroup (64 rows of 128256: 40
+// 30 us, 37 by bins; a batch with rows of 200 65 against 58), the slabs it sorts,
+// and the largest whose rows need no masses of bins.
+constexpr int kSlabTopK = 64, kSlabsMax = 1024, kListTopK = 2048;
 
 struct Border {  // kept: key > this one, or the same key at an index up to this one
     uint32_t key;
@@ -373,7 +376,6 @@ struct Plan {
     int mode;          // see kNone ..
     int from, last;    // bins that are collected (none: 0, -1)
     int bin;           // the border's bin, kBins: none
-    uint32_t floor;    // not 0: keys from here on are collected instead
     uint32_t before;   // tokens in the bins above the border's
     uint32_t tokens;   // of the row that top_k leaves
     float top;         // the row's largest logit
@@ -387,6 +389,7 @@ enum : int {
     kFree,    // no border with weight below it: every token, by chunks
     kBorder,  // the collected tokens are the border's bin
     kAll,     // every token that may be kept is collected
+    kSlabs,   // the same, by the last workgroup itself, from the slabs that top_k reaches
 };
 
 struct SampleWs {
@@ -440,7 +443,7 @@ __global__ __launch_bounds__(kScan) void sample_range_kernel(SampleArgs a, Sampl
 #pragma unroll
         for (int j = 0; j < 4; j++) {
             const float top = wave_top(fmaxf(fmaxf(l[j][0], l[j][1]), fmaxf(l[j][2], l[j][3])));
-            if (lane == 63) ws.tops[kSlabs * at + 4 * j + wave] = top;
+            if (lane == 63) ws.tops[kChunkSlabs * at + 4 * j + wave] = top;
 #pragma unroll
             for (int i = 0; i < 4; i++)
                 if (l[j][i] > -__builtin_inff()) low = fmaxf(low, -l[j][i]);
@@ -459,8 +462,8 @@ template <int THREADS>
 __device__ __forceinline__ Range row_range(const SampleWs &ws, int row) {
     __shared__ Range part[THREADS / 64];
     Range r = {-__builtin_inff(), __builtin_inff(), 0};
-    for (int i = (int)threadIdx.x; i < kSlabs * ws.chunks; i += THREADS) {
-        const float t = ws.tops[(int64_t)row * kSlabs * ws.chunks + i];
+    for (int i = (int)threadIdx.x; i < kChunkSlabs * ws.chunks; i += THREADS) {
+        const float t = ws.tops[(int64_t)row * kChunkSlabs * ws.chunks + i];
         r.top = fmaxf(r.top, t);
         r.slabs += t > -__builtin_inff() ? 1 : 0;
     }
@@ -486,12 +489,15 @@ __device__ __forceinline__ Bins row_bins(const SampleArgs &a, const Wish &w, con
     return {r.top, range > 0.0f ? fminf((float)(kBins - 1) / range, 0x1p100f) : 0.0f, far};
 }
 
+// Whether the masses of the bins are needed: not where top_k bounds the list.
+__device__ __forceinline__ bool needs_mass(const Wish &w) { return w.has_p && w.top_k > kListTopK; }
+
 // How a row's border is looked for.
 enum : int { kEmpty, kNoBorder, kBySlabs, kByBins, kBySearch };
 __device__ __forceinline__ int border_way(const SampleArgs &a, const SampleWs &ws, const Wish &w, const Range &r) {
     if (!(r.top > -__builtin_inff())) return kEmpty;
     if (!w.has_p && w.top_k >= a.vocab) return kNoBorder;
-    if (w.top_k <= r.slabs && w.top_k <= kSlabTopK && kSlabs * ws.chunks <= kSlabsMax) return kBySlabs;
+    if (w.top_k <= r.slabs && w.top_k <= kSlabTopK && kChunkSlabs * ws.chunks <= kSlabsMax) return kBySlabs;
     // bins do not count tokens of weight 0 that a tiny min_p keeps
     return w.min_p > 0.0 && w.min_p < __builtin_ldexp(1.0, 2 - a.shift) ? kBySearch : kByBins;
 }
@@ -514,44 +520,6 @@ __device__ __forceinline__ void scan_sum(u64 &mass, uint32_t &n, u64 *pm, uint32
     }
 }
 
-// The upper half of the k-th largest slab maximum's key (k slabs at least hold a
-// token that large), by a workgroup of kScan threads: the bin of its first byte,
-// then of its second (bit by bit, in one wave, it took 2 us).
-__device__ __forceinline__ uint32_t slab_floor(const SampleWs &ws, int row, uint32_t k) {
-    static_assert(kScan == 256, "a thread a bin");
-    __shared__ uint32_t count[256], upto[kScan / 64], digit, before;
-    constexpr int kPer = kSlabsMax / kScan;
-    const int tid = (int)threadIdx.x, lane = tid & 63, wave = tid >> 6, slabs = kSlabs * ws.chunks;
-    uint32_t key[kPer];
-#pragma unroll
-    for (int j = 0; j < kPer; j++)
-        key[j] = tid + kScan * j < slabs ? logit_key(ws.tops[(int64_t)row * slabs + tid + kScan * j]) : 0u;
-    uint32_t floor = 0;
-#pragma unroll
-    for (int at = 24; at >= 16; at -= 8) {
-        __syncthreads();
-        count[tid] = 0;
-        __syncthreads();
-#pragma unroll
-        for (int j = 0; j < kPer; j++)
-            if (key[j] > 0 && (at == 24 || key[j] >> 24 == floor >> 24)) atomicAdd(&count[(key[j] >> at) & 255u], 1u);  // LDS
-        __syncthreads();
-        const uint32_t mine = count[255 - tid];  // from the top
-        uint32_t end = wave_scan(mine);
-        if (lane == 63) upto[wave] = end;
-        __syncthreads();
-        for (int w = 0; w < wave; w++) end += upto[w];
-        if (end >= k && end - mine < k) {  // one thread
-            digit = (uint32_t)(255 - tid);
-            before = end - mine;
-        }
-        __syncthreads();
-        floor |= digit << at;
-        k -= before;
-    }
-    return floor > 0u ? floor : 1u;  // (0 is no token)
-}
-
 __global__ __launch_bounds__(kScan) void sample_bins_kernel(SampleArgs a, SampleWs ws) {
     __shared__ u64 mass[kBins];
     __shared__ uint32_t count[kBins];
@@ -569,7 +537,7 @@ __global__ __launch_bounds__(kScan) void sample_bins_kernel(SampleArgs a, Sample
     if (way == kBySlabs || way == kBySearch || way == kEmpty) return;  // (nothing to count)
     const Scale sc(r.top, wish.inv_t, a.shift);
     const Bins bins = row_bins(a, wish, r);
-    const bool border = way == kByBins;
+    const bool border = way == kByBins, weigh = needs_mass(wish);
     if (border) {
         for (int b = tid; b < kBins; b += kScan) {
             mass[b] = 0;
@@ -586,7 +554,7 @@ __global__ __launch_bounds__(kScan) void sample_bins_kernel(SampleArgs a, Sample
                 if (!(v > -__builtin_inff())) continue;
                 const int b = bins.of(v);
                 atomicAdd(&count[b], 1u);  // LDS
-                if (wish.has_p && !(bins.far && b == kBins - 1)) atomicAdd(&mass[b], sc.fixed(sc.weight(v)));
+                if (weigh && !(bins.far && b == kBins - 1)) atomicAdd(&mass[b], sc.fixed(sc.weight(v)));
             }
         } else {
             u64 t = 0;
@@ -612,7 +580,7 @@ __global__ __launch_bounds__(kScan) void sample_bins_kernel(SampleArgs a, Sample
     const int64_t at = ((int64_t)row * ws.parts + part) * kBins;
     for (int b = tid; b < kBins; b += kScan) {
         ws.count[at + b] = count[b];
-        if (wish.has_p) ws.mass[at + b] = mass[b];
+        if (weigh) ws.mass[at + b] = mass[b];
     }
 }
 
@@ -657,14 +625,13 @@ __device__ __forceinline__ Plan make_plan(const SampleArgs &a, const SampleWs &w
     const Wish wish = row_wish(a, row);
     const Range r = row_range<kScan>(ws, row);
     const int way = border_way(a, ws, wish, r);
-    Plan plan = {kFree, 0, -1, kBins, 0, 0, 0x7FFFFFFF, r.top, row_bins(a, wish, r), 0, 0.0};
+    Plan plan = {kFree, 0, -1, kBins, 0, 0x7FFFFFFF, r.top, row_bins(a, wish, r), 0, 0.0};
     if (way == kEmpty || way == kBySearch || way == kNoBorder) {
         plan.mode = way == kEmpty ? kNone : way == kBySearch ? kWhole : kFree;
         return plan;
     }
     if (way == kBySlabs) {
-        plan.mode = kAll;
-        plan.floor = slab_floor(ws, row, (uint32_t)wish.top_k);
+        plan.mode = kSlabs;
         plan.tokens = (uint32_t)wish.top_k;
         return plan;
     }
@@ -678,7 +645,7 @@ __device__ __forceinline__ Plan make_plan(const SampleArgs &a, const SampleWs &w
         n.x += v.x;
         n.y += v.y;
     }
-    if (wish.has_p) {
+    if (needs_mass(wish)) {
 #pragma unroll 16
         for (int p = 0; p < ws.parts; p++) {
             const ulonglong2 v = *reinterpret_cast<const ulonglong2 *>(ws.mass + at + p * kBins);
@@ -720,7 +687,7 @@ __device__ __forceinline__ Plan make_plan(const SampleArgs &a, const SampleWs &w
                 before_k = c[j];
                 in_k = c[j + 1] - c[j];
             }
-            if (wish.has_p && (double)q[j] < target && !((double)q[j + 1] < target)) {
+            if (needs_mass(wish) && (double)q[j] < target && !((double)q[j + 1] < target)) {
                 cut_p = 2 * tid + j;
                 before_p = c[j];
                 in_p = c[j + 1] - c[j];
@@ -734,6 +701,11 @@ __device__ __forceinline__ Plan make_plan(const SampleArgs &a, const SampleWs &w
     if (k_cuts && before_k + in_k <= (uint32_t)kList) {
         plan.mode = kAll;
         plan.last = cut_k;
+    } else if (wish.has_p && !needs_mass(wish) && !k_cuts) {
+        // fewer tokens than top_k, all of them or all that have weight
+        plan.mode = kAll;
+        plan.last = cut_k < kBins ? cut_k - 1 : kBins - 1;
+        plan.tokens = cut_k < kBins ? before_k : all;
     } else if (k_cuts) {
         plan.mode = wish.has_p || in_k > (uint32_t)kList ? kWhole : kBorder;
         plan.bin = plan.from = plan.last = cut_k;
@@ -775,26 +747,22 @@ __global__ __launch_bounds__(kScan) void sample_collect_kernel(SampleArgs a, Sam
         plan = ws.plan[row];
     }
     const Wish wish = row_wish(a, row);
-    if (plan.mode == kNone || plan.mode == kWhole) return;
+    if (plan.mode == kNone || plan.mode == kWhole || plan.mode == kSlabs) return;
     if (plan.mode == kFree && !wish.has_p && wish.top_k >= a.vocab) return;  // (the second launch has its masses)
     const Scale sc(plan.top, wish.inv_t, a.shift);
-    const float *const tops = ws.tops + (int64_t)row * kSlabs * ws.chunks;
-    // Tokens that are collected, and others whose mass counts.
-    const bool by_key = plan.floor > 0;
-    const int deepest = plan.last > plan.bin - 1 ? plan.last : plan.mode == kAll ? plan.last : plan.bin - 1;
-    auto concerns = [&](float top) {
-        if (!(top > -__builtin_inff())) return false;
-        return by_key ? logit_key(top) >= plan.floor : plan.bins.of(top) <= deepest;
-    };
+    const float *const tops = ws.tops + (int64_t)row * kChunkSlabs * ws.chunks;
+    // The bins of tokens that are collected, or whose mass counts.
+    const int deepest = plan.mode == kAll || plan.last > plan.bin - 1 ? plan.last : plan.bin - 1;
+    auto concerns = [&](float top) { return top > -__builtin_inff() && plan.bins.of(top) <= deepest; };
     for (int c = ws.first(part); c < ws.first(part + 1); c++) {
         bool any = plan.mode != kAll;  // (then the chunk's mass is written, if it is 0)
 #pragma unroll
-        for (int j = 0; j < kSlabs; j++) any |= concerns(tops[kSlabs * c + j]);
+        for (int j = 0; j < kChunkSlabs; j++) any |= concerns(tops[kChunkSlabs * c + j]);
         if (!any) continue;
         float l[4][4];
 #pragma unroll
         for (int j = 0; j < 4; j++) {
-            if (concerns(tops[kSlabs * c + 4 * j + wave])) {
+            if (concerns(tops[kChunkSlabs * c + 4 * j + wave])) {
                 load4(a, base, c * kChunk + j * 1024 + 4 * tid, l[j]);
             } else {
 #pragma unroll
@@ -802,33 +770,28 @@ __global__ __launch_bounds__(kScan) void sample_collect_kernel(SampleArgs a, Sam
             }
         }
         uint32_t listed = 0;  // bit j: token j is collected
-        if (by_key) {
+        u64 t = 0;
+        uint32_t kept = 0;
 #pragma unroll
-            for (int j = 0; j < 16; j++) listed |= logit_key(l[j >> 2][j & 3]) >= plan.floor ? 1u << j : 0u;
-        } else {
-            u64 t = 0;
-            uint32_t kept = 0;
-#pragma unroll
-            for (int j = 0; j < 16; j++) {
-                const float v = l[j >> 2][j & 3];
-                if (!(v > -__builtin_inff())) continue;
-                const int b = plan.bins.of(v);
-                if (b >= plan.from && b <= plan.last) {
-                    listed |= 1u << j;
-                } else if (plan.mode != kAll && b < plan.bin) {
-                    const double w = sc.weight(v);
-                    if (w >= wish.min_p) {
-                        t += sc.fixed(w);
-                        kept++;
-                    }
+        for (int j = 0; j < 16; j++) {
+            const float v = l[j >> 2][j & 3];
+            if (!(v > -__builtin_inff())) continue;
+            const int b = plan.bins.of(v);
+            if (b >= plan.from && b <= plan.last) {
+                listed |= 1u << j;
+            } else if (plan.mode != kAll && b < plan.bin) {
+                const double w = sc.weight(v);
+                if (w >= wish.min_p) {
+                    t += sc.fixed(w);
+                    kept++;
                 }
             }
-            if (plan.mode != kAll) {
-                scan_sum(t, kept, pm, pn);
-                if (tid == 0) {
-                    ws.chunk_mass[(int64_t)row * ws.chunks + c] = t;
-                    ws.chunk_kept[(int64_t)row * ws.chunks + c] = kept;
-                }
+        }
+        if (plan.mode != kAll) {
+            scan_sum(t, kept, pm, pn);
+            if (tid == 0) {
+                ws.chunk_mass[(int64_t)row * ws.chunks + c] = t;
+                ws.chunk_kept[(int64_t)row * ws.chunks + c] = kept;
             }
         }
         collect(ws, row, c, l, listed, cn, &place);
@@ -908,7 +871,10 @@ __device__ void sort_list(SortLds &s, RowLds &rl, int n, BUCKET &&bucket) {
             if (tid + j * kThreads >= n) continue;
             const uint32_t from = b[j] > 0 ? s.slot[b[j] - 1] : 0u, to = s.slot[b[j]];
             uint32_t place = from;
-            for (uint32_t i = from; i < to; i++) place += s.spare[i] < v[j] ? 1u : 0u;
+            for (uint32_t i = from; i < to; i += 4) {  // (four reads on the way at a time)
+#pragma unroll
+                for (uint32_t q = 0; q < 4; q++) place += s.spare[i + q < to ? i + q : i] < v[j] && i + q < to ? 1u : 0u;
+            }
             s.list[place] = v[j];
         }
         __syncthreads();
@@ -930,6 +896,74 @@ __device__ void sort_list(SortLds &s, RowLds &rl, int n, BUCKET &&bucket) {
             }
             __syncthreads();
         }
+}
+
+// The tokens of a row that a top_k of k can keep, into the list (its length is
+// returned; past kList only counted): k slabs at least hold a token as large as
+// the k-th largest slab maximum, so none below it is among the first k.  Of that
+// maximum's key the upper half suffices, found by a histogram of the first byte,
+// then of the second.
+__device__ __forceinline__ int collect_slabs(const SampleArgs &a, const SampleWs &ws, int row, uint32_t k, SortLds &so,
+                                             RowLds &s) {
+    static_assert(kSlabsMax <= kThreads, "a thread a slab");
+    const int tid = (int)threadIdx.x, lane = tid & 63, wave = tid >> 6, slabs = kChunkSlabs * ws.chunks;
+    const uint32_t key = tid < slabs ? logit_key(ws.tops[(int64_t)row * slabs + tid]) : 0u;
+    uint32_t floor = 0;
+#pragma unroll
+    for (int at = 24; at >= 16; at -= 8) {
+        if (tid < 256) s.count[tid] = 0;
+        if (tid == 0) so.most = s.found = 0;
+        __syncthreads();
+        if (key > 0 && (at == 24 || key >> 24 == floor >> 24)) atomicAdd(&s.count[(key >> at) & 255u], 1u);  // LDS
+        __syncthreads();
+        const uint32_t mine = tid < 256 ? s.count[255 - tid] : 0u;  // from the top
+        uint32_t end = wave_scan(mine);
+        if (lane == 63) s.part[wave] = end;
+        __syncthreads();
+        for (int w = 0; w < wave; w++) end += (uint32_t)s.part[w];
+        if (end >= k && end - mine < k) {  // one thread
+            s.digit = (uint32_t)(255 - tid);
+            s.before_count = end - mine;
+        }
+        __syncthreads();
+        floor |= s.digit << at;
+        k -= s.before_count;
+    }
+    if (floor == 0) floor = 1;  // (0 is no token)
+    if (key >= floor) so.slot[atomicAdd(&s.found, 1)] = (uint32_t)tid;  // LDS
+    __syncthreads();
+    const int n = s.found;
+    const int64_t base = (int64_t)row * a.stride;
+    constexpr int kAhead = 4;
+    for (int i0 = wave; i0 < n; i0 += kAhead * kWaves) {
+        float l[kAhead][4];
+        int at[kAhead];
+#pragma unroll
+        for (int j = 0; j < kAhead; j++) {
+            const int i = i0 + j * kWaves;
+            at[j] = i < n ? 256 * (int)so.slot[i] + 4 * lane : a.vocab;  // (a slab is 256 neighbours)
+            load4(a, base, at[j], l[j]);
+        }
+#pragma unroll
+        for (int j = 0; j < kAhead; j++) {
+            uint32_t count = 0;
+#pragma unroll
+            for (int i = 0; i < 4; i++) count += logit_key(l[j][i]) >= floor ? 1u : 0u;
+            const uint32_t upto = wave_scan(count);
+            uint32_t place = 0;
+            if (lane == 63 && upto > 0) place = atomicAdd(&so.most, upto);  // LDS
+            place = (uint32_t)__builtin_amdgcn_readlane((int)place, 63) + upto - count;
+#pragma unroll
+            for (int i = 0; i < 4; i++) {
+                const uint32_t t = logit_key(l[j][i]);
+                if (t < floor) continue;
+                if (place < (uint32_t)kList) so.list[place] = ((u64)(0xFFFFFFFFu - t) << 32) | (uint32_t)(at[j] + i);
+                place++;
+            }
+        }
+    }
+    __syncthreads();
+    return (int)so.most;
 }
 
 // One workgroup per row.
@@ -954,7 +988,15 @@ __global__ __launch_bounds__(kThreads) void sample_draw_kernel(SampleArgs a, Sam
         }
         return;
     }
-    const int n = plan.mode == kAll || plan.mode == kBorder ? (int)ws.listed[kLine * row] : 0;
+    const bool all = plan.mode == kAll || plan.mode == kSlabs;  // every token that may be kept is in the list
+    int n = 0;
+    if (plan.mode == kSlabs) {
+        n = collect_slabs(a, ws, row, plan.tokens, so, s);
+    } else if (plan.mode == kAll || plan.mode == kBorder) {
+        n = (int)ws.listed[kLine * row];
+        for (int i = tid; i < n && i < kList; i += kThreads) so.list[i] = ws.list[(int64_t)row * kList + i];
+        __syncthreads();
+    }
     if (plan.mode == kWhole || n > kList) {
         whole_row(a, row, wish, plan.top, s);
         return;
@@ -967,15 +1009,14 @@ __global__ __launch_bounds__(kThreads) void sample_draw_kernel(SampleArgs a, Sam
     };
     auto logit_of = [](u64 v) { return key_logit(0xFFFFFFFFu - (uint32_t)(v >> 32)); };
 
-    if (plan.mode == kAll && n <= 128) {
+    if (all && n <= 128) {
         // Few tokens, two a lane of one wave, without a barrier: places by
         // counting, by key and then by index.
         if (tid >= 64) return;
         u64 v[2] = {~0ull, ~0ull};
 #pragma unroll
         for (int j = 0; j < 2; j++) {
-            if (tid + 64 * j < n) v[j] = ws.list[(int64_t)row * kList + tid + 64 * j];
-            so.list[tid + 64 * j] = v[j];
+            if (tid + 64 * j < n) v[j] = so.list[tid + 64 * j];
         }
         auto place = [&](int count, bool (&in)[2]) {  // those of `in` below each value, of the first `count`
             __builtin_amdgcn_wave_barrier();          // (a wave's LDS accesses complete in order)
@@ -1052,10 +1093,8 @@ __global__ __launch_bounds__(kThreads) void sample_draw_kernel(SampleArgs a, Sam
     if (n > 0) {
         float low = __builtin_inff(), high = -__builtin_inff();
         for (int i = tid; i < n; i += kThreads) {
-            const u64 v = ws.list[(int64_t)row * kList + i];
-            so.list[i] = v;
-            low = fminf(low, logit_of(v));
-            high = fmaxf(high, logit_of(v));
+            low = fminf(low, logit_of(so.list[i]));
+            high = fmaxf(high, logit_of(so.list[i]));
         }
         for (int d = 1; d < 64; d <<= 1) {
             low = fminf(low, __shfl_xor(low, d));
@@ -1076,7 +1115,7 @@ __global__ __launch_bounds__(kThreads) void sample_draw_kernel(SampleArgs a, Sam
             const float x = inv > 0.0f ? fminf((high - logit_of(v)) * inv, 1.0f) : 0.0f;
             return (int)(x * (0.4f + 0.6f * x) * (float)(kThreads - 1));
         });
-        const int k = plan.mode == kAll && plan.tokens < (uint32_t)n ? (int)plan.tokens : n;
+        const int k = all && plan.tokens < (uint32_t)n ? (int)plan.tokens : n;
         u64 sum = 0, total;
         double w[kPer];
 #pragma unroll
@@ -1110,7 +1149,7 @@ __global__ __launch_bounds__(kThreads) void sample_draw_kernel(SampleArgs a, Sam
     __syncthreads();
     // The chunks' kept mass, and the one that the random number falls into.
     u64 mine = tid < ws.chunks ? chunk[tid] : 0;
-    if (plan.mode != kAll && tid < ws.chunks) {
+    if (!all && tid < ws.chunks) {
         mine += ws.chunk_mass[(int64_t)row * ws.chunks + tid];
         kept += ws.chunk_kept[(int64_t)row * ws.chunks + tid];
     }
@@ -1126,7 +1165,7 @@ __global__ __launch_bounds__(kThreads) void sample_draw_kernel(SampleArgs a, Sam
     }
     __syncthreads();
     u64 cum = before_chunk;
-    if (plan.mode == kAll) {
+    if (all) {
         // the chunk's kept tokens by index: upper half the index, lower half the key
         u64 v[kPer];
 #pragma unroll
@@ -1207,7 +1246,7 @@ SampleLayout sample_layout(int rows, int vocab) {
         return at;
     };
     const size_t r = (size_t)rows, rc = r * o.chunks, rb = r * o.parts * kBins;
-    o.tops = take(rc * kSlabs * sizeof(float));
+    o.tops = take(rc * kChunkSlabs * sizeof(float));
     o.least = take(rc * 4 * sizeof(float));
     o.mass = take(rb * sizeof(u64));
     o.chunk_mass = take(rc * sizeof(u64));

@@ -113,9 +113,9 @@ __global__ __launch_bounds__(64 * WAVES) void moe_route_kernel(RouteArgs a) {
             p[j] = exp((double)l[j] - (double)mx);
             if (lane + 64 * j < E) s += p[j];
         }
-        s = wave_sum(s);
+        const double over = 1.0 / wave_sum(s);
 #pragma unroll
-        for (int j = 0; j < PER; j++) p[j] /= s;
+        for (int j = 0; j < PER; j++) p[j] *= over;
     }
     u64 key[PER];
 #pragma unroll
@@ -180,10 +180,8 @@ __global__ __launch_bounds__(64 * WAVES) void moe_route_kernel(RouteArgs a) {
             }
     };
     look();
-    double sum = 0.0;
-    const bool few = K <= 64;
+    const bool few = K <= 64;  // lane r keeps rank r
     int id = 0;
-    double pw = 0.0;
     for (int r = 0; r < K; r++) {
         const uint32_t hi = (uint32_t)(mine >> 32);
         u64 who = __ballot(hi == wave_max(hi));
@@ -201,16 +199,8 @@ __global__ __launch_bounds__(64 * WAVES) void moe_route_kernel(RouteArgs a) {
             winner = (int)((0xFFFFFFFFu - low) & 63u);
         }
         const int e = winner + 64 * __builtin_amdgcn_readlane(at, winner);
-        const double pe = ps[e];
-        sum += pe;
-        if (few) {
-            if (lane == r) {
-                id = e;
-                pw = pe;
-            }
-        } else if (lane == 0) {
-            a.ids[(int64_t)t * K + r] = e;
-        }
+        if (few) id = lane == r ? e : id;
+        else if (lane == 0) a.ids[(int64_t)t * K + r] = e;
         if (lane == winner) {
 #pragma unroll
             for (int j = 0; j < PER; j++)
@@ -218,16 +208,15 @@ __global__ __launch_bounds__(64 * WAVES) void moe_route_kernel(RouteArgs a) {
             look();
         }
     }
+    if (!few) __threadfence_block();  // lane 0's ids
+    double sum = 0.0;
+    for (int r = lane; r < K; r += 64) sum += ps[few ? id : a.ids[(int64_t)t * K + r]];
+    sum = wave_sum(sum);
     const double over = a.renormalize && sum > 0.0 ? sum : 1.0;
-    if (few) {
-        if (lane < K) {
-            a.ids[(int64_t)t * K + lane] = id;
-            a.weights[(int64_t)t * K + lane] = (float)(pw / over * (double)a.scale);
-        }
-    } else {
-        __threadfence_block();  // lane 0's ids
-        for (int r = lane; r < K; r += 64)
-            a.weights[(int64_t)t * K + r] = (float)(ps[a.ids[(int64_t)t * K + r]] / over * (double)a.scale);
+    for (int r = lane; r < K; r += 64) {
+        const int e = few ? id : a.ids[(int64_t)t * K + r];
+        if (few) a.ids[(int64_t)t * K + r] = e;
+        a.weights[(int64_t)t * K + r] = (float)(ps[e] / over * (double)a.scale);
     }
 }
 

@@ -42,7 +42,7 @@ struct gollek_hip_weight {
 
 namespace {
 
-constexpr int32_t kAbiVersion = 1 * 10000 + 0 * 100 + 0;
+constexpr int32_t kAbiVersion = 1 * 10000 + 1 * 100 + 0;
 constexpr int64_t kRouterMaxExperts = 4096;  // router LDS: 8 B per expert + 4 B per rank
 
 thread_local std::string g_last_error;
@@ -931,9 +931,10 @@ int32_t make_epilogue(const gollek_hip_weight *w, int64_t m, const float *bias, 
     for (auto &b : each) {
         if (*b.stride == 0) *b.stride = n;
         if (b.p == nullptr) continue;
-        if (*b.stride < n || *b.stride > (int64_t)1 << 40)
-            return fail(GOLLEK_HIP_ERR_ARG, err, err_len, "The %s's row stride %lld is not at least %lld columns",
-                        b.name, (long long)*b.stride, (long long)n);
+        if (*b.stride < n || *b.stride > ((int64_t)1 << 56) / (m > 0 ? m : 1))
+            return fail(GOLLEK_HIP_ERR_ARG, err, err_len,
+                        "The %s's row stride %lld is not at least %lld columns, or out of range", b.name,
+                        (long long)*b.stride, (long long)n);
         if (reinterpret_cast<uintptr_t>(b.p) % (uintptr_t)size != 0)
             return fail(GOLLEK_HIP_ERR_ARG, err, err_len, "The %s is not aligned to its %d-byte elements", b.name, size);
         if (b.p != y && m > 0 && n > 0 && overlaps(y, y_stride, b.p, *b.stride, m, n, size))
@@ -1340,7 +1341,8 @@ int32_t gollek_hip_moe_select_topk(const float *logits, int64_t tokens, int64_t 
 
 static int32_t check_route(int32_t logits_type, const void *logits, int64_t tokens, int64_t n_experts,
                            const float *bias, int32_t scoring, int64_t n_groups, int64_t top_groups, int32_t group_top,
-                           int64_t top_k, float scale, char *err, size_t err_len) {
+                           int64_t top_k, float scale, const int32_t *ids, const float *weights, char *err,
+                           size_t err_len) {
     const int32_t rc = check_router(tokens, n_experts, top_k, scoring, err, err_len);
     if (rc != GOLLEK_HIP_OK) return rc;
     const int size = element_size(logits_type);
@@ -1357,9 +1359,10 @@ static int32_t check_route(int32_t logits_type, const void *logits, int64_t toke
         return fail(GOLLEK_HIP_ERR_ARG, err, err_len, "top_k %lld is more than the %lld experts of %lld groups",
                     (long long)top_k, (long long)(top_groups * (n_experts / n_groups)), (long long)top_groups);
     if (!(scale - scale == 0.0f)) return fail(GOLLEK_HIP_ERR_ARG, err, err_len, "The scale is not finite");
-    if (reinterpret_cast<uintptr_t>(logits) % (uintptr_t)size != 0 ||
-        reinterpret_cast<uintptr_t>(bias) % sizeof(float) != 0)
-        return fail(GOLLEK_HIP_ERR_ARG, err, err_len, "The logits or the bias are not aligned to their elements");
+    const uintptr_t four = reinterpret_cast<uintptr_t>(bias) | reinterpret_cast<uintptr_t>(ids) |
+                           reinterpret_cast<uintptr_t>(weights);
+    if (reinterpret_cast<uintptr_t>(logits) % (uintptr_t)size != 0 || (four & 3u) != 0)
+        return fail(GOLLEK_HIP_ERR_ARG, err, err_len, "The routing buffers are not aligned to their elements");
     return GOLLEK_HIP_OK;
 }
 
@@ -1368,7 +1371,7 @@ int32_t gollek_hip_moe_route_device(const void *logits, int32_t logits_type, int
                                     int32_t group_top, int64_t top_k, int32_t renormalize, float scale, int32_t *ids,
                                     float *weights, void *stream, char *err, size_t err_len) {
     const int32_t rc = check_route(logits_type, logits, tokens, n_experts, bias, scoring, n_groups, top_groups,
-                                   group_top, top_k, scale, err, err_len);
+                                   group_top, top_k, scale, ids, weights, err, err_len);
     if (rc != GOLLEK_HIP_OK) return rc;
     if (tokens == 0) {
         ok(err, err_len);
@@ -1390,7 +1393,7 @@ int32_t gollek_hip_moe_route(const void *logits, int32_t logits_type, int64_t to
                              int32_t group_top, int64_t top_k, int32_t renormalize, float scale, int32_t *ids,
                              float *weights, char *err, size_t err_len) {
     int32_t rc = check_route(logits_type, logits, tokens, n_experts, bias, scoring, n_groups, top_groups, group_top,
-                             top_k, scale, err, err_len);
+                             top_k, scale, ids, weights, err, err_len);
     if (rc != GOLLEK_HIP_OK) return rc;
     if (tokens == 0) {
         ok(err, err_len);
@@ -1433,7 +1436,7 @@ int32_t gollek_hip_moe_block_routed_device(gollek_hip_weight *gate, gollek_hip_w
     if (rc != GOLLEK_HIP_OK) return rc;
     // every check before the first launch: a refused call leaves ids and weights alone
     rc = check_route(logits_type, logits, tokens, n_experts, bias, scoring, n_groups, top_groups, group_top, top_k,
-                     scale, err, err_len);
+                     scale, ids, weights, err, err_len);
     if (rc != GOLLEK_HIP_OK) return rc;
     if (tokens == 0) {
         ok(err, err_len);

@@ -256,3 +256,63 @@ def test_next_token_is_the_mat_vec_and_the_sample(compact):
     with pytest.raises(ops.IllegalArgumentError):
         ops.next_token(t, x[:-1], 0.5)
     t.close()
+
+
+# The ways a border is found: bins whose tokens fill the list, past it (the border's
+# bin alone), a far bin of weight 0 (low temperatures), a min_p below the weights' unit,
+# a top_k past the slabs, and the whole row by one workgroup.
+WAYS = [dict(k=6000), dict(k=6000, t=0.05), dict(k=20000, t=0.03), dict(k=300, t=0.05, p=0.9), dict(k=64, t=0.02),
+        dict(k=65), dict(k=2000, p=0.99, t=2.0), dict(k=2100, p=0.99, t=2.0), dict(k=2100, t=0.04, p=0.95),
+        dict(mp=1e-15), dict(p=0.9, mp=1e-15), dict(k=30, mp=1e-15), dict(p=0.97, t=1.6), dict(p=0.999, t=4.0, mp=1e-3),
+        dict(k=120000, p=0.95, t=1.5), dict(p=1e-9), dict(k=10**9, p=0.5)]
+
+
+@pytest.mark.parametrize("i", range(len(WAYS)))
+@pytest.mark.parametrize("vocab,rows,kind", [(128256, 3, _native.F32), (50257, 6, _native.BF16)])
+def test_every_way_to_a_border(vocab, rows, kind, i):
+    l = logits_of(rows, vocab, 100 + i, DTYPE[kind])
+    u = np.random.default_rng(200 + i).random(rows).astype(np.float32)
+    compare(sample(l, u, **WAYS[i]), l, u, f"{vocab} {WAYS[i]}", **WAYS[i])
+
+
+@pytest.mark.parametrize("vocab", [262144, 300001, 4194304])
+@pytest.mark.parametrize("kw", [dict(), dict(k=40, p=0.9), dict(p=0.9), dict(k=700, t=1.2), dict(mp=0.01)])
+def test_large_vocabularies(vocab, kw):
+    l = logits_of(2, vocab, vocab % 97)
+    u = np.array([0.37, 0.93], np.float32)
+    compare(sample(l, u, **kw), l, u, f"{vocab} {kw}", **kw)
+
+
+def test_masks_of_the_lowest_value():
+    """A mask written as the type's lowest finite value: tokens, of weight 0."""
+    vocab = 40000
+    for dtype in (torch.float32, torch.bfloat16, torch.float16):
+        l = logits_of(4, vocab, 12).to(dtype)
+        mask = torch.rand(4, vocab, generator=torch.Generator().manual_seed(1)) > 0.01
+        l[mask.cuda()] = torch.finfo(dtype).min
+        l[3] = torch.finfo(dtype).min
+        u = np.array([0.1, 0.5, 0.9, 0.7], np.float32)
+        for kw in (dict(), dict(k=50, p=0.9), dict(k=1000, p=0.9), dict(p=0.95), dict(mp=0.02), dict(k=900)):
+            compare(sample(l, u, **kw), l, u, f"{dtype} {kw}", **kw)
+
+
+def test_calls_on_two_streams_at_once():
+    rows, vocab = 5, 60000
+    side = [torch.cuda.Stream(), torch.cuda.Stream()]
+    runs = []
+    for i, s in enumerate(side):
+        l = logits_of(rows, vocab, 60 + i)
+        u = torch.from_numpy(np.random.default_rng(i).random(rows).astype(np.float32)).cuda()
+        p = torch.full((rows,), 0.9, device="cuda")
+        out = [torch.zeros(rows, device="cuda", dtype=d) for d in (torch.int32, torch.float32, torch.int32)]
+        ws = torch.zeros(ops.sample_workspace_bytes(rows, vocab), device="cuda", dtype=torch.uint8)
+        runs.append((s, l, u, p, out, ws))
+    torch.cuda.synchronize()
+    for _ in range(6):
+        for s, l, u, p, out, ws in runs:
+            ops.sample_device(l.data_ptr(), _native.F32, rows, vocab, u.data_ptr(), out[0].data_ptr(),
+                              top_p_ptr=p.data_ptr(), probs_ptr=out[1].data_ptr(), kept_ptr=out[2].data_ptr(),
+                              ws_ptr=ws.data_ptr(), ws_bytes=ws.numel(), stream=s.cuda_stream)
+    torch.cuda.synchronize()
+    for _, l, u, _, out, _ in runs:
+        compare([o.cpu().numpy() for o in out], l, u.cpu().numpy(), "two streams", p=0.9)

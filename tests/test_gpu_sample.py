@@ -316,3 +316,15 @@ def test_calls_on_two_streams_at_once():
     torch.cuda.synchronize()
     for _, l, u, _, out, _ in runs:
         compare([o.cpu().numpy() for o in out], l, u.cpu().numpy(), "two streams", p=0.9)
+
+
+@pytest.mark.parametrize("vocab,stride", [(40001, 40003), (16384, 16385), (16385, 16388), (8192, 8192), (8193, 8200)])
+def test_settings_of_their_own_over_long_rows(vocab, stride):
+    rows = 24
+    wide = logits_of(rows, stride, vocab)
+    wide[:, vocab:] = 1e4  # behind the vocabulary: never read as a token
+    rng = np.random.default_rng(vocab)
+    kw = dict(t=rng.choice([0.0, 0.1, 0.6, 1.0, 1.7, 6.0], rows), k=rng.choice([0, 1, 7, 50, 64, 900, 3000, 10**6], rows),
+              p=rng.choice([0.5, 0.9, 0.99, 1.0], rows), mp=rng.choice([0.0, 0.02, 0.3], rows))
+    u = rng.random(rows).astype(np.float32)
+    compare(sample(wide, u, vocab=vocab, **kw), wide[:, :vocab], u, "rows", **kw)

@@ -39,6 +39,9 @@ import java.util.WeakHashMap;
  * <li>GgufTensorOps.dotRow and dequantizeRow (RT/GgufTensorOps.java:636-650),
  * after checkLayoutRow: {@code tryDotRow} / {@code tryDequantizeRow}, falling
  * through to the Java code when they return false.</li>
+ * <li>A generation loop that runs the lm_head's mat-vec and samples from its
+ * logits: {@code tryNextToken}, which does both on the device and returns the
+ * token alone.</li>
  * <li>GgufTensorOps.clearPreparedMatrixCaches, which JavaNativeGgufBackend.close
  * calls (core/plugin/gollek-plugin-runner-gguf/.../JavaNativeGgufBackend.java:139-143):
  * {@code GgufHipMatVec.release(model)}.</li>
@@ -185,6 +188,36 @@ final class GgufHipMatVec {
             return (short) ((bits >>> 16) | 0x0040);
         }
         return (short) ((bits + 0x7FFF + ((bits >>> 16) & 1)) >>> 16);
+    }
+
+    /**
+     * token[0] = the token sampled from the logits tensor . vector
+     * (gollek_hip_next_token; -1 when every logit is -inf or NaN): the first
+     * topK of them (topK &lt;= 0: all), of these the shortest prefix holding
+     * topP of their mass at the given temperature (&lt;= 0: the largest logit),
+     * of these the ones of at least minP of the largest's probability, and
+     * among those the one that u, a random number in [0, 1), falls on in the
+     * order of the vocabulary.  The logits, half a megabyte for a vocabulary of
+     * 128k, stay on the device.  False when the route is not taken.
+     */
+    static boolean tryNextToken(GGUFModel model, GGUFTensorInfo tensor, long rows, int columns, long rowBytes,
+                                float[] vector, float temperature, int topK, float topP, float minP, float u,
+                                int[] token) {
+        Binding b = Binding.get();
+        if (b == null || !supportsType(tensor.typeId())) {
+            return false;
+        }
+        if (token.length < 1) {
+            throw new IllegalArgumentException("No room for the token");
+        }
+        MemorySegment w = handle(b, model, tensor, rows, columns, rowBytes);
+        try (Arena arena = Arena.ofConfined()) {
+            MemorySegment err = arena.allocate(ERR_LEN);
+            int rc = b.nextToken(w, MemorySegment.ofArray(vector), (long) vector.length, temperature, topK, topP, minP,
+                    u, MemorySegment.ofArray(token), MemorySegment.NULL, MemorySegment.NULL, err, (long) ERR_LEN);
+            check(rc, err);
+        }
+        return true;
     }
 
     /** Row {@code row} of the tensor . vector into out[0]; false when the route is not taken. */
@@ -413,6 +446,7 @@ final class GgufHipMatVec {
         private final MethodHandle moeBlock;
         private final MethodHandle moeSharedExpert;
         private final MethodHandle gemmBf16;
+        private final MethodHandle nextToken;
 
         /** The binding, or null when the route is disabled or the library cannot be used here. */
         static Binding get() {
@@ -508,6 +542,12 @@ final class GgufHipMatVec {
                             ValueLayout.ADDRESS, ValueLayout.ADDRESS, ValueLayout.JAVA_LONG, ValueLayout.JAVA_LONG,
                             ValueLayout.ADDRESS, ValueLayout.JAVA_LONG, ValueLayout.ADDRESS, ValueLayout.JAVA_LONG),
                     true);
+            this.nextToken = downcall(linker, lookup, "gollek_hip_next_token",
+                    FunctionDescriptor.of(ValueLayout.JAVA_INT,
+                            ValueLayout.ADDRESS, ValueLayout.ADDRESS, ValueLayout.JAVA_LONG, ValueLayout.JAVA_FLOAT,
+                            ValueLayout.JAVA_INT, ValueLayout.JAVA_FLOAT, ValueLayout.JAVA_FLOAT,
+                            ValueLayout.JAVA_FLOAT, ValueLayout.ADDRESS, ValueLayout.ADDRESS, ValueLayout.ADDRESS,
+                            ValueLayout.ADDRESS, ValueLayout.JAVA_LONG), true);
             int abi = (int) version.invokeExact();
             if (abi / 10000 != ABI_MAJOR) {
                 throw new IllegalStateException("libgollek_hip ABI " + abi + " is not major " + ABI_MAJOR);
@@ -634,6 +674,17 @@ final class GgufHipMatVec {
                      MemorySegment err, long errLen) {
             try {
                 return (int) gemmBf16.invokeExact(weight, x, xLen, m, y, yLen, err, errLen);
+            } catch (Throwable t) {
+                throw propagate(t);
+            }
+        }
+
+        int nextToken(MemorySegment weight, MemorySegment x, long xLen, float temperature, int topK, float topP,
+                      float minP, float u, MemorySegment token, MemorySegment prob, MemorySegment kept,
+                      MemorySegment err, long errLen) {
+            try {
+                return (int) nextToken.invokeExact(weight, x, xLen, temperature, topK, topP, minP, u, token, prob, kept,
+                        err, errLen);
             } catch (Throwable t) {
                 throw propagate(t);
             }

@@ -201,3 +201,23 @@ def test_sample_refuses():
         ops.next_token(None, u, 0.5)
     assert lib.gollek_hip_next_token(None, u.ctypes.data, 2, 1.0, 0, 1.0, 0.0, 0.5, u.ctypes.data, None, None, e.buf,
                                      e.size) == _native.ERR_NULL
+
+
+def test_sample_checks_the_workspace_of_long_rows():
+    lib, e = _native.load(), _err()
+    need = lib.gollek_hip_sample_workspace_bytes(3, 100000)
+    assert need > 0 and need % 256 == 0
+
+    def rc(ws, ws_bytes):
+        return lib.gollek_hip_sample_device(4096, 0, 3, 100000, 0, 0, 0, 0, 0, 4096, 4096, 0, 0, ws, ws_bytes, None,
+                                            e.buf, e.size)
+
+    assert rc(0, need) == _native.ERR_NULL
+    assert rc(4096, need - 1) == rc(4096 + 128, need) == _native.ERR_ARG
+
+
+def test_route_refuses_misaligned_results():
+    lib, e = _native.load(), _err()
+    for ids, w in ((4098, 4096), (4096, 4097)):
+        assert lib.gollek_hip_moe_route_device(4096, 0, 1, 32, 0, 0, 1, 1, 1, 2, 1, 1.0, ids, w, None, e.buf,
+                                               e.size) == _native.ERR_ARG

@@ -296,7 +296,7 @@ inline constexpr bool kHasEpilogue<Epilogue> = true;
 
 // Host side: workspace bytes left for the S - 1 partials that a split plan
 // counts (an epilogue's split 0 takes one more), and whether a product's
-// splits can be added four floats at a time.
+// splits can be added (a plain one's four floats at a time).
 template <class OUT>
 size_t split_bytes(const float *workspace, size_t bytes, int M, int N) {
     if (workspace == nullptr) return 0;
@@ -307,8 +307,8 @@ inline bool splits_aligned(const float *y, const float *workspace, int M, int N)
     return ((int64_t)M * N) % 4 == 0 &&
            ((reinterpret_cast<uintptr_t>(workspace) | reinterpret_cast<uintptr_t>(y)) & 15u) == 0;
 }
-inline bool splits_aligned(const Epilogue &, const float *workspace, int M, int N) {
-    return ((int64_t)M * N) % 4 == 0 && (reinterpret_cast<uintptr_t>(workspace) & 15u) == 0;
+inline bool splits_aligned(const Epilogue &, const float *workspace, int, int) {
+    return (reinterpret_cast<uintptr_t>(workspace) & 15u) == 0;
 }
 
 }  // namespace gollek

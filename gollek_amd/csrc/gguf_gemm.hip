@@ -624,8 +624,9 @@ hipError_t launch_gemm_bf16(int type_id, const uint8_t *w, int64_t row_bytes, co
 }
 
 size_t linear_workspace_bytes(int type_id, int M, int N, int K) {
-    const size_t most = gemm_workspace_bytes(type_id, M, N, K);
-    return most > 0 ? most + (size_t)M * N * sizeof(float) : 0;
+    if (type_id == kQ4_K || type_id == kQ5_K || type_id == kQ6_K) return linear_kq_workspace_bytes(type_id, M, N, K);
+    if (type_id == kQ8_0 && M <= 32 && N % 16 == 0 && K % 256 == 0) return 0;  // the skinny kernel
+    return linear_tile_workspace_bytes(M, N, K);
 }
 
 hipError_t launch_linear(int type_id, const uint8_t *w, int64_t row_bytes, const uint16_t *x, const Epilogue &y,

@@ -43,6 +43,7 @@
 // the release writes back and the acquire invalidates each XCD's L2.)
 #include "gguf_blocks.hpp"
 #include "gguf_dot4.hpp"
+#include "gguf_gemm_plan.hpp"
 #include "gguf_kernels.hpp"
 
 namespace gollek {
@@ -267,9 +268,11 @@ __global__ __launch_bounds__(kThreads) void gemm_tile_kernel(const uint8_t *__re
     // it (its X and W bytes are the next row's, or zeros).  (K rounded up where
     // it is whole cost those kernels 0.8 % over 112 shapes, Q4_0 M = 64, 4096 x
     // 11008 85.7 -> 87.8 us, with the same instructions in the loops.)
-    const int nst = (RAGGED ? (K + 63) / 64 : K / 64) / S;
-    const int s0 = split * nst;
-    const bool half_last = RAGGED && (K & 32) != 0;
+    // An epilogue's splits take any number of stages, one more in some of them.
+    const int stages = RAGGED ? (K + 63) / 64 : K / 64;
+    const int s0 = kHasEpilogue<OUT> ? split * stages / S : split * (stages / S);
+    const int nst = kHasEpilogue<OUT> ? (split + 1) * stages / S - s0 : stages / S;
+    const bool half_last = RAGGED && (K & 32) != 0 && (!kHasEpilogue<OUT> || split == S - 1);
 
     // Buffers from the split's first column; rows past M / N and bytes past
     // the end read as zeros (W's end rounded up to a dword: a buffer load drops
@@ -609,6 +612,42 @@ int tile_splits(int type_id, int M, int N, int K, size_t workspace_bytes) {
 
 }  // namespace
 
+// The linear layer's tile height and splits (parts of K, whole stages, one more in
+// some of them): the pair with the shortest time by the constants of tile_mt, 2.9 us
+// for the launch that adds the splits and 0.2 us a MB of them, written and read.
+// Against the plain product's rule, which splits a K of whole 512 by powers of two:
+// 0.97 of its times over 140 shapes of such K (0.70 to 1.07), 0.6 over those of other
+// K (Q4_0 4096 x 11008: M = 16 63.9 -> 18.0 us, M = 100 125 -> 31.4).
+struct LinearTiles {
+    int mt, splits;
+};
+static LinearTiles linear_tiles(int M, int N, int K, size_t workspace_bytes) {
+    const size_t mn = (size_t)M * N * sizeof(float);
+    constexpr float kStage[4] = {0.46f, 0.54f, 0.69f, 0.95f};
+    const int stages = (K + 63) / 64;
+    LinearTiles best = {8, 1};
+    float best_us = 0.0f;
+    for (int i = 0; i < 4; i++) {
+        const int mt = 1 << i;
+        const int64_t tiles = (int64_t)((M + 16 * mt - 1) / (16 * mt)) * ((N + kTileN - 1) / kTileN);
+        for (int S = 1; S <= 8 && S <= stages && (S == 1 || (size_t)S * mn <= workspace_bytes); S++) {
+            float us = (float)((tiles * S + device_cus() - 1) / device_cus()) *
+                       (3.0f + kStage[i] * ((stages + S - 1) / S));
+            if (S > 1) us += 2.9f + 0.4f * S * (float)mn * 1e-6f;
+            if (best_us == 0.0f || us < best_us) {
+                best = {mt, S};
+                best_us = us;
+            }
+        }
+    }
+    return best;
+}
+
+size_t linear_tile_workspace_bytes(int M, int N, int K) {
+    const LinearTiles t = linear_tiles(M, N, K, kGemmMaxSplitBytes);
+    return t.splits > 1 ? (size_t)t.splits * M * N * sizeof(float) : 0;
+}
+
 bool gemm_tile_supported(int type_id, int64_t row_bytes, int M, int N, int K, const void *w, const void *x) {
     if (type_id != kQ8_0 && type_id != kQ4_0) return false;
     if (M <= 0 || N <= 0 || K <= 0 || K % 32 != 0) return false;
@@ -636,9 +675,18 @@ hipError_t launch_gemm_tile(int type_id, const uint8_t *w, int64_t row_bytes, co
                             OUT y, int M, int N, int K, hipStream_t stream, float *workspace,
                             size_t workspace_bytes) {
     if (M <= 0) return hipSuccess;
-    int S = tile_splits(type_id, M, N, K, split_bytes<OUT>(workspace, workspace_bytes, M, N));
-    if (!splits_aligned(y, workspace, M, N)) S = 1;
-    const int mt = tile_mt(type_id, M, N, K), tm = 16 * mt;
+    int S, mt;
+    if constexpr (kHasEpilogue<OUT>) {
+        const bool split = workspace != nullptr && splits_aligned(y, workspace, M, N);
+        const LinearTiles t = linear_tiles(M, N, K, split ? workspace_bytes : 0);
+        S = t.splits;
+        mt = t.mt;
+    } else {
+        S = tile_splits(type_id, M, N, K, workspace != nullptr ? workspace_bytes : 0);
+        if (!splits_aligned(y, workspace, M, N)) S = 1;
+        mt = tile_mt(type_id, M, N, K);
+    }
+    const int tm = 16 * mt;
     const unsigned tiles = (unsigned)(((M + tm - 1) / tm) * ((N + kTileN - 1) / kTileN));
     const dim3 grid(tiles * (unsigned)S), block(kThreads);
     float *part = S > 1 ? workspace : nullptr;

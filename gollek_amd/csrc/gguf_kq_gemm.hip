@@ -348,6 +348,11 @@ size_t kq_gemm_workspace_bytes(int type_id, int M, int N, int K) {
     return gemm_plan_bytes(kq_plan(type_id, M, N, K, kGemmMaxSplitBytes), M, N);
 }
 
+size_t linear_kq_workspace_bytes(int type_id, int M, int N, int K) {
+    const size_t partials = gemm_plan_bytes(kq_plan(type_id, M, N, K, kGemmMaxSplitBytes), M, N);
+    return partials > 0 ? partials + (size_t)M * N * sizeof(float) : 0;
+}
+
 void kq_gemm_plan(int type_id, int M, int N, int K, int32_t (&plan)[4]) {
     const bool split = gemm_may_split(type_id, M, N, K) && ((int64_t)M * N) % 4 == 0;
     const GemmPlan p = kq_plan(type_id, M, N, K, split ? kGemmMaxSplitBytes : 0);
@@ -360,7 +365,9 @@ void kq_gemm_plan(int type_id, int M, int N, int K, int32_t (&plan)[4]) {
 template <class OUT>
 hipError_t launch_kq_gemm(int type_id, const uint8_t *w, int64_t row_bytes, const uint16_t *x, OUT y, int M, int N,
                           int K, hipStream_t stream, float *workspace, size_t workspace_bytes) {
-    const bool split = workspace != nullptr && gemm_may_split(type_id, M, N, K) && splits_aligned(y, workspace, M, N);
+    // (a linear layer's caller owns the workspace: it splits wherever that pays)
+    const bool split = workspace != nullptr && (kHasEpilogue<OUT> || gemm_may_split(type_id, M, N, K)) &&
+                       splits_aligned(y, workspace, M, N);
     const GemmPlan p = kq_plan(type_id, M, N, K, split ? split_bytes<OUT>(workspace, workspace_bytes, M, N) : 0);
     const unsigned grid =
         (unsigned)(((M + 16 * p.mt - 1) / (16 * p.mt)) * ((N + 32 * p.nw - 1) / (32 * p.nw)) * p.splits);

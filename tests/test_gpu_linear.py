@@ -403,3 +403,19 @@ def test_refusals():
     assert lib.gollek_hip_linear(*args[:2], xs.size - 1, *args[3:], ys.size, e.buf, e.size) == _native.ERR_ARG
     assert ctypes.sizeof(ctypes.c_void_p) == 8
     t.close()
+
+
+@pytest.mark.parametrize("t,rows,cols,m", [("q8_0", 256, 2880, 8), ("q8_0", 130, 2912, 70), ("q4_0", 256, 2816, 40),
+                                           ("q4_0", 131, 11008, 17), ("q8_0", 97, 11008, 50), ("q4_k", 256, 2816, 16),
+                                           ("q5_k", 259, 3840, 33), ("q6_k", 255, 2816, 9), ("q4_k", 130, 11008, 7)])
+def test_uneven_splits_of_k(t, rows, cols, m):
+    """K in parts of unequal length, outputs that are no multiple of four."""
+    wt = Weight(TYPES[t], rows, cols, 23)
+    assert wt.handle.linear_workspace_bytes(m) >= 2 * 4 * m * rows
+    xb = syn.activation_bf16(m, cols, seed=m)
+    x = torch.from_numpy(xb.view(np.int16)).cuda()
+    for y_type in (_native.F32, _native.F16):
+        b, mu, re = operands(m, rows, y_type, 6, True, True, True)
+        y = re.clone()
+        call(wt, x, m, y, y_type, ops.ACT_GELU_TANH, b, mu, y, wt.workspace(m))
+        check(y, expected(wt, xb, ops.ACT_GELU_TANH, b, mu, re, y_type), f"{t} {rows}x{cols} m={m} type {y_type}")

@@ -547,6 +547,15 @@ hipError_t launch_gemm(int type_id, const uint8_t *w, int64_t row_bytes, const u
     if (gemm_col_supported(type_id, row_bytes, M, N, K, w != nullptr ? w : prep, x))
         return launch_gemm_col(type_id, w, row_bytes, x, y, M, N, K, stream, prep, prep_rows);
     if (w == nullptr) return hipErrorInvalidValue;  // the GGUF rows are needed
+    // One token of the linear layer where the column kernel takes no such weight:
+    // the mat-vec's 16-row tiles against the K-quant GEMM's tiles, whose rows
+    // would be 15 of 16 empty: Q6_K 4096 x 4096 7.1 against 12.4 us,
+    // 4096 x 14336 14.3 against 25.3, 1024 x 4096 6.8 against 9.7, 128256 x 4096
+    // 81 against 164; Q4_K 32000 x 4096 15.5 against 22.2.
+    if constexpr (kHasEpilogue<OUT>) {
+        if (M == 1 && linear_vec_supported(type_id, row_bytes, N, K, w, x))
+            return launch_linear_vec(type_id, w, row_bytes, N, K, x, y, stream);
+    }
     // M <= 32 with Q8_0 weights: the buffer->LDS ring over 16-row column tiles.
     if (type_id == kQ8_0 && aligned && M <= 32 && N % 16 == 0 && K % 256 == 0 &&
         (int64_t)16 * row_bytes < ((int64_t)1 << 31) && (int64_t)M * K * 2 < ((int64_t)1 << 31)) {

@@ -544,10 +544,11 @@ constexpr int kT2MaxRows = 1024;                                // rows per work
 
 }  // namespace
 
-template <int NSLOT>
+// XB: x holds bf16 bit patterns (the linear layer's), widened to fp32 exactly.
+template <int NSLOT, bool XB = false, class OUT = float *__restrict__>
 __global__ __launch_bounds__(kT2Threads) void gemv_q4_k_mfma_tile_kernel(
     const uint8_t *__restrict__ w, int64_t row_bytes64, int nsb, const float *__restrict__ x,
-    float *__restrict__ y, int64_t rows, int64_t rows_per_wg) {
+    OUT y, int64_t rows, int64_t rows_per_wg) {
     static_assert(kT2DmaPerWave * kT2Waves >= kT2Dma, "tile loads");
     static_assert(kT2Waves * 1024 <= kT2Slot, "x scratch fits a slot");
     __shared__ __attribute__((aligned(16))) uint8_t ring[NSLOT * kT2Slot + 1024];  // + sink
@@ -597,7 +598,7 @@ __global__ __launch_bounds__(kT2Threads) void gemv_q4_k_mfma_tile_kernel(
     // nsb converts superblock 0 (its operands are never used).
     const int sb = wv;
     const bool active = sb < nsb;  // wave-uniform
-    const float4 xv = reinterpret_cast<const float4 *>(x)[64 * (active ? sb : 0) + lane];
+    const float4 xv = load_x4<XB>(x, 64 * (active ? sb : 0) + lane);
     __builtin_amdgcn_sched_barrier(0);
     issue(0, 0);
     float4 xr = xv;  // the conversion stays below the tile loads
@@ -644,7 +645,7 @@ __global__ __launch_bounds__(kT2Threads) void gemv_q4_k_mfma_tile_kernel(
         if (row < nr) yout[row] = s;
     }
     __syncthreads();
-    for (int r = threadIdx.x; r < nr; r += kT2Threads) y[r0 + r] = yout[r];
+    for (int r = threadIdx.x; r < nr; r += kT2Threads) put(y, 0, r0 + r, rows, yout[r]);
 }
 
 
@@ -1109,6 +1110,36 @@ bool q4k_mfma_supported(int64_t row_bytes, int64_t cols, int64_t rows, const voi
            (reinterpret_cast<uintptr_t>(w) & 15u) == 0 && (reinterpret_cast<uintptr_t>(x) & 15u) == 0;
 }
 
+template <bool XB, class OUT>
+static hipError_t launch_q4k_tiles(const uint8_t *w, int64_t row_bytes, int nsb, const float *x, OUT y, int64_t rows,
+                                   hipStream_t stream) {
+    const int64_t cus = device_cus();
+    // one workgroup per CU, at most kT2MaxRows rows each, at least one tile each
+    int64_t grid = (rows + kTileRows - 1) / kTileRows;
+    if (grid > cus) grid = cus;
+    int64_t per = (rows + grid - 1) / grid;
+    if (per > kT2MaxRows) per = kT2MaxRows;
+    grid = (rows + per - 1) / per;
+    per = (rows + grid - 1) / grid;
+    grid = (rows + per - 1) / per;
+    hipLaunchKernelGGL((gemv_q4_k_mfma_tile_kernel<3, XB, OUT>), dim3((unsigned)grid), dim3(kT2Threads), 0, stream, w,
+                       row_bytes, nsb, x, y, rows, per);
+    return hipGetLastError();
+}
+
+bool linear_vec_supported(int type_id, int64_t row_bytes, int64_t rows, int64_t cols, const void *w, const void *x) {
+    const float *xf = static_cast<const float *>(x);
+    if (type_id == kQ6_K) return q6k_mfma_supported(row_bytes, cols, rows, w, xf);
+    return type_id == kQ4_K && cols <= 16 * kQK && cols % kQK == 0 && q4k_mfma_supported(row_bytes, cols, rows, w, xf);
+}
+
+hipError_t launch_linear_vec(int type_id, const uint8_t *w, int64_t row_bytes, int64_t rows, int64_t cols,
+                             const uint16_t *x, const Epilogue &y, hipStream_t stream) {
+    if (type_id == kQ6_K) return launch_linear_vec_q6k(w, row_bytes, cols, x, y, rows, stream);
+    return launch_q4k_tiles<true, Epilogue>(w, row_bytes, (int)(cols / kQK), reinterpret_cast<const float *>(x), y,
+                                            rows, stream);
+}
+
 hipError_t launch_gemv_q4k_mfma(const uint8_t *w, int64_t row_bytes, int64_t cols,
                                 const float *x, float *y, int64_t rows, hipStream_t stream,
                                 const uint8_t *prep, int64_t prep_rows) {
@@ -1140,17 +1171,7 @@ hipError_t launch_gemv_q4k_mfma(const uint8_t *w, int64_t row_bytes, int64_t col
         return hipGetLastError();
     }
     if (nsb <= 16) {
-        // one workgroup per CU, at most kT2MaxRows rows each, at least one tile each
-        int64_t grid = (rows + kTileRows - 1) / kTileRows;
-        if (grid > cus) grid = cus;
-        int64_t per = (rows + grid - 1) / grid;
-        if (per > kT2MaxRows) per = kT2MaxRows;
-        grid = (rows + per - 1) / per;
-        per = (rows + grid - 1) / grid;
-        grid = (rows + per - 1) / per;
-        hipLaunchKernelGGL((gemv_q4_k_mfma_tile_kernel<3>), dim3((unsigned)grid), dim3(kT2Threads), 0,
-                           stream, w, row_bytes, nsb, x, y, rows, per);
-        return hipGetLastError();
+        return launch_q4k_tiles<false, float *__restrict__>(w, row_bytes, nsb, x, y, rows, stream);
     }
     const MfmaPlan p = plan_mfma(rows, nsb);
     hipLaunchKernelGGL((gemv_q4_k_mfma_kernel<kQ4_K, 2, 64>), dim3((unsigned)p.grid), dim3(kMfThreads), 0,

@@ -44,6 +44,7 @@
 // 210 bytes, so every other one starts 2 bytes off a dword in LDS: a lane
 // reads aligned dwords and v_alignbyte_b32 realigns them (the shift is 0 or
 // 2, uniform per wave).
+#include "gguf_epilogue.hpp"
 #include "gguf_mfma_q4k.hpp"
 
 namespace gollek {
@@ -191,11 +192,12 @@ __device__ __forceinline__ void q6_x_operands_sums(uint32_t a01, uint32_t a23, u
 
 }  // namespace
 
-// XLDS: K > 4096, x's planes and digit sums for every superblock in LDS.
-template <bool XLDS>
+// XLDS: K > 4096, x's planes and digit sums for every superblock in LDS.  XB: x
+// holds bf16 bit patterns (the linear layer's), widened to fp32 exactly as they load.
+template <bool XLDS, bool XB = false, class OUT = float *__restrict__>
 __global__ __launch_bounds__(kQ6Threads) void gemv_q6_k_mfma_tile_kernel(
     const uint8_t *__restrict__ w, int64_t row_bytes64, int nsb, const float *__restrict__ x,
-    float *__restrict__ y, int64_t rows, int64_t rows_per_wg) {
+    OUT y, int64_t rows, int64_t rows_per_wg) {
     constexpr int kQ6Slots = XLDS ? 3 : 5;
     static_assert(kQ6DmaPerWave * kQ6Waves >= kQ6Dma, "item loads");
     static_assert(kQ6Waves * 1024 <= kQ6Slot, "x scratch fits a slot");
@@ -253,7 +255,7 @@ __global__ __launch_bounds__(kQ6Threads) void gemv_q6_k_mfma_tile_kernel(
     constexpr int kXl = (kQ6MaxSbLds + kQ6Waves - 1) / kQ6Waves;  // x superblocks per wave (XLDS)
     float4 xq[XLDS ? kXl : 1];
     if constexpr (!XLDS) {
-        const float4 xv = reinterpret_cast<const float4 *>(x)[64 * (active ? sb : 0) + lane];
+        const float4 xv = load_x4<XB>(x, 64 * (active ? sb : 0) + lane);
         __builtin_amdgcn_sched_barrier(0);
         issue(0, 0);
         xr = xv;  // the conversion stays below the first item's loads
@@ -265,7 +267,7 @@ __global__ __launch_bounds__(kQ6Threads) void gemv_q6_k_mfma_tile_kernel(
 #pragma unroll
         for (int i = 0; i < kXl; i++) {
             const int s2 = wv + kQ6Waves * i;
-            xq[i] = reinterpret_cast<const float4 *>(x)[64 * (s2 < nsb ? s2 : nsb - 1) + lane];
+            xq[i] = load_x4<XB>(x, 64 * (s2 < nsb ? s2 : nsb - 1) + lane);
         }
         __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
@@ -444,7 +446,7 @@ __global__ __launch_bounds__(kQ6Threads) void gemv_q6_k_mfma_tile_kernel(
         if (row < nr) yout[row] = s;
     }
     __syncthreads();
-    for (int r = threadIdx.x; r < nr; r += kQ6Threads) y[r0 + r] = yout[r];
+    for (int r = threadIdx.x; r < nr; r += kQ6Threads) put(y, 0, r0 + r, rows, yout[r]);
 }
 
 bool q6k_mfma_supported(int64_t row_bytes, int64_t cols, int64_t rows, const void *w, const float *x) {
@@ -458,10 +460,12 @@ bool q6k_mfma_supported(int64_t row_bytes, int64_t cols, int64_t rows, const voi
     return (int64_t)kQ6MaxRows * row_bytes < ((int64_t)1 << 31);
 }
 
-hipError_t launch_gemv_q6k_mfma(const uint8_t *w, int64_t row_bytes, int64_t cols, const float *x, float *y,
-                                int64_t rows, hipStream_t stream) {
+// XB and OUT as the kernel's (one workgroup per CU, at most kQ6MaxRows rows
+// each, at least one tile each).
+template <bool XB, class OUT>
+static hipError_t launch_q6k_tiles(const uint8_t *w, int64_t row_bytes, int64_t cols, const float *x, OUT y,
+                                   int64_t rows, hipStream_t stream) {
     const int64_t cus = device_cus();
-    // one workgroup per CU, at most kQ6MaxRows rows each, at least one tile each
     int64_t grid = (rows + kQ6TileRows - 1) / kQ6TileRows;
     if (grid > cus) grid = cus;
     int64_t per = (rows + grid - 1) / grid;
@@ -471,12 +475,22 @@ hipError_t launch_gemv_q6k_mfma(const uint8_t *w, int64_t row_bytes, int64_t col
     grid = (rows + per - 1) / per;
     const int nsb = (int)(cols / kQK);
     if (nsb <= 2 * kQ6HalfSb)
-        hipLaunchKernelGGL(gemv_q6_k_mfma_tile_kernel<false>, dim3((unsigned)grid), dim3(kQ6Threads), 0, stream, w,
-                           row_bytes, nsb, x, y, rows, per);
+        hipLaunchKernelGGL((gemv_q6_k_mfma_tile_kernel<false, XB, OUT>), dim3((unsigned)grid), dim3(kQ6Threads), 0,
+                           stream, w, row_bytes, nsb, x, y, rows, per);
     else
-        hipLaunchKernelGGL(gemv_q6_k_mfma_tile_kernel<true>, dim3((unsigned)grid), dim3(kQ6Threads), 0, stream, w,
-                           row_bytes, nsb, x, y, rows, per);
+        hipLaunchKernelGGL((gemv_q6_k_mfma_tile_kernel<true, XB, OUT>), dim3((unsigned)grid), dim3(kQ6Threads), 0,
+                           stream, w, row_bytes, nsb, x, y, rows, per);
     return hipGetLastError();
+}
+
+hipError_t launch_gemv_q6k_mfma(const uint8_t *w, int64_t row_bytes, int64_t cols, const float *x, float *y,
+                                int64_t rows, hipStream_t stream) {
+    return launch_q6k_tiles<false, float *__restrict__>(w, row_bytes, cols, x, y, rows, stream);
+}
+
+hipError_t launch_linear_vec_q6k(const uint8_t *w, int64_t row_bytes, int64_t cols, const uint16_t *x,
+                                 const Epilogue &y, int64_t rows, hipStream_t stream) {
+    return launch_q6k_tiles<true, Epilogue>(w, row_bytes, cols, reinterpret_cast<const float *>(x), y, rows, stream);
 }
 
 }  // namespace gollek

@@ -160,6 +160,14 @@ size_t linear_tile_workspace_bytes(int M, int N, int K);
 hipError_t launch_linear(int type_id, const uint8_t *w, int64_t row_bytes, const uint16_t *x, const Epilogue &y, int M,
                          int N, int K, hipStream_t stream, float *workspace, size_t workspace_bytes,
                          const uint8_t *prep, int64_t prep_rows);
+// Its M = 1 where the column kernel does not take the weight and a mat-vec kernel
+// of 16-row tiles does: Q6_K (K a multiple of 2048 up to 14336) and Q4_K up to
+// K = 4096; x and w 16-byte aligned.
+bool linear_vec_supported(int type_id, int64_t row_bytes, int64_t rows, int64_t cols, const void *w, const void *x);
+hipError_t launch_linear_vec(int type_id, const uint8_t *w, int64_t row_bytes, int64_t rows, int64_t cols,
+                             const uint16_t *x, const Epilogue &y, hipStream_t stream);
+hipError_t launch_linear_vec_q6k(const uint8_t *w, int64_t row_bytes, int64_t cols, const uint16_t *x,
+                                 const Epilogue &y, int64_t rows, hipStream_t stream);
 
 // Workspace layout of the grouped MoE FFN (byte offsets; gguf_moe.hip).
 struct MoeLayout {

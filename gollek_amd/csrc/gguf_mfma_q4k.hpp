@@ -89,6 +89,18 @@ __device__ __forceinline__ void col_load(__amdgpu_buffer_rsrc_t rs, uint8_t *dst
     __builtin_amdgcn_raw_ptr_buffer_load_lds(rs, (lds_ptr)dst, 16, off, 0, 0, kStreamLoad);
 }
 
+// Elements 4 i .. 4 i + 3 of x (XB: bf16 bit patterns, 8-byte aligned, widened exactly).
+template <bool XB>
+__device__ __forceinline__ float4 load_x4(const float *x, int i) {
+    if constexpr (XB) {
+        const uint2 u = reinterpret_cast<const uint2 *>(x)[i];
+        return float4{__uint_as_float(u.x << 16), __uint_as_float(u.x & 0xFFFF0000u), __uint_as_float(u.y << 16),
+                      __uint_as_float(u.y & 0xFFFF0000u)};
+    } else {
+        return reinterpret_cast<const float4 *>(x)[i];
+    }
+}
+
 // Wave-wide: lane l holds elements 4 l .. 4 l + 3 of a superblock of x.
 // Writes the four balanced signed-byte digit planes of X = trunc(x /
 // 2^(e-30)), max |x| < 2^e, to `scratch` (1 KB of LDS private to the wave:

@@ -419,3 +419,29 @@ def test_uneven_splits_of_k(t, rows, cols, m):
         y = re.clone()
         call(wt, x, m, y, y_type, ops.ACT_GELU_TANH, b, mu, y, wt.workspace(m))
         check(y, expected(wt, xb, ops.ACT_GELU_TANH, b, mu, re, y_type), f"{t} {rows}x{cols} m={m} type {y_type}")
+
+
+# The mat-vec's 16-row tiles at one token: Q6_K with one and with several
+# superblocks a wave, rows from one to several tiles a workgroup, and Q4_K
+# beyond 64 rows a compute unit; in place, unaligned y, no workspace.
+@pytest.mark.parametrize("t,rows,cols", [("q6_k", 1, 2048), ("q6_k", 17, 4096), ("q6_k", 500, 2048), ("q6_k", 4100, 4096),
+                                         ("q6_k", 16, 6144), ("q6_k", 333, 14336), ("q6_k", 9000, 2048),
+                                         ("q4_k", 16400, 256), ("q4_k", 20001, 512), ("q4_k", 16390, 4096)])
+@pytest.mark.parametrize("y_type", [_native.F32, _native.BF16])
+def test_one_token_on_row_tiles(t, rows, cols, y_type):
+    print(f"[gpu] linear {t} {rows}x{cols} m=1 type={y_type}", flush=True)
+    wt = Weight(TYPES[t], rows, cols, 17)
+    xb = syn.activation_bf16(1, cols, seed=rows)
+    x = torch.from_numpy(xb.view(np.int16)).cuda()
+    b, mu, re = operands(1, rows, y_type, cols, True, True, True)
+    out = torch.full((rows + 2,), 7.0, device="cuda", dtype=DTYPE[y_type])
+    y = out[1:rows + 1]
+    y.copy_(re[0])
+    call(wt, x, 1, y, y_type, ops.ACT_SILU, b, mu, y)
+    check(y.reshape(1, rows), expected(wt, xb, ops.ACT_SILU, b, mu, re, y_type), f"{t} {rows}x{cols}")
+    assert out[0] == 7.0 and out[-1] == 7.0
+    call(wt, x, 1, y, y_type)
+    check(y.reshape(1, rows), expected(wt, xb, 0, None, None, None, y_type), f"{t} {rows}x{cols} alone")
+    xb[0, cols // 2] = 0x7FC0  # a NaN in x reaches every sum
+    call(wt, torch.from_numpy(xb.view(np.int16)).cuda(), 1, y, y_type)
+    assert torch.isnan(y).all() and out[0] == 7.0 and out[-1] == 7.0

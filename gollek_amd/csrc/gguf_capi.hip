@@ -912,6 +912,12 @@ bool overlaps(const void *y, int64_t y_stride, const void *b, int64_t b_stride, 
     return !(apart >= width && row - apart >= width);
 }
 
+// Whether matrix y and `bytes` bytes at b share a byte (y's gaps between rows counted as y's).
+bool within(const void *y, int64_t m, int64_t n, int64_t y_stride, int64_t size, const void *b, int64_t bytes) {
+    const uintptr_t ya = reinterpret_cast<uintptr_t>(y), ba = reinterpret_cast<uintptr_t>(b);
+    return ba < ya + (uintptr_t)(((m - 1) * y_stride + n) * size) && ya < ba + (uintptr_t)bytes;
+}
+
 // Checks a linear call's epilogue and fills `out`.  Strides of 0 are packed rows.
 int32_t make_epilogue(const gollek_hip_weight *w, int64_t m, const float *bias, int32_t activation, const void *mul,
                       int64_t mul_stride, const void *residual, int64_t residual_stride, void *y, int32_t y_type,
@@ -945,6 +951,8 @@ int32_t make_epilogue(const gollek_hip_weight *w, int64_t m, const float *bias, 
     }
     if (reinterpret_cast<uintptr_t>(bias) % sizeof(float) != 0)
         return fail(GOLLEK_HIP_ERR_ARG, err, err_len, "The bias is not aligned to its 4-byte elements");
+    if (bias != nullptr && m > 0 && n > 0 && within(y, m, n, y_stride, size, bias, n * (int64_t)sizeof(float)))
+        return fail(GOLLEK_HIP_ERR_ARG, err, err_len, "The output overlaps the bias");
     *out = gollek::make_epilogue(y, bias, mul, residual, y_stride, mul_stride, residual_stride, activation, y_type);
     return GOLLEK_HIP_OK;
 }
@@ -976,10 +984,10 @@ int32_t gollek_hip_linear_device(gollek_hip_weight *w, const uint16_t *x, int64_
         ok(err, err_len);
         return GOLLEK_HIP_OK;
     }
-    const uintptr_t ya = reinterpret_cast<uintptr_t>(y), xa = reinterpret_cast<uintptr_t>(x);
-    const uintptr_t ye = ya + (uintptr_t)(((m - 1) * epi.y_stride + w->rows) * element_size(y_type));
-    if (xa < ye && ya < xa + (uintptr_t)(2 * m * w->cols))
+    if (within(y, m, w->rows, epi.y_stride, element_size(y_type), x, 2 * m * w->cols))
         return fail(GOLLEK_HIP_ERR_ARG, err, err_len, "The output overlaps the input");
+    if (workspace != nullptr && within(y, m, w->rows, epi.y_stride, element_size(y_type), workspace, workspace_bytes))
+        return fail(GOLLEK_HIP_ERR_ARG, err, err_len, "The output overlaps the workspace");
     const DeviceGuard device(w->device);
     const hipError_t e = gollek::launch_linear(w->type_id, w->data, w->row_bytes, x, epi, (int)m, (int)w->rows,
                                                (int)w->cols, static_cast<hipStream_t>(stream),

@@ -505,11 +505,13 @@ __global__ __launch_bounds__(kThreads) void gemm_tile_kernel(const uint8_t *__re
 }
 
 // A linear layer's split product: the partials in split order, then the
-// epilogue (4 elements of a row a thread).
+// epilogue (4 elements of a row a thread; rows and columns share one grid axis,
+// so neither is bound by the other axes' 65535).
 __global__ __launch_bounds__(256) void linear_reduce_kernel(const float *__restrict__ part, int S, int M, int N,
                                                             Epilogue y) {
-    const int n = 4 * ((int)blockIdx.x * 256 + (int)threadIdx.x), m = (int)blockIdx.y;
-    if (n >= N) return;
+    const uint32_t i4 = blockIdx.x * 256u + threadIdx.x, across = ((uint32_t)N + 3u) / 4u;
+    const int m = (int)(i4 / across), n = 4 * (int)(i4 - (uint32_t)m * across);
+    if (m >= M) return;
     const int64_t mn = (int64_t)M * N;
     const float *const p = part + (int64_t)m * N + n;
     if ((N & 3) == 0) {
@@ -727,8 +729,9 @@ hipError_t launch_gemm_reduce(const float *part, int S, int M, int N, float *y, 
 }
 
 hipError_t launch_gemm_reduce(const float *part, int S, int M, int N, const Epilogue &y, hipStream_t stream) {
-    hipLaunchKernelGGL(linear_reduce_kernel, dim3((unsigned)((N + 1023) / 1024), (unsigned)M), dim3(256), 0, stream,
-                       part, S, M, N, y);
+    const int64_t blocks = ((int64_t)M * (((int64_t)N + 3) / 4) + 255) / 256;
+    if (blocks > (int64_t)1 << 23) return hipErrorInvalidValue;  // (no plan splits 2^33 elements)
+    hipLaunchKernelGGL(linear_reduce_kernel, dim3((unsigned)blocks), dim3(256), 0, stream, part, S, M, N, y);
     return hipGetLastError();
 }
 

@@ -233,9 +233,10 @@ int64_t gollek_hip_linear_workspace_bytes(const gollek_hip_weight *weight, int64
  * device; allocates nothing, so it can be captured into a graph.  The strides
  * are elements between rows, at least `rows` (0: packed).  Y may be mul or
  * residual (the same address and stride), or another column range of one wider
- * matrix; any other overlap of Y with mul, residual or X -> ARG, and Y must not
- * overlap bias, workspace or the weight.  Elements of Y's rows past column
- * `rows` are left as they are.  Pointers are aligned to their elements (else
+ * matrix; any other overlap of Y with mul or residual, and any of Y with X, bias
+ * or workspace, -> ARG (the gaps between Y's rows counted in; Y must not overlap
+ * the weight either).  Elements of Y's rows past column `rows` are left as they
+ * are.  Pointers are aligned to their elements (else
  * ARG).  workspace (256-byte aligned, else ARG) may be smaller than
  * gollek_hip_linear_workspace_bytes, or NULL: the call splits less, which
  * changes Y by the rounding of the sums' order alone.  Calls that share a

@@ -445,3 +445,52 @@ def test_one_token_on_row_tiles(t, rows, cols, y_type):
     xb[0, cols // 2] = 0x7FC0  # a NaN in x reaches every sum
     call(wt, torch.from_numpy(xb.view(np.int16)).cuda(), 1, y, y_type)
     assert torch.isnan(y).all() and out[0] == 7.0 and out[-1] == 7.0
+
+
+def test_more_rows_than_a_grid_axis():
+    # a tall and narrow product that splits K: more than 65535 rows go through the reduction
+    rows, cols, m = 8, 4096, 66560
+    print(f"[gpu] linear q8_0 {rows}x{cols} m={m}", flush=True)
+    wt = Weight(syn.Q8_0, rows, cols, 18)
+    assert wt.handle.linear_workspace_bytes(m) >= 2 * m * rows * 4
+    some = syn.activation_bf16(64, cols, seed=18)
+    x = torch.from_numpy(some.view(np.int16)).cuda().repeat(m // 64, 1)
+    re = torch.from_numpy(np.random.default_rng(18).normal(size=(64, rows)).astype(np.float32)).to(torch.bfloat16).cuda()
+    y = re.repeat(m // 64, 1)
+    call(wt, x, m, y, _native.BF16, ops.ACT_SILU, None, None, y, wt.workspace(m))
+    want, tol = expected(wt, some, ops.ACT_SILU, None, None, re, _native.BF16)
+    check(y, (np.tile(want, (m // 64, 1)), np.tile(tol, (m // 64, 1))), "tall")
+
+
+@pytest.mark.parametrize("t,rows,cols,m", [("q4_k", 300, 512, 3), ("q8_0", 256, 512, 20), ("q6_k", 160, 512, 70),
+                                           ("q4_0", 256, 4096, 40)])
+def test_16_bit_operands_in_place(t, rows, cols, m):
+    wt = Weight(TYPES[t], rows, cols, 19)
+    xb = syn.activation_bf16(m, cols, seed=19)
+    x = torch.from_numpy(xb.view(np.int16)).cuda()
+    for y_type in (_native.BF16, _native.F16):
+        b, mu, re = operands(m, rows, y_type, 19, True, True, True)
+        y = re.clone()
+        call(wt, x, m, y, y_type, ops.ACT_SILU, b, mu, y, wt.workspace(m))
+        check(y, expected(wt, xb, ops.ACT_SILU, b, mu, re, y_type), "y is the residual")
+        y = mu.clone()
+        call(wt, x, m, y, y_type, ops.ACT_SILU, b, y, y, wt.workspace(m))
+        check(y, expected(wt, xb, ops.ACT_SILU, b, mu, mu, y_type), "y is mul and the residual")
+
+
+def test_output_over_its_bias_or_workspace_is_refused():
+    rows, cols, m = 64, 256, 4
+    wt = Weight(syn.Q8_0, rows, cols, 22)
+    x = torch.zeros((m, cols), device="cuda", dtype=torch.int16)
+    y = torch.zeros(m * rows + 256, device="cuda")
+    yp = (y.data_ptr() + 255) // 256 * 256
+    for kw in ({"bias_ptr": yp}, {"bias_ptr": yp + 4 * (m * rows - 1)}, {"bias_ptr": yp - 4 * (rows - 1)},
+               {"ws_ptr": yp, "ws_bytes": 256}, {"ws_ptr": yp - 256, "ws_bytes": 512}):
+        with pytest.raises(ops.IllegalArgumentError):
+            wt.handle.linear(x.data_ptr(), m, yp, _native.F32, **kw)
+    room = torch.zeros(512 + m * rows + rows, device="cuda")
+    zp = (room.data_ptr() + 255) // 256 * 256 + 4 * rows
+    for bias in (zp - 4 * rows, zp + 4 * m * rows):  # right before it, right behind it
+        wt.handle.linear(x.data_ptr(), m, zp, _native.F32, bias_ptr=bias, ws_ptr=zp - 4 * rows, ws_bytes=4 * rows,
+                         stream=stream())
+    torch.cuda.synchronize()

@@ -17,6 +17,8 @@
 #include <hip/hip_runtime.h>
 #include <stdint.h>
 
+#include <type_traits>
+
 namespace gollek {
 
 enum ElementType : int { kF32 = 0, kF16 = 1, kBF16 = 30 };  // ggml type ids
@@ -78,6 +80,17 @@ __device__ __forceinline__ void store_element(void *p, int type, int64_t i, floa
     else static_cast<__bf16 *>(p)[i] = (__bf16)v;
 }
 
+template <class OUT>
+constexpr bool kHasEpilogue = false;
+template <>
+inline constexpr bool kHasEpilogue<Epilogue> = true;
+
+// The type a kernel takes for OUT.  Launches name it: a plain output deduced from
+// an argument, or passed on as float *, would lose its __restrict__.
+typedef float *__restrict__ PlainOut;
+template <class OUT>
+using KernelOut = std::conditional_t<kHasEpilogue<OUT>, OUT, PlainOut>;
+
 // Element (m, n) of an output with N columns.
 __device__ __forceinline__ void put(float *y, int64_t m, int64_t n, int64_t N, float v) { y[m * N + n] = v; }
 __device__ __forceinline__ void put(const Epilogue &e, int64_t m, int64_t n, int64_t, float v) {
@@ -111,17 +124,17 @@ __device__ __forceinline__ void put(const Epilogue &e, int64_t m, int64_t n, int
     store_element(e.y, e.type, m * e.y_stride + n, v);
 }
 
-// 16 bytes of elements: 4 floats, 8 halves.
-template <int TYPE>
-struct Elements {
-    static constexpr int kSize = TYPE == kF32 ? 4 : 2, kCount = 16 / kSize;
-    typedef uint32_t v4 __attribute__((ext_vector_type(4)));
-    v4 bits;
+// Elements in W words: 16 bytes of them (Elements), or four (Quad).
+template <int TYPE, int W>
+struct Words {
+    static constexpr int kSize = TYPE == kF32 ? 4 : 2, kCount = 4 * W / kSize;
+    typedef uint32_t words __attribute__((ext_vector_type(W)));
+    words bits;
     __device__ __forceinline__ void load(const void *p, int64_t i) {
-        bits = *reinterpret_cast<const v4 *>(static_cast<const uint8_t *>(p) + i * kSize);
+        bits = *reinterpret_cast<const words *>(static_cast<const uint8_t *>(p) + i * kSize);
     }
     __device__ __forceinline__ void store(void *p, int64_t i) const {
-        *reinterpret_cast<v4 *>(static_cast<uint8_t *>(p) + i * kSize) = bits;
+        *reinterpret_cast<words *>(static_cast<uint8_t *>(p) + i * kSize) = bits;
     }
     __device__ __forceinline__ float get(int j) const {
         if constexpr (TYPE == kF32) return __uint_as_float(bits[j]);
@@ -131,7 +144,7 @@ struct Elements {
     }
     __device__ __forceinline__ void set(const float *v) {
 #pragma unroll
-        for (int j = 0; j < 4; j++) {
+        for (int j = 0; j < W; j++) {
             if constexpr (TYPE == kF32) {
                 bits[j] = __float_as_uint(v[j]);
             } else if constexpr (TYPE == kBF16) {
@@ -144,6 +157,10 @@ struct Elements {
         }
     }
 };
+template <int TYPE>
+using Elements = Words<TYPE, 4>;
+template <int TYPE>
+using Quad = Words<TYPE, TYPE == kF32 ? 4 : 2>;
 
 // The activations of C values (one uniform branch for all of them).
 template <bool FAST, int C>
@@ -167,9 +184,9 @@ __device__ __forceinline__ void activate_all(int act, float (&v)[C]) {
 // time, in rounds of THREADS of them; the mul and residual of up to four rounds
 // (a batch) are loaded together, a batch before it is used: the first by
 // tile_ahead, which may stand anywhere before, the next while one is computed.
-// (Element by element, straight from the accumulators, every load waited behind
-// the store before it: Q4_K M = 2048, 14336 x 4096 with SiLU and mul 464 against
-// 378 us.)
+// (Q4_K M = 2048, 14336 x 4096 with SiLU and mul: 464 us element by element,
+// straight from the accumulators, where every load waited behind the store before
+// it; 378 in rows; 344 with the loads a batch ahead and activations FAST.)
 template <int COLS>
 constexpr int kTilePitch = COLS + 4;
 
@@ -288,11 +305,6 @@ __device__ __forceinline__ float *split_output(float *y, float *part, int split,
 __device__ __forceinline__ float *split_output(const Epilogue &, float *part, int split, int64_t mn) {
     return part + split * mn;
 }
-
-template <class OUT>
-constexpr bool kHasEpilogue = false;
-template <>
-inline constexpr bool kHasEpilogue<Epilogue> = true;
 
 // Host side: workspace bytes left for the S - 1 partials that a split plan
 // counts (an epilogue's split 0 takes one more), and whether a product's

@@ -539,6 +539,7 @@ template <class OUT>
 hipError_t launch_gemm(int type_id, const uint8_t *w, int64_t row_bytes, const uint16_t *x, OUT y,
                        int M, int N, int K, hipStream_t stream, float *workspace, size_t workspace_bytes,
                        const uint8_t *prep, int64_t prep_rows) {
+    using Out = KernelOut<OUT>;
     if (M <= 0) return hipSuccess;
     const bool aligned = (reinterpret_cast<uintptr_t>(w) & 3u) == 0 && (row_bytes & 3) == 0 &&
                          (reinterpret_cast<uintptr_t>(x) & 15u) == 0;
@@ -560,10 +561,10 @@ hipError_t launch_gemm(int type_id, const uint8_t *w, int64_t row_bytes, const u
     if (type_id == kQ8_0 && aligned && M <= 32 && N % 16 == 0 && K % 256 == 0 &&
         (int64_t)16 * row_bytes < ((int64_t)1 << 31) && (int64_t)M * K * 2 < ((int64_t)1 << 31)) {
         if (M <= 16)
-            hipLaunchKernelGGL((gemm_q8_0_bf16_skinny_kernel<1, 4, OUT>), dim3(N / 16), dim3(256), 0, stream, w,
+            hipLaunchKernelGGL((gemm_q8_0_bf16_skinny_kernel<1, 4, Out>), dim3(N / 16), dim3(256), 0, stream, w,
                                row_bytes, x, y, M, N, K);
         else
-            hipLaunchKernelGGL((gemm_q8_0_bf16_skinny_kernel<2, 4, OUT>), dim3(N / 16), dim3(256), 0, stream, w,
+            hipLaunchKernelGGL((gemm_q8_0_bf16_skinny_kernel<2, 4, Out>), dim3(N / 16), dim3(256), 0, stream, w,
                                row_bytes, x, y, M, N, K);
         return hipGetLastError();
     }
@@ -583,25 +584,25 @@ hipError_t launch_gemm(int type_id, const uint8_t *w, int64_t row_bytes, const u
         const int64_t wide = (int64_t)((N + 63) / 64) * ((M + 63) / 64);
         if (mt == 4 && wide >= 2 * (int64_t)device_cus()) {
             const dim3 g6((unsigned)((N + 63) / 64), (unsigned)((M + 63) / 64));
-            hipLaunchKernelGGL((gemm_q6k_f32_kernel<4, 4, OUT>), g6, dim3(256), 0, stream, w, row_bytes, x, y, M, N, K);
+            hipLaunchKernelGGL((gemm_q6k_f32_kernel<4, 4, Out>), g6, dim3(256), 0, stream, w, row_bytes, x, y, M, N, K);
         } else {
             const dim3 g6((unsigned)((N + 15) / 16), (unsigned)((M + 16 * mt - 1) / (16 * mt)));
             if (mt == 1)
-                hipLaunchKernelGGL((gemm_q6k_f32_kernel<1, 1, OUT>), g6, dim3(256), 0, stream, w, row_bytes, x, y, M, N, K);
+                hipLaunchKernelGGL((gemm_q6k_f32_kernel<1, 1, Out>), g6, dim3(256), 0, stream, w, row_bytes, x, y, M, N, K);
             else if (mt == 2)
-                hipLaunchKernelGGL((gemm_q6k_f32_kernel<2, 1, OUT>), g6, dim3(256), 0, stream, w, row_bytes, x, y, M, N, K);
+                hipLaunchKernelGGL((gemm_q6k_f32_kernel<2, 1, Out>), g6, dim3(256), 0, stream, w, row_bytes, x, y, M, N, K);
             else
-                hipLaunchKernelGGL((gemm_q6k_f32_kernel<4, 1, OUT>), g6, dim3(256), 0, stream, w, row_bytes, x, y, M, N, K);
+                hipLaunchKernelGGL((gemm_q6k_f32_kernel<4, 1, Out>), g6, dim3(256), 0, stream, w, row_bytes, x, y, M, N, K);
         }
         return hipGetLastError();
     }
     if (type_id == kQ5_K || type_id == kQ6_K) {
         const dim3 g16((unsigned)((N + 15) / 16), (unsigned)((M + 15) / 16));
         if (type_id == kQ5_K)
-            hipLaunchKernelGGL((gemm_kquant_generic_kernel<kQ5_K, OUT>), g16, dim3(256), 0, stream, w, row_bytes, x, y, M,
+            hipLaunchKernelGGL((gemm_kquant_generic_kernel<kQ5_K, Out>), g16, dim3(256), 0, stream, w, row_bytes, x, y, M,
                                N, K);
         else
-            hipLaunchKernelGGL((gemm_kquant_generic_kernel<kQ6_K, OUT>), g16, dim3(256), 0, stream, w, row_bytes, x, y, M,
+            hipLaunchKernelGGL((gemm_kquant_generic_kernel<kQ6_K, Out>), g16, dim3(256), 0, stream, w, row_bytes, x, y, M,
                                N, K);
         return hipGetLastError();
     }
@@ -609,13 +610,13 @@ hipError_t launch_gemm(int type_id, const uint8_t *w, int64_t row_bytes, const u
     const dim3 grid((unsigned)((total + 255) / 256)), block(256);
     switch (type_id) {
     case kQ8_0:
-        hipLaunchKernelGGL(gemm_q8_0_generic_kernel<OUT>, grid, block, 0, stream, w, row_bytes, x, y, M, N, K);
+        hipLaunchKernelGGL(gemm_q8_0_generic_kernel<Out>, grid, block, 0, stream, w, row_bytes, x, y, M, N, K);
         break;
     case kQ4_0:
-        hipLaunchKernelGGL((gemm_generic_kernel<kQ4_0, OUT>), grid, block, 0, stream, w, row_bytes, x, y, M, N, K);
+        hipLaunchKernelGGL((gemm_generic_kernel<kQ4_0, Out>), grid, block, 0, stream, w, row_bytes, x, y, M, N, K);
         break;
     case kQ4_K:
-        hipLaunchKernelGGL((gemm_generic_kernel<kQ4_K, OUT>), grid, block, 0, stream, w, row_bytes, x, y, M, N, K);
+        hipLaunchKernelGGL((gemm_generic_kernel<kQ4_K, Out>), grid, block, 0, stream, w, row_bytes, x, y, M, N, K);
         break;
     default:
         return hipErrorInvalidValue;

@@ -506,7 +506,50 @@ __global__ __launch_bounds__(kThreads) void gemm_tile_kernel(const uint8_t *__re
 
 // A linear layer's split product: the partials in split order, then the
 // epilogue (4 elements of a row a thread; rows and columns share one grid axis,
-// so neither is bound by the other axes' 65535).
+// so neither is bound by the other axes' 65535).  Whole quads of aligned rows load
+// all that they need before they store anything.
+template <int TYPE>
+__device__ __forceinline__ void linear_reduce_quad(const float *p, int S, int64_t mn, const Epilogue &y, int m, int n) {
+    Quad<TYPE> mul, residual;
+    float bias[4];
+    if (y.mul != nullptr) mul.load(y.mul, m * y.mul_stride + n);
+    if (y.residual != nullptr) residual.load(y.residual, m * y.residual_stride + n);
+    if (y.bias != nullptr) {
+#pragma unroll
+        for (int i = 0; i < 4; i++) bias[i] = y.bias[n + i];
+    }
+    float4 b[8];
+#pragma unroll
+    for (int k = 0; k < 8; k++)
+        if (k < S) b[k] = *reinterpret_cast<const float4 *>(p + k * mn);
+    float v[4] = {b[0].x, b[0].y, b[0].z, b[0].w};
+#pragma unroll
+    for (int k = 1; k < 8; k++) {
+        if (k < S) {
+            v[0] += b[k].x;
+            v[1] += b[k].y;
+            v[2] += b[k].z;
+            v[3] += b[k].w;
+        }
+    }
+    if (y.bias != nullptr) {
+#pragma unroll
+        for (int i = 0; i < 4; i++) v[i] += bias[i];
+    }
+    activate_all<TYPE != kF32>(y.act, v);
+    if (y.mul != nullptr) {
+#pragma unroll
+        for (int i = 0; i < 4; i++) v[i] *= mul.get(i);
+    }
+    if (y.residual != nullptr) {
+#pragma unroll
+        for (int i = 0; i < 4; i++) v[i] += residual.get(i);
+    }
+    Quad<TYPE> out;
+    out.set(v);
+    out.store(y.y, m * y.y_stride + n);
+}
+
 __global__ __launch_bounds__(256) void linear_reduce_kernel(const float *__restrict__ part, int S, int M, int N,
                                                             Epilogue y) {
     const uint32_t i4 = blockIdx.x * 256u + threadIdx.x, across = ((uint32_t)N + 3u) / 4u;
@@ -514,29 +557,16 @@ __global__ __launch_bounds__(256) void linear_reduce_kernel(const float *__restr
     if (m >= M) return;
     const int64_t mn = (int64_t)M * N;
     const float *const p = part + (int64_t)m * N + n;
-    if ((N & 3) == 0) {
-        float4 b[8];
-#pragma unroll
-        for (int k = 0; k < 8; k++)
-            if (k < S) b[k] = *reinterpret_cast<const float4 *>(p + k * mn);
-        float4 a = b[0];
-#pragma unroll
-        for (int k = 1; k < 8; k++) {
-            if (k < S) {
-                a.x += b[k].x;
-                a.y += b[k].y;
-                a.z += b[k].z;
-                a.w += b[k].w;
-            }
-        }
-        const float v[4] = {a.x, a.y, a.z, a.w};
-        for (int i = 0; i < 4; i++) put(y, m, n + i, N, v[i]);
-    } else {
-        for (int i = 0; i < 4 && n + i < N; i++) {
-            float a = p[i];
-            for (int k = 1; k < S; k++) a += p[k * mn + i];
-            put(y, m, n + i, N, a);
-        }
+    if ((N & 3) == 0 && y.vec) {
+        if (y.type == kF32) linear_reduce_quad<kF32>(p, S, mn, y, m, n);
+        else if (y.type == kF16) linear_reduce_quad<kF16>(p, S, mn, y, m, n);
+        else linear_reduce_quad<kBF16>(p, S, mn, y, m, n);
+        return;
+    }
+    for (int i = 0; i < 4 && n + i < N; i++) {
+        float a = p[i];
+        for (int k = 1; k < S; k++) a += p[k * mn + i];
+        put(y, m, n + i, N, a);
     }
 }
 
@@ -698,10 +728,10 @@ hipError_t launch_gemm_tile(int type_id, const uint8_t *w, int64_t row_bytes, co
     };
 #define GOLLEK_TILE_LAUNCH(TY)                                                                              \
     do {                                                                                                    \
-        if (mt == 1) ragged ? run(&gemm_tile_kernel<TY, 1, true, OUT>) : run(&gemm_tile_kernel<TY, 1, false, OUT>);   \
-        else if (mt == 2) ragged ? run(&gemm_tile_kernel<TY, 2, true, OUT>) : run(&gemm_tile_kernel<TY, 2, false, OUT>); \
-        else if (mt == 4) ragged ? run(&gemm_tile_kernel<TY, 4, true, OUT>) : run(&gemm_tile_kernel<TY, 4, false, OUT>); \
-        else ragged ? run(&gemm_tile_kernel<TY, 8, true, OUT>) : run(&gemm_tile_kernel<TY, 8, false, OUT>);           \
+        if (mt == 1) ragged ? run(&gemm_tile_kernel<TY, 1, true, KernelOut<OUT>>) : run(&gemm_tile_kernel<TY, 1, false, KernelOut<OUT>>);   \
+        else if (mt == 2) ragged ? run(&gemm_tile_kernel<TY, 2, true, KernelOut<OUT>>) : run(&gemm_tile_kernel<TY, 2, false, KernelOut<OUT>>); \
+        else if (mt == 4) ragged ? run(&gemm_tile_kernel<TY, 4, true, KernelOut<OUT>>) : run(&gemm_tile_kernel<TY, 4, false, KernelOut<OUT>>); \
+        else ragged ? run(&gemm_tile_kernel<TY, 8, true, KernelOut<OUT>>) : run(&gemm_tile_kernel<TY, 8, false, KernelOut<OUT>>);           \
     } while (0)
     switch (type_id) {
     case kQ8_0:

@@ -545,7 +545,8 @@ constexpr int kT2MaxRows = 1024;                                // rows per work
 }  // namespace
 
 // XB: x holds bf16 bit patterns (the linear layer's), widened to fp32 exactly.
-template <int NSLOT, bool XB = false, class OUT = float *__restrict__>
+// OUT: Epilogue or PlainOut.
+template <int NSLOT, bool XB, class OUT>
 __global__ __launch_bounds__(kT2Threads) void gemv_q4_k_mfma_tile_kernel(
     const uint8_t *__restrict__ w, int64_t row_bytes64, int nsb, const float *__restrict__ x,
     OUT y, int64_t rows, int64_t rows_per_wg) {
@@ -727,7 +728,7 @@ struct ColGeom {
 // take a second operand set (a second MFMA per chunk on the same B).
 // Vector v is x + v K, its results y + v rows.  XB: x holds bf16 bit
 // patterns (the GEMM's input), widened to fp32 exactly as they load.
-template <int TYPE, bool PREP, int NV = 1, bool XB = false, class OUT = float *__restrict__>
+template <int TYPE, bool PREP, int NV, bool XB, class OUT>
 __global__ __launch_bounds__(kColThreads) void gemv_mfma_col_kernel(
     const uint8_t *__restrict__ w, int64_t row_bytes64, int nsb, const float *__restrict__ x,
     OUT y, int64_t rows, int rows_per_wg) {
@@ -910,7 +911,7 @@ constexpr int kWideMaxCols = 4;  // columns per wave (K <= 16384)
 // NV = 2, XB: as the column kernel's (the small-M GEMM's M = 2 on bf16 X):
 // the second vector's digits in A rows 8..15 of the same compact operands,
 // its sums in output lanes 32..63 and a second row-sum buffer.
-template <int TYPE, bool PREP, int NV = 1, bool XB = false, class OUT = float *__restrict__>
+template <int TYPE, bool PREP, int NV, bool XB, class OUT>
 __global__ __launch_bounds__(kColThreads) void gemv_mfma_wide_kernel(
     const uint8_t *__restrict__ w, int64_t row_bytes64, int nsb, const float *__restrict__ x,
     OUT y, int64_t rows, int rows_per_wg) {
@@ -1155,23 +1156,23 @@ hipError_t launch_gemv_q4k_mfma(const uint8_t *w, int64_t row_bytes, int64_t col
         const uint8_t *src = use_prep ? prep : w;
         if (nsb <= kColWaves) {
             if (use_prep)
-                hipLaunchKernelGGL((gemv_mfma_col_kernel<kQ4_K, true>), grid, dim3(kColThreads), 0, stream, src,
+                hipLaunchKernelGGL((gemv_mfma_col_kernel<kQ4_K, true, 1, false, PlainOut>), grid, dim3(kColThreads), 0, stream, src,
                                    row_bytes, nsb, x, y, rows, (int)col_rows);
             else
-                hipLaunchKernelGGL((gemv_mfma_col_kernel<kQ4_K, false>), grid, dim3(kColThreads), 0, stream, src,
+                hipLaunchKernelGGL((gemv_mfma_col_kernel<kQ4_K, false, 1, false, PlainOut>), grid, dim3(kColThreads), 0, stream, src,
                                    row_bytes, nsb, x, y, rows, (int)col_rows);
         } else {
             if (use_prep)
-                hipLaunchKernelGGL((gemv_mfma_wide_kernel<kQ4_K, true>), grid, dim3(kColThreads), 0, stream, src,
+                hipLaunchKernelGGL((gemv_mfma_wide_kernel<kQ4_K, true, 1, false, PlainOut>), grid, dim3(kColThreads), 0, stream, src,
                                    row_bytes, nsb, x, y, rows, (int)col_rows);
             else
-                hipLaunchKernelGGL((gemv_mfma_wide_kernel<kQ4_K, false>), grid, dim3(kColThreads), 0, stream, src,
+                hipLaunchKernelGGL((gemv_mfma_wide_kernel<kQ4_K, false, 1, false, PlainOut>), grid, dim3(kColThreads), 0, stream, src,
                                    row_bytes, nsb, x, y, rows, (int)col_rows);
         }
         return hipGetLastError();
     }
     if (nsb <= 16) {
-        return launch_q4k_tiles<false, float *__restrict__>(w, row_bytes, nsb, x, y, rows, stream);
+        return launch_q4k_tiles<false, PlainOut>(w, row_bytes, nsb, x, y, rows, stream);
     }
     const MfmaPlan p = plan_mfma(rows, nsb);
     hipLaunchKernelGGL((gemv_q4_k_mfma_kernel<kQ4_K, 2, 64>), dim3((unsigned)p.grid), dim3(kMfThreads), 0,
@@ -1241,22 +1242,23 @@ hipError_t launch_gemm_col(int type_id, const uint8_t *w, int64_t row_bytes, con
     if (src == nullptr) return hipErrorInvalidValue;  // no GGUF rows and no layout for this partition
     const dim3 grid((unsigned)((N + col_rows - 1) / col_rows));
     const float *xf = reinterpret_cast<const float *>(x);
+    using Out = KernelOut<OUT>;
 #define GOLLEK_GEMM_COL_NV(T, NV)                                                                              \
     do {                                                                                                       \
         if (use_prep)                                                                                          \
-            hipLaunchKernelGGL((gemv_mfma_col_kernel<T, true, NV, true, OUT>), grid, dim3(kColThreads), 0, stream,   \
+            hipLaunchKernelGGL((gemv_mfma_col_kernel<T, true, NV, true, Out>), grid, dim3(kColThreads), 0, stream,   \
                                src, row_bytes, nsb, xf, y, (int64_t)N, (int)col_rows);                        \
         else                                                                                                   \
-            hipLaunchKernelGGL((gemv_mfma_col_kernel<T, false, NV, true, OUT>), grid, dim3(kColThreads), 0, stream,  \
+            hipLaunchKernelGGL((gemv_mfma_col_kernel<T, false, NV, true, Out>), grid, dim3(kColThreads), 0, stream,  \
                                src, row_bytes, nsb, xf, y, (int64_t)N, (int)col_rows);                        \
     } while (0)
 #define GOLLEK_GEMM_WIDE_NV(T, NV)                                                                             \
     do {                                                                                                       \
         if (use_prep)                                                                                          \
-            hipLaunchKernelGGL((gemv_mfma_wide_kernel<T, true, NV, true, OUT>), grid, dim3(kColThreads), 0, stream,  \
+            hipLaunchKernelGGL((gemv_mfma_wide_kernel<T, true, NV, true, Out>), grid, dim3(kColThreads), 0, stream,  \
                                src, row_bytes, nsb, xf, y, (int64_t)N, (int)col_rows);                        \
         else                                                                                                   \
-            hipLaunchKernelGGL((gemv_mfma_wide_kernel<T, false, NV, true, OUT>), grid, dim3(kColThreads), 0, stream, \
+            hipLaunchKernelGGL((gemv_mfma_wide_kernel<T, false, NV, true, Out>), grid, dim3(kColThreads), 0, stream, \
                                src, row_bytes, nsb, xf, y, (int64_t)N, (int)col_rows);                        \
     } while (0)
 #define GOLLEK_GEMM_COL(T)                                                                                      \
@@ -1295,16 +1297,16 @@ hipError_t launch_gemv_q32_mfma(int type_id, const uint8_t *w, int64_t row_bytes
 #define GOLLEK_COL(T)                                                                                      \
     do {                                                                                                   \
         if (nsb <= kColWaves && use_prep)                                                                  \
-            hipLaunchKernelGGL((gemv_mfma_col_kernel<T, true>), grid, dim3(kColThreads), 0, stream, src,   \
+            hipLaunchKernelGGL((gemv_mfma_col_kernel<T, true, 1, false, PlainOut>), grid, dim3(kColThreads), 0, stream, src,   \
                                row_bytes, nsb, x, y, rows, (int)col_rows);                                \
         else if (nsb <= kColWaves)                                                                         \
-            hipLaunchKernelGGL((gemv_mfma_col_kernel<T, false>), grid, dim3(kColThreads), 0, stream, src,  \
+            hipLaunchKernelGGL((gemv_mfma_col_kernel<T, false, 1, false, PlainOut>), grid, dim3(kColThreads), 0, stream, src,  \
                                row_bytes, nsb, x, y, rows, (int)col_rows);                                \
         else if (use_prep)                                                                                 \
-            hipLaunchKernelGGL((gemv_mfma_wide_kernel<T, true>), grid, dim3(kColThreads), 0, stream, src,  \
+            hipLaunchKernelGGL((gemv_mfma_wide_kernel<T, true, 1, false, PlainOut>), grid, dim3(kColThreads), 0, stream, src,  \
                                row_bytes, nsb, x, y, rows, (int)col_rows);                                \
         else                                                                                               \
-            hipLaunchKernelGGL((gemv_mfma_wide_kernel<T, false>), grid, dim3(kColThreads), 0, stream, src, \
+            hipLaunchKernelGGL((gemv_mfma_wide_kernel<T, false, 1, false, PlainOut>), grid, dim3(kColThreads), 0, stream, src, \
                                row_bytes, nsb, x, y, rows, (int)col_rows);                                \
     } while (0)
     if (type_id == kQ8_0) GOLLEK_COL(kQ8_0);

@@ -194,7 +194,7 @@ __device__ __forceinline__ void q6_x_operands_sums(uint32_t a01, uint32_t a23, u
 
 // XLDS: K > 4096, x's planes and digit sums for every superblock in LDS.  XB: x
 // holds bf16 bit patterns (the linear layer's), widened to fp32 exactly as they load.
-template <bool XLDS, bool XB = false, class OUT = float *__restrict__>
+template <bool XLDS, bool XB, class OUT>
 __global__ __launch_bounds__(kQ6Threads) void gemv_q6_k_mfma_tile_kernel(
     const uint8_t *__restrict__ w, int64_t row_bytes64, int nsb, const float *__restrict__ x,
     OUT y, int64_t rows, int64_t rows_per_wg) {
@@ -485,7 +485,7 @@ static hipError_t launch_q6k_tiles(const uint8_t *w, int64_t row_bytes, int64_t 
 
 hipError_t launch_gemv_q6k_mfma(const uint8_t *w, int64_t row_bytes, int64_t cols, const float *x, float *y,
                                 int64_t rows, hipStream_t stream) {
-    return launch_q6k_tiles<false, float *__restrict__>(w, row_bytes, cols, x, y, rows, stream);
+    return launch_q6k_tiles<false, PlainOut>(w, row_bytes, cols, x, y, rows, stream);
 }
 
 hipError_t launch_linear_vec_q6k(const uint8_t *w, int64_t row_bytes, int64_t cols, const uint16_t *x,

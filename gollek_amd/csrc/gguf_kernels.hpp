@@ -152,7 +152,7 @@ hipError_t launch_gemm_reduce(const float *part, int S, int M, int N, float *y, 
 hipError_t launch_gemm_reduce(const float *part, int S, int M, int N, const Epilogue &y, hipStream_t stream);
 
 // The linear layer (gguf_epilogue.hpp) on the kernels of launch_gemm_bf16, whose
-// sums it shares.  Splits keep all S partials in the workspace, so it takes
+// sums it shares (but for linear_vec_supported's).  Splits keep all S partials in the workspace, so it takes
 // linear_workspace_bytes (0: never splits; with less it splits less).
 size_t linear_workspace_bytes(int type_id, int M, int N, int K);
 size_t linear_kq_workspace_bytes(int type_id, int M, int N, int K);

@@ -310,7 +310,7 @@ GemmPlan kq_plan(int type_id, int M, int N, int K, size_t ws_bytes) {
 template <int T, int MT, int NW, int KW, class OUT>
 void launch(unsigned grid, hipStream_t stream, const uint8_t *w, int64_t row_bytes, const uint16_t *x, OUT y,
             int M, int N, int K, int S, float *part) {
-    hipLaunchKernelGGL((gemm_kq_kernel<T, MT, NW, KW, OUT>), dim3(grid), dim3(64 * NW * KW), 0, stream, w, row_bytes, x, y,
+    hipLaunchKernelGGL((gemm_kq_kernel<T, MT, NW, KW, KernelOut<OUT>>), dim3(grid), dim3(64 * NW * KW), 0, stream, w, row_bytes, x, y,
                        M, N, K, S, part);
 }
 

@@ -442,6 +442,11 @@ def test_one_token_on_row_tiles(t, rows, cols, y_type):
     assert out[0] == 7.0 and out[-1] == 7.0
     call(wt, x, 1, y, y_type)
     check(y.reshape(1, rows), expected(wt, xb, 0, None, None, None, y_type), f"{t} {rows}x{cols} alone")
+    if y_type == _native.F32:  # the mat-vec's own sums, bit for bit
+        xf = torch.from_numpy((xb.astype(np.uint32) << 16).view(np.float32)).cuda()
+        ref = torch.empty(rows, device="cuda")
+        wt.handle.matvec(xf.data_ptr(), ref.data_ptr(), stream=stream())
+        assert torch.equal(y.view(torch.int32), ref.view(torch.int32))
     xb[0, cols // 2] = 0x7FC0  # a NaN in x reaches every sum
     call(wt, torch.from_numpy(xb.view(np.int16)).cuda(), 1, y, y_type)
     assert torch.isnan(y).all() and out[0] == 7.0 and out[-1] == 7.0

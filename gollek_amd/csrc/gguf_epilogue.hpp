@@ -59,12 +59,31 @@ __device__ __forceinline__ float gated(float v, float s) {
     return v / (1.0f + expf(-s));
 }
 
+// v Phi(v) without 1 + erf, which cancels below 0 (4 % off at v = -5, 0 at -6):
+//   Phi(-a) = t (1/2 + c1 s + .. + c7 s^7) exp(-a^2 / 2),  t = 1 / (1 + 0.3 a),  s = 1 - t = 0.3 a t,
+// the coefficients a minimax fit of the relative error over a in [0, 14]: 2^-22.7;
+// in fp32 3 units of 2^-23 from v = -1 on and 6 at -3; below it is exp's argument,
+// a^2 / 2, that rounds, as v's own last bit would.  At 16, where a stops, exp has
+// left fp32's range.  Serves fp32 results too: the library's erfc is as exact and
+// cost a 96 x 256 tile's products 4 to 8 %.
+__device__ __forceinline__ float gelu(float v) {
+    const float a = fminf(fabsf(v), 16.0f), pa = 0.3f * a;
+    const float t = __builtin_amdgcn_rcpf(1.0f + pa), s = pa * t;
+    constexpr float kTerm[8] = {0.5f,           -0.829805851f, 0.618176758f,  -0.0820174515f,
+                                -0.131090671f, -0.0126647931f, 0.0927853063f, -0.0357543267f};
+    float q = kTerm[7];
+#pragma unroll
+    for (int k = 6; k >= 0; k--) q = __builtin_fmaf(q, s, kTerm[k]);
+    q = q * t * __builtin_amdgcn_exp2f(-0.72134752044448170f * a * a);
+    return v * (v < 0.0f ? q : 1.0f - q);
+}
+
 template <bool FAST>
 __device__ __forceinline__ float activate(int act, float v) {
     switch (act) {
     case kActRelu: return v < 0.0f ? 0.0f : v;  // (NaN stays)
     case kActSilu: return gated<FAST>(v, v);
-    case kActGelu: return 0.5f * v * (1.0f + erff(v * 0.70710678118654752f));
+    case kActGelu: return gelu(v);
     // 0.5 (1 + tanh(z)) is 1 / (1 + exp(-2 z))
     case kActGeluTanh: return gated<FAST>(v, 1.5957691216057308f * (v + 0.044715f * v * v * v));
     default: return v;

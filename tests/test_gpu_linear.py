@@ -512,3 +512,34 @@ def test_one_token_of_few_long_rows_with_and_without_a_workspace(rows, cols):
         y = torch.full((1, rows), float("nan"), device="cuda", dtype=torch.bfloat16)
         call(wt, x, 1, y, _native.BF16, ops.ACT_SILU, b, mu, re, ws)
         check(y, want, f"{rows}x{cols} workspace {ws is not None}")
+
+
+# v Phi(v) = v erfc(z) / 2 at z = -v / sqrt(2): z by one rounded constant and one
+# product, 2^-23 relative, of which erfc makes at most (2 z^2 + 2 z) 2^-23 for z > 0
+# (|erfc'(z)| <= (2 z + 2 / z) erfc(z) from z = 1 on) and 2^-23 below; erfc itself
+# 16 units of 2^-23 (the bound OpenCL sets its own), two products and the cast's half step.
+@pytest.mark.parametrize("y_type", [_native.F32, _native.F16, _native.BF16])
+@pytest.mark.parametrize("t,cols,m", [("q4_k", 512, 1), ("q8_0", 512, 20), ("q4_k", 4096, 40), ("q8_0", 32, 3),
+                                      ("q8_0", 512, 100)])
+def test_gelu_keeps_its_precision_below_zero(t, cols, m, y_type):
+    from scipy.special import erfc
+
+    v = np.concatenate([np.linspace(-12.5, 9.0, 498), [-0.0, 0.0, 1e-20, -1e-20, 1e30, -1e30]]).astype(np.float32)
+    wt = Weight(TYPES[t], v.size, cols, 24)
+    x = torch.zeros((m, cols), device="cuda", dtype=torch.int16)  # the product is 0: v is the bias alone
+    for odd in (0, 1):  # whole vectors of a row, and single elements
+        room = torch.full((m, v.size + 16), 7.0, device="cuda", dtype=DTYPE[y_type])
+        y = room[:, odd:odd + v.size]
+        call(wt, x, m, y, y_type, ops.ACT_GELU, torch.from_numpy(v).cuda(), ws=wt.workspace(m), y_stride=room.shape[1])
+        v64 = v.astype(np.float64)
+        want = np.where(v64 < -1e3, -0.0, 0.5 * v64 * erfc(-v64 / np.sqrt(2.0)))
+        z = np.clip(-v64 / np.sqrt(2.0), 0.0, 10.0)
+        rel = (2 * z * z + 2 * z + 1 + 16 + 1) * 2.0**-23 + HALF_STEP[y_type]
+        over = np.abs(want) > 65504.0 if y_type == _native.F16 else np.zeros(v.size, bool)
+        got = f64(y)
+        assert np.isinf(got[:, over]).all() and np.isfinite(got[:, ~over]).all()
+        err = np.abs(got - want)[:, ~over] - (2.0**-25 if y_type == _native.F16 else 2.0**-149)
+        worst = (err / np.maximum(rel * np.abs(want), 1e-300)[~over]).max()
+        print(f"[gpu] gelu {t} m={m} type={y_type}: largest error {worst:.3f} of its bound", flush=True)
+        assert worst <= 1.0
+        assert (room[:, odd + v.size:] == 7.0).all()

@@ -598,16 +598,26 @@ def moe_block_device(gate: DeviceWeight, up: DeviceWeight, down: DeviceWeight, n
     check(rc, err)
 
 
+def _logits(a):
+    """A host array of logits as it is passed on, and its element type: float16
+    and bf16 bit patterns (uint16) as they are, every other type as float32."""
+    a = np.ascontiguousarray(a)
+    if a.dtype == np.float16:
+        return a, _native.F16
+    if a.dtype == np.uint16:
+        return a, _native.BF16
+    return np.ascontiguousarray(a, dtype=np.float32), _native.F32
+
+
 def moe_route(logits, top_k: int, scoring: int, *, bias=None, n_groups: int = 1, top_groups: int = 1,
               group_top: int = 1, renormalize: bool = True, scale: float = 1.0):
     """Routing with a balancing bias and groups (gollek_hip_moe_route) on host
-    arrays: logits (tokens, n_experts) float32 or float16 -> ids (tokens, top_k)
-    int32, weights (tokens, top_k) float32."""
+    arrays: logits (tokens, n_experts) float32, float16 or uint16 bf16 bit
+    patterns (as linear returns them) -> ids (tokens, top_k) int32, weights
+    (tokens, top_k) float32."""
     if logits is None:
         raise NullPointerError("logits")
-    lv = np.ascontiguousarray(logits)
-    if lv.dtype != np.float16:
-        lv = np.ascontiguousarray(lv, dtype=np.float32)
+    lv, kind = _logits(logits)
     if lv.ndim != 2:
         raise IllegalArgumentError("logits must be (tokens, n_experts)")
     tokens, n_experts = lv.shape
@@ -617,10 +627,10 @@ def moe_route(logits, top_k: int, scoring: int, *, bias=None, n_groups: int = 1,
     ids = np.zeros((tokens, max(top_k, 0)), np.int32)
     w = np.zeros((tokens, max(top_k, 0)), np.float32)
     err = _native.ErrBuf()
-    check(_native.load().gollek_hip_moe_route(lv.ctypes.data, _native.F16 if lv.dtype == np.float16 else _native.F32,
-                                              tokens, n_experts, None if bv is None else bv.ctypes.data, scoring,
-                                              n_groups, top_groups, group_top, top_k, int(renormalize), scale,
-                                              ids.ctypes.data, w.ctypes.data, err.buf, err.size), err)
+    check(_native.load().gollek_hip_moe_route(lv.ctypes.data, kind, tokens, n_experts,
+                                              None if bv is None else bv.ctypes.data, scoring, n_groups, top_groups,
+                                              group_top, top_k, int(renormalize), scale, ids.ctypes.data,
+                                              w.ctypes.data, err.buf, err.size), err)
     return ids, w
 
 
@@ -691,16 +701,15 @@ def moe_shared_expert_device(gate: DeviceWeight, up: DeviceWeight, down: DeviceW
 
 def sample(logits, u, *, temperature=None, top_k=None, top_p=None, min_p=None):
     """One token per row of logits (gollek_hip_sample) on host arrays: logits
-    (rows, vocab) float32 or float16, u (rows,) the random numbers, settings
-    scalars or (rows,) arrays (None: off, temperature 1) -> tokens int32, probs
-    float32, kept int32, each (rows,)."""
+    (rows, vocab) float32, float16 or uint16 bf16 bit patterns (as linear returns
+    them), u (rows,) the random numbers, settings scalars or (rows,) arrays
+    (None: off, temperature 1) -> tokens int32, probs float32, kept int32, each
+    (rows,)."""
     if logits is None:
         raise NullPointerError("logits")
     if u is None:
         raise NullPointerError("u")
-    lv = np.ascontiguousarray(logits)
-    if lv.dtype != np.float16:
-        lv = np.ascontiguousarray(lv, dtype=np.float32)
+    lv, kind = _logits(logits)
     if lv.ndim != 2:
         raise IllegalArgumentError("logits must be (rows, vocab)")
     rows, vocab = lv.shape
@@ -720,10 +729,9 @@ def sample(logits, u, *, temperature=None, top_k=None, top_p=None, min_p=None):
                                              (u, "u", np.float32))]
     tokens, probs, kept = np.empty(rows, np.int32), np.empty(rows, np.float32), np.empty(rows, np.int32)
     err = _native.ErrBuf()
-    check(_native.load().gollek_hip_sample(lv.ctypes.data, _native.F16 if lv.dtype == np.float16 else _native.F32,
-                                           rows, vocab, *(None if a is None else a.ctypes.data for a in args),
-                                           tokens.ctypes.data, probs.ctypes.data, kept.ctypes.data, err.buf,
-                                           err.size), err)
+    check(_native.load().gollek_hip_sample(lv.ctypes.data, kind, rows, vocab,
+                                           *(None if a is None else a.ctypes.data for a in args), tokens.ctypes.data,
+                                           probs.ctypes.data, kept.ctypes.data, err.buf, err.size), err)
     return tokens, probs, kept
 
 
@@ -744,10 +752,13 @@ def sample_device(logits_ptr: int, logits_type: int, rows: int, vocab: int, u_pt
 
 def next_token(lm_head: GgufTensor, vector, u: float, *, temperature: float = 1.0, top_k: int = 0, top_p: float = 1.0,
                min_p: float = 0.0):
-    """The lm_head's mat-vec of `vector` and a token sampled from it
-    (gollek_hip_next_token; the logits stay on the device) -> token, prob, kept."""
+    """The lm_head's mat-vec of `vector` (floats, or uint16 bf16 bit patterns as
+    linear returns them) and a token sampled from it (gollek_hip_next_token; the
+    logits stay on the device) -> token, prob, kept."""
     if lm_head is None:
         raise NullPointerError("tensor")
+    if getattr(vector, "dtype", None) == np.uint16:
+        vector = (np.asarray(vector, np.uint32) << 16).view(np.float32)  # exact
     x = _f32_in(vector, "vector")
     token, prob, kept = ctypes.c_int32(), ctypes.c_float(), ctypes.c_int32()
     err = _native.err_buf()

@@ -221,3 +221,39 @@ def test_route_refuses_misaligned_results():
     for ids, w in ((4098, 4096), (4096, 4097)):
         assert lib.gollek_hip_moe_route_device(4096, 0, 1, 32, 0, 0, 1, 1, 1, 2, 1, 1.0, ids, w, None, e.buf,
                                                e.size) == _native.ERR_ARG
+
+
+@pytest.mark.parametrize("dtype,kind", [(np.float32, _native.F32), (np.float64, _native.F32), (np.float16, _native.F16),
+                                        (np.uint16, _native.BF16)])
+def test_logits_go_on_as_what_they_are(monkeypatch, dtype, kind):
+    """uint16 logits are bf16 bit patterns, as linear returns them, not numbers."""
+    calls = []
+
+    class Library:
+        def __getattr__(self, name):
+            return lambda *a: calls.append((name, a)) or _native.OK
+
+    monkeypatch.setattr(_native, "load", Library)
+    values = np.array([[1, 0x4000, 0x3F80, 7]], dtype)
+    ops.sample(values, [0.5])
+    ops.moe_route(values, 2, ops.ROUTER_SOFTMAX)
+    assert [name for name, _ in calls] == ["gollek_hip_sample", "gollek_hip_moe_route"]
+    assert [a[1] for _, a in calls] == [kind, kind]
+
+
+def test_next_token_takes_bf16_bit_patterns(monkeypatch):
+    seen = []
+
+    class Library:
+        def gollek_hip_next_token(self, handle, x, n, *rest):
+            seen.append(list((ctypes.c_float * n).from_address(x)))
+            return _native.OK
+
+    class Head:
+        def handle(self):
+            return None
+
+    monkeypatch.setattr(_native, "load", Library)
+    ops.next_token(Head(), np.array([0x3F80, 0xC000, 0, 0x3E20], np.uint16), 0.5)
+    ops.next_token(Head(), [1, 2.5], 0.5)
+    assert seen == [[1.0, -2.0, 0.0, 0.15625], [1.0, 2.5]]

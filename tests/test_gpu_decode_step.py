@@ -143,3 +143,20 @@ def test_decode_step(m):
         torch.cuda.synchronize()
         for a, b in zip(replayed, (step.h, step.f, step.ffn, step.moe, step.vocab, step.tokens)):
             assert torch.equal(a, b), turn
+
+
+def test_bf16_results_of_the_host_forms_go_on():
+    """linear's bf16 logits (uint16 bit patterns) into the host router and sampler."""
+    ops.init(0)
+    rows, cols, m = 64, 256, 5
+    data = syn.matrix(syn.Q8_0, rows, cols, seed=3)
+    t = ops.GgufTensor("w", (cols, rows), syn.Q8_0, data.reshape(-1))
+    logits = ops.linear(t, syn.activation_bf16(m, cols, seed=4), _native.BF16)
+    values = (logits.astype(np.uint32) << 16).view(np.float32)
+    for a, b in zip(ops.moe_route(logits, 6, ops.ROUTER_SOFTMAX, n_groups=8, top_groups=4),
+                    ops.moe_route(values, 6, ops.ROUTER_SOFTMAX, n_groups=8, top_groups=4)):
+        assert np.array_equal(a, b)
+    u = np.linspace(0.05, 0.95, m).astype(np.float32)
+    for a, b in zip(ops.sample(logits, u, temperature=20.0, top_p=0.9), ops.sample(values, u, temperature=20.0, top_p=0.9)):
+        assert np.array_equal(a, b)
+    t.close()

@@ -1525,9 +1525,10 @@ __global__ __launch_bounds__(kThreads) void sample_small_kernel(SampleArgs a) {
 
 // Workgroups a row is dealt to: one a chunk, so that rows whose weights are
 // summed do not wait behind others, up to the 64 whose histograms are read back.
+constexpr int kDealt = 2048, kMaxParts = 64;
 int row_parts(int rows, int chunks) {
-    int want = 2048 / rows;
-    if (want > 64) want = 64;
+    int want = kDealt / rows;
+    if (want > kMaxParts) want = kMaxParts;
     if (want > chunks) want = chunks;
     return want > 1 ? want : 1;
 }
@@ -1545,7 +1546,12 @@ SampleLayout sample_layout(int rows, int vocab) {
         o.total += (bytes + 255) / 256 * 256;
         return at;
     };
-    const size_t r = (size_t)rows, rc = r * o.chunks, rb = r * o.parts * kBins;
+    // Histograms: room for those of any smaller batch too (its rows are dealt to
+    // more parts: 93 of 128256 to 22, 96 to 21), so that a workspace never shrinks
+    // with rows or vocab.
+    const int64_t spread = (int64_t)rows * (o.chunks < kMaxParts ? o.chunks : kMaxParts);
+    const int64_t dealt = spread < kDealt ? spread : kDealt;
+    const size_t r = (size_t)rows, rc = r * o.chunks, rb = (size_t)(dealt > rows ? dealt : rows) * kBins;
     o.tops = take(rc * kChunkSlabs * sizeof(float));
     o.least = take(rc * 4 * sizeof(float));
     o.mass = take(rb * sizeof(u64));

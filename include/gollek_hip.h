@@ -450,7 +450,9 @@ int32_t gollek_hip_moe_shared_expert_device(gollek_hip_weight *gate, gollek_hip_
 int32_t gollek_hip_sample(const void *logits, int32_t logits_type, int64_t rows, int64_t vocab,
                           const float *temperature, const int32_t *top_k, const float *top_p, const float *min_p,
                           const float *u, int32_t *tokens, float *probs, int32_t *kept, char *err, size_t err_len);
-/* Device workspace bytes gollek_hip_sample_device needs (-1: out of range). */
+/* Device workspace bytes gollek_hip_sample_device needs (-1: out of range).  They
+ * never fall as rows or vocab rise: the workspace of the largest batch and
+ * vocabulary serves every smaller call. */
 int64_t gollek_hip_sample_workspace_bytes(int64_t rows, int64_t vocab);
 /* Device variant (every pointer on the device; `workspace` 256-byte aligned and
  * of at least gollek_hip_sample_workspace_bytes, else ARG; calls sharing it must

@@ -257,3 +257,16 @@ def test_next_token_takes_bf16_bit_patterns(monkeypatch):
     ops.next_token(Head(), np.array([0x3F80, 0xC000, 0, 0x3E20], np.uint16), 0.5)
     ops.next_token(Head(), [1, 2.5], 0.5)
     assert seen == [[1.0, -2.0, 0.0, 0.15625], [1.0, 2.5]]
+
+
+def test_sample_workspace_never_shrinks():
+    """A workspace for the largest batch and vocabulary serves every smaller one."""
+    size = _native.load().gollek_hip_sample_workspace_bytes
+    for vocab in (1, 16384, 16385, 32000, 128256, 262145, 4194304):
+        rows = list(range(0, 2200)) + [4095, 4096, 4097, 30000, 65535]
+        sizes = [size(r, vocab) for r in rows]
+        assert sizes == sorted(sizes) and sizes[0] >= 0, vocab
+    for rows in (1, 2, 31, 32, 33, 96, 1025, 65535):
+        sizes = [size(rows, v) for v in (1, 5000, 16384, 16385, 20480, 20481, 50257, 128256, 131072, 131073, 262144,
+                                         262145, 1 << 20, 1 << 22)]
+        assert sizes == sorted(sizes), rows

@@ -360,3 +360,26 @@ def test_few_keys_on_both_sides_of_zero(dtype):
     u = rng.random(3).astype(np.float32)
     for kw in (dict(k=2000), dict(k=3900), dict(k=9001, p=0.2003), dict(p=0.1507)):
         compare(sample(dev, u, **kw), dev, u, f"{dtype} {kw}", **kw)
+
+
+def test_the_largest_batchs_workspace_serves_smaller_ones():
+    vocab, most = 50257, 200  # (13 chunks a row: 200 rows are dealt to 10 parts, 150 and fewer to all 13)
+    need = ops.sample_workspace_bytes(most, vocab)
+    ws = torch.full((need,), 255, device="cuda", dtype=torch.uint8)
+    l = logits_of(most, vocab, 70)
+    u = torch.from_numpy(np.random.default_rng(71).random(most).astype(np.float32)).cuda()
+    p = torch.full((most,), 0.9, device="cuda")
+    out = [torch.zeros(most, device="cuda", dtype=d) for d in (torch.int32, torch.float32, torch.int32)]
+    wants = None
+    for rows in (most, 186, 171, 170, 157, 93, 33, 1):
+        assert ops.sample_workspace_bytes(rows, vocab) <= need
+        for o in out:
+            o.fill_(-5)
+        ops.sample_device(l.data_ptr(), _native.F32, rows, vocab, u.data_ptr(), out[0].data_ptr(), top_p_ptr=p.data_ptr(),
+                          probs_ptr=out[1].data_ptr(), kept_ptr=out[2].data_ptr(), ws_ptr=ws.data_ptr(), ws_bytes=need,
+                          stream=torch.cuda.current_stream().cuda_stream)
+        got = [o.cpu().numpy() for o in out]
+        if wants is None:
+            compare([g[:9] for g in got], l[:9], u[:9].cpu().numpy(), "200 rows", p=0.9)
+            wants = got
+        assert all(np.array_equal(g[:rows], w[:rows]) and (g[rows:] == -5).all() for g, w in zip(got, wants)), rows

@@ -646,15 +646,23 @@ int tile_splits(int type_id, int M, int N, int K, size_t workspace_bytes) {
 
 // The linear layer's tile height and splits (parts of K, whole stages, one more in
 // some of them): the pair with the shortest time by the constants of tile_mt, 2.9 us
-// for the launch that adds the splits and 0.2 us a MB of them, written and read.
+// for the launch that adds the splits and 0.2 us a MB of them, written and read
+// (twice that where rows are no whole quads and the launch adds element by element).
 // Against the plain product's rule, which splits a K of whole 512 by powers of two:
 // 0.97 of its times over 140 shapes of such K (0.70 to 1.07), 0.6 over those of other
-// K (Q4_0 4096 x 11008: M = 16 63.9 -> 18.0 us, M = 100 125 -> 31.4).
+// K (Q4_0 4096 x 11008: M = 16 63.9 -> 18.0 us, M = 100 125 -> 31.4).  Plans of more
+// than kFewPartials have to win 10 %, which is how far off the constants are for long
+// prompts.  (160 shapes that such partials reach, M = 24 to 2032, against partials up
+// to 16 MB: 0.91 of the times, 0.74 to 1.00; without the 10 % and the factor of two
+// 0.90, but 1.02 to 1.19 for eleven of them.  Q8_0 4096 x 14336, M = 600: 162 us
+// unsplit, 138 in three parts.)
 struct LinearTiles {
     int mt, splits;
 };
+constexpr size_t kFewPartials = (size_t)16 << 20;
 static LinearTiles linear_tiles(int M, int N, int K, size_t workspace_bytes) {
     const size_t mn = (size_t)M * N * sizeof(float);
+    const float byte_us = N % 4 == 0 ? 0.4e-6f : 0.8e-6f;
     constexpr float kStage[4] = {0.46f, 0.54f, 0.69f, 0.95f};
     const int stages = (K + 63) / 64;
     LinearTiles best = {8, 1};
@@ -665,7 +673,8 @@ static LinearTiles linear_tiles(int M, int N, int K, size_t workspace_bytes) {
         for (int S = 1; S <= 8 && S <= stages && (S == 1 || (size_t)S * mn <= workspace_bytes); S++) {
             float us = (float)((tiles * S + device_cus() - 1) / device_cus()) *
                        (3.0f + kStage[i] * ((stages + S - 1) / S));
-            if (S > 1) us += 2.9f + 0.4f * S * (float)mn * 1e-6f;
+            if (S > 1) us += 2.9f + byte_us * S * (float)mn;
+            if (S > 1 && S * mn > kFewPartials) us *= 1.1f;
             if (best_us == 0.0f || us < best_us) {
                 best = {mt, S};
                 best_us = us;
@@ -676,7 +685,7 @@ static LinearTiles linear_tiles(int M, int N, int K, size_t workspace_bytes) {
 }
 
 size_t linear_tile_workspace_bytes(int M, int N, int K) {
-    const LinearTiles t = linear_tiles(M, N, K, kGemmMaxSplitBytes);
+    const LinearTiles t = linear_tiles(M, N, K, (size_t)-1);
     return t.splits > 1 ? (size_t)t.splits * M * N * sizeof(float) : 0;
 }
 

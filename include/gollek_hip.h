@@ -227,8 +227,8 @@ int32_t gollek_hip_linear(gollek_hip_weight *weight, const uint16_t *x_bf16, int
                           int32_t y_type, int64_t y_len, char *err, size_t err_len);
 
 /* Device workspace bytes with which gollek_hip_linear_device splits K as far as
- * it pays (0: a call of m rows never splits); -1 for a NULL weight or m out of
- * range. */
+ * it pays (0: a call of m rows never splits), up to some hundred MB for long
+ * prompts; -1 for a NULL weight or m out of range. */
 int64_t gollek_hip_linear_workspace_bytes(const gollek_hip_weight *weight, int64_t m);
 
 /* Device variant, asynchronous on `stream`, which belongs to the weight's
@@ -241,8 +241,9 @@ int64_t gollek_hip_linear_workspace_bytes(const gollek_hip_weight *weight, int64
  * are.  Pointers are aligned to their elements (else
  * ARG).  workspace (256-byte aligned, else ARG) may be smaller than
  * gollek_hip_linear_workspace_bytes, or NULL: the call splits less, which
- * changes Y by the rounding of the sums' order alone.  Calls that share a
- * workspace must not overlap. */
+ * changes Y by the rounding of the sums' order alone.  A larger one changes
+ * nothing: bytes past those are not touched, so one workspace may serve calls of
+ * different needs.  Calls that share a workspace must not overlap. */
 int32_t gollek_hip_linear_device(gollek_hip_weight *weight, const uint16_t *x_bf16, int64_t m, const float *bias,
                                  int32_t activation, const void *mul, int64_t mul_stride, const void *residual,
                                  int64_t residual_stride, void *y, int32_t y_type, int64_t y_stride, void *workspace,

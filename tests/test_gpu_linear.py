@@ -543,3 +543,22 @@ def test_gelu_keeps_its_precision_below_zero(t, cols, m, y_type):
         print(f"[gpu] gelu {t} m={m} type={y_type}: largest error {worst:.3f} of its bound", flush=True)
         assert worst <= 1.0
         assert (room[:, odd + v.size:] == 7.0).all()
+
+
+@pytest.mark.parametrize("t,rows,cols,m", [("q8_0", 1024, 14336, 1111), ("q4_0", 2048, 11008, 1129), ("q8_0", 257, 2080, 900),
+                                           ("q4_k", 1024, 8192, 300), ("q6_k", 512, 8192, 1), ("q8_0", 256, 4096, 8)])
+def test_a_larger_workspace_changes_no_bit(t, rows, cols, m):
+    """The plan is the stated workspace's, whatever a caller has beyond it; and what is beyond stays as it is."""
+    print(f"[gpu] linear {t} {rows}x{cols} m={m} larger workspace", flush=True)
+    wt = Weight(TYPES[t], rows, cols, 25)
+    xb = syn.activation_bf16(m, cols, seed=25)
+    x = torch.from_numpy(xb.view(np.int16)).cuda()
+    need = wt.handle.linear_workspace_bytes(m)
+    y, z = (torch.full((m, rows), float("nan"), device="cuda") for _ in range(2))
+    call(wt, x, m, y, _native.F32, ops.ACT_SILU, ws=wt.workspace(m))
+    big = torch.full((need + (128 << 20),), 171, device="cuda", dtype=torch.uint8)
+    call(wt, x, m, z, _native.F32, ops.ACT_SILU, ws=big)
+    assert torch.equal(y.view(torch.int32), z.view(torch.int32))
+    assert (big[need:] == 171).all()
+    some = np.unique(np.r_[0:min(m, 20), m // 2, m - 1])
+    check(z[some], expected(wt, xb[some], ops.ACT_SILU, None, None, None, _native.F32), f"{t} {rows}x{cols} m={m}")

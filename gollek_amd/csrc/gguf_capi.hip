@@ -962,7 +962,9 @@ int32_t make_epilogue(const gollek_hip_weight *w, int64_t m, const float *bias, 
 int64_t gollek_hip_linear_workspace_bytes(const gollek_hip_weight *w, int64_t m) {
     if (w == nullptr || m < 0 || m > (int64_t)0x7FFFFFFF || w->rows > 0x7FFFFFFF || w->cols > 0x7FFFFFFF) return -1;
     if (m == 0 || w->rows == 0 || w->compact) return 0;
-    return (int64_t)align_up(gollek::linear_workspace_bytes(w->type_id, (int)m, (int)w->rows, (int)w->cols), 256);
+    return (int64_t)align_up(gollek::linear_workspace_bytes(w->type_id, w->data, w->row_bytes, (int)m, (int)w->rows,
+                                                            (int)w->cols),
+                             256);
 }
 
 int32_t gollek_hip_linear_device(gollek_hip_weight *w, const uint16_t *x, int64_t m, const float *bias,
@@ -1022,7 +1024,9 @@ int32_t gollek_hip_linear(gollek_hip_weight *w, const uint16_t *x, int64_t x_len
     if (rc != GOLLEK_HIP_OK) return rc;
     const size_t xn = (size_t)(m * w->cols) * sizeof(uint16_t), bn = (size_t)w->rows * sizeof(float);
     const size_t yn = (size_t)(m * w->rows) * element_size(y_type);
-    const size_t ws_bytes = gollek::linear_workspace_bytes(w->type_id, (int)m, (int)w->rows, (int)w->cols);
+    const size_t ws_bytes =
+        w->compact ? 0
+                   : gollek::linear_workspace_bytes(w->type_id, w->data, w->row_bytes, (int)m, (int)w->rows, (int)w->cols);
     const size_t b_off = align_up(xn, 256), m_off = b_off + (bias != nullptr ? align_up(bn, 256) : 0);
     const size_t r_off = m_off + (mul != nullptr ? align_up(yn, 256) : 0);
     const size_t y_off = r_off + (residual != nullptr ? align_up(yn, 256) : 0), ws_off = y_off + align_up(yn, 256);

@@ -535,14 +535,22 @@ size_t gemm_workspace_max_bytes(int type_id, int N, int K) {
 
 namespace {
 
+bool skinny_supported(int type_id, int64_t row_bytes, int M, int N, int K, const void *w, const void *x) {
+    return type_id == kQ8_0 && M <= 32 && N % 16 == 0 && K % 256 == 0 && (reinterpret_cast<uintptr_t>(w) & 3u) == 0 &&
+           (row_bytes & 3) == 0 && (reinterpret_cast<uintptr_t>(x) & 15u) == 0 &&
+           (int64_t)16 * row_bytes < ((int64_t)1 << 31) && (int64_t)M * K * 2 < ((int64_t)1 << 31);
+}
+
+// One token's weights whose K the GEMM splits even where the mat-vec's 16-row
+// tiles take them (launch_gemm).
+bool few_long_rows(int N, int K) { return K > 6144 && N <= 4 * device_cus(); }
+
 template <class OUT>
 hipError_t launch_gemm(int type_id, const uint8_t *w, int64_t row_bytes, const uint16_t *x, OUT y,
                        int M, int N, int K, hipStream_t stream, float *workspace, size_t workspace_bytes,
                        const uint8_t *prep, int64_t prep_rows) {
     using Out = KernelOut<OUT>;
     if (M <= 0) return hipSuccess;
-    const bool aligned = (reinterpret_cast<uintptr_t>(w) & 3u) == 0 && (row_bytes & 3) == 0 &&
-                         (reinterpret_cast<uintptr_t>(x) & 15u) == 0;
     // M <= 4: the GEMV's column kernel, two vectors in each MFMA (on the
     // prepared column layout when there is one for its partition).
     if (gemm_col_supported(type_id, row_bytes, M, N, K, w != nullptr ? w : prep, x))
@@ -557,15 +565,14 @@ hipError_t launch_gemm(int type_id, const uint8_t *w, int64_t row_bytes, const u
     // 1024 x 8192 9.1 against 8.2, 1024 x 14336 13.2 against 11.0 (but 1024 x 6144
     // 7.7 against 7.9, 2048 x 14336 13.4 against 14.7).
     if constexpr (kHasEpilogue<OUT>) {
-        const bool splits = M == 1 && K > 6144 && N <= 4 * device_cus() && workspace != nullptr &&
-                            workspace_bytes >= linear_workspace_bytes(type_id, M, N, K) &&
+        const bool splits = few_long_rows(N, K) && workspace != nullptr &&
+                            workspace_bytes >= linear_kq_workspace_bytes(type_id, M, N, K) &&
                             splits_aligned(y, workspace, M, N);
         if (M == 1 && !splits && linear_vec_supported(type_id, row_bytes, N, K, w, x))
             return launch_linear_vec(type_id, w, row_bytes, N, K, x, y, stream);
     }
     // M <= 32 with Q8_0 weights: the buffer->LDS ring over 16-row column tiles.
-    if (type_id == kQ8_0 && aligned && M <= 32 && N % 16 == 0 && K % 256 == 0 &&
-        (int64_t)16 * row_bytes < ((int64_t)1 << 31) && (int64_t)M * K * 2 < ((int64_t)1 << 31)) {
+    if (skinny_supported(type_id, row_bytes, M, N, K, w, x)) {
         if (M <= 16)
             hipLaunchKernelGGL((gemm_q8_0_bf16_skinny_kernel<1, 4, Out>), dim3(N / 16), dim3(256), 0, stream, w,
                                row_bytes, x, y, M, N, K);
@@ -639,10 +646,14 @@ hipError_t launch_gemm_bf16(int type_id, const uint8_t *w, int64_t row_bytes, co
                                 prep_rows);
 }
 
-size_t linear_workspace_bytes(int type_id, int M, int N, int K) {
-    if (type_id == kQ4_K || type_id == kQ5_K || type_id == kQ6_K) return linear_kq_workspace_bytes(type_id, M, N, K);
-    if (type_id == kQ8_0 && M <= 32 && N % 16 == 0 && K % 256 == 0) return 0;  // the skinny kernel
-    return linear_tile_workspace_bytes(M, N, K);
+// (the order of launch_gemm, for x on a 16-byte boundary: every kernel that splits needs it)
+size_t linear_workspace_bytes(int type_id, const uint8_t *w, int64_t row_bytes, int M, int N, int K) {
+    if (gemm_col_supported(type_id, row_bytes, M, N, K, w, nullptr)) return 0;
+    if (M == 1 && !few_long_rows(N, K) && linear_vec_supported(type_id, row_bytes, N, K, w, nullptr)) return 0;
+    if (skinny_supported(type_id, row_bytes, M, N, K, w, nullptr)) return 0;
+    if (kq_gemm_supported(type_id, row_bytes, N, K, w, nullptr)) return linear_kq_workspace_bytes(type_id, M, N, K);
+    if (gemm_tile_supported(type_id, row_bytes, M, N, K, w, nullptr)) return linear_tile_workspace_bytes(M, N, K);
+    return 0;
 }
 
 hipError_t launch_linear(int type_id, const uint8_t *w, int64_t row_bytes, const uint16_t *x, const Epilogue &y,
@@ -650,7 +661,7 @@ hipError_t launch_linear(int type_id, const uint8_t *w, int64_t row_bytes, const
                          const uint8_t *prep, int64_t prep_rows) {
     // What the query did not ask for stays unused: the plans, and so the sums'
     // order, do not depend on what else a caller's workspace serves.
-    const size_t need = linear_workspace_bytes(type_id, M, N, K);
+    const size_t need = w != nullptr ? linear_workspace_bytes(type_id, w, row_bytes, M, N, K) : 0;
     if (workspace_bytes > need) workspace_bytes = need;
     if (workspace_bytes == 0) workspace = nullptr;
     return launch_gemm<Epilogue>(type_id, w, row_bytes, x, y, M, N, K, stream, workspace, workspace_bytes, prep,

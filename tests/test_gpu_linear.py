@@ -562,3 +562,23 @@ def test_a_larger_workspace_changes_no_bit(t, rows, cols, m):
     assert (big[need:] == 171).all()
     some = np.unique(np.r_[0:min(m, 20), m // 2, m - 1])
     check(z[some], expected(wt, xb[some], ops.ACT_SILU, None, None, None, _native.F32), f"{t} {rows}x{cols} m={m}")
+
+
+# One to four tokens on the mat-vec's kernels and up to 32 on the skinny one never split,
+# others of the same weights do: K-quants from few rows on, and a Q6_K weight of few long rows.
+@pytest.mark.parametrize("t,rows,cols,never,splits", [
+    ("q4_0", 300, 2048, (1, 2, 3, 4), (5, 40)), ("q4_k", 512, 8192, (1, 2), (3, 16)), ("q5_k", 256, 4096, (1, 4), (5,)),
+    ("q8_0", 512, 8192, (1, 2, 3, 32), (33,)), ("q8_0", 500, 8192, (1, 2), (3, 32)), ("q6_k", 2048, 4096, (1,), (8,)),
+    ("q6_k", 1024, 6144, (1,), (2,)), ("q6_k", 1024, 8192, (), (1, 2)), ("q4_k", 16400, 256, (1,), ())])
+def test_no_workspace_is_asked_for_where_none_is_used(t, rows, cols, never, splits):
+    wt = Weight(TYPES[t], rows, cols, 26)
+    for m in never:
+        assert wt.handle.linear_workspace_bytes(m) == 0, m
+        x = torch.from_numpy(syn.activation_bf16(m, cols, seed=26).view(np.int16)).cuda()
+        ws = torch.full((16 << 20,), 171, device="cuda", dtype=torch.uint8)
+        y, z = (torch.full((m, rows), float("nan"), device="cuda") for _ in range(2))
+        call(wt, x, m, y, _native.F32)
+        call(wt, x, m, z, _native.F32, ws=ws)
+        assert torch.equal(y.view(torch.int32), z.view(torch.int32)) and (ws == 171).all(), m
+    for m in splits:
+        assert wt.handle.linear_workspace_bytes(m) >= 2 * 4 * m * rows, m

@@ -582,3 +582,15 @@ def test_no_workspace_is_asked_for_where_none_is_used(t, rows, cols, never, spli
         assert torch.equal(y.view(torch.int32), z.view(torch.int32)) and (ws == 171).all(), m
     for m in splits:
         assert wt.handle.linear_workspace_bytes(m) >= 2 * 4 * m * rows, m
+
+
+def test_without_a_workspace_the_bits_are_the_gemms():
+    """Shapes that the plain GEMM does not split, whatever a workspace would change."""
+    for t, rows, cols, m in (("q4_0", 300, 2048, 3), ("q8_0", 100, 2080, 40), ("q4_0", 131, 2848, 300), ("q4_k", 512, 1024, 2),
+                             ("q6_k", 14336, 512, 128), ("q8_0", 512, 1024, 16)):
+        wt = Weight(TYPES[t], rows, cols, 27)
+        x = torch.from_numpy(syn.activation_bf16(m, cols, seed=27).view(np.int16)).cuda()
+        y, ref = (torch.full((m, rows), float("nan"), device="cuda") for _ in range(2))
+        call(wt, x, m, y, _native.F32)
+        wt.handle.gemm_bf16(x.data_ptr(), m, ref.data_ptr(), stream())
+        assert torch.equal(y.view(torch.int32), ref.view(torch.int32)), (t, rows, cols, m)

@@ -990,12 +990,28 @@ int32_t gollek_hip_linear_device(gollek_hip_weight *w, const uint16_t *x, int64_
         return fail(GOLLEK_HIP_ERR_ARG, err, err_len, "The output overlaps the input");
     if (workspace != nullptr && within(y, m, w->rows, epi.y_stride, element_size(y_type), workspace, workspace_bytes))
         return fail(GOLLEK_HIP_ERR_ARG, err, err_len, "The output overlaps the workspace");
+    // What the query did not ask for stays unused: the plans, and so the sums'
+    // order, do not depend on what else a caller's workspace serves.
+    const int64_t n = w->rows;
+    int64_t ws_bytes = workspace != nullptr && !w->compact ? workspace_bytes : 0;
+    if (ws_bytes > 0) {
+        const int64_t need = (int64_t)gollek::linear_workspace_bytes(w->type_id, w->data, w->row_bytes, (int)m, (int)n,
+                                                                     (int)w->cols);
+        if (ws_bytes > need) ws_bytes = need;
+    }
+    if (ws_bytes > 0) {
+        const int64_t size = element_size(y_type);
+        const bool inputs = within(x, m, w->cols, w->cols, 2, workspace, ws_bytes) ||
+                            (bias != nullptr && within(bias, 1, n, n, 4, workspace, ws_bytes)) ||
+                            (mul != nullptr && within(mul, m, n, epi.mul_stride, size, workspace, ws_bytes)) ||
+                            (residual != nullptr && within(residual, m, n, epi.residual_stride, size, workspace, ws_bytes));
+        if (inputs) return fail(GOLLEK_HIP_ERR_ARG, err, err_len, "The workspace overlaps an input");
+    }
     const DeviceGuard device(w->device);
-    const hipError_t e = gollek::launch_linear(w->type_id, w->data, w->row_bytes, x, epi, (int)m, (int)w->rows,
-                                               (int)w->cols, static_cast<hipStream_t>(stream),
-                                               static_cast<float *>(workspace),
-                                               workspace != nullptr ? (size_t)workspace_bytes : 0, w->prep,
-                                               w->prep_rows);
+    const hipError_t e = gollek::launch_linear(w->type_id, w->data, w->row_bytes, x, epi, (int)m, (int)n, (int)w->cols,
+                                               static_cast<hipStream_t>(stream),
+                                               ws_bytes > 0 ? static_cast<float *>(workspace) : nullptr, (size_t)ws_bytes,
+                                               w->prep, w->prep_rows);
     if (e != hipSuccess) return hip_fail(e, "linear launch", err, err_len);
     ok(err, err_len);
     return GOLLEK_HIP_OK;

@@ -659,11 +659,6 @@ size_t linear_workspace_bytes(int type_id, const uint8_t *w, int64_t row_bytes, 
 hipError_t launch_linear(int type_id, const uint8_t *w, int64_t row_bytes, const uint16_t *x, const Epilogue &y,
                          int M, int N, int K, hipStream_t stream, float *workspace, size_t workspace_bytes,
                          const uint8_t *prep, int64_t prep_rows) {
-    // What the query did not ask for stays unused: the plans, and so the sums'
-    // order, do not depend on what else a caller's workspace serves.
-    const size_t need = w != nullptr ? linear_workspace_bytes(type_id, w, row_bytes, M, N, K) : 0;
-    if (workspace_bytes > need) workspace_bytes = need;
-    if (workspace_bytes == 0) workspace = nullptr;
     return launch_gemm<Epilogue>(type_id, w, row_bytes, x, y, M, N, K, stream, workspace, workspace_bytes, prep,
                                  prep_rows);
 }

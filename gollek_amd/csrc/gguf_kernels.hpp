@@ -153,8 +153,7 @@ hipError_t launch_gemm_reduce(const float *part, int S, int M, int N, const Epil
 
 // The linear layer (gguf_epilogue.hpp) on the kernels of launch_gemm_bf16, whose
 // sums it shares (but for linear_vec_supported's).  Splits keep all S partials in the workspace, so it takes
-// linear_workspace_bytes (0: never splits; with less it splits less, what is past
-// them it leaves alone).
+// linear_workspace_bytes at most (0: never splits; with less it splits less).
 size_t linear_workspace_bytes(int type_id, const uint8_t *w, int64_t row_bytes, int M, int N, int K);
 size_t linear_kq_workspace_bytes(int type_id, int M, int N, int K);
 size_t linear_tile_workspace_bytes(int M, int N, int K);

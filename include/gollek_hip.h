@@ -243,7 +243,8 @@ int64_t gollek_hip_linear_workspace_bytes(const gollek_hip_weight *weight, int64
  * gollek_hip_linear_workspace_bytes, or NULL: the call splits less, which
  * changes Y by the rounding of the sums' order alone.  A larger one changes
  * nothing: bytes past those are not touched, so one workspace may serve calls of
- * different needs.  Calls that share a workspace must not overlap. */
+ * different needs.  The bytes that the call may use must not overlap X, bias, mul
+ * or residual (-> ARG).  Calls that share a workspace must not overlap. */
 int32_t gollek_hip_linear_device(gollek_hip_weight *weight, const uint16_t *x_bf16, int64_t m, const float *bias,
                                  int32_t activation, const void *mul, int64_t mul_stride, const void *residual,
                                  int64_t residual_stride, void *y, int32_t y_type, int64_t y_stride, void *workspace,

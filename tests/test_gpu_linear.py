@@ -594,3 +594,32 @@ def test_without_a_workspace_the_bits_are_the_gemms():
         call(wt, x, m, y, _native.F32)
         wt.handle.gemm_bf16(x.data_ptr(), m, ref.data_ptr(), stream())
         assert torch.equal(y.view(torch.int32), ref.view(torch.int32)), (t, rows, cols, m)
+
+
+@pytest.mark.parametrize("t,m", [("q4_k", 40), ("q8_0", 64)])
+def test_a_workspace_over_an_input_is_refused(t, m):
+    rows, cols = 256, 4096
+    wt = Weight(TYPES[t], rows, cols, 28)
+    need = wt.handle.linear_workspace_bytes(m)
+    assert need > 0
+    xb = syn.activation_bf16(m, cols, seed=28)
+    b, mu, re = operands(m, rows, _native.F32, 28, True, True, True)
+    size = 2 * m * cols
+    room = torch.zeros(need + 4 * size, device="cuda", dtype=torch.uint8)
+    base = (room.data_ptr() + 255) // 256 * 256
+    y = torch.full((m, rows), 7.0, device="cuda")
+    xp = torch.from_numpy(xb.view(np.int16)).cuda()
+    put = dict(bias_ptr=b.data_ptr(), mul_ptr=mu.data_ptr(), residual_ptr=re.data_ptr(), stream=stream())
+    for at in (base, base + need - 16):  # at the workspace's start and over its last bytes
+        with pytest.raises(ops.IllegalArgumentError):
+            wt.handle.linear(at, m, y.data_ptr(), _native.F32, ws_ptr=base, ws_bytes=need, **put)
+        for name in ("bias_ptr", "mul_ptr", "residual_ptr"):
+            with pytest.raises(ops.IllegalArgumentError):
+                wt.handle.linear(xp.data_ptr(), m, y.data_ptr(), _native.F32, ws_ptr=base, ws_bytes=need, **{**put, name: at})
+    torch.cuda.synchronize()
+    assert (y == 7.0).all()
+    # right behind what the call uses an input may stand, whatever the workspace's length
+    at = base - room.data_ptr() + need
+    room[at:at + size].view(torch.int16).copy_(xp.reshape(-1))
+    wt.handle.linear(base + need, m, y.data_ptr(), _native.F32, ws_ptr=base, ws_bytes=need + size, activation=ops.ACT_SILU, **put)
+    check(y, expected(wt, xb, ops.ACT_SILU, b, mu, re, _native.F32), "x behind the workspace")

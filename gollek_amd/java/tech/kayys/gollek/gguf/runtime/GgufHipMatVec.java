@@ -198,13 +198,14 @@ final class GgufHipMatVec {
      * of these the ones of at least minP of the largest's probability, and
      * among those the one that u, a random number in [0, 1), falls on in the
      * order of the vocabulary.  The logits, half a megabyte for a vocabulary of
-     * 128k, stay on the device.  False when the route is not taken.
+     * 128k, stay on the device.  False when the route is not taken, or with a
+     * library of ABI 1.0, which has no such entry.
      */
     static boolean tryNextToken(GGUFModel model, GGUFTensorInfo tensor, long rows, int columns, long rowBytes,
                                 float[] vector, float temperature, int topK, float topP, float minP, float u,
                                 int[] token) {
         Binding b = Binding.get();
-        if (b == null || !supportsType(tensor.typeId())) {
+        if (b == null || !b.hasNextToken() || !supportsType(tensor.typeId())) {
             return false;
         }
         if (token.length < 1) {
@@ -542,7 +543,9 @@ final class GgufHipMatVec {
                             ValueLayout.ADDRESS, ValueLayout.ADDRESS, ValueLayout.JAVA_LONG, ValueLayout.JAVA_LONG,
                             ValueLayout.ADDRESS, ValueLayout.JAVA_LONG, ValueLayout.ADDRESS, ValueLayout.JAVA_LONG),
                     true);
-            this.nextToken = downcall(linker, lookup, "gollek_hip_next_token",
+            // Since ABI 1.1: a 1.0 library still serves every other call.
+            this.nextToken = lookup.find("gollek_hip_next_token").isEmpty() ? null
+                    : downcall(linker, lookup, "gollek_hip_next_token",
                     FunctionDescriptor.of(ValueLayout.JAVA_INT,
                             ValueLayout.ADDRESS, ValueLayout.ADDRESS, ValueLayout.JAVA_LONG, ValueLayout.JAVA_FLOAT,
                             ValueLayout.JAVA_INT, ValueLayout.JAVA_FLOAT, ValueLayout.JAVA_FLOAT,
@@ -677,6 +680,10 @@ final class GgufHipMatVec {
             } catch (Throwable t) {
                 throw propagate(t);
             }
+        }
+
+        boolean hasNextToken() {
+            return nextToken != null;
         }
 
         int nextToken(MemorySegment weight, MemorySegment x, long xLen, float temperature, int topK, float topP,

@@ -24,3 +24,14 @@ def test_try_next_token_passes_its_arguments_in_order():
                     "u", "MemorySegment.ofArray(token)", "MemorySegment.NULL", "MemorySegment.NULL", "err",
                     "(long) ERR_LEN"]
     assert "token.length < 1" in body
+
+
+def test_a_library_without_the_entry_serves_the_others():
+    # ABI 1.0 has no gollek_hip_next_token: its handle is optional, the others' are not
+    text = java_text()
+    optional = re.findall(r'lookup\.find\("(\w+)"\)\.isEmpty\(\) \? null\s*: downcall\(linker, lookup, "(\w+)"', text)
+    assert optional == [("gollek_hip_next_token", "gollek_hip_next_token")]
+    body = re.search(r"static boolean tryNextToken\(.*?\n    \}\n", text, flags=re.S).group(0)
+    assert "if (b == null || !b.hasNextToken() || !supportsType(tensor.typeId())) {\n            return false;" in body
+    assert body.index("hasNextToken") < body.index("handle(b, ")
+    assert re.search(r"boolean hasNextToken\(\) \{\s*return nextToken != null;", text)

@@ -144,6 +144,14 @@ int32_t use_device(int device, char *err, size_t err_len) {
     return GOLLEK_HIP_OK;
 }
 
+// use_device for the host forms that have no weight to name one.
+int32_t use_current_device(char *err, size_t err_len) {
+    int device = 0;
+    const hipError_t e = hipGetDevice(&device);
+    if (e != hipSuccess) return hip_fail(e, "hipGetDevice", err, err_len);
+    return use_device(device, err, err_len);
+}
+
 // GC/core/GgmlType.java:70-81 and RT/GgufTensorShape.java:185-198.
 int32_t check_shape(int32_t type_id, int64_t rows, int64_t cols, int64_t row_bytes, char *err,
                     size_t err_len) {
@@ -1342,15 +1350,12 @@ int32_t gollek_hip_moe_select_topk(const float *logits, int64_t tokens, int64_t 
         ok(err, err_len);
         return GOLLEK_HIP_OK;
     }
-    int device = 0;
-    hipError_t e = hipGetDevice(&device);
-    if (e != hipSuccess) return hip_fail(e, "hipGetDevice", err, err_len);
-    rc = use_device(device, err, err_len);
+    rc = use_current_device(err, err_len);
     if (rc != GOLLEK_HIP_OK) return rc;
     const size_t lb = align_up((size_t)(tokens * n_experts) * 4, 256);
     const size_t rb = align_up((size_t)(tokens * top_k) * 4, 256);
     uint8_t *buf = nullptr;
-    e = hipMalloc(reinterpret_cast<void **>(&buf), lb + 2 * rb);
+    hipError_t e = hipMalloc(reinterpret_cast<void **>(&buf), lb + 2 * rb);
     if (e != hipSuccess) return hip_fail(e, "hipMalloc(router)", err, err_len);
     float *d_l = reinterpret_cast<float *>(buf);
     int32_t *d_ids = reinterpret_cast<int32_t *>(buf + lb);
@@ -1429,6 +1434,8 @@ int32_t gollek_hip_moe_route(const void *logits, int32_t logits_type, int64_t to
     }
     if (logits == nullptr || ids == nullptr || weights == nullptr)
         return fail(GOLLEK_HIP_ERR_NULL, err, err_len, "router buffers");
+    rc = use_current_device(err, err_len);
+    if (rc != GOLLEK_HIP_OK) return rc;
     const size_t ln = (size_t)(tokens * n_experts) * element_size(logits_type), rn = (size_t)(tokens * top_k) * 4;
     const size_t lb = align_up(ln, 256), rb = align_up(rn, 256), bn = (size_t)n_experts * 4;
     uint8_t *buf = nullptr;
@@ -1651,13 +1658,15 @@ int32_t gollek_hip_sample_device(const void *logits, int32_t logits_type, int64_
 int32_t gollek_hip_sample(const void *logits, int32_t logits_type, int64_t rows, int64_t vocab,
                           const float *temperature, const int32_t *top_k, const float *top_p, const float *min_p,
                           const float *u, int32_t *tokens, float *probs, int32_t *kept, char *err, size_t err_len) {
-    const int32_t rc = check_sample(logits, logits_type, rows, vocab, vocab, temperature, top_k, top_p, min_p, u,
-                                    tokens, probs, kept, err, err_len);
+    int32_t rc = check_sample(logits, logits_type, rows, vocab, vocab, temperature, top_k, top_p, min_p, u, tokens,
+                              probs, kept, err, err_len);
     if (rc != GOLLEK_HIP_OK) return rc;
     if (rows == 0) {
         ok(err, err_len);
         return GOLLEK_HIP_OK;
     }
+    rc = use_current_device(err, err_len);
+    if (rc != GOLLEK_HIP_OK) return rc;
     // one allocation: logits | temperature, top_k, top_p, min_p, u | tokens, probs, kept | workspace
     const size_t ln = (size_t)(rows * vocab) * element_size(logits_type), rn = (size_t)rows * 4;
     const size_t lb = align_up(ln, 256), rb = align_up(rn, 256);

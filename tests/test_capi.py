@@ -270,3 +270,20 @@ def test_sample_workspace_never_shrinks():
         sizes = [size(rows, v) for v in (1, 5000, 16384, 16385, 20480, 20481, 50257, 128256, 131072, 131073, 262144,
                                          262145, 1 << 20, 1 << 22)]
         assert sizes == sorted(sizes), rows
+
+
+def test_host_forms_without_a_weight_ask_for_the_device_first():
+    import torch
+    if torch.cuda.is_available():
+        pytest.skip("a device is there")
+    lib, e = _native.load(), _err()
+    x, out = np.zeros(64, np.float32), np.zeros(64, np.float32)
+    xp, op = x.ctypes.data, out.ctypes.data
+    calls = {
+        "select_topk": lambda: lib.gollek_hip_moe_select_topk(xp, 2, 8, 2, 0, op, op + 64, e.buf, e.size),
+        "route": lambda: lib.gollek_hip_moe_route(xp, 0, 2, 8, None, 0, 1, 1, 1, 2, 1, 1.0, op, op + 64, e.buf, e.size),
+        "sample": lambda: lib.gollek_hip_sample(xp, 0, 2, 8, None, None, None, None, xp, op, None, None, e.buf, e.size),
+    }
+    for name, call in calls.items():
+        assert call() == _native.ERR_DEVICE, name
+        assert b"hipGetDevice failed" in e.buf.value or b"hipSetDevice failed" in e.buf.value, (name, e.buf.value)

@@ -926,6 +926,12 @@ bool within(const void *y, int64_t m, int64_t n, int64_t y_stride, int64_t size,
     return ba < ya + (uintptr_t)(((m - 1) * y_stride + n) * size) && ya < ba + (uintptr_t)bytes;
 }
 
+// Whether two stretches of bytes share one (NULL shares none).
+bool share(const void *a, int64_t a_bytes, const void *b, int64_t b_bytes) {
+    const uintptr_t x = reinterpret_cast<uintptr_t>(a), y = reinterpret_cast<uintptr_t>(b);
+    return a != nullptr && b != nullptr && y < x + (uintptr_t)a_bytes && x < y + (uintptr_t)b_bytes;
+}
+
 // Checks a linear call's epilogue and fills `out`.  Strides of 0 are packed rows.
 int32_t make_epilogue(const gollek_hip_weight *w, int64_t m, const float *bias, int32_t activation, const void *mul,
                       int64_t mul_stride, const void *residual, int64_t residual_stride, void *y, int32_t y_type,
@@ -1399,12 +1405,23 @@ static int32_t check_route(int32_t logits_type, const void *logits, int64_t toke
     return GOLLEK_HIP_OK;
 }
 
+// The device forms: a wave writes its token's routes while others still read theirs.
+static int32_t check_route_overlap(const void *logits, int32_t logits_type, int64_t tokens, int64_t n_experts,
+                                   const float *bias, int64_t top_k, const int32_t *ids, const float *weights, char *err,
+                                   size_t err_len) {
+    const int64_t ln = tokens * n_experts * element_size(logits_type), rn = tokens * top_k * 4;
+    if (share(ids, rn, logits, ln) || share(weights, rn, logits, ln) || share(ids, rn, bias, 4 * n_experts) ||
+        share(weights, rn, bias, 4 * n_experts) || share(ids, rn, weights, rn))
+        return fail(GOLLEK_HIP_ERR_ARG, err, err_len, "The routes overlap the logits, the bias or each other");
+    return GOLLEK_HIP_OK;
+}
+
 int32_t gollek_hip_moe_route_device(const void *logits, int32_t logits_type, int64_t tokens, int64_t n_experts,
                                     const float *bias, int32_t scoring, int64_t n_groups, int64_t top_groups,
                                     int32_t group_top, int64_t top_k, int32_t renormalize, float scale, int32_t *ids,
                                     float *weights, void *stream, char *err, size_t err_len) {
-    const int32_t rc = check_route(logits_type, logits, tokens, n_experts, bias, scoring, n_groups, top_groups,
-                                   group_top, top_k, scale, ids, weights, err, err_len);
+    int32_t rc = check_route(logits_type, logits, tokens, n_experts, bias, scoring, n_groups, top_groups, group_top,
+                             top_k, scale, ids, weights, err, err_len);
     if (rc != GOLLEK_HIP_OK) return rc;
     if (tokens == 0) {
         ok(err, err_len);
@@ -1412,6 +1429,8 @@ int32_t gollek_hip_moe_route_device(const void *logits, int32_t logits_type, int
     }
     if (logits == nullptr || ids == nullptr || weights == nullptr)
         return fail(GOLLEK_HIP_ERR_NULL, err, err_len, "router buffers");
+    rc = check_route_overlap(logits, logits_type, tokens, n_experts, bias, top_k, ids, weights, err, err_len);
+    if (rc != GOLLEK_HIP_OK) return rc;
     const DeviceGuard device(pointer_device(logits));
     const hipError_t e = gollek::launch_moe_expert_route(
         logits, logits_type, (int)tokens, (int)n_experts, bias, scoring == GOLLEK_HIP_ROUTER_SIGMOID, (int)n_groups,
@@ -1480,6 +1499,8 @@ int32_t gollek_hip_moe_block_routed_device(gollek_hip_weight *gate, gollek_hip_w
     if (x == nullptr || logits == nullptr || ids == nullptr || weights == nullptr || out == nullptr ||
         workspace == nullptr)
         return fail(GOLLEK_HIP_ERR_NULL, err, err_len, "MoE block buffers");
+    rc = check_route_overlap(logits, logits_type, tokens, n_experts, bias, top_k, ids, weights, err, err_len);
+    if (rc != GOLLEK_HIP_OK) return rc;
     const int64_t need = gollek_hip_moe_workspace_bytes(tokens, top_k, sh.H, sh.I, sh.E);
     if (workspace_bytes < need || (reinterpret_cast<uintptr_t>(workspace) & 255u) != 0)
         return fail(GOLLEK_HIP_ERR_ARG, err, err_len,

@@ -379,7 +379,8 @@ int32_t gollek_hip_moe_block_device(gollek_hip_weight *gate, gollek_hip_weight *
  * top_k.  n_experts in [1, 4096]; n_groups in [1, 64] dividing it, top_groups in
  * [1, n_groups]; top_k in [1, top_groups * n_experts / n_groups]; tokens * top_k up
  * to 2^24 and tokens * n_experts up to 2^30; a finite scale; aligned pointers:
- * else ARG; another logits_type -> UNSUPPORTED.  No reference
+ * else ARG; another logits_type -> UNSUPPORTED.  In the device forms ids and
+ * weights must not overlap the logits, the bias or each other (-> ARG).  No reference
  * counterpart: MoeForwardPass.java:174-203 routes by plain scores alone. */
 int32_t gollek_hip_moe_route(const void *logits, int32_t logits_type, int64_t tokens, int64_t n_experts,
                              const float *bias, int32_t scoring, int64_t n_groups, int64_t top_groups,

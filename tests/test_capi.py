@@ -287,3 +287,28 @@ def test_host_forms_without_a_weight_ask_for_the_device_first():
     for name, call in calls.items():
         assert call() == _native.ERR_DEVICE, name
         assert b"hipGetDevice failed" in e.buf.value or b"hipSetDevice failed" in e.buf.value, (name, e.buf.value)
+
+
+def _no_device():
+    import torch
+    if torch.cuda.is_available():
+        pytest.skip("made-up addresses: only where nothing can be launched")
+
+
+def test_route_refuses_routes_over_what_it_reads():
+    _no_device()
+    lib, e = _native.load(), _err()
+    t, n, k = 10, 32, 2
+
+    def rc(ids, w, bias=0, kind=0):
+        return lib.gollek_hip_moe_route_device(1 << 20, kind, t, n, bias, 0, 1, 1, 1, k, 1, 1.0, ids, w, None, e.buf, e.size)
+
+    free, end, r = 1 << 21, (1 << 20) + 4 * t * n, 4 * t * k
+    for over in (1 << 20, (1 << 20) + 4 - r, end - 4):
+        assert rc(over, free) == rc(free, over) == _native.ERR_ARG
+    assert rc(free, free) == rc(free, free + r - 4) == rc(free + r - 4, free) == _native.ERR_ARG
+    assert rc(free, free + r, bias=free - 4 * n + 4) == rc(free, free + 8 * r, bias=free + 9 * r - 4) == _native.ERR_ARG
+    # side by side they may stand: these calls end at the device that is not there
+    for call in (lambda: rc((1 << 20) - r, end), lambda: rc(end, end + r, bias=end + 2 * r),
+                 lambda: rc((1 << 20) + 2 * t * n, free, kind=30)):
+        assert call() == _native.ERR_DEVICE

@@ -1644,6 +1644,37 @@ static int32_t check_sample(const void *logits, int32_t logits_type, int64_t row
     return GOLLEK_HIP_OK;
 }
 
+// Whether `bytes` at b share one with the logits' rows (not with the gaps between them).
+static bool share_rows(const void *logits, int64_t rows, int64_t vocab, int64_t stride, int64_t size, const void *b,
+                       int64_t bytes) {
+    if (!share(logits, ((rows - 1) * stride + vocab) * size, b, bytes)) return false;
+    const uintptr_t at = reinterpret_cast<uintptr_t>(logits), from = reinterpret_cast<uintptr_t>(b);
+    if (from < at) return true;
+    const uintptr_t pitch = (uintptr_t)(stride * size), in = (from - at) % pitch;
+    return in < (uintptr_t)(vocab * size) || in + (uintptr_t)bytes > pitch;  // (in a gap, and up to the next row)
+}
+
+// The device form: rows are read by several workgroups and launches, and written by
+// the last; a row's results may take the place of its settings, whose readers are done.
+static int32_t check_sample_overlap(const void *logits, int64_t rows, int64_t vocab, int64_t stride, int64_t size,
+                                    const void *const (&settings)[5], const void *const (&results)[3],
+                                    const void *workspace, int64_t workspace_bytes, char *err, size_t err_len) {
+    const int64_t rn = rows * 4;
+    bool bad = workspace != nullptr && share_rows(logits, rows, vocab, stride, size, workspace, workspace_bytes);
+    for (int i = 0; i < 3; i++) {
+        const void *const r = results[i];
+        bad |= r != nullptr && share_rows(logits, rows, vocab, stride, size, r, rn);
+        bad |= share(r, rn, workspace, workspace_bytes);
+        for (int j = 0; j < i; j++) bad |= share(r, rn, results[j], rn);
+        for (const void *const s : settings) bad |= r != s && share(r, rn, s, rn);
+    }
+    for (const void *const s : settings) bad |= share(s, rn, workspace, workspace_bytes);
+    if (bad)
+        return fail(GOLLEK_HIP_ERR_ARG, err, err_len,
+                    "The sampling results or the workspace overlap the logits, a setting or each other");
+    return GOLLEK_HIP_OK;
+}
+
 int64_t gollek_hip_sample_workspace_bytes(int64_t rows, int64_t vocab) {
     if (rows < 0 || rows > kSampleMaxRows || vocab < 1 || vocab > kSampleMaxVocab) return -1;
     return (int64_t)align_up(gollek::sample_workspace_bytes((int)rows, (int)vocab), 256);
@@ -1655,8 +1686,8 @@ int32_t gollek_hip_sample_device(const void *logits, int32_t logits_type, int64_
                                  int32_t *kept, void *workspace, int64_t workspace_bytes, void *stream, char *err,
                                  size_t err_len) {
     if (logits_stride == 0) logits_stride = vocab;
-    const int32_t rc = check_sample(logits, logits_type, rows, vocab, logits_stride, temperature, top_k, top_p, min_p,
-                                    u, tokens, probs, kept, err, err_len);
+    int32_t rc = check_sample(logits, logits_type, rows, vocab, logits_stride, temperature, top_k, top_p, min_p, u,
+                              tokens, probs, kept, err, err_len);
     if (rc != GOLLEK_HIP_OK) return rc;
     if (rows == 0) {
         ok(err, err_len);
@@ -1667,6 +1698,9 @@ int32_t gollek_hip_sample_device(const void *logits, int32_t logits_type, int64_
     if (workspace_bytes < need || (reinterpret_cast<uintptr_t>(workspace) & 255u) != 0)
         return fail(GOLLEK_HIP_ERR_ARG, err, err_len, "Workspace of %lld bytes (256-byte aligned) needed, got %lld",
                     (long long)need, (long long)workspace_bytes);
+    rc = check_sample_overlap(logits, rows, vocab, logits_stride, element_size(logits_type),
+                              {temperature, top_k, top_p, min_p, u}, {tokens, probs, kept}, workspace, need, err, err_len);
+    if (rc != GOLLEK_HIP_OK) return rc;
     const DeviceGuard device(pointer_device(logits));
     const hipError_t e = gollek::launch_sample(logits, logits_type, (int)rows, (int)vocab, logits_stride, temperature,
                                                top_k, top_p, min_p, u, tokens, probs, kept,

@@ -459,7 +459,9 @@ int32_t gollek_hip_sample(const void *logits, int32_t logits_type, int64_t rows,
 int64_t gollek_hip_sample_workspace_bytes(int64_t rows, int64_t vocab);
 /* Device variant (every pointer on the device; `workspace` 256-byte aligned and
  * of at least gollek_hip_sample_workspace_bytes, else ARG; calls sharing it must
- * not overlap).  Allocates nothing: it can be captured into a graph. */
+ * not overlap).  The results and the workspace's bytes must not overlap the
+ * logits' rows, a setting or each other (-> ARG), but a result may be a setting's
+ * own array.  Allocates nothing: it can be captured into a graph. */
 int32_t gollek_hip_sample_device(const void *logits, int32_t logits_type, int64_t rows, int64_t vocab,
                                  int64_t logits_stride, const float *temperature, const int32_t *top_k,
                                  const float *top_p, const float *min_p, const float *u, int32_t *tokens, float *probs,

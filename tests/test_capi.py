@@ -312,3 +312,34 @@ def test_route_refuses_routes_over_what_it_reads():
     for call in (lambda: rc((1 << 20) - r, end), lambda: rc(end, end + r, bias=end + 2 * r),
                  lambda: rc((1 << 20) + 2 * t * n, free, kind=30)):
         assert call() == _native.ERR_DEVICE
+
+
+@pytest.mark.parametrize("vocab", [100, 20000])
+def test_sample_refuses_results_over_what_it_reads(vocab):
+    _no_device()
+    lib, e = _native.load(), _err()
+    rows, stride = 6, vocab + 12  # gaps of 48 bytes; the results are 24 bytes each
+    need = lib.gollek_hip_sample_workspace_bytes(rows, vocab)
+    l0, u, ws, free, n = 1 << 20, 1 << 30, 1 << 31, 1 << 33, 4 * rows
+    end = l0 + 4 * ((rows - 1) * stride + vocab)
+
+    def rc(tok=free, prob=0, kept=0, ws=ws, t=0, k=0):
+        return lib.gollek_hip_sample_device(l0, 0, rows, vocab, stride, t, k, 0, 0, u, tok, prob, kept, ws, 1 << 40, None,
+                                            e.buf, e.size)
+
+    gap = l0 + 4 * vocab  # behind the first row
+    for over in (l0, l0 + 4 - n, end - 4, gap - 4, gap + 28, l0 + 4 * stride):
+        assert rc(tok=over) == rc(prob=over) == rc(kept=over) == _native.ERR_ARG, over - l0
+    for over in (u + 4, u - n + 4, free, free + n - 4):
+        assert rc(prob=over) == rc(kept=over) == _native.ERR_ARG
+    assert rc(tok=u + 4) == rc(k=free + 4) == rc(prob=free + n, kept=free + 2 * n - 4) == _native.ERR_ARG
+    if need > 0:
+        base = (end + 255) // 256 * 256
+        for at in (l0, base - need // 256 * 256, base - 256):
+            assert rc(ws=at) == _native.ERR_ARG
+        assert rc(tok=ws) == rc(kept=ws + need - 4) == rc(t=ws + 256) == _native.ERR_ARG
+        assert rc(ws=u) == rc(ws=u - 256) == _native.ERR_ARG
+    # side by side, in a gap between rows, in a setting's own place: these end at the device that is not there
+    for kw in (dict(tok=gap, prob=gap + n), dict(tok=l0 - n, prob=end, kept=end + n), dict(tok=u), dict(prob=u, t=u),
+               dict(k=free, tok=free), dict(ws=(end + 255) // 256 * 256), dict(tok=ws + need)):
+        assert rc(**kw) == _native.ERR_DEVICE, kw

@@ -383,3 +383,19 @@ def test_the_largest_batchs_workspace_serves_smaller_ones():
             compare([g[:9] for g in got], l[:9], u[:9].cpu().numpy(), "200 rows", p=0.9)
             wants = got
         assert all(np.array_equal(g[:rows], w[:rows]) and (g[rows:] == -5).all() for g, w in zip(got, wants)), rows
+
+
+@pytest.mark.parametrize("vocab,rows", [(900, 40), (40000, 70)])
+def test_results_in_the_place_of_their_settings(vocab, rows):
+    l = logits_of(rows, vocab, 80)
+    rng = np.random.default_rng(81)
+    kw = dict(t=rng.choice([0.0, 0.7, 1.3], rows), k=rng.choice([0, 1, 40, 900], rows), p=rng.choice([0.8, 1.0], rows))
+    u = rng.random(rows).astype(np.float32)
+    t, p, du = (torch.from_numpy(np.asarray(a, np.float32)).cuda() for a in (kw["t"], kw["p"], u))
+    k, kept = torch.from_numpy(kw["k"].astype(np.int32)).cuda(), torch.zeros(rows, device="cuda", dtype=torch.int32)
+    ws = torch.zeros(max(ops.sample_workspace_bytes(rows, vocab), 256), device="cuda", dtype=torch.uint8)
+    ops.sample_device(l.data_ptr(), _native.F32, rows, vocab, du.data_ptr(), k.data_ptr(), temperature_ptr=t.data_ptr(),
+                      top_k_ptr=k.data_ptr(), top_p_ptr=p.data_ptr(), probs_ptr=du.data_ptr(), kept_ptr=kept.data_ptr(),
+                      ws_ptr=ws.data_ptr(), ws_bytes=ws.numel(), stream=torch.cuda.current_stream().cuda_stream)
+    torch.cuda.synchronize()
+    compare([a.cpu().numpy() for a in (k, du, kept)], l, u, "in place", **kw)

@@ -1054,9 +1054,13 @@ int32_t gollek_hip_linear(gollek_hip_weight *w, const uint16_t *x, int64_t x_len
     if (rc != GOLLEK_HIP_OK) return rc;
     const size_t xn = (size_t)(m * w->cols) * sizeof(uint16_t), bn = (size_t)w->rows * sizeof(float);
     const size_t yn = (size_t)(m * w->rows) * element_size(y_type);
-    const size_t ws_bytes =
+    size_t ws_bytes =
         w->compact ? 0
                    : gollek::linear_workspace_bytes(w->type_id, w->data, w->row_bytes, (int)m, (int)w->rows, (int)w->cols);
+    // Every handle keeps its staging: no more than 16 MiB of partials beyond the
+    // first (the copies of a long prompt take longer than its splits save).
+    const size_t most = kGemmScratchBytes + (size_t)(m * w->rows) * sizeof(float);
+    if (ws_bytes > most) ws_bytes = most;
     const size_t b_off = align_up(xn, 256), m_off = b_off + (bias != nullptr ? align_up(bn, 256) : 0);
     const size_t r_off = m_off + (mul != nullptr ? align_up(yn, 256) : 0);
     const size_t y_off = r_off + (residual != nullptr ? align_up(yn, 256) : 0), ws_off = y_off + align_up(yn, 256);

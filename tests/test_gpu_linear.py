@@ -623,3 +623,22 @@ def test_a_workspace_over_an_input_is_refused(t, m):
     room[at:at + size].view(torch.int16).copy_(xp.reshape(-1))
     wt.handle.linear(base + need, m, y.data_ptr(), _native.F32, ws_ptr=base, ws_bytes=need + size, activation=ops.ACT_SILU, **put)
     check(y, expected(wt, xb, ops.ACT_SILU, b, mu, re, _native.F32), "x behind the workspace")
+
+
+def test_the_host_form_keeps_its_handles_small():
+    """A handle's staging stays: x, y and no more than 16 MiB of partials beyond the first."""
+    rows, cols, m = 2048, 11008, 1129
+    wt = Weight(syn.Q4_0, rows, cols, 29)
+    y_bytes = 4 * m * rows
+    assert wt.handle.linear_workspace_bytes(m) > (16 << 20) + 2 * y_bytes  # the device form splits further
+    t = ops.GgufTensor("w", (cols, rows), syn.Q4_0, wt.data.reshape(-1))
+    xb = syn.activation_bf16(m, cols, seed=29)
+    ops.linear(t, xb[:1])
+    torch.cuda.synchronize()
+    before = torch.cuda.mem_get_info()[0]
+    y = ops.linear(t, xb, _native.F32, activation=ops.ACT_RELU)
+    held = before - torch.cuda.mem_get_info()[0]
+    assert held <= 2 * m * cols + 2 * y_bytes + (16 << 20) + (8 << 20)  # (and the allocator's granularity)
+    some = np.r_[0:20, m - 1]
+    check(torch.from_numpy(y[some]), expected(wt, xb[some], ops.ACT_RELU, None, None, None, _native.F32), "host form")
+    t.close()

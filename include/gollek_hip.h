@@ -212,9 +212,11 @@ int32_t gollek_hip_gemm_bf16(gollek_hip_weight *weight, const uint16_t *x_bf16, 
  * in fp32, rounded once to y_type (F32, F16 or BF16; nearest, ties to even).
  * bias (`rows` floats), mul and residual (m x rows of y_type) may each be NULL
  * and are then left out.  The sums are gollek_hip_gemm_bf16's for the same
- * weight, X and m (bit for bit where neither splits K); one row of X with a
- * Q6_K weight, or a Q4_K one of too many rows for the mat-vec's column layout,
- * has gollek_hip_matvec_rows's of that X row widened to fp32 (unless it splits K).
+ * weight, X and m (bit for bit where neither splits K); one row of X, 16-byte
+ * aligned, has gollek_hip_matvec_rows's of that row widened to fp32 with a Q6_K
+ * weight of a multiple of 2048 columns up to 14336 (unless it splits K) and with
+ * a Q4_K one of up to 4096 columns and too many rows for the mat-vec's column
+ * layout.
  * A gated FFN is two calls: the up product, then the gate's with
  * activation SILU and mul = the up product's Y.  The reference adds biases and
  * residuals in Java after its linear (AccelOps.java:370-376).
@@ -227,8 +229,9 @@ int32_t gollek_hip_linear(gollek_hip_weight *weight, const uint16_t *x_bf16, int
                           int32_t y_type, int64_t y_len, char *err, size_t err_len);
 
 /* Device workspace bytes with which gollek_hip_linear_device splits K as far as
- * it pays (0: a call of m rows never splits), up to some hundred MB for long
- * prompts; -1 for a NULL weight or m out of range. */
+ * it pays (0: a call of m rows never splits): for Q8_0 and Q4_0 up to some
+ * hundred MB for long prompts, for the others partials of at most 16 MiB beyond
+ * the first; -1 for a NULL weight or m out of range. */
 int64_t gollek_hip_linear_workspace_bytes(const gollek_hip_weight *weight, int64_t m);
 
 /* Device variant, asynchronous on `stream`, which belongs to the weight's

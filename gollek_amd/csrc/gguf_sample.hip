@@ -272,7 +272,7 @@ __device__ Border select(const SampleArgs &a, int64_t base, const Scale &sc, Bor
     } else {
         r = count - seen;
     }
-    if (r >= ties) return Border{prefix, 0x7FFFFFFF};
+    if (r >= ties) return Border{prefix, prefix == in.key ? in.index : 0x7FFFFFFF};  // (all within `in`)
     // the index of the r-th of them: kThreads indexes at a time
     if (threadIdx.x == 0) s.found = 0x7FFFFFFF;
     uint32_t had = 0;

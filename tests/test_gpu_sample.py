@@ -399,3 +399,18 @@ def test_results_in_the_place_of_their_settings(vocab, rows):
                       ws_ptr=ws.data_ptr(), ws_bytes=ws.numel(), stream=torch.cuda.current_stream().cuda_stream)
     torch.cuda.synchronize()
     compare([a.cpu().numpy() for a in (k, du, kept)], l, u, "in place", **kw)
+
+
+@pytest.mark.parametrize("vocab", [5000, 16384, 40000])
+@pytest.mark.parametrize("kw", [dict(k=200, p=0.999), dict(k=1, p=0.9), dict(t=0.0, p=0.5), dict(k=2, p=0.99, mp=0.3),
+                                dict(k=65, p=0.9999, t=3.0), dict(k=4500, p=0.99999), dict(k=3, p=0.7, t=float("inf"))])
+def test_top_p_that_keeps_all_of_top_k_in_a_crowd(vocab, kw):
+    """Thousands of equal logits through which top_k cuts; top_p then keeps every token that it left."""
+    l = torch.full((4, vocab), -3.5, device="cuda")
+    l[1, 100:103] = -3.0                     # the crowd is the second value
+    l[2, ::7] = float("-inf")
+    l[3, vocab // 2:] = float("-inf")
+    l[3, :vocab // 2] = 0.0
+    u = np.array([0.05, 0.9, 0.5, 0.99], np.float32)
+    for dtype in (torch.float32, torch.bfloat16):
+        compare(sample(l.to(dtype), u, **kw), l, u, f"crowd {vocab} {kw} {dtype}", **kw)

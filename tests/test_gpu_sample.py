@@ -414,3 +414,21 @@ def test_top_p_that_keeps_all_of_top_k_in_a_crowd(vocab, kw):
     u = np.array([0.05, 0.9, 0.5, 0.99], np.float32)
     for dtype in (torch.float32, torch.bfloat16):
         compare(sample(l.to(dtype), u, **kw), l, u, f"crowd {vocab} {kw} {dtype}", **kw)
+
+
+@pytest.mark.parametrize("kind", [syn.Q6_K, syn.Q8_0])
+def test_next_token_of_a_long_vocabulary(kind):
+    rows, cols = 20011, 512
+    t = ops.GgufTensor("output.weight", (cols, rows), kind, syn.matrix(kind, rows, cols, seed=12).reshape(-1))
+    rng = np.random.default_rng(13)
+    for i in range(8):
+        x = rng.normal(size=cols).astype(np.float32) * (0.0 if i == 7 else 1.0)  # (the last: equal logits)
+        y = np.zeros(rows, np.float32)
+        ops.mat_vec(t, x, y)
+        kw = dict(temperature=(0.0, 5.0, 20.0, 1.0)[i % 4], top_k=(0, 50, 700)[i % 3], top_p=(1.0, 0.9)[i % 2], min_p=0.0)
+        u = np.float32(0.07 + 0.12 * i)
+        got = ops.next_token(t, x, float(u), **kw)
+        host = ops.sample(y[None], [u], **kw)
+        assert got == tuple(a[0] for a in host)
+        compare(host, y[None], u, f"next token {kw}", t=kw["temperature"], k=kw["top_k"], p=kw["top_p"])
+    t.close()

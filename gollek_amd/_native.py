@@ -89,6 +89,22 @@ SIGNATURES: dict[str, tuple[object, list[object]]] = {
     "gollek_hip_sample_device": (_I32, [_P, _I32, _I64, _I64, _I64, _P, _P, _P, _P, _P, _P, _P, _P, _P, _I64, _P,
                                         _CHARP, _SZ]),
     "gollek_hip_next_token": (_I32, [_P, _P, _I64, _F32, _I32, _F32, _F32, _F32, _P, _P, _P, _CHARP, _SZ]),
+    "gollek_hip_norm": (_I32, [_P, _I32, _I64, _I64, _P, _P, _F32, _P, _P, _I32, _P, _P, _I32, _F32, _P, _I32, _CHARP,
+                               _SZ]),
+    "gollek_hip_norm_device": (_I32, [_P, _I32, _I64, _I64, _I64, _P, _P, _F32, _P, _I64, _P, _I32, _I64, _P, _P, _I32,
+                                      _F32, _P, _I32, _I64, _P, _CHARP, _SZ]),
+    "gollek_hip_rope_frequencies": (_I32, [_I64, _F32, _I32, _F32, _F32, _F32, _F32, _F32, _P, _P, _P, _CHARP, _SZ]),
+    "gollek_hip_rope_create": (_P, [_I32, _I64, _F32, _I32, _F32, _F32, _F32, _F32, _F32, _P, _CHARP, _SZ]),
+    "gollek_hip_rope_free": (None, [_P]),
+    "gollek_hip_rope_apply": (_I32, [_P, _P, _I32, _I64, _I64, _I64, _P, _P, _CHARP, _SZ]),
+    "gollek_hip_rope_apply_device": (_I32, [_P, _P, _I32, _I64, _I64, _I64, _I64, _P, _P, _I64, _P, _CHARP, _SZ]),
+    "gollek_hip_kv_cache_wrap_device": (_P, [_I32, _P, _P, _I64, _I64, _I64, _I64, _CHARP, _SZ]),
+    "gollek_hip_kv_cache_free": (None, [_P]),
+    "gollek_hip_kv_append_device": (_I32, [_P, _P, _P, _I64, _P, _I64, _P, _I64, _I64, _I32, _I64, _P, _P, _F32, _P, _P,
+                                           _P, _I64, _I64, _P, _I64, _P, _CHARP, _SZ]),
+    "gollek_hip_attention_device": (_I32, [_P, _P, _I64, _I64, _I64, _P, _P, _I64, _F32, _F32, _I64, _P, _P, _I32, _I64,
+                                           _P, _I64, _P, _CHARP, _SZ]),
+    "gollek_hip_attention_workspace_bytes": (_I64, [_P, _I64, _I64, _I64]),
     "gollek_hip_gguf_open": (_P, [_CHARP, _CHARP, _SZ]),
     "gollek_hip_gguf_close": (None, [_P]),
     "gollek_hip_gguf_info": (_I32, [_P, _P, _P, _P, _P, _P, _P]),

@@ -40,6 +40,10 @@ HIP_SOURCES = (
     "gguf_sample.hip",
     "gguf_moe_gemm.hip",
     "gguf_kq_gemm.hip",
+    "layer_capi.hip",
+    "layer_norm.hip",
+    "layer_heads.hip",
+    "layer_attention.hip",
 )
 
 ARCH = "gfx950"

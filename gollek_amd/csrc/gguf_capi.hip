@@ -15,6 +15,7 @@
 #include <new>
 #include <string>
 
+#include "gguf_capi_util.hpp"
 #include "gguf_kernels.hpp"
 #include "gollek_hip.h"
 #include "gollek_hip_testing.h"
@@ -41,6 +42,13 @@ struct gollek_hip_weight {
 };
 
 namespace {
+
+using gollek::DeviceGuard;
+using gollek::element_size;
+using gollek::overlaps;
+using gollek::pointer_device;
+using gollek::share;
+using gollek::within;
 
 constexpr int32_t kAbiVersion = 1 * 10000 + 1 * 100 + 0;
 constexpr int64_t kRouterMaxExperts = 4096;  // router LDS: 8 B per expert + 4 B per rank
@@ -865,72 +873,6 @@ int32_t gollek_hip_gemm_bf16_device_noalloc(gollek_hip_weight *w, const uint16_t
 // ---- the linear layer: a product with its epilogue -----------------------
 
 namespace {
-
-// A device current for the calls inside, the caller's again afterwards.
-class DeviceGuard {
-public:
-    explicit DeviceGuard(int device) {
-        if (hipGetDevice(&before_) != hipSuccess || before_ == device) before_ = -1;
-        else if (hipSetDevice(device) != hipSuccess) before_ = -1;
-    }
-    ~DeviceGuard() {
-        if (before_ >= 0) (void)hipSetDevice(before_);
-    }
-    DeviceGuard(const DeviceGuard &) = delete;
-    DeviceGuard &operator=(const DeviceGuard &) = delete;
-
-private:
-    int before_ = -1;
-};
-
-// The device that holds device memory p (the current one where there is no
-// other, or p is not known).
-int pointer_device(const void *p) {
-    static const int devices = [] {
-        int n = 0;
-        return hipGetDeviceCount(&n) == hipSuccess ? n : 0;
-    }();
-    int device = 0;
-    if (devices > 1) {
-        hipPointerAttribute_t at;
-        if (hipPointerGetAttributes(&at, p) == hipSuccess && at.type == hipMemoryTypeDevice) return at.device;
-        (void)hipGetLastError();
-    }
-    (void)hipGetDevice(&device);
-    return device;
-}
-
-int element_size(int32_t type) {
-    return type == GOLLEK_HIP_F32 ? 4 : type == GOLLEK_HIP_F16 || type == GOLLEK_HIP_BF16 ? 2 : 0;
-}
-
-// Whether writing matrix y (m rows of n elements, y_stride apart) changes an
-// element of matrix b other than the one at the same place: the same matrix
-// is fine, and so are two column ranges of one wider matrix.
-bool overlaps(const void *y, int64_t y_stride, const void *b, int64_t b_stride, int64_t m, int64_t n, int64_t size) {
-    const uintptr_t ya = reinterpret_cast<uintptr_t>(y), ba = reinterpret_cast<uintptr_t>(b);
-    const uintptr_t ye = ya + (uintptr_t)(((m - 1) * y_stride + n) * size);
-    const uintptr_t be = ba + (uintptr_t)(((m - 1) * b_stride + n) * size);
-    if (ye <= ba || be <= ya) return false;
-    if (m == 1) return ya != ba;
-    if (y_stride != b_stride) return true;
-    if (ya == ba) return false;
-    const uintptr_t row = (uintptr_t)(y_stride * size), width = (uintptr_t)(n * size);
-    const uintptr_t apart = (ya > ba ? ya - ba : ba - ya) % row;
-    return !(apart >= width && row - apart >= width);
-}
-
-// Whether matrix y and `bytes` bytes at b share a byte (y's gaps between rows counted as y's).
-bool within(const void *y, int64_t m, int64_t n, int64_t y_stride, int64_t size, const void *b, int64_t bytes) {
-    const uintptr_t ya = reinterpret_cast<uintptr_t>(y), ba = reinterpret_cast<uintptr_t>(b);
-    return ba < ya + (uintptr_t)(((m - 1) * y_stride + n) * size) && ya < ba + (uintptr_t)bytes;
-}
-
-// Whether two stretches of bytes share one (NULL shares none).
-bool share(const void *a, int64_t a_bytes, const void *b, int64_t b_bytes) {
-    const uintptr_t x = reinterpret_cast<uintptr_t>(a), y = reinterpret_cast<uintptr_t>(b);
-    return a != nullptr && b != nullptr && y < x + (uintptr_t)a_bytes && x < y + (uintptr_t)b_bytes;
-}
 
 // Checks a linear call's epilogue and fills `out`.  Strides of 0 are packed rows.
 int32_t make_epilogue(const gollek_hip_weight *w, int64_t m, const float *bias, int32_t activation, const void *mul,
@@ -1815,6 +1757,8 @@ int32_t gollek_hip_next_token(gollek_hip_weight *w, const float *x, int64_t x_le
 }  // extern "C"
 
 namespace gollek {
+
+int32_t ready_current_device(char *err, size_t err_len) { return use_current_device(err, err_len); }
 
 void record_status(int32_t code, const char *message) {
     g_last_status = code;

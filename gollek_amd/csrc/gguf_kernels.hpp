@@ -266,6 +266,8 @@ namespace gollek {
 
 // Sets what gollek_hip_last_status / gollek_hip_last_error report.
 void record_status(int32_t code, const char *message);
+// Makes the current device ready for launches (its CU count, its scratch).
+int32_t ready_current_device(char *err, size_t err_len);
 // A weight handle on the current device that owns an uninitialised
 // rows * row_bytes device buffer; same validation and messages as
 // gollek_hip_weight_upload.  nullptr (with the error recorded) on failure.

@@ -766,3 +766,198 @@ def next_token(lm_head: GgufTensor, vector, u: float, *, temperature: float = 1.
                                                min_p, u, ctypes.byref(token), ctypes.byref(prob), ctypes.byref(kept),
                                                err.buf, err.size), err)
     return token.value, prob.value, kept.value
+
+
+# ---- between the products of a decoder layer -----------------------------------
+
+NORM_RMS = 0
+NORM_LAYER = 1
+ROPE_HALF = 0
+ROPE_INTERLEAVED = 1
+ROPE_NONE = 0
+ROPE_LINEAR = 1
+ROPE_YARN = 2
+ROPE_LLAMA3 = 3
+
+
+def _typed(a, name):
+    """A host array as it is passed on and its element type (as _logits)."""
+    if a is None:
+        raise NullPointerError(name)
+    return _logits(a)
+
+
+def norm(x, weight=None, *, bias=None, kind: int = NORM_RMS, eps: float = 1e-6, post_weight=None, gate=None,
+         scale: float = 1.0, residual=None, hidden_type: int | None = None, y_type: int = _native.F32):
+    """The norms around a block (gollek_hip_norm) on host arrays: x (rows, cols)
+    float32, float16 or uint16 bf16 bit patterns, residual likewise (its type is
+    hidden's; without one hidden_type, by default x's), vectors (cols,) float32 ->
+    hidden, y."""
+    xv, x_type = _typed(x, "input")
+    if xv.ndim != 2:
+        raise IllegalArgumentError("input must be (rows, cols)")
+    rows, cols = xv.shape
+    rv = None
+    if residual is not None:
+        rv, r_type = _logits(residual)
+        if rv.shape != xv.shape or hidden_type not in (None, r_type):
+            raise IllegalArgumentError(f"residual must be {xv.shape} of the hidden type")
+        hidden_type = r_type
+    hidden_type = x_type if hidden_type is None else hidden_type
+    for t in (hidden_type, y_type):
+        if t not in _LINEAR_DTYPES:
+            raise UnsupportedOperationError(f"Unsupported norm type id: {t} (F32, F16 or BF16)")
+
+    def vector(v, name):
+        if v is None:
+            return None
+        v = np.ascontiguousarray(v, dtype=np.float32)
+        if v.shape != (cols,):
+            raise IllegalArgumentError(f"{name} must be ({cols},)")
+        return v
+
+    vs = [vector(v, n) for v, n in ((post_weight, "post_weight"), (gate, "gate"), (weight, "weight"), (bias, "bias"))]
+    at = [None if v is None else v.ctypes.data for v in vs]
+    h, y = np.empty(xv.shape, _LINEAR_DTYPES[hidden_type]), np.empty(xv.shape, _LINEAR_DTYPES[y_type])
+    err = _native.ErrBuf()
+    check(_native.load().gollek_hip_norm(xv.ctypes.data, x_type, rows, cols, at[0], at[1], scale,
+                                         None if rv is None else rv.ctypes.data, h.ctypes.data, hidden_type, at[2], at[3],
+                                         kind, eps, y.ctypes.data, y_type, err.buf, err.size), err)
+    return h, y
+
+
+def norm_device(x_ptr: int, x_type: int, rows: int, cols: int, *, x_stride: int = 0, post_weight_ptr: int = 0,
+                gate_ptr: int = 0, scale: float = 1.0, residual_ptr: int = 0, residual_stride: int = 0,
+                hidden_ptr: int = 0, hidden_type: int = _native.F32, hidden_stride: int = 0, weight_ptr: int = 0,
+                bias_ptr: int = 0, kind: int = NORM_RMS, eps: float = 1e-6, y_ptr: int = 0, y_type: int = _native.BF16,
+                y_stride: int = 0, stream: int = 0) -> None:
+    """hidden = residual + scale * gate * (norm of x by post_weight, or x), y = norm
+    of that by weight and bias (gollek_hip_norm_device); 0 leaves a part out."""
+    err = _native.err_buf()
+    check(_native.load().gollek_hip_norm_device(x_ptr, x_type, rows, cols, x_stride, post_weight_ptr, gate_ptr, scale,
+                                                residual_ptr, residual_stride, hidden_ptr, hidden_type, hidden_stride,
+                                                weight_ptr, bias_ptr, kind, eps, y_ptr, y_type, y_stride, stream,
+                                                err.buf, err.size), err)
+
+
+def _factors(factors, dims):
+    if factors is None:
+        return None
+    f = np.ascontiguousarray(factors, dtype=np.float32)
+    if f.shape != (dims // 2,):
+        raise IllegalArgumentError(f"factors must be ({dims // 2},)")
+    return f
+
+
+def rope_frequencies(dims: int, *, base: float = 10000.0, scaling: int = ROPE_NONE, factor: float = 1.0,
+                     original_context: float = 0.0, low: float = 0.0, high: float = 0.0, magnitude: float = 0.0,
+                     factors=None):
+    """Radians a position of each pair (dims / 2,) float32 and the magnitude
+    (gollek_hip_rope_frequencies; needs no GPU)."""
+    f = _factors(factors, dims)
+    out, result = np.empty(max(dims, 0) // 2, np.float32), ctypes.c_float()
+    err = _native.ErrBuf()
+    check(_native.load().gollek_hip_rope_frequencies(dims, base, scaling, factor, original_context, low, high, magnitude,
+                                                     None if f is None else f.ctypes.data, out.ctypes.data,
+                                                     ctypes.addressof(result), err.buf, err.size), err)
+    return out, result.value
+
+
+class Rope:
+    """A model's rotary table on the current device (gollek_hip_rope)."""
+
+    def __init__(self, dims: int, *, layout: int = ROPE_HALF, base: float = 10000.0, scaling: int = ROPE_NONE,
+                 factor: float = 1.0, original_context: float = 0.0, low: float = 0.0, high: float = 0.0,
+                 magnitude: float = 0.0, factors=None):
+        f = _factors(factors, dims)
+        err = _native.ErrBuf()
+        lib = _native.load()
+        self.handle = lib.gollek_hip_rope_create(layout, dims, base, scaling, factor, original_context, low, high,
+                                                 magnitude, None if f is None else f.ctypes.data, err.buf, err.size)
+        if not self.handle:
+            check(lib.gollek_hip_last_status(), err)
+        self.dims = dims
+
+    def close(self) -> None:
+        if self.handle:
+            _native.load().gollek_hip_rope_free(self.handle)
+            self.handle = None
+
+    def __del__(self):
+        try:
+            self.close()
+        except Exception:
+            pass
+
+    def apply(self, x, positions) -> np.ndarray:
+        """x (tokens, heads, head_dim) float32, float16 or uint16 bf16 bit patterns,
+        rotated to positions (tokens,)."""
+        xv, kind = _typed(x, "input")
+        if positions is None:
+            raise NullPointerError("positions")
+        pv = np.ascontiguousarray(positions, dtype=np.int32)
+        if xv.ndim != 3 or pv.shape != xv.shape[:1]:
+            raise IllegalArgumentError("input must be (tokens, heads, head_dim) and positions (tokens,)")
+        out = np.empty_like(xv)
+        err = _native.ErrBuf()
+        check(_native.load().gollek_hip_rope_apply(self.handle, xv.ctypes.data, kind, *xv.shape, pv.ctypes.data,
+                                                   out.ctypes.data, err.buf, err.size), err)
+        return out
+
+    def apply_device(self, x_ptr: int, type_id: int, tokens: int, heads: int, head_dim: int, positions_ptr: int,
+                     out_ptr: int, *, x_stride: int = 0, out_stride: int = 0, stream: int = 0) -> None:
+        err = _native.err_buf()
+        check(_native.load().gollek_hip_rope_apply_device(self.handle, x_ptr, type_id, tokens, heads, head_dim, x_stride,
+                                                          positions_ptr, out_ptr, out_stride, stream, err.buf,
+                                                          err.size), err)
+
+
+class KvCache:
+    """A paged cache of keys and values in the caller's device memory
+    (gollek_hip_kv_cache): k and v (pages, kv_heads, page_size, head_dim) of F16 or
+    BF16, which must outlive it."""
+
+    def __init__(self, type_id: int, k_ptr: int, v_ptr: int, pages: int, page_size: int, kv_heads: int, head_dim: int):
+        err = _native.ErrBuf()
+        lib = _native.load()
+        self.handle = lib.gollek_hip_kv_cache_wrap_device(type_id, k_ptr, v_ptr, pages, page_size, kv_heads, head_dim,
+                                                          err.buf, err.size)
+        if not self.handle:
+            check(lib.gollek_hip_last_status(), err)
+
+    def close(self) -> None:
+        if self.handle:
+            _native.load().gollek_hip_kv_cache_free(self.handle)
+            self.handle = None
+
+    def __del__(self):
+        try:
+            self.close()
+        except Exception:
+            pass
+
+    def append(self, k_ptr: int, v_ptr: int, type_id: int, tokens: int, positions_ptr: int, page_table_ptr: int,
+               sequences: int, max_pages: int, *, rope: Rope | None = None, k_stride: int = 0, v_stride: int = 0,
+               q_ptr: int = 0, q_heads: int = 0, q_stride: int = 0, q_out_ptr: int = 0, q_out_stride: int = 0,
+               q_norm_ptr: int = 0, k_norm_ptr: int = 0, eps: float = 1e-6, sequence_ptr: int = 0,
+               stream: int = 0) -> None:
+        """New tokens' keys (normalised, rotated) and values into their pages, their
+        queries (normalised, rotated) to q_out (gollek_hip_kv_append_device)."""
+        err = _native.err_buf()
+        check(_native.load().gollek_hip_kv_append_device(
+            self.handle, None if rope is None else rope.handle, k_ptr, k_stride, v_ptr, v_stride, q_ptr, q_heads,
+            q_stride, type_id, tokens, q_norm_ptr, k_norm_ptr, eps, positions_ptr, sequence_ptr, page_table_ptr,
+            sequences, max_pages, q_out_ptr, q_out_stride, stream, err.buf, err.size), err)
+
+    def attend_workspace_bytes(self, sequences: int, q_heads: int, max_pages: int) -> int:
+        return int(_native.load().gollek_hip_attention_workspace_bytes(self.handle, sequences, q_heads, max_pages))
+
+    def attend(self, q_ptr: int, sequences: int, q_heads: int, lengths_ptr: int, page_table_ptr: int, max_pages: int,
+               out_ptr: int, out_type: int, *, scale: float, softcap: float = 0.0, window: int = 0, sinks_ptr: int = 0,
+               q_stride: int = 0, out_stride: int = 0, ws_ptr: int = 0, ws_bytes: int = 0, stream: int = 0) -> None:
+        """Attention of one new token a sequence over the first lengths of its pages
+        (gollek_hip_attention_device)."""
+        err = _native.err_buf()
+        check(_native.load().gollek_hip_attention_device(
+            self.handle, q_ptr, q_stride, sequences, q_heads, lengths_ptr, page_table_ptr, max_pages, scale, softcap,
+            window, sinks_ptr, out_ptr, out_type, out_stride, ws_ptr, ws_bytes, stream, err.buf, err.size), err)

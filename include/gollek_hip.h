@@ -480,6 +480,144 @@ int32_t gollek_hip_next_token(gollek_hip_weight *lm_head, const float *x, int64_
                               int32_t top_k, float top_p, float min_p, float u, int32_t *token, float *prob,
                               int32_t *kept, char *err, size_t err_len);
 
+/* ---- between the products of a decoder layer ------------------------------- */
+
+/* Element types of these calls: F32, F16 and BF16 (ggml type ids 0, 1, 30); any
+ * other -> UNSUPPORTED.  Computed in fp32 and rounded once (to nearest).  Device
+ * forms are asynchronous on the caller's stream, allocate nothing and can be
+ * captured into a graph; their arrays are aligned to their elements (else ARG), and
+ * what a call writes must not share memory with what it reads or with its other
+ * results, unless said otherwise (-> ARG).  A stride is the number of elements
+ * between two rows (0: packed).  The reference's GGUF path leaves these to its Java
+ * runner; none of them replaces an entry of it. */
+
+#define GOLLEK_HIP_NORM_RMS 0   /* N(v) = v / sqrt(mean(v^2) + eps) */
+#define GOLLEK_HIP_NORM_LAYER 1 /* N(v) = (v - mean(v)) / sqrt(mean((v - mean(v))^2) + eps) */
+
+/* The norms around a block, row by row (rows x cols):
+ *   b = post_weight ? N(x) * post_weight : x
+ *   h = residual + scale * gate * b               -> hidden, of hidden_type
+ *   y = N(h) * weight + bias                      -> y, of y_type
+ * with N by `kind` and h unrounded in N(h).  post_weight, gate, weight, bias: cols
+ * floats; residual: of hidden_type; NULL: no first norm, gate 1, residual 0, weight 1,
+ * bias 0; hidden or y may be NULL (not both).  rows up to 2^31 - 1, cols in
+ * [1, 65536], a finite scale, eps >= 0 and finite: else ARG.  hidden may be x or the
+ * residual itself, y may be x or the residual (the same address, type size and
+ * stride).  A row of zeros with eps 0 divides 0 by 0 (NaN).
+ * The host form takes packed rows and copies them up (synchronous). */
+int32_t gollek_hip_norm(const void *x, int32_t x_type, int64_t rows, int64_t cols, const float *post_weight,
+                        const float *gate, float scale, const void *residual, void *hidden, int32_t hidden_type,
+                        const float *weight, const float *bias, int32_t kind, float eps, void *y, int32_t y_type,
+                        char *err, size_t err_len);
+int32_t gollek_hip_norm_device(const void *x, int32_t x_type, int64_t rows, int64_t cols, int64_t x_stride,
+                               const float *post_weight, const float *gate, float scale, const void *residual,
+                               int64_t residual_stride, void *hidden, int32_t hidden_type, int64_t hidden_stride,
+                               const float *weight, const float *bias, int32_t kind, float eps, void *y,
+                               int32_t y_type, int64_t y_stride, void *stream, char *err, size_t err_len);
+
+/* Rotary positions: which elements of a head's first `dims` make a pair. */
+#define GOLLEK_HIP_ROPE_HALF 0        /* i and i + dims / 2 */
+#define GOLLEK_HIP_ROPE_INTERLEAVED 1 /* 2 i and 2 i + 1 */
+/* How their frequencies f_i = base^(-2 i / dims) are scaled for long contexts. */
+#define GOLLEK_HIP_ROPE_NONE 0
+#define GOLLEK_HIP_ROPE_LINEAR 1 /* f / factor */
+#define GOLLEK_HIP_ROPE_YARN 2   /* f / factor where a pair turns fewer than `low` times in original_context, f where more
+                                  * than `high` times, mixed by a ramp over the pairs between; magnitude 0.1 ln(factor) + 1 */
+#define GOLLEK_HIP_ROPE_LLAMA3 3 /* the same borders, mixed by the number of turns; magnitude 1 */
+
+/* Opaque table of a model's rotary frequencies, on the device that was current. */
+typedef struct gollek_hip_rope gollek_hip_rope;
+
+/* Frequencies (radians a position, dims / 2 floats) and magnitude (one float) that
+ * a table of these arguments has; either may be NULL; needs no GPU.  Pair i of a head
+ * turns by position * f_i and is multiplied by the magnitude; magnitude 0 stands for
+ * the scaling's own (1, or YARN's).  factors: dims / 2 floats that divide the
+ * frequencies first (a GGUF file's rope_freqs.weight), or NULL.  dims even in
+ * [2, 256], base > 1, and where the scaling uses them factor > 0, original_context > 0
+ * and 0 < low < high; everything finite, magnitude >= 0, factors > 0: else ARG.  The
+ * table itself is in 64 bits: a position of 2^31 keeps its angle. */
+int32_t gollek_hip_rope_frequencies(int64_t dims, float base, int32_t scaling, float factor, float original_context,
+                                    float low, float high, float magnitude, const float *factors, float *frequencies,
+                                    float *resulting_magnitude, char *err, size_t err_len);
+/* NULL on failure.  An unknown layout -> ARG. */
+gollek_hip_rope *gollek_hip_rope_create(int32_t layout, int64_t dims, float base, int32_t scaling, float factor,
+                                        float original_context, float low, float high, float magnitude,
+                                        const float *factors, char *err, size_t err_len);
+/* Waits for the device's work first.  NULL is a no-op. */
+void gollek_hip_rope_free(gollek_hip_rope *rope);
+
+/* out = x (tokens x heads x head_dim) with every head's first dims elements rotated
+ * to its token's position, the others as they are; out of x's type, may be x itself
+ * (with its stride).  head_dim even in [dims, 256], heads in [1, 65535], tokens up to
+ * 2^31 - 1: else ARG.  The host form takes packed rows and copies them up. */
+int32_t gollek_hip_rope_apply(const gollek_hip_rope *rope, const void *x, int32_t type, int64_t tokens, int64_t heads,
+                              int64_t head_dim, const int32_t *positions, void *out, char *err, size_t err_len);
+int32_t gollek_hip_rope_apply_device(const gollek_hip_rope *rope, const void *x, int32_t type, int64_t tokens,
+                                     int64_t heads, int64_t head_dim, int64_t x_stride, const int32_t *positions,
+                                     void *out, int64_t out_stride, void *stream, char *err, size_t err_len);
+
+/* Opaque paged cache of keys and values: a view of two device arrays that the
+ * caller keeps, each (pages x kv_heads x page_size x head_dim) of `type`, F16 or BF16. */
+typedef struct gollek_hip_kv_cache gollek_hip_kv_cache;
+
+/* page_size a power of two in [16, 65536], head_dim a multiple of 8 in [8, 256],
+ * kv_heads in [1, 65535], pages in [1, 2^31 - 1], k and v 16-byte aligned and apart:
+ * else ARG; another type -> UNSUPPORTED.  NULL on failure. */
+gollek_hip_kv_cache *gollek_hip_kv_cache_wrap_device(int32_t type, void *k, void *v, int64_t pages, int64_t page_size,
+                                                     int64_t kv_heads, int64_t head_dim, char *err, size_t err_len);
+/* Frees the handle, not the arrays.  NULL is a no-op. */
+void gollek_hip_kv_cache_free(gollek_hip_kv_cache *cache);
+
+/* Appends new tokens to a cache, and makes their queries ready for it:
+ *   k, v (tokens x kv_heads x head_dim of `type`): k by k_norm and rope -> the cache
+ *     at the token's place, v as it is;
+ *   q (tokens x q_heads x head_dim of `type`, NULL with q_heads 0): by q_norm and
+ *     rope -> q_out, of the cache's type.
+ * q_norm, k_norm (head_dim floats, NULL: none): RMS norms of each head before it
+ * turns; rope NULL: no rotation.  The place of token t is position positions[t] of
+ * sequence sequence[t] (NULL: t), in page page_table[sequence * max_pages +
+ * position / page_size].  A token whose position is below 0, or whose sequence is
+ * outside [0, sequences), is padding: nothing of it is written.  Where the position
+ * is past the table (max_pages * page_size) or the page outside [0, pages), k and v
+ * are dropped.  Two tokens of a call must not have one place: which of them stays is
+ * not determined.  q_out may be q itself where the types have one size (and with its
+ * stride).  tokens up to 2^31 - 1, q_heads in [0, 65535], max_pages >= 1 with
+ * max_pages * page_size < 2^31, rope's dims at most head_dim, rope on the cache's
+ * device: else ARG. */
+int32_t gollek_hip_kv_append_device(const gollek_hip_kv_cache *cache, const gollek_hip_rope *rope, const void *k,
+                                    int64_t k_stride, const void *v, int64_t v_stride, const void *q, int64_t q_heads,
+                                    int64_t q_stride, int32_t type, int64_t tokens, const float *q_norm,
+                                    const float *k_norm, float eps, const int32_t *positions, const int32_t *sequence,
+                                    const int32_t *page_table, int64_t sequences, int64_t max_pages, void *q_out,
+                                    int64_t q_out_stride, void *stream, char *err, size_t err_len);
+
+/* Attention of one new token a sequence over the cache.  q (sequences x q_heads x
+ * head_dim of the cache's type, as gollek_hip_kv_append_device leaves it); q_heads a
+ * multiple of kv_heads, whose q_heads / kv_heads neighbours share keys and values:
+ *   s_j = scale * q . k_j,  capped: softcap * tanh(s_j / softcap) (softcap 0: not)
+ *   out = sum_j exp(s_j) v_j / (sum_j exp(s_j) + exp(sinks[head]))   (sinks NULL: no such term)
+ * over the last `window` (0: all) of the first lengths[sequence] tokens, -> out
+ * (sequences x q_heads x head_dim of out_type).  A length past the table counts as
+ * the table's, one below 1 as 0; a token whose page is outside [0, pages) is not
+ * there; a row without any token is 0.  Nothing behind a sequence's length or before
+ * its window changes a result, whatever it holds.  Several new tokens of one
+ * sequence are rows of their own, with equal page_table rows and growing lengths.
+ * Results depend in their last bits on the lengths in the batch (they set how the
+ * sums are split), not on timing.  sequences and q_heads in [0, 65535] and
+ * [1, 65535], sequences * q_heads < 2^24, max_pages as above, scale finite, softcap
+ * >= 0 and finite, window >= 0, workspace (256-byte aligned; calls sharing it must not
+ * overlap) of at least gollek_hip_attention_workspace_bytes: else ARG. */
+int32_t gollek_hip_attention_device(const gollek_hip_kv_cache *cache, const void *q, int64_t q_stride,
+                                    int64_t sequences, int64_t q_heads, const int32_t *lengths,
+                                    const int32_t *page_table, int64_t max_pages, float scale, float softcap,
+                                    int64_t window, const float *sinks, void *out, int32_t out_type,
+                                    int64_t out_stride, void *workspace, int64_t workspace_bytes, void *stream,
+                                    char *err, size_t err_len);
+/* Device workspace bytes that call needs (-1: out of range).  They never fall as
+ * sequences or max_pages rise. */
+int64_t gollek_hip_attention_workspace_bytes(const gollek_hip_kv_cache *cache, int64_t sequences, int64_t q_heads,
+                                             int64_t max_pages);
+
 /* ---- GGUF files --------------------------------------------------------- */
 /* GC/ = runner/gguf/gollek-gguf-core/src/main/java/tech/kayys/gollek/gguf/. */
 

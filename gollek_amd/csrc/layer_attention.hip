@@ -4,8 +4,27 @@
 //   s_j = scale * q . k_j [softcap * tanh(s_j / softcap)]
 //   out = sum_j exp(s_j) v_j / (sum_j exp(s_j) [+ exp(sink)])
 //
-// in one pass: m the largest s so far, l = sum exp(s_j - m), o = sum exp(s_j - m) v_j,
-// the last two scaled by exp(m_old - m) whenever m grows.
+// in one pass: m a bound of the s so far, l = sum exp(s_j - m), o = sum exp(s_j - m) v_j,
+// the last two scaled by exp(m_old - m) when m grows.
+//
+// A wave takes 32 keys at a time for up to 16 query heads that share them, straight
+// from memory to registers:
+//   S^T = K Q^T   (two tiles of 16 keys): lane (c, g) = (lane % 16, lane / 16) gets for
+//                 query c the keys 4 g .. 4 g + 3 of each tile;
+//   O^T += V^T P^T over those 32 keys: the lane's eight weights are, in this order, the
+//                 lane's part of the second operand as they stand, when the product's
+//                 inner index 8 g + j means key 4 g + j of the first tile (j < 4) or
+//                 4 g + j - 4 of the second.
+// So weights never cross lanes, and m, l and the accumulators of a query sit in the lanes
+// of its column.  For V^T a lane reads the same 8 keys, 8 (or 4) neighbouring dims each,
+// and turns them in registers (one v_perm for two elements): fragment i has dim 8 c + i in
+// row c.  No LDS in the loop; the next keys are loaded as soon as the scores have used the
+// registers, the next values behind the second product.
+//
+// A sequence's tiles are cut into chunks of equal size for workgroups that share the chip
+// evenly whatever the lengths are: every workgroup adds up the batch's tiles, takes the
+// chunk length from the sum and finds its own sequence and chunk.  Sequences of more than
+// one chunk leave (o, m, l) in the workspace, and a second launch joins them.
 #include <hip/hip_runtime.h>
 
 #include "layer_kernels.hpp"
@@ -13,73 +32,488 @@
 namespace gollek {
 namespace {
 
-constexpr int kWaves = 4;
+typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
+typedef float f32x4 __attribute__((ext_vector_type(4)));
 
-// One workgroup a query head; its waves take every fourth token.
-__global__ __launch_bounds__(64 * kWaves) void attend_kernel(AttendArgs a) {
-    __shared__ float part_m[kWaves], part_l[kWaves], part_o[kWaves][256];
-    const int lane = (int)threadIdx.x & 63, wave = (int)threadIdx.x >> 6, dim = a.kv.head_dim;
-    const int head = (int)blockIdx.x % a.q_heads, kv_head = head / (a.q_heads / a.kv.kv_heads);
-    const int64_t sequence = blockIdx.x / a.q_heads;
+constexpr int kWaves = 4, kThreads = 64 * kWaves;
+constexpr int kTile = 32;           // keys of a step
+constexpr int kRows = 16;           // query heads of a workgroup
+constexpr int kLeast = 8;           // tiles of a chunk at least: two steps a wave
+constexpr int kTarget = 1024;       // workgroups a batch is cut into: two rounds of two a CU
+constexpr int kScanMost = 1024;     // sequences whose tiles every workgroup adds up
+constexpr float kSlack = 8.0f;      // how far a score may pass m, in powers of two
+constexpr float kLog2e = 1.4426950408889634f;
+
+struct AttendPlan {
+    int row_tiles;  // workgroups for the query heads of one key head
+    int slots;      // chunks of a key head that the batch is cut into (0: a chunk a sequence)
+    int items;      // chunks at most
+    bool q_vec;     // queries on 16-byte borders
+    float *part_o, *part_ml;
+};
+
+// A sequence's keys: [begin, length), in tiles from begin's on.
+struct Span {
+    int begin, length, first, tiles;
+};
+__device__ __forceinline__ Span span_of(const AttendArgs &a, int length) {
     const int64_t table = a.max_pages << a.kv.page_shift;
-    const int64_t length = min((int64_t)max(a.lengths[sequence], 0), table);
-    const int64_t begin = a.window > 0 && length > a.window ? length - a.window : 0;
-    const float ninf = -__builtin_inff();
+    Span s;
+    s.length = (int)min((int64_t)max(length, 0), table);
+    s.begin = a.window > 0 && s.length > a.window ? s.length - a.window : 0;
+    s.first = s.begin / kTile;
+    s.tiles = (int)(((int64_t)s.length + kTile - 1) / kTile) - s.first;
+    if (s.length == 0) s.tiles = 0;
+    return s;
+}
 
-    float q[4], o[4] = {};
+__device__ __forceinline__ int lane_of(int v, int lane) { return __builtin_amdgcn_readlane(v, lane); }
+
+// What a workgroup works on: chunk `chunk` of `chunks` of a sequence, the batch's
+// chunk number `item`.  By every wave for itself.
+struct Item {
+    int sequence, chunk, chunks;
+};
+
+// Tiles of a chunk: above the batch's tiles / slots, so all sequences together
+// have at most sequences + slots chunks.
+__device__ __forceinline__ int chunk_tiles(const AttendArgs &a, const AttendPlan &p, int lane) {
+    unsigned long long total = 0;
+    for (int s = lane; s < a.sequences; s += 64) total += (unsigned)span_of(a, a.lengths[s]).tiles;
 #pragma unroll
-    for (int i = 0; i < 4; i++) {
-        const int d = lane + 64 * i;
-        q[i] = d < dim ? load_element(a.q, a.kv.type, sequence * a.q_stride + (int64_t)head * dim + d) : 0.0f;
-    }
-    float m = ninf, l = 0.0f;
-    for (int64_t j = begin + wave; j < length; j += kWaves) {
-        const int64_t page = a.page_table[sequence * a.max_pages + (j >> a.kv.page_shift)];
-        if (page < 0 || page >= a.kv.pages) continue;
-        const int64_t slot = j & ((1 << a.kv.page_shift) - 1);
-        const int64_t at = (((page * a.kv.kv_heads + kv_head) << a.kv.page_shift) + slot) * dim;
-        float s = 0.0f;
+    for (int m = 1; m < 64; m <<= 1) total += __shfl_xor(total, m);
+    const float each = (float)total / (float)p.slots * 1.000001f;  // (2^26 tiles a sequence at most)
+    return max(kLeast, (int)fminf(each, 1.0e9f) + 1);
+}
+
+// The sequence that item belongs to; false past the last.
+__device__ __forceinline__ bool find_item(const AttendArgs &a, const AttendPlan &p, int item, int lane, Item &it) {
+    const int each = chunk_tiles(a, p, lane);
+    int before = 0;
+    for (int s0 = 0; s0 < a.sequences; s0 += 64) {
+        const int s = s0 + lane;
+        const int n = s < a.sequences ? max(1, (span_of(a, a.lengths[s]).tiles + each - 1) / each) : 0;
+        int upto = n;
 #pragma unroll
-        for (int i = 0; i < 4; i++)
-            if (lane + 64 * i < dim) s += q[i] * load_element(a.kv.k, a.kv.type, at + lane + 64 * i);
-#pragma unroll
-        for (int x = 1; x < 64; x <<= 1) s += __shfl_xor(s, x);
-        s *= a.scale;
-        if (a.softcap > 0.0f) s = a.softcap * tanhf(s / a.softcap);
-        const float most = fmaxf(m, s), base = most == ninf ? 0.0f : most;
-        const float keep = expf(m - base), p = expf(s - base);
-        l = l * keep + p;
-#pragma unroll
-        for (int i = 0; i < 4; i++) {
-            o[i] *= keep;
-            if (lane + 64 * i < dim) o[i] += p * load_element(a.kv.v, a.kv.type, at + lane + 64 * i);
+        for (int m = 1; m < 64; m <<= 1) {
+            const int below = __shfl_up(upto, m);
+            if (lane >= m) upto += below;
         }
-        m = most;
+        const unsigned long long here = __ballot(before + upto > item);
+        if (here != 0) {
+            const int l = __builtin_ctzll(here);
+            it.sequence = s0 + l;
+            it.chunks = lane_of(n, l);
+            it.chunk = item - (before + lane_of(upto, l) - it.chunks);
+            return true;
+        }
+        before += lane_of(upto, 63);
     }
-#pragma unroll
-    for (int i = 0; i < 4; i++) part_o[wave][lane + 64 * i] = o[i];
-    if (lane == 0) part_m[wave] = m, part_l[wave] = l;
-    __syncthreads();
-    float most = a.sinks != nullptr ? a.sinks[head] : ninf;
-    const float sink = most;
-    for (int w = 0; w < kWaves; w++) most = fmaxf(most, part_m[w]);
-    const float base = most == ninf ? 0.0f : most;
-    float total = a.sinks != nullptr ? expf(sink - base) : 0.0f;
-    for (int w = 0; w < kWaves; w++) total += part_l[w] * expf(part_m[w] - base);
-    for (int d = (int)threadIdx.x; d < dim; d += 64 * kWaves) {
-        float v = 0.0f;
-        for (int w = 0; w < kWaves; w++) v += part_o[w][d] * expf(part_m[w] - base);
-        store_element(a.out, a.out_type, sequence * a.out_stride + (int64_t)head * dim + d, total > 0.0f || total != total ? v / total : 0.0f);
+    return false;
+}
+
+__device__ __forceinline__ f32x4 mfma(u32x4 a, u32x4 b, f32x4 c, std::integral_constant<int, kBF16>) {
+    typedef __bf16 v8 __attribute__((ext_vector_type(8)));
+    return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(v8, a), __builtin_bit_cast(v8, b), c, 0, 0, 0);
+}
+__device__ __forceinline__ f32x4 mfma(u32x4 a, u32x4 b, f32x4 c, std::integral_constant<int, kF16>) {
+    typedef _Float16 v8 __attribute__((ext_vector_type(8)));
+    return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(v8, a), __builtin_bit_cast(v8, b), c, 0, 0, 0);
+}
+
+// Two floats rounded to the type, and what that took off.
+template <int TYPE>
+__device__ __forceinline__ uint32_t round_pair(float &a, float &b) {
+    if constexpr (TYPE == kBF16) {
+        typedef __bf16 b2 __attribute__((ext_vector_type(2)));
+        const b2 r = {(__bf16)a, (__bf16)b};
+        a -= (float)r[0], b -= (float)r[1];
+        return __builtin_bit_cast(uint32_t, r);
+    } else {
+        typedef _Float16 h2 __attribute__((ext_vector_type(2)));
+        const h2 r = {(_Float16)a, (_Float16)b};
+        a -= (float)r[0], b -= (float)r[1];
+        return __builtin_bit_cast(uint32_t, r);
     }
 }
 
+// Dims of a head as the second product takes them: 16 lanes of kWide0 neighbours,
+// then (past 128) 16 of kWide1.
+template <int NK>
+struct Dims {
+    static constexpr int kWide0 = NK <= 2 ? 4 : 8, kWide1 = NK <= 4 ? 0 : NK <= 6 ? 4 : 8;
+    static constexpr int kFragments = kWide0 + kWide1, kWords = kFragments / 2;
+    static constexpr int kPitch = 16 * kFragments + 4;  // floats of a row in LDS
+};
+
+// The keys or values of one step as they stand in registers.
+template <int NK>
+struct KeyTile {
+    u32x4 word[2][NK];
+};
+template <int NK>
+struct ValueTile {
+    uint32_t word[8][Dims<NK>::kWords];
+};
+
+// TYPE: of cache and queries.  NK: head_dim / 32, rounded up (EXACT: without a rest).
+// PARTS: the pieces a weight is split into, of 8 (bf16) or 11 (fp16) bits each.
+template <int TYPE, int NK, bool EXACT, int PARTS>
+__global__ __launch_bounds__(kThreads) void attend_kernel(AttendArgs a, AttendPlan plan) {
+    using D = Dims<NK>;
+    constexpr std::integral_constant<int, TYPE> type;
+    // fp16 weights: exp(s - m) times 2^7, so that all but the smallest are normal numbers
+    // (2^15 with the slack, below fp16's largest)
+    constexpr float kLift = TYPE == kF16 ? 7.0f : 0.0f;
+    const float ninf = -__builtin_inff();
+    __shared__ __attribute__((aligned(16))) float lds_o[kWaves][kRows * D::kPitch];
+    __shared__ float lds_m[kWaves][kRows], lds_l[kWaves][kRows];
+
+    const int lane = (int)threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
+    const int c = lane & 15, g = lane >> 4;
+    const int dim = EXACT ? 32 * NK : a.kv.head_dim;
+    const int group = a.q_heads / a.kv.kv_heads;
+    // workgroups of one chunk's heads that read the same keys: eight apart, on one XCD
+    const int id = (int)blockIdx.x, row_tile = id / 8 % plan.row_tiles, unit = id / (8 * plan.row_tiles) * 8 + id % 8;
+    const int item = unit / a.kv.kv_heads, kv_head = unit % a.kv.kv_heads;
+    Item it = {item, 0, 1};
+    if (plan.slots > 0) {
+        if (!find_item(a, plan, item, lane, it)) return;
+    } else if (item >= a.sequences) {
+        return;
+    }
+    const Span span = span_of(a, __builtin_amdgcn_readfirstlane(a.lengths[it.sequence]));
+    const int each = (span.tiles + it.chunks - 1) / it.chunks;
+    const int tile0 = span.first + it.chunk * each, tile1 = min(tile0 + each, span.first + span.tiles);
+    const int row0 = row_tile * kRows, rows = min(kRows, group - row0);
+    const int64_t head0 = (int64_t)kv_head * group + row0;
+
+    // queries: row c, dims 32 i + 8 g ..
+    u32x4 q[NK];
+    {
+        const uint16_t *const from =
+            static_cast<const uint16_t *>(a.q) + it.sequence * a.q_stride + (head0 + (c < rows ? c : 0)) * dim;
+#pragma unroll
+        for (int i = 0; i < NK; i++) {
+            const bool in = c < rows && (EXACT || 32 * i + 8 * g < dim);
+            q[i] = u32x4{};
+            if (!in) continue;
+            if (plan.q_vec) {
+                q[i] = *reinterpret_cast<const u32x4 *>(from + 32 * i + 8 * g);
+            } else {
+#pragma unroll
+                for (int w = 0; w < 4; w++)
+                    q[i][w] = (uint32_t)from[32 * i + 8 * g + 2 * w] | (uint32_t)from[32 * i + 8 * g + 2 * w + 1] << 16;
+            }
+        }
+    }
+
+    // where a lane reads in a tile of 16 keys, in bytes: its key's row for K, four
+    // rows for V (dims past the head's read its first ones, and are not used)
+    const uint32_t k_lane = (uint32_t)(c * dim + 8 * g) * 2;
+    const bool k_rest = !EXACT && 32 * (NK - 1) + 8 * g >= dim;
+    const uint32_t k_last = k_rest ? (uint32_t)(c * dim) * 2 : k_lane + 64 * (NK - 1);
+    const uint32_t v_lane0 = (uint32_t)(4 * g * dim + (D::kWide0 * c < dim ? D::kWide0 * c : 0)) * 2;
+    const uint32_t v_lane1 = (uint32_t)(4 * g * dim + (128 + D::kWide1 * c < dim ? 128 + D::kWide1 * c : 0)) * 2;
+
+    const auto table = reinterpret_cast<const __attribute__((address_space(4))) int32_t *>(
+        reinterpret_cast<uintptr_t>(a.page_table + (int64_t)it.sequence * a.max_pages));
+    // byte offset of 16 keys from `key` on; -1 where there is no page
+    const auto place = [&](int key) -> int64_t {
+        if (key >= span.length) return -1;
+        const int page = table[key >> a.kv.page_shift];
+        if (page < 0 || page >= a.kv.pages) return -1;
+        const int64_t row = ((int64_t)page * a.kv.kv_heads + kv_head) << a.kv.page_shift;
+        return (row + (key & ((1 << a.kv.page_shift) - 1))) * dim * 2;
+    };
+    const int64_t nowhere = (((int64_t)kv_head) << a.kv.page_shift) * dim * 2;  // (page 0: memory of the cache)
+
+    KeyTile<NK> k;
+    ValueTile<NK> v;
+    const auto load_keys = [&](const int64_t (&at)[2]) {
+#pragma unroll
+        for (int h = 0; h < 2; h++) {
+            const uint8_t *const base = static_cast<const uint8_t *>(a.kv.k) + (at[h] < 0 ? nowhere : at[h]);
+#pragma unroll
+            for (int i = 0; i < NK; i++)
+                k.word[h][i] = *reinterpret_cast<const u32x4 *>(base + (i < NK - 1 ? k_lane + 64 * i : k_last));
+        }
+    };
+    const auto load_values = [&](const int64_t (&at)[2]) {
+#pragma unroll
+        for (int h = 0; h < 2; h++) {
+            const uint8_t *const base = static_cast<const uint8_t *>(a.kv.v) + (at[h] < 0 ? nowhere : at[h]);
+#pragma unroll
+            for (int j = 0; j < 4; j++) {
+                uint32_t *const w = v.word[4 * h + j];
+                const uint32_t off = v_lane0 + (uint32_t)(2 * j * dim);
+                if constexpr (D::kWide0 == 8) {
+                    const u32x4 x = *reinterpret_cast<const u32x4 *>(base + off);
+                    w[0] = x[0], w[1] = x[1], w[2] = x[2], w[3] = x[3];
+                } else {
+                    const uint2 x = *reinterpret_cast<const uint2 *>(base + off);
+                    w[0] = x.x, w[1] = x.y;
+                }
+                if constexpr (D::kWide1 == 8) {
+                    const u32x4 x = *reinterpret_cast<const u32x4 *>(base + v_lane1 + (uint32_t)(2 * j * dim));
+                    w[4] = x[0], w[5] = x[1], w[6] = x[2], w[7] = x[3];
+                } else if constexpr (D::kWide1 == 4) {
+                    const uint2 x = *reinterpret_cast<const uint2 *>(base + v_lane1 + (uint32_t)(2 * j * dim));
+                    w[4] = x.x, w[5] = x.y;
+                }
+            }
+        }
+    };
+
+    f32x4 o[D::kFragments] = {};
+    float m = ninf, base = 0.0f, l = 0.0f;  // l of this lane's keys
+    const float scale2 = a.scale * kLog2e, cap2 = a.softcap * kLog2e;
+    const float turn = a.softcap > 0.0f ? 2.0f * kLog2e * a.scale / a.softcap : 0.0f;
+
+    int tile = tile0 + wave;
+    if (tile < tile1) {
+        int64_t at[2] = {place(kTile * tile), place(kTile * tile + 16)};
+        load_keys(at);
+        load_values(at);
+        while (true) {
+            f32x4 s[2];
+#pragma unroll
+            for (int h = 0; h < 2; h++) {
+                s[h] = f32x4{};
+                if constexpr (!EXACT) {
+                    if (k_rest) k.word[h][NK - 1] = u32x4{};
+                }
+#pragma unroll
+                for (int i = 0; i < NK; i++) s[h] = mfma(k.word[h][i], q[i], s[h], type);
+            }
+            const int key0 = kTile * tile;
+            const bool whole = key0 >= span.begin && span.length - key0 >= kTile && at[0] >= 0 && at[1] >= 0;
+            const bool half[2] = {at[0] >= 0, at[1] >= 0};
+            const bool more = tile + kWaves < tile1;
+            if (more) {
+                const int next = kTile * (tile + kWaves);
+                at[0] = place(next), at[1] = place(next + 16);
+                load_keys(at);
+            }
+
+            float x[8];
+            if (a.softcap > 0.0f) {
+#pragma unroll
+                for (int j = 0; j < 8; j++)  // cap * tanh(z) = cap * (1 - 2 / (1 + exp(2 z)))
+                    x[j] = cap2 - 2.0f * cap2 * __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(turn * s[j >> 2][j & 3]));
+            } else {
+#pragma unroll
+                for (int j = 0; j < 8; j++) x[j] = scale2 * s[j >> 2][j & 3];
+            }
+            if (!whole) {
+#pragma unroll
+                for (int j = 0; j < 8; j++) {
+                    const int key = key0 + 16 * (j >> 2) + 4 * g + (j & 3);
+                    const bool in = half[j >> 2] && key >= span.begin && key < span.length;
+                    x[j] = in ? x[j] : ninf;
+#pragma unroll
+                    for (int w = 0; w < D::kWords; w++) v.word[j][w] = in ? v.word[j][w] : 0;
+                }
+            }
+            float most = x[0];
+#pragma unroll
+            for (int j = 1; j < 8; j++) most = fmaxf(most, x[j]);
+            if (__any(most > m + kSlack)) {
+                most = fmaxf(most, __shfl_xor(most, 16));
+                most = fmaxf(fmaxf(most, __shfl_xor(most, 32)), m);
+                const float before = m == ninf ? ninf : base;
+                m = most;
+                base = m == ninf ? 0.0f : m - kLift;
+                const float keep = __builtin_amdgcn_exp2f(before - base);
+                l *= keep;
+#pragma unroll
+                for (int i = 0; i < D::kFragments; i++) o[i] *= keep;
+            }
+#pragma unroll
+            for (int j = 0; j < 8; j++) {
+                x[j] = __builtin_amdgcn_exp2f(x[j] - base);
+                l += x[j];
+            }
+            u32x4 p[PARTS];
+#pragma unroll
+            for (int n = 0; n < PARTS; n++)
+#pragma unroll
+                for (int j = 0; j < 4; j++) p[n][j] = round_pair<TYPE>(x[2 * j], x[2 * j + 1]);
+#pragma unroll
+            for (int i = 0; i < D::kFragments; i++) {
+                u32x4 t;
+#pragma unroll
+                for (int j = 0; j < 4; j++)
+                    t[j] = __builtin_amdgcn_perm(v.word[2 * j + 1][i / 2], v.word[2 * j][i / 2],
+                                                 i % 2 == 0 ? 0x05040100u : 0x07060302u);
+#pragma unroll
+                for (int n = 0; n < PARTS; n++) o[i] = mfma(t, p[n], o[i], type);
+            }
+            if (!more) break;
+            load_values(at);
+            tile += kWaves;
+        }
+    }
+
+    // the waves' sums, rescaled to their common bound, through LDS
+    l += __shfl_xor(l, 16);
+    l += __shfl_xor(l, 32);
+    const float bound = m == ninf ? ninf : base;
+    if (g == 0) lds_m[wave][c] = bound, lds_l[wave][c] = l;
+    __syncthreads();
+    float top = ninf;
+#pragma unroll
+    for (int w = 0; w < kWaves; w++) top = fmaxf(top, lds_m[w][c]);
+    const float keep = __builtin_amdgcn_exp2f(bound - (top == ninf ? 0.0f : top));
+    if (c < rows) {
+#pragma unroll
+        for (int r = 0; r < 4; r++) {  // dims wide * (4 g + r) + i
+            float *const to = lds_o[wave] + c * D::kPitch;
+#pragma unroll
+            for (int i = 0; i < D::kWide0; i++) to[D::kWide0 * (4 * g + r) + i] = keep * o[i][r];
+#pragma unroll
+            for (int i = 0; i < D::kWide1; i++) to[16 * D::kWide0 + D::kWide1 * (4 * g + r) + i] = keep * o[D::kWide0 + i][r];
+        }
+    }
+    __syncthreads();
+    for (int e = (int)threadIdx.x; e < rows * dim; e += kThreads) {
+        const int r = e / dim, d = e - r * dim;
+        float sum = 0.0f, total = 0.0f, most = ninf;
+#pragma unroll
+        for (int w = 0; w < kWaves; w++) {
+            sum += lds_o[w][r * D::kPitch + d];
+            most = fmaxf(most, lds_m[w][r]);
+        }
+        const float at0 = most == ninf ? 0.0f : most;
+#pragma unroll
+        for (int w = 0; w < kWaves; w++) total += lds_l[w][r] * __builtin_amdgcn_exp2f(lds_m[w][r] - at0);
+        if (it.chunks > 1) {
+            const int64_t row = (int64_t)item * a.q_heads + head0 + r;
+            plan.part_o[row * dim + d] = sum;
+            if (d == 0) plan.part_ml[2 * row] = most, plan.part_ml[2 * row + 1] = total;
+        } else {
+            if (a.sinks != nullptr) {
+                const float sink = a.sinks[head0 + r] * kLog2e, up = fmaxf(sink, most), at1 = up == ninf ? 0.0f : up;
+                const float f = __builtin_amdgcn_exp2f(at0 - at1);
+                sum *= f;
+                total = total * f + __builtin_amdgcn_exp2f(sink - at1);
+            }
+            store_element(a.out, a.out_type, it.sequence * a.out_stride + (head0 + r) * dim + d,
+                          total == 0.0f ? 0.0f : sum / total);
+        }
+    }
+}
+
+// The chunks of a sequence's query head joined: a workgroup each.
+__global__ __launch_bounds__(256) void join_kernel(AttendArgs a, AttendPlan plan) {
+    __shared__ float lds[4][256], lds_l[4];
+    const int lane = (int)threadIdx.x & 63, wave = (int)threadIdx.x >> 6, dim = a.kv.head_dim;
+    const float ninf = -__builtin_inff();
+    const int sequence = (int)blockIdx.x / a.q_heads, head = (int)blockIdx.x % a.q_heads;
+    const int each = chunk_tiles(a, plan, lane);
+    int first = 0, chunks = 0;
+    for (int s0 = 0; s0 <= sequence; s0 += 64) {
+        const int s = s0 + lane;
+        const int n = s <= sequence ? max(1, (span_of(a, a.lengths[s]).tiles + each - 1) / each) : 0;
+        int sum = n;
+#pragma unroll
+        for (int m = 1; m < 64; m <<= 1) sum += __shfl_xor(sum, m);
+        first += sum;
+        if (s0 + 64 > sequence) chunks = __shfl(n, sequence - s0);
+    }
+    first -= chunks;
+    if (chunks <= 1) return;
+    float most = ninf;
+    for (int i = lane; i < chunks; i += 64) most = fmaxf(most, plan.part_ml[2 * ((int64_t)(first + i) * a.q_heads + head)]);
+#pragma unroll
+    for (int m = 1; m < 64; m <<= 1) most = fmaxf(most, __shfl_xor(most, m));
+    const float sink = a.sinks != nullptr ? a.sinks[head] * kLog2e : ninf;
+    most = fmaxf(most, sink);
+    const float at = most == ninf ? 0.0f : most;
+    float o[4] = {}, l = 0.0f;
+    for (int i = wave; i < chunks; i += 4) {
+        const int64_t row = (int64_t)(first + i) * a.q_heads + head;
+        const float f = __builtin_amdgcn_exp2f(plan.part_ml[2 * row] - at);
+        l += f * plan.part_ml[2 * row + 1];
+#pragma unroll
+        for (int j = 0; j < 4; j++)
+            if (lane + 64 * j < dim) o[j] += f * plan.part_o[row * dim + lane + 64 * j];
+    }
+#pragma unroll
+    for (int j = 0; j < 4; j++) lds[wave][lane + 64 * j] = o[j];
+    if (lane == 0) lds_l[wave] = l;
+    __syncthreads();
+    const int d = (int)threadIdx.x;
+    if (d >= dim) return;
+    float sum = 0.0f, total = a.sinks != nullptr ? __builtin_amdgcn_exp2f(sink - at) : 0.0f;
+#pragma unroll
+    for (int w = 0; w < 4; w++) sum += lds[w][d], total += lds_l[w];
+    store_element(a.out, a.out_type, sequence * a.out_stride + (int64_t)head * dim + d, total == 0.0f ? 0.0f : sum / total);
+}
+
+AttendPlan make_plan(const KvPages &kv, int sequences, int q_heads, int64_t max_pages) {
+    AttendPlan p = {};
+    p.row_tiles = (q_heads / kv.kv_heads + kRows - 1) / kRows;
+    const int64_t tiles = ((max_pages << kv.page_shift) + kTile - 1) / kTile;
+    p.items = sequences;
+    if (sequences > kScanMost || tiles <= kLeast) return p;  // a chunk a sequence
+    const int64_t per = (int64_t)kv.kv_heads * p.row_tiles;
+    const int slots = (int)(per < kTarget ? kTarget / per : 1);
+    p.slots = slots;
+    const int64_t most = sequences * ((tiles + kLeast - 1) / kLeast);
+    p.items = (int)(most < sequences + slots ? most : sequences + slots);
+    return p;
+}
+
+template <int TYPE, int PARTS>
+void launch(int dim, const AttendArgs &a, const AttendPlan &p, unsigned grid, hipStream_t stream) {
+#define GOLLEK_ATTEND(NK)                                                                                               \
+    case NK:                                                                                                            \
+        if (dim == 32 * NK)                                                                                             \
+            hipLaunchKernelGGL((attend_kernel<TYPE, NK, true, PARTS>), dim3(grid), dim3(kThreads), 0, stream, a, p);    \
+        else                                                                                                            \
+            hipLaunchKernelGGL((attend_kernel<TYPE, NK, false, PARTS>), dim3(grid), dim3(kThreads), 0, stream, a, p);   \
+        break
+    switch ((dim + 31) / 32) {
+        GOLLEK_ATTEND(1);
+        GOLLEK_ATTEND(2);
+        GOLLEK_ATTEND(3);
+        GOLLEK_ATTEND(4);
+        GOLLEK_ATTEND(5);
+        GOLLEK_ATTEND(6);
+        GOLLEK_ATTEND(7);
+        GOLLEK_ATTEND(8);
+    }
+#undef GOLLEK_ATTEND
+}
+
+size_t part_rows(const AttendPlan &p, int q_heads) { return p.slots > 0 ? (size_t)p.items * (size_t)q_heads : 0; }
+
 }  // namespace
 
-size_t attend_workspace_bytes(const KvPages &, int, int, int64_t) { return 0; }
+size_t attend_workspace_bytes(const KvPages &kv, int sequences, int q_heads, int64_t max_pages) {
+    // (past kScanMost nothing is split; the size stays what the batch before needed)
+    const AttendPlan p = make_plan(kv, sequences < kScanMost ? sequences : kScanMost, q_heads, max_pages);
+    return (part_rows(p, q_heads) * (size_t)(kv.head_dim + 2) * sizeof(float) + 255) / 256 * 256;
+}
 
-hipError_t launch_attend(const AttendArgs &a, uint8_t *, hipStream_t stream) {
-    hipLaunchKernelGGL(attend_kernel, dim3((unsigned)(a.sequences * a.q_heads)), dim3(64 * kWaves), 0, stream, a);
-    return hipGetLastError();
+hipError_t launch_attend(const AttendArgs &a, uint8_t *workspace, hipStream_t stream) {
+    AttendPlan p = make_plan(a.kv, a.sequences, a.q_heads, a.max_pages);
+    p.part_o = reinterpret_cast<float *>(workspace);
+    p.part_ml = p.part_o + part_rows(p, a.q_heads) * (size_t)a.kv.head_dim;
+    p.q_vec = ((reinterpret_cast<uintptr_t>(a.q) | (uintptr_t)(a.q_stride * 2)) & 15u) == 0;
+    const int64_t units = ((int64_t)p.items * a.kv.kv_heads + 7) / 8 * 8, grid = units * p.row_tiles;
+    if (grid > 0x7FFFFFFF) return hipErrorInvalidValue;
+    const int dim = a.kv.head_dim;
+    if (a.kv.type == kF16) launch<kF16, 2>(dim, a, p, (unsigned)grid, stream);
+    else if (a.out_type == kF32) launch<kBF16, 3>(dim, a, p, (unsigned)grid, stream);
+    else launch<kBF16, 2>(dim, a, p, (unsigned)grid, stream);
+    hipError_t e = hipGetLastError();
+    if (e == hipSuccess && p.slots > 0) {
+        hipLaunchKernelGGL(join_kernel, dim3((unsigned)(a.sequences * a.q_heads)), dim3(256), 0, stream, a, p);
+        e = hipGetLastError();
+    }
+    return e;
 }
 
 }  // namespace gollek

@@ -27,19 +27,26 @@
 // one chunk leave (o, m, l) in the workspace, and a second launch joins them.
 #include <hip/hip_runtime.h>
 
+#include <type_traits>
+
 #include "layer_kernels.hpp"
 
 namespace gollek {
 namespace {
 
 typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
+typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
 typedef float f32x4 __attribute__((ext_vector_type(4)));
 
 constexpr int kWaves = 4, kThreads = 64 * kWaves;
 constexpr int kTile = 32;           // keys of a step
 constexpr int kRows = 16;           // query heads of a workgroup
 constexpr int kLeast = 8;           // tiles of a chunk at least: two steps a wave
-constexpr int kTarget = 1024;       // workgroups a batch is cut into: two rounds of two a CU
+// Workgroups that a batch is cut into: one sequence, whose chunks are all alike, into one
+// round of three a CU (131072 tokens of 4 heads of 128: 44.9 us, in 1024 46.4, in 1536
+// 48.8); several, whose chunks come out between half of T and T, into twice that, so
+// that the last round is short (64 of up to 8192: 225 in 768, 216 in 1536).
+constexpr int kTargetOne = 768, kTarget = 1536;
 constexpr int kScanMost = 1024;     // sequences whose tiles every workgroup adds up
 constexpr float kSlack = 8.0f;      // how far a score may pass m, in powers of two
 constexpr float kLog2e = 1.4426950408889634f;
@@ -49,7 +56,11 @@ struct AttendPlan {
     int slots;      // chunks of a key head that the batch is cut into (0: a chunk a sequence)
     int items;      // chunks at most
     bool q_vec;     // queries on 16-byte borders
-    float *part_o, *part_ml;
+    // workspace: a chunk's sums, (bound, weight) for each query head, and a sequence's
+    // first chunk and how many it has
+    float *part_o;
+    float2 *part_ml;
+    int2 *joins;
 };
 
 // A sequence's keys: [begin, length), in tiles from begin's on.
@@ -69,40 +80,54 @@ __device__ __forceinline__ Span span_of(const AttendArgs &a, int length) {
 
 __device__ __forceinline__ int lane_of(int v, int lane) { return __builtin_amdgcn_readlane(v, lane); }
 
-// What a workgroup works on: chunk `chunk` of `chunks` of a sequence, the batch's
-// chunk number `item`.  By every wave for itself.
-struct Item {
-    int sequence, chunk, chunks;
-};
-
-// Tiles of a chunk: above the batch's tiles / slots, so all sequences together
-// have at most sequences + slots chunks.
-__device__ __forceinline__ int chunk_tiles(const AttendArgs &a, const AttendPlan &p, int lane) {
-    unsigned long long total = 0;
-    for (int s = lane; s < a.sequences; s += 64) total += (unsigned)span_of(a, a.lengths[s]).tiles;
-#pragma unroll
-    for (int m = 1; m < 64; m <<= 1) total += __shfl_xor(total, m);
-    const float each = (float)total / (float)p.slots * 1.000001f;  // (2^26 tiles a sequence at most)
-    return max(kLeast, (int)fminf(each, 1.0e9f) + 1);
+template <int CTRL, int ROWS>
+__device__ __forceinline__ int dpp(int v) {
+    return __builtin_amdgcn_update_dpp(0, v, CTRL, ROWS, 0xF, false);
+}
+// Of the values of the lanes up to each: their sum.  (row_shr 1, 2, 4, 8 within 16
+// lanes, then row_bcast 15 and 31.)
+template <class T>
+__device__ __forceinline__ T prefix_sum(T v) {
+    const auto add = [&](int moved) { v += __builtin_bit_cast(T, moved); };
+    add(dpp<0x111, 0xF>(__builtin_bit_cast(int, v)));
+    add(dpp<0x112, 0xF>(__builtin_bit_cast(int, v)));
+    add(dpp<0x114, 0xF>(__builtin_bit_cast(int, v)));
+    add(dpp<0x118, 0xF>(__builtin_bit_cast(int, v)));
+    add(dpp<0x142, 0xA>(__builtin_bit_cast(int, v)));
+    add(dpp<0x143, 0xC>(__builtin_bit_cast(int, v)));
+    return v;
 }
 
-// The sequence that item belongs to; false past the last.
+// What a workgroup works on: chunk `chunk` of `chunks` of a sequence.
+struct Item {
+    int sequence, length, chunk, chunks;
+};
+
+// The sequence that chunk number `item` of the batch belongs to; false past the last.
+// By every wave for itself: the batch's tiles are added up, the chunk length T is just
+// above tiles / slots, so that all sequences together have at most sequences + slots
+// chunks, and the sequences' chunks are counted up to the item.  (The sum is in fp32:
+// 22 additions, 2^-19.5 off at most; T is rounded up by more.)
 __device__ __forceinline__ bool find_item(const AttendArgs &a, const AttendPlan &p, int item, int lane, Item &it) {
-    const int each = chunk_tiles(a, p, lane);
+    const int length0 = lane < a.sequences ? a.lengths[lane] : 0;  // (kept: most batches have no more)
+    float total = 0.0f;
+    for (int s0 = 0; s0 < a.sequences; s0 += 64) {
+        const int s = s0 + lane;
+        if (s < a.sequences) total += (float)span_of(a, s0 == 0 ? length0 : a.lengths[s]).tiles;
+    }
+    total = __int_as_float(lane_of(__float_as_int(prefix_sum(total)), 63));
+    const int each = max(kLeast, (int)fminf(total / (float)p.slots * 1.00001f, 1.0e9f) + 1);
     int before = 0;
     for (int s0 = 0; s0 < a.sequences; s0 += 64) {
         const int s = s0 + lane;
-        const int n = s < a.sequences ? max(1, (span_of(a, a.lengths[s]).tiles + each - 1) / each) : 0;
-        int upto = n;
-#pragma unroll
-        for (int m = 1; m < 64; m <<= 1) {
-            const int below = __shfl_up(upto, m);
-            if (lane >= m) upto += below;
-        }
+        const int length = s0 == 0 ? length0 : s < a.sequences ? a.lengths[s] : 0;
+        const int n = s < a.sequences ? max(1, (span_of(a, length).tiles + each - 1) / each) : 0;
+        const int upto = prefix_sum(n);
         const unsigned long long here = __ballot(before + upto > item);
         if (here != 0) {
             const int l = __builtin_ctzll(here);
             it.sequence = s0 + l;
+            it.length = lane_of(length, l);
             it.chunks = lane_of(n, l);
             it.chunk = item - (before + lane_of(upto, l) - it.chunks);
             return true;
@@ -146,6 +171,12 @@ struct Dims {
     static constexpr int kPitch = 16 * kFragments + 4;  // floats of a row in LDS
 };
 
+// Keys and values are used once a call: loads that do not stay in the caches.
+template <class T>
+__device__ __forceinline__ T stream(const T *p) {
+    return __builtin_nontemporal_load(p);
+}
+
 // The keys or values of one step as they stand in registers.
 template <int NK>
 struct KeyTile {
@@ -176,35 +207,36 @@ __global__ __launch_bounds__(kThreads) void attend_kernel(AttendArgs a, AttendPl
     // workgroups of one chunk's heads that read the same keys: eight apart, on one XCD
     const int id = (int)blockIdx.x, row_tile = id / 8 % plan.row_tiles, unit = id / (8 * plan.row_tiles) * 8 + id % 8;
     const int item = unit / a.kv.kv_heads, kv_head = unit % a.kv.kv_heads;
-    Item it = {item, 0, 1};
+    Item it = {item, 0, 0, 1};
     if (plan.slots > 0) {
         if (!find_item(a, plan, item, lane, it)) return;
-    } else if (item >= a.sequences) {
-        return;
+        if (it.chunk == 0 && kv_head == 0 && row_tile == 0 && threadIdx.x == 0)
+            plan.joins[it.sequence] = make_int2(item, it.chunks);
+    } else {
+        if (item >= a.sequences) return;
+        it.length = __builtin_amdgcn_readfirstlane(a.lengths[item]);
     }
-    const Span span = span_of(a, __builtin_amdgcn_readfirstlane(a.lengths[it.sequence]));
+    const Span span = span_of(a, it.length);
     const int each = (span.tiles + it.chunks - 1) / it.chunks;
     const int tile0 = span.first + it.chunk * each, tile1 = min(tile0 + each, span.first + span.tiles);
     const int row0 = row_tile * kRows, rows = min(kRows, group - row0);
     const int64_t head0 = (int64_t)kv_head * group + row0;
 
-    // queries: row c, dims 32 i + 8 g ..
+    // queries: row c, dims 32 i + 8 g .. (rows and dims there are none of: 0)
     u32x4 q[NK];
     {
         const uint16_t *const from =
             static_cast<const uint16_t *>(a.q) + it.sequence * a.q_stride + (head0 + (c < rows ? c : 0)) * dim;
+        const auto dims = [&](int i) { return EXACT || 32 * i + 8 * g < dim ? 32 * i + 8 * g : 0; };
+        if (plan.q_vec) {
 #pragma unroll
-        for (int i = 0; i < NK; i++) {
-            const bool in = c < rows && (EXACT || 32 * i + 8 * g < dim);
-            q[i] = u32x4{};
-            if (!in) continue;
-            if (plan.q_vec) {
-                q[i] = *reinterpret_cast<const u32x4 *>(from + 32 * i + 8 * g);
-            } else {
+            for (int i = 0; i < NK; i++) q[i] = *reinterpret_cast<const u32x4 *>(from + dims(i));
+        } else {
+#pragma unroll
+            for (int i = 0; i < NK; i++)
 #pragma unroll
                 for (int w = 0; w < 4; w++)
-                    q[i][w] = (uint32_t)from[32 * i + 8 * g + 2 * w] | (uint32_t)from[32 * i + 8 * g + 2 * w + 1] << 16;
-            }
+                    q[i][w] = (uint32_t)from[dims(i) + 2 * w] | (uint32_t)from[dims(i) + 2 * w + 1] << 16;
         }
     }
 
@@ -218,13 +250,16 @@ __global__ __launch_bounds__(kThreads) void attend_kernel(AttendArgs a, AttendPl
 
     const auto table = reinterpret_cast<const __attribute__((address_space(4))) int32_t *>(
         reinterpret_cast<uintptr_t>(a.page_table + (int64_t)it.sequence * a.max_pages));
-    // byte offset of 16 keys from `key` on; -1 where there is no page
-    const auto place = [&](int key) -> int64_t {
-        if (key >= span.length) return -1;
-        const int page = table[key >> a.kv.page_shift];
-        if (page < 0 || page >= a.kv.pages) return -1;
+    // the pages of a tile's two halves (past the length: some page of the sequence)
+    const auto pages_of = [&](int tile, int (&page)[2]) {
+        page[0] = table[min(kTile * tile, span.length - 1) >> a.kv.page_shift];
+        page[1] = table[min(kTile * tile + 16, span.length - 1) >> a.kv.page_shift];
+    };
+    // byte offset of 16 keys from `key` on, which lie in `page`; -1 where there is none
+    const auto place = [&](int page, int key) -> int64_t {
         const int64_t row = ((int64_t)page * a.kv.kv_heads + kv_head) << a.kv.page_shift;
-        return (row + (key & ((1 << a.kv.page_shift) - 1))) * dim * 2;
+        const int64_t at = (row + (key & ((1 << a.kv.page_shift) - 1))) * dim * 2;
+        return key < span.length && page >= 0 && page < a.kv.pages ? at : -1;
     };
     const int64_t nowhere = (((int64_t)kv_head) << a.kv.page_shift) * dim * 2;  // (page 0: memory of the cache)
 
@@ -236,7 +271,7 @@ __global__ __launch_bounds__(kThreads) void attend_kernel(AttendArgs a, AttendPl
             const uint8_t *const base = static_cast<const uint8_t *>(a.kv.k) + (at[h] < 0 ? nowhere : at[h]);
 #pragma unroll
             for (int i = 0; i < NK; i++)
-                k.word[h][i] = *reinterpret_cast<const u32x4 *>(base + (i < NK - 1 ? k_lane + 64 * i : k_last));
+                k.word[h][i] = stream(reinterpret_cast<const u32x4 *>(base + (i < NK - 1 ? k_lane + 64 * i : k_last)));
         }
     };
     const auto load_values = [&](const int64_t (&at)[2]) {
@@ -248,18 +283,18 @@ __global__ __launch_bounds__(kThreads) void attend_kernel(AttendArgs a, AttendPl
                 uint32_t *const w = v.word[4 * h + j];
                 const uint32_t off = v_lane0 + (uint32_t)(2 * j * dim);
                 if constexpr (D::kWide0 == 8) {
-                    const u32x4 x = *reinterpret_cast<const u32x4 *>(base + off);
+                    const u32x4 x = stream(reinterpret_cast<const u32x4 *>(base + off));
                     w[0] = x[0], w[1] = x[1], w[2] = x[2], w[3] = x[3];
                 } else {
-                    const uint2 x = *reinterpret_cast<const uint2 *>(base + off);
-                    w[0] = x.x, w[1] = x.y;
+                    const u32x2 x = stream(reinterpret_cast<const u32x2 *>(base + off));
+                    w[0] = x[0], w[1] = x[1];
                 }
                 if constexpr (D::kWide1 == 8) {
-                    const u32x4 x = *reinterpret_cast<const u32x4 *>(base + v_lane1 + (uint32_t)(2 * j * dim));
+                    const u32x4 x = stream(reinterpret_cast<const u32x4 *>(base + v_lane1 + (uint32_t)(2 * j * dim)));
                     w[4] = x[0], w[5] = x[1], w[6] = x[2], w[7] = x[3];
                 } else if constexpr (D::kWide1 == 4) {
-                    const uint2 x = *reinterpret_cast<const uint2 *>(base + v_lane1 + (uint32_t)(2 * j * dim));
-                    w[4] = x.x, w[5] = x.y;
+                    const u32x2 x = stream(reinterpret_cast<const u32x2 *>(base + v_lane1 + (uint32_t)(2 * j * dim)));
+                    w[4] = x[0], w[5] = x[1];
                 }
             }
         }
@@ -270,89 +305,100 @@ __global__ __launch_bounds__(kThreads) void attend_kernel(AttendArgs a, AttendPl
     const float scale2 = a.scale * kLog2e, cap2 = a.softcap * kLog2e;
     const float turn = a.softcap > 0.0f ? 2.0f * kLog2e * a.scale / a.softcap : 0.0f;
 
-    int tile = tile0 + wave;
-    if (tile < tile1) {
-        int64_t at[2] = {place(kTile * tile), place(kTile * tile + 16)};
-        load_keys(at);
-        load_values(at);
-        while (true) {
-            f32x4 s[2];
+    // One step; MORE: of another one after it, whose keys are loaded when the scores have
+    // used the registers, and whose values behind the second product.  (Two copies: a load
+    // under a branch would have the wait for this step's values wait for it too.)
+    int tile = tile0 + wave, page[2];
+    int64_t at[2];
+    const auto step = [&](auto MORE) {
+        constexpr bool more = decltype(MORE)::value;
+        f32x4 s[2];
 #pragma unroll
-            for (int h = 0; h < 2; h++) {
-                s[h] = f32x4{};
-                if constexpr (!EXACT) {
-                    if (k_rest) k.word[h][NK - 1] = u32x4{};
-                }
-#pragma unroll
-                for (int i = 0; i < NK; i++) s[h] = mfma(k.word[h][i], q[i], s[h], type);
+        for (int h = 0; h < 2; h++) {
+            s[h] = f32x4{};
+            if constexpr (!EXACT) {
+                if (k_rest) k.word[h][NK - 1] = u32x4{};
             }
-            const int key0 = kTile * tile;
-            const bool whole = key0 >= span.begin && span.length - key0 >= kTile && at[0] >= 0 && at[1] >= 0;
-            const bool half[2] = {at[0] >= 0, at[1] >= 0};
-            const bool more = tile + kWaves < tile1;
-            if (more) {
-                const int next = kTile * (tile + kWaves);
-                at[0] = place(next), at[1] = place(next + 16);
-                load_keys(at);
-            }
-
-            float x[8];
-            if (a.softcap > 0.0f) {
+        }
 #pragma unroll
-                for (int j = 0; j < 8; j++)  // cap * tanh(z) = cap * (1 - 2 / (1 + exp(2 z)))
-                    x[j] = cap2 - 2.0f * cap2 * __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(turn * s[j >> 2][j & 3]));
-            } else {
+        for (int h = 0; h < 2; h++)
 #pragma unroll
-                for (int j = 0; j < 8; j++) x[j] = scale2 * s[j >> 2][j & 3];
-            }
-            if (!whole) {
+            for (int i = 0; i < NK; i++) s[h] = mfma(k.word[h][i], q[i], s[h], type);
+        const int key0 = kTile * tile;
+        const bool half[2] = {at[0] >= 0, at[1] >= 0};
+        const bool whole = key0 >= span.begin && span.length - key0 >= kTile && half[0] && half[1];
+        if constexpr (more) {
+            tile += kWaves;
+            at[0] = place(page[0], kTile * tile), at[1] = place(page[1], kTile * tile + 16);
+            load_keys(at);
+            pages_of(min(tile + kWaves, tile1 - 1), page);
+        }
+        float x[8];
+        if (a.softcap > 0.0f) {
 #pragma unroll
-                for (int j = 0; j < 8; j++) {
-                    const int key = key0 + 16 * (j >> 2) + 4 * g + (j & 3);
-                    const bool in = half[j >> 2] && key >= span.begin && key < span.length;
-                    x[j] = in ? x[j] : ninf;
+            for (int j = 0; j < 8; j++)  // cap * tanh(z) = cap * (1 - 2 / (1 + exp(2 z)))
+                x[j] = cap2 - 2.0f * cap2 * __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(turn * s[j >> 2][j & 3]));
+        } else {
 #pragma unroll
-                    for (int w = 0; w < D::kWords; w++) v.word[j][w] = in ? v.word[j][w] : 0;
-                }
-            }
-            float most = x[0];
-#pragma unroll
-            for (int j = 1; j < 8; j++) most = fmaxf(most, x[j]);
-            if (__any(most > m + kSlack)) {
-                most = fmaxf(most, __shfl_xor(most, 16));
-                most = fmaxf(fmaxf(most, __shfl_xor(most, 32)), m);
-                const float before = m == ninf ? ninf : base;
-                m = most;
-                base = m == ninf ? 0.0f : m - kLift;
-                const float keep = __builtin_amdgcn_exp2f(before - base);
-                l *= keep;
-#pragma unroll
-                for (int i = 0; i < D::kFragments; i++) o[i] *= keep;
-            }
+            for (int j = 0; j < 8; j++) x[j] = scale2 * s[j >> 2][j & 3];
+        }
+        if (!whole) {
 #pragma unroll
             for (int j = 0; j < 8; j++) {
-                x[j] = __builtin_amdgcn_exp2f(x[j] - base);
-                l += x[j];
+                const int key = key0 + 16 * (j >> 2) + 4 * g + (j & 3);
+                const bool in = half[j >> 2] && key >= span.begin && key < span.length;
+                x[j] = in ? x[j] : ninf;
+#pragma unroll
+                for (int w = 0; w < D::kWords; w++) v.word[j][w] = in ? v.word[j][w] : 0;
             }
-            u32x4 p[PARTS];
-#pragma unroll
-            for (int n = 0; n < PARTS; n++)
-#pragma unroll
-                for (int j = 0; j < 4; j++) p[n][j] = round_pair<TYPE>(x[2 * j], x[2 * j + 1]);
-#pragma unroll
-            for (int i = 0; i < D::kFragments; i++) {
-                u32x4 t;
-#pragma unroll
-                for (int j = 0; j < 4; j++)
-                    t[j] = __builtin_amdgcn_perm(v.word[2 * j + 1][i / 2], v.word[2 * j][i / 2],
-                                                 i % 2 == 0 ? 0x05040100u : 0x07060302u);
-#pragma unroll
-                for (int n = 0; n < PARTS; n++) o[i] = mfma(t, p[n], o[i], type);
-            }
-            if (!more) break;
-            load_values(at);
-            tile += kWaves;
         }
+        float most = x[0];
+#pragma unroll
+        for (int j = 1; j < 8; j++) most = fmaxf(most, x[j]);
+        if (__any(most > m + kSlack)) {
+            most = fmaxf(most, __shfl_xor(most, 16));
+            most = fmaxf(fmaxf(most, __shfl_xor(most, 32)), m);
+            const float before = m == ninf ? ninf : base;
+            m = most;
+            base = m == ninf ? 0.0f : m - kLift;
+            const float keep = __builtin_amdgcn_exp2f(before - base);
+            l *= keep;
+#pragma unroll
+            for (int i = 0; i < D::kFragments; i++) o[i] *= keep;
+        }
+#pragma unroll
+        for (int j = 0; j < 8; j++) {
+            x[j] = __builtin_amdgcn_exp2f(x[j] - base);
+            l += x[j];
+        }
+        u32x4 p[PARTS];
+#pragma unroll
+        for (int n = 0; n < PARTS; n++)
+#pragma unroll
+            for (int j = 0; j < 4; j++) p[n][j] = round_pair<TYPE>(x[2 * j], x[2 * j + 1]);
+#pragma unroll
+        for (int i = 0; i < D::kFragments; i++) {
+            u32x4 t;
+#pragma unroll
+            for (int j = 0; j < 4; j++)
+                t[j] = __builtin_amdgcn_perm(v.word[2 * j + 1][i / 2], v.word[2 * j][i / 2],
+                                             i % 2 == 0 ? 0x05040100u : 0x07060302u);
+#pragma unroll
+            for (int n = 0; n < PARTS; n++) o[i] = mfma(t, p[n], o[i], type);
+        }
+        if constexpr (more) load_values(at);
+    };
+    if (tile < tile1) {
+        pages_of(tile, page);
+        at[0] = place(page[0], kTile * tile), at[1] = place(page[1], kTile * tile + 16);
+        load_keys(at);
+        load_values(at);
+        pages_of(min(tile + kWaves, tile1 - 1), page);
+#pragma unroll
+        for (int i = 0; i < NK; i++)
+            if (c >= rows || (!EXACT && 32 * i + 8 * g >= dim)) q[i] = u32x4{};
+        while (tile + kWaves < tile1) step(std::true_type{});
+        step(std::false_type{});
     }
 
     // the waves' sums, rescaled to their common bound, through LDS
@@ -390,7 +436,7 @@ __global__ __launch_bounds__(kThreads) void attend_kernel(AttendArgs a, AttendPl
         if (it.chunks > 1) {
             const int64_t row = (int64_t)item * a.q_heads + head0 + r;
             plan.part_o[row * dim + d] = sum;
-            if (d == 0) plan.part_ml[2 * row] = most, plan.part_ml[2 * row + 1] = total;
+            if (d == 0) plan.part_ml[row] = make_float2(most, total);
         } else {
             if (a.sinks != nullptr) {
                 const float sink = a.sinks[head0 + r] * kLog2e, up = fmaxf(sink, most), at1 = up == ninf ? 0.0f : up;
@@ -404,61 +450,78 @@ __global__ __launch_bounds__(kThreads) void attend_kernel(AttendArgs a, AttendPl
     }
 }
 
-// The chunks of a sequence's query head joined: a workgroup each.
-__global__ __launch_bounds__(256) void join_kernel(AttendArgs a, AttendPlan plan) {
-    __shared__ float lds[4][256], lds_l[4];
-    const int lane = (int)threadIdx.x & 63, wave = (int)threadIdx.x >> 6, dim = a.kv.head_dim;
+// The chunks of a sequence's query head joined, by one workgroup: groups of `across`
+// threads take a chunk at a time, four dims a thread.
+template <int WAVES>
+__global__ __launch_bounds__(64 * WAVES) void join_kernel(AttendArgs a, AttendPlan plan) {
+    constexpr int kThreads = 64 * WAVES, kEach = 4;  // (chunks: at most slots, at most 256 a wave)
+    __shared__ float weight[kEach * kThreads], lds_m[WAVES], lds_l[WAVES];
+    __shared__ __attribute__((aligned(16))) float lds[4 * kThreads];
+    const int tid = (int)threadIdx.x, lane = tid & 63, wave = tid >> 6, dim = a.kv.head_dim;
     const float ninf = -__builtin_inff();
     const int sequence = (int)blockIdx.x / a.q_heads, head = (int)blockIdx.x % a.q_heads;
-    const int each = chunk_tiles(a, plan, lane);
-    int first = 0, chunks = 0;
-    for (int s0 = 0; s0 <= sequence; s0 += 64) {
-        const int s = s0 + lane;
-        const int n = s <= sequence ? max(1, (span_of(a, a.lengths[s]).tiles + each - 1) / each) : 0;
-        int sum = n;
-#pragma unroll
-        for (int m = 1; m < 64; m <<= 1) sum += __shfl_xor(sum, m);
-        first += sum;
-        if (s0 + 64 > sequence) chunks = __shfl(n, sequence - s0);
-    }
-    first -= chunks;
+    const int2 join = plan.joins[sequence];
+    const int64_t row0 = (int64_t)join.x * a.q_heads + head;
+    const int chunks = join.y;
     if (chunks <= 1) return;
-    float most = ninf;
-    for (int i = lane; i < chunks; i += 64) most = fmaxf(most, plan.part_ml[2 * ((int64_t)(first + i) * a.q_heads + head)]);
+    const float sink = a.sinks != nullptr ? a.sinks[head] * kLog2e : ninf;
+    float2 ml[kEach];
+    float most = sink;
+#pragma unroll
+    for (int n = 0; n < kEach; n++) {
+        const int i = tid + n * kThreads;
+        ml[n] = i < chunks ? plan.part_ml[row0 + (int64_t)i * a.q_heads] : make_float2(ninf, 0.0f);
+        most = fmaxf(most, ml[n].x);
+    }
 #pragma unroll
     for (int m = 1; m < 64; m <<= 1) most = fmaxf(most, __shfl_xor(most, m));
-    const float sink = a.sinks != nullptr ? a.sinks[head] * kLog2e : ninf;
-    most = fmaxf(most, sink);
-    const float at = most == ninf ? 0.0f : most;
-    float o[4] = {}, l = 0.0f;
-    for (int i = wave; i < chunks; i += 4) {
-        const int64_t row = (int64_t)(first + i) * a.q_heads + head;
-        const float f = __builtin_amdgcn_exp2f(plan.part_ml[2 * row] - at);
-        l += f * plan.part_ml[2 * row + 1];
+    if (lane == 0) lds_m[wave] = most;
+    __syncthreads();
 #pragma unroll
-        for (int j = 0; j < 4; j++)
-            if (lane + 64 * j < dim) o[j] += f * plan.part_o[row * dim + lane + 64 * j];
+    for (int w = 0; w < WAVES; w++) most = fmaxf(most, lds_m[w]);
+    const float at = most == ninf ? 0.0f : most;
+    float l = 0.0f;
+#pragma unroll
+    for (int n = 0; n < kEach; n++) {
+        const int i = tid + n * kThreads;
+        const float f = __builtin_amdgcn_exp2f(ml[n].x - at);
+        if (i < chunks) weight[i] = f;
+        l += f * ml[n].y;
     }
 #pragma unroll
-    for (int j = 0; j < 4; j++) lds[wave][lane + 64 * j] = o[j];
+    for (int m = 1; m < 64; m <<= 1) l += __shfl_xor(l, m);
     if (lane == 0) lds_l[wave] = l;
     __syncthreads();
-    const int d = (int)threadIdx.x;
-    if (d >= dim) return;
+    const int across = 1 << (32 - __builtin_clz((unsigned)(dim / 4 - 1))), slices = kThreads / across;
+    const int slice = tid / across, d0 = 4 * (tid % across);
+    f32x4 o = {};
+    if (d0 < dim) {
+        const float *const from = plan.part_o + row0 * dim + d0;
+        const int64_t pitch = (int64_t)a.q_heads * dim;
+#pragma unroll 8
+        for (int i = slice; i < chunks; i += slices)
+            o += weight[i] * *reinterpret_cast<const f32x4 *>(from + (int64_t)i * pitch);
+        *reinterpret_cast<f32x4 *>(lds + slice * dim + d0) = o;
+    }
+    __syncthreads();
+    if (tid >= dim) return;
     float sum = 0.0f, total = a.sinks != nullptr ? __builtin_amdgcn_exp2f(sink - at) : 0.0f;
+    for (int w = 0; w < min(slices, chunks); w++) sum += lds[w * dim + tid];
 #pragma unroll
-    for (int w = 0; w < 4; w++) sum += lds[w][d], total += lds_l[w];
-    store_element(a.out, a.out_type, sequence * a.out_stride + (int64_t)head * dim + d, total == 0.0f ? 0.0f : sum / total);
+    for (int w = 0; w < WAVES; w++) total += lds_l[w];
+    store_element(a.out, a.out_type, sequence * a.out_stride + (int64_t)head * dim + tid, total == 0.0f ? 0.0f : sum / total);
 }
 
-AttendPlan make_plan(const KvPages &kv, int sequences, int q_heads, int64_t max_pages) {
+AttendPlan make_plan(const KvPages &kv, int sequences, int q_heads, int64_t max_pages, int window) {
     AttendPlan p = {};
     p.row_tiles = (q_heads / kv.kv_heads + kRows - 1) / kRows;
-    const int64_t tiles = ((max_pages << kv.page_shift) + kTile - 1) / kTile;
+    int64_t tiles = ((max_pages << kv.page_shift) + kTile - 1) / kTile;
+    if (window > 0 && tiles > window / kTile + 2) tiles = window / kTile + 2;
     p.items = sequences;
     if (sequences > kScanMost || tiles <= kLeast) return p;  // a chunk a sequence
     const int64_t per = (int64_t)kv.kv_heads * p.row_tiles;
-    const int slots = (int)(per < kTarget ? kTarget / per : 1);
+    const int target = sequences == 1 ? kTargetOne : kTarget;
+    const int slots = (int)(per < target ? target / per : 1);
     p.slots = slots;
     const int64_t most = sequences * ((tiles + kLeast - 1) / kLeast);
     p.items = (int)(most < sequences + slots ? most : sequences + slots);
@@ -487,20 +550,28 @@ void launch(int dim, const AttendArgs &a, const AttendPlan &p, unsigned grid, hi
 #undef GOLLEK_ATTEND
 }
 
-size_t part_rows(const AttendPlan &p, int q_heads) { return p.slots > 0 ? (size_t)p.items * (size_t)q_heads : 0; }
+// Bytes of the workspace's parts; p's pointers where there is one.
+size_t lay_out(AttendPlan &p, const KvPages &kv, int sequences, int q_heads, uint8_t *workspace) {
+    if (p.slots == 0) return 0;
+    const size_t rows = (size_t)p.items * (size_t)q_heads, o = rows * (size_t)kv.head_dim * sizeof(float);
+    p.part_o = reinterpret_cast<float *>(workspace);
+    p.part_ml = reinterpret_cast<float2 *>(workspace + o);
+    p.joins = reinterpret_cast<int2 *>(workspace + o + rows * sizeof(float2));
+    return (o + rows * sizeof(float2) + (size_t)sequences * sizeof(int2) + 255) / 256 * 256;
+}
 
 }  // namespace
 
 size_t attend_workspace_bytes(const KvPages &kv, int sequences, int q_heads, int64_t max_pages) {
     // (past kScanMost nothing is split; the size stays what the batch before needed)
-    const AttendPlan p = make_plan(kv, sequences < kScanMost ? sequences : kScanMost, q_heads, max_pages);
-    return (part_rows(p, q_heads) * (size_t)(kv.head_dim + 2) * sizeof(float) + 255) / 256 * 256;
+    if (sequences > kScanMost) sequences = kScanMost;
+    AttendPlan p = make_plan(kv, sequences, q_heads, max_pages, 0);
+    return lay_out(p, kv, sequences, q_heads, nullptr);
 }
 
 hipError_t launch_attend(const AttendArgs &a, uint8_t *workspace, hipStream_t stream) {
-    AttendPlan p = make_plan(a.kv, a.sequences, a.q_heads, a.max_pages);
-    p.part_o = reinterpret_cast<float *>(workspace);
-    p.part_ml = p.part_o + part_rows(p, a.q_heads) * (size_t)a.kv.head_dim;
+    AttendPlan p = make_plan(a.kv, a.sequences, a.q_heads, a.max_pages, a.window);
+    (void)lay_out(p, a.kv, a.sequences, a.q_heads, workspace);
     p.q_vec = ((reinterpret_cast<uintptr_t>(a.q) | (uintptr_t)(a.q_stride * 2)) & 15u) == 0;
     const int64_t units = ((int64_t)p.items * a.kv.kv_heads + 7) / 8 * 8, grid = units * p.row_tiles;
     if (grid > 0x7FFFFFFF) return hipErrorInvalidValue;
@@ -510,7 +581,10 @@ hipError_t launch_attend(const AttendArgs &a, uint8_t *workspace, hipStream_t st
     else launch<kBF16, 2>(dim, a, p, (unsigned)grid, stream);
     hipError_t e = hipGetLastError();
     if (e == hipSuccess && p.slots > 0) {
-        hipLaunchKernelGGL(join_kernel, dim3((unsigned)(a.sequences * a.q_heads)), dim3(256), 0, stream, a, p);
+        const dim3 rows((unsigned)(a.sequences * a.q_heads));
+        if (p.slots > 16 * a.sequences || p.slots > 1024) hipLaunchKernelGGL(join_kernel<16>, rows, dim3(1024), 0, stream, a, p);
+        else if (p.slots <= 4 * a.sequences && p.slots <= 256) hipLaunchKernelGGL(join_kernel<1>, rows, dim3(64), 0, stream, a, p);
+        else hipLaunchKernelGGL(join_kernel<4>, rows, dim3(256), 0, stream, a, p);
         e = hipGetLastError();
     }
     return e;

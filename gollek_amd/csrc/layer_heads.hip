@@ -96,35 +96,18 @@ __global__ __launch_bounds__(64 * kWaves) void heads_kernel(HeadsArgs a, HeadsPl
     const int slice = (int)(unit - t * plan.slices);
     const int kv_heads = CACHE ? a.kv.kv_heads : 0, heads = a.q_heads + 2 * kv_heads;
     const int dim = a.head_dim, dims = a.rope.dims, pairs = dim / 2;
+    // everything that waits for nothing is loaded first: a decoded token's call is a chain
+    // of loads, position to page to place, and the angles on the way
     const int64_t position = a.positions[t];
-    for (int p = lane; p < dims / 2; p += 64) {
-        const double turn = (double)position * a.rope.turns[p];
-        float s, c;
-        sincospif(2.0f * (float)(turn - rint(turn)), &s, &c);
-        turns[wave][p] = make_float2(a.rope.magnitude * c, a.rope.magnitude * s);
-    }
-    __syncthreads();
-    if (!in) return;
-
-    // the token's place in the cache: of head 0, in elements (-1: nowhere)
-    int64_t place = -1;
+    int64_t sequence = t, page = -1;
     if constexpr (CACHE) {
-        const int64_t sequence = a.sequence != nullptr ? a.sequence[t] : t;
-        if (position < 0 || sequence < 0 || sequence >= a.sequences) return;  // padding
-        const int64_t column = position >> a.kv.page_shift;
-        if (column < a.max_pages) {
-            const int64_t page = a.page_table[sequence * a.max_pages + column];
-            const int64_t slot = position & ((1 << a.kv.page_shift) - 1);
-            if (page >= 0 && page < a.kv.pages) place = (((page * kv_heads) << a.kv.page_shift) + slot) * dim;
-        }
+        if (a.sequence != nullptr) sequence = a.sequence[t];
     }
-
     // this lane's pairs: p .. p + V - 1; their first and second elements stand at
     // e0 and e1 .. (half), or together from e0 on (interleaved, or behind what turns)
     const int groups = 64 / plan.lanes, mine = lane % plan.lanes;
     int e0[NS], e1[NS];
     bool has[NS], turned[NS];
-    float2 cs[NS][V];
     Run<4, V> qn[NS][2], kn[NS][2];
 #pragma unroll
     for (int n = 0; n < NS; n++) {
@@ -134,30 +117,67 @@ __global__ __launch_bounds__(64 * kWaves) void heads_kernel(HeadsArgs a, HeadsPl
         const bool half = turned[n] && !a.rope.interleaved;
         e0[n] = half ? p : 2 * p;
         e1[n] = half ? p + dims / 2 : 2 * p + V;
-#pragma unroll
-        for (int j = 0; j < V; j++) cs[n][j] = turned[n] ? turns[wave][p + j] : make_float2(1.0f, 0.0f);
         if (!has[n]) continue;
         if (a.q_norm != nullptr) qn[n][0].load(a.q_norm, e0[n]), qn[n][1].load(a.q_norm, e1[n]);
         if (a.k_norm != nullptr) kn[n][0].load(a.k_norm, e0[n]), kn[n][1].load(a.k_norm, e1[n]);
     }
-
-    const int step = plan.slices * groups;
+    // the token's rows (as numbers that the compiler does not know to stand side by side
+    // in the arguments: it would choose between them through memory)
+    const uint8_t *q_row = static_cast<const uint8_t *>(a.q) + t * a.q_stride * IN;
+    const uint8_t *k_row = nullptr, *v_row = nullptr;
+    if constexpr (CACHE) {
+        k_row = static_cast<const uint8_t *>(a.k) + t * a.k_stride * IN;
+        v_row = static_cast<const uint8_t *>(a.v) + t * a.v_stride * IN;
+    }
     Run<IN, V> x[NS][2];
     const auto fetch = [&](int head) {
-        const void *from = a.q;
-        int64_t at = t * a.q_stride + (int64_t)head * dim;
+        const uint8_t *from = q_row + (int64_t)head * dim * IN;
         if (CACHE && head >= a.q_heads) {
             const bool key = head < a.q_heads + kv_heads;
-            from = key ? a.k : a.v;
-            at = t * (key ? a.k_stride : a.v_stride) + (int64_t)(head - a.q_heads - (key ? 0 : kv_heads)) * dim;
+            from = (key ? k_row : v_row) + (int64_t)(head - a.q_heads - (key ? 0 : kv_heads)) * dim * IN;
         }
 #pragma unroll
         for (int n = 0; n < NS; n++)
-            if (has[n]) x[n][0].load(from, at + e0[n]), x[n][1].load(from, at + e1[n]);
+            if (has[n]) x[n][0].load(from, e0[n]), x[n][1].load(from, e1[n]);
     };
     int head = slice * groups + lane / plan.lanes;
-    const int rounds = (heads - slice * groups + step - 1) / step;  // (of the wave; its last may lack heads)
     if (head < heads) fetch(head);
+    double angle[2];
+#pragma unroll
+    for (int n = 0; n < 2; n++) angle[n] = lane + 64 * n < dims / 2 ? a.rope.turns[lane + 64 * n] : 0.0;
+
+    // the token's place in the cache: of head 0, in elements (-1: nowhere)
+    int64_t place = -1;
+    bool padding = false;
+    if constexpr (CACHE) {
+        const int64_t column = position >> a.kv.page_shift;
+        padding = position < 0 || sequence < 0 || sequence >= a.sequences;
+        if (!padding && column < a.max_pages) page = a.page_table[sequence * a.max_pages + column];
+    }
+#pragma unroll
+    for (int n = 0; n < 2; n++) {
+        if (lane + 64 * n >= dims / 2) continue;
+        const double turn = (double)position * angle[n];
+        float s, c;
+        sincospif(2.0f * (float)(turn - rint(turn)), &s, &c);
+        turns[wave][lane + 64 * n] = make_float2(a.rope.magnitude * c, a.rope.magnitude * s);
+    }
+    __syncthreads();
+    if (!in || padding) return;
+    if constexpr (CACHE) {
+        const int64_t slot = position & ((1 << a.kv.page_shift) - 1);
+        if (page >= 0 && page < a.kv.pages) place = (((page * kv_heads) << a.kv.page_shift) + slot) * dim;
+    }
+    float2 cs[NS][V];
+#pragma unroll
+    for (int n = 0; n < NS; n++)
+#pragma unroll
+        for (int j = 0; j < V; j++)
+            cs[n][j] = turned[n] ? turns[wave][V * (mine + 64 * n) + j] : make_float2(1.0f, 0.0f);
+
+    const int64_t v_from_k = static_cast<uint8_t *>(a.kv.v) - static_cast<uint8_t *>(a.kv.k);
+    const int step = plan.slices * groups;
+    const int rounds = (heads - slice * groups + step - 1) / step;  // (of the wave; its last may lack heads)
     for (int i = 0; i < rounds; i++, head += step) {
         float u[NS][2][V];
         float sum = 0.0f;
@@ -187,10 +207,10 @@ __global__ __launch_bounds__(64 * kWaves) void heads_kernel(HeadsArgs a, HeadsPl
             }
         }
         if (head >= heads || (!query && place < 0)) continue;
-        void *to = a.q_out;
+        uint8_t *to = static_cast<uint8_t *>(a.q_out);
         int64_t at = t * a.q_out_stride + (int64_t)head * dim;
         if (CACHE && !query) {
-            to = key ? a.kv.k : a.kv.v;
+            to = static_cast<uint8_t *>(a.kv.k) + (key ? 0 : v_from_k);
             at = place + ((int64_t)(head - a.q_heads - (key ? 0 : kv_heads)) << a.kv.page_shift) * dim;
         }
 #pragma unroll

@@ -303,7 +303,7 @@ __global__ __launch_bounds__(kThreads) void attend_kernel(AttendArgs a, AttendPl
     f32x4 o[D::kFragments] = {};
     float m = ninf, base = 0.0f, l = 0.0f;  // l of this lane's keys
     const float scale2 = a.scale * kLog2e, cap2 = a.softcap * kLog2e;
-    const float turn = a.softcap > 0.0f ? 2.0f * kLog2e * a.scale / a.softcap : 0.0f;
+    const float turn = a.softcap > 0.0f ? a.scale / a.softcap : 0.0f;
 
     // One step; MORE: of another one after it, whose keys are loaded when the scores have
     // used the registers, and whose values behind the second product.  (Two copies: a load
@@ -335,9 +335,17 @@ __global__ __launch_bounds__(kThreads) void attend_kernel(AttendArgs a, AttendPl
         }
         float x[8];
         if (a.softcap > 0.0f) {
+            if (a.out_type == kF32) {
 #pragma unroll
-            for (int j = 0; j < 8; j++)  // cap * tanh(z) = cap * (1 - 2 / (1 + exp(2 z)))
-                x[j] = cap2 - 2.0f * cap2 * __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(turn * s[j >> 2][j & 3]));
+                for (int j = 0; j < 8; j++) x[j] = cap2 * tanhf(turn * s[j >> 2][j & 3]);
+            } else {
+                // 1 - 2 / (1 + exp(2 z)): off by 2^-21.5 of the cap at most, for a cap of 50 a
+                // weight by 2e-5, a 25th of fp16's half step; 8 % of the exact form's instructions
+#pragma unroll
+                for (int j = 0; j < 8; j++)
+                    x[j] = cap2 - 2.0f * cap2 *
+                                      __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(2.0f * kLog2e * turn * s[j >> 2][j & 3]));
+            }
         } else {
 #pragma unroll
             for (int j = 0; j < 8; j++) x[j] = scale2 * s[j >> 2][j & 3];
@@ -504,12 +512,14 @@ __global__ __launch_bounds__(64 * WAVES) void join_kernel(AttendArgs a, AttendPl
         *reinterpret_cast<f32x4 *>(lds + slice * dim + d0) = o;
     }
     __syncthreads();
-    if (tid >= dim) return;
-    float sum = 0.0f, total = a.sinks != nullptr ? __builtin_amdgcn_exp2f(sink - at) : 0.0f;
-    for (int w = 0; w < min(slices, chunks); w++) sum += lds[w * dim + tid];
+    float total = a.sinks != nullptr ? __builtin_amdgcn_exp2f(sink - at) : 0.0f;
 #pragma unroll
     for (int w = 0; w < WAVES; w++) total += lds_l[w];
-    store_element(a.out, a.out_type, sequence * a.out_stride + (int64_t)head * dim + tid, total == 0.0f ? 0.0f : sum / total);
+    for (int d = tid; d < dim; d += kThreads) {
+        float sum = 0.0f;
+        for (int w = 0; w < min(slices, chunks); w++) sum += lds[w * dim + d];
+        store_element(a.out, a.out_type, sequence * a.out_stride + (int64_t)head * dim + d, total == 0.0f ? 0.0f : sum / total);
+    }
 }
 
 AttendPlan make_plan(const KvPages &kv, int sequences, int q_heads, int64_t max_pages, int window) {

@@ -178,6 +178,16 @@ def test_many_sequences():
     Batch([(5 * i) % 9 for i in range(3000)], 2, 1, 32, BF16, seed=17).check(F32)
 
 
+@pytest.mark.parametrize("sequences,kv_heads,dim", [(50, 8, 128), (50, 8, 256), (50, 8, 40), (20, 8, 128), (3, 1, 256), (2, 1, 8),
+                                                    (97, 16, 64), (300, 2, 192), (1024, 1, 64), (1025, 1, 64)])
+def test_few_long_among_many(sequences, kv_heads, dim):
+    # every way to join chunks: many a sequence, a few, at most one on the average
+    lengths = [(11 * i) % 67 for i in range(sequences)]
+    lengths[0], lengths[sequences // 2], lengths[-1] = 3000, 1111, 5000
+    rows = sorted({0, 1, sequences // 3, sequences // 2, sequences - 2, sequences - 1})
+    Batch(lengths, 2 * kv_heads, kv_heads, dim, BF16, page=64, seed=sequences).check(F32, rows)
+
+
 def test_lengths_past_the_table_and_below_zero():
     b = Batch([64, 64, 64, 64], 4, 2, 64, BF16, seed=18)
     b.lengths = [65, 2**31 - 1, -5, -(2**31)]

@@ -41,7 +41,15 @@ typedef float f32x4 __attribute__((ext_vector_type(4)));
 constexpr int kWaves = 4, kThreads = 64 * kWaves;
 constexpr int kTile = 32;           // keys of a step
 constexpr int kRows = 16;           // query heads of a workgroup
-constexpr int kLeast = 8;           // tiles of a chunk at least: two steps a wave
+// Tiles of a chunk at least: a step a wave.  (A CU takes in some 60 GB/s, 64 KB a step's
+// round of its four waves, so a short sequence is as fast as it has CUs: 700 tokens of 8
+// heads in chunks of 8 tiles 7.0 us, of 4 6.2, of 2 5.7, to which a join adds 4.3 to 4.5.)
+constexpr int kLeast = 4;
+// Tables of no more tiles than this are not cut at all, which saves the second launch:
+// with workgroups for fewer than 256 CUs (700 tokens, 22 tiles: 10.5 us whole, 6.2 and 4.3
+// cut; 1000, 32 tiles: 13.1, 6.2 and 4.4), and with more (32 sequences of 1000: 20.0, 20.5
+// and 4.0; of 2000, 63 tiles: 36.4, 31.5 and 4.6).
+constexpr int kWholeFew = 24, kWholeMany = 32, kFew = 256;
 // Workgroups that a batch is cut into: one sequence, whose chunks are all alike, into one
 // round of three a CU (131072 tokens of 4 heads of 128: 44.9 us, in 1024 46.4, in 1536
 // 48.8); several, whose chunks come out between half of T and T, into twice that, so
@@ -190,7 +198,7 @@ struct ValueTile {
 // TYPE: of cache and queries.  NK: head_dim / 32, rounded up (EXACT: without a rest).
 // PARTS: the pieces a weight is split into, of 8 (bf16) or 11 (fp16) bits each.
 template <int TYPE, int NK, bool EXACT, int PARTS>
-__global__ __launch_bounds__(kThreads) void attend_kernel(AttendArgs a, AttendPlan plan) {
+__global__ __launch_bounds__(kThreads, NK <= 2 ? 4 : 2) void attend_kernel(AttendArgs a, AttendPlan plan) {
     using D = Dims<NK>;
     constexpr std::integral_constant<int, TYPE> type;
     // fp16 weights: exp(s - m) times 2^7, so that all but the smallest are normal numbers
@@ -528,8 +536,8 @@ AttendPlan make_plan(const KvPages &kv, int sequences, int q_heads, int64_t max_
     int64_t tiles = ((max_pages << kv.page_shift) + kTile - 1) / kTile;
     if (window > 0 && tiles > window / kTile + 2) tiles = window / kTile + 2;
     p.items = sequences;
-    if (sequences > kScanMost || tiles <= kLeast) return p;  // a chunk a sequence
     const int64_t per = (int64_t)kv.kv_heads * p.row_tiles;
+    if (sequences > kScanMost || tiles <= (sequences * per < kFew ? kWholeFew : kWholeMany)) return p;  // a chunk a sequence
     const int target = sequences == 1 ? kTargetOne : kTarget;
     const int slots = (int)(per < target ? target / per : 1);
     p.slots = slots;

@@ -50,7 +50,7 @@ using gollek::pointer_device;
 using gollek::share;
 using gollek::within;
 
-constexpr int32_t kAbiVersion = 1 * 10000 + 1 * 100 + 0;
+constexpr int32_t kAbiVersion = 1 * 10000 + 2 * 100 + 0;
 constexpr int64_t kRouterMaxExperts = 4096;  // router LDS: 8 B per expert + 4 B per rank
 
 thread_local std::string g_last_error;

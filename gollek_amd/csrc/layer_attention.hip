@@ -50,11 +50,13 @@ constexpr int kLeast = 4;
 // cut; 1000, 32 tiles: 13.1, 6.2 and 4.4), and with more (32 sequences of 1000: 20.0, 20.5
 // and 4.0; of 2000, 63 tiles: 36.4, 31.5 and 4.6).
 constexpr int kWholeFew = 24, kWholeMany = 32, kFew = 256;
-// Workgroups that a batch is cut into: one sequence, whose chunks are all alike, into one
-// round of three a CU (131072 tokens of 4 heads of 128: 44.9 us, in 1024 46.4, in 1536
-// 48.8); several, whose chunks come out between half of T and T, into twice that, so
-// that the last round is short (64 of up to 8192: 225 in 768, 216 in 1536).
-constexpr int kTargetOne = 768, kTarget = 1536;
+// Workgroups that a batch is cut into: one for every CU and sequence, up to kTargetMost.
+// The chunks of one sequence are all alike, and one round of them does best (131072 tokens
+// of 4 heads of 128, main kernel and join: 44.1 + 4.8 us, in 512 44.5 + 5.3, in 768 45.1 +
+// 5.8); several sequences' come out between half of T and T, and the more there are the
+// shorter the last round should be (two of 65536: 39.1 in 512, 51.8 in 256; 64 of up to
+// 8192: 216 in 1536, 225 in 768).
+constexpr int kTargetEach = 256, kTargetMost = 1536;
 constexpr int kScanMost = 1024;     // sequences whose tiles every workgroup adds up
 constexpr float kSlack = 8.0f;      // how far a score may pass m, in powers of two
 constexpr float kLog2e = 1.4426950408889634f;
@@ -538,7 +540,7 @@ AttendPlan make_plan(const KvPages &kv, int sequences, int q_heads, int64_t max_
     p.items = sequences;
     const int64_t per = (int64_t)kv.kv_heads * p.row_tiles;
     if (sequences > kScanMost || tiles <= (sequences * per < kFew ? kWholeFew : kWholeMany)) return p;  // a chunk a sequence
-    const int target = sequences == 1 ? kTargetOne : kTarget;
+    const int target = sequences < kTargetMost / kTargetEach ? sequences * kTargetEach : kTargetMost;
     const int slots = (int)(per < target ? target / per : 1);
     p.slots = slots;
     const int64_t most = sequences * ((tiles + kLeast - 1) / kLeast);

@@ -503,7 +503,8 @@ int32_t gollek_hip_next_token(gollek_hip_weight *lm_head, const float *x, int64_
  * bias 0; hidden or y may be NULL (not both).  rows up to 2^31 - 1, cols in
  * [1, 65536], a finite scale, eps >= 0 and finite: else ARG.  hidden may be x or the
  * residual itself, y may be x or the residual (the same address, type size and
- * stride).  A row of zeros with eps 0 divides 0 by 0 (NaN).
+ * stride).  A row of zeros with eps 0 divides 0 by 0 (NaN); squares are fp32's, so
+ * rows of magnitudes past 1e18 overflow.
  * The host form takes packed rows and copies them up (synchronous). */
 int32_t gollek_hip_norm(const void *x, int32_t x_type, int64_t rows, int64_t cols, const float *post_weight,
                         const float *gate, float scale, const void *residual, void *hidden, int32_t hidden_type,
@@ -599,7 +600,7 @@ int32_t gollek_hip_kv_append_device(const gollek_hip_kv_cache *cache, const goll
  * over the last `window` (0: all) of the first lengths[sequence] tokens, -> out
  * (sequences x q_heads x head_dim of out_type).  A length past the table counts as
  * the table's, one below 1 as 0; a token whose page is outside [0, pages) is not
- * there; a row without any token is 0.  Nothing behind a sequence's length or before
+ * there; a row without any token (or with every s_j -inf) is 0.  Nothing behind a sequence's length or before
  * its window changes a result, whatever it holds.  Several new tokens of one
  * sequence are rows of their own, with equal page_table rows and growing lengths.
  * Results depend in their last bits on the lengths in the batch (they set how the

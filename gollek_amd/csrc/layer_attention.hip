@@ -28,8 +28,8 @@
 //
 // Bound by bytes: 64 sequences of up to 8192 tokens of 8 heads of 128 217 us (1.37 GB, 6.3
 // TB/s; reads alone outrun a copy's 5.0), one of 131072 of 4 heads 44.0 (268 MB, 6.1
-// TB/s) and 4.8 for the join.  Loads that do not stay in the caches are an eighth of that
-// (251 and 51 with plain ones).  Short sequences are bound by what a CU takes in (60 GB/s)
+// TB/s) and 4.8 for the join.  Loads that do not stay in the caches give an eighth of
+// that (plain ones: 246 and 51).  Short sequences are bound by what a CU takes in (60 GB/s)
 // and the chain length, page, keys: 700 tokens 10.4.
 //
 // A sequence's tiles are cut into chunks of equal size for workgroups that share the chip
@@ -61,6 +61,12 @@ constexpr int kLeast = 4;
 // cut; 1000, 32 tiles: 13.1, 6.2 and 4.4), and with more (32 sequences of 1000: 20.0, 20.5
 // and 4.0; of 2000, 63 tiles: 36.4, 31.5 and 4.6).
 constexpr int kWholeFew = 24, kWholeMany = 32, kFew = 256;
+// Many units of few tiles take a wave each, which saves their join through LDS and the
+// idle waves (256 sequences in a window of 128, 64 / 8 heads of 64: 17.5 us, by
+// workgroups 20.2; 1000 of up to 60, 16 / 4 of 128: 24.0, 28.5).  From eight tiles on, or
+// with fewer waves than the chip holds, it loses (256 of up to 256, 32 / 8 of 128: 38.4,
+// 33.8; 32 of up to 300: 20.5, 9.1).
+constexpr int kAloneTiles = 6, kAloneUnits = 2048;
 // Workgroups that a batch is cut into: one for every CU and sequence, up to kTargetMost.
 // The chunks of one sequence are all alike, and one round of them does best (131072 tokens
 // of 4 heads of 128, main kernel and join: 44.1 + 4.8 us, in 512 44.5 + 5.3, in 768 45.1 +
@@ -76,6 +82,7 @@ struct AttendPlan {
     int row_tiles;  // workgroups for the query heads of one key head
     int slots;      // chunks of a key head that the batch is cut into (0: a chunk a sequence)
     int items;      // chunks at most
+    int share;      // waves that share a unit (one key head of a chunk, up to kRows query heads)
     bool q_vec;     // queries on 16-byte borders
     // workspace: a chunk's sums, (bound, weight) for each query head, and a sequence's
     // first chunk and how many it has
@@ -192,6 +199,24 @@ struct Dims {
     static constexpr int kPitch = 16 * kFragments + 4;  // floats of a row in LDS
 };
 
+// N neighbouring floats to elements of the output, at any alignment of the element.
+template <int N>
+__device__ __forceinline__ void store_run(void *p, int type, int64_t i, const float (&v)[N]) {
+    if (type == kF32) {
+        __builtin_memcpy(static_cast<float *>(p) + i, v, sizeof(v));
+    } else {
+        uint32_t w[N / 2];
+#pragma unroll
+        for (int j = 0; j < N / 2; j++) {
+            typedef __bf16 b2 __attribute__((ext_vector_type(2)));
+            typedef _Float16 h2 __attribute__((ext_vector_type(2)));
+            w[j] = type == kBF16 ? __builtin_bit_cast(uint32_t, b2{(__bf16)v[2 * j], (__bf16)v[2 * j + 1]})
+                                 : __builtin_bit_cast(uint32_t, h2{(_Float16)v[2 * j], (_Float16)v[2 * j + 1]});
+        }
+        __builtin_memcpy(static_cast<uint16_t *>(p) + i, w, sizeof(w));
+    }
+}
+
 // Keys and values are used once a call: loads that do not stay in the caches.
 template <class T>
 __device__ __forceinline__ T stream(const T *p) {
@@ -210,26 +235,34 @@ struct ValueTile {
 
 // TYPE: of cache and queries.  NK: head_dim / 32, rounded up (EXACT: without a rest).
 // PARTS: the pieces a weight is split into, of 8 (bf16) or 11 (fp16) bits each.
-template <int TYPE, int NK, bool EXACT, int PARTS>
-__global__ __launch_bounds__(kThreads, NK <= 2 ? 4 : 2) void attend_kernel(AttendArgs a, AttendPlan plan) {
+template <int TYPE, int NK, bool EXACT, int PARTS, int SHARE>
+__global__ __launch_bounds__(kThreads, NK <= 2 ? 4 : NK <= 6 ? 2 : 1) void attend_kernel(AttendArgs a, AttendPlan plan) {
     using D = Dims<NK>;
     constexpr std::integral_constant<int, TYPE> type;
     // fp16 weights: exp(s - m) times 2^7, so that all but the smallest are normal numbers
     // (2^15 with the slack, below fp16's largest)
     constexpr float kLift = TYPE == kF16 ? 7.0f : 0.0f;
     const float ninf = -__builtin_inff();
-    __shared__ __attribute__((aligned(16))) float lds_o[kWaves][kRows * D::kPitch];
-    __shared__ float lds_m[kWaves][kRows], lds_l[kWaves][kRows];
 
     const int lane = (int)threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
     const int c = lane & 15, g = lane >> 4;
     const int dim = EXACT ? 32 * NK : a.kv.head_dim;
     const int group = a.q_heads / a.kv.kv_heads;
-    // workgroups of one chunk's heads that read the same keys: eight apart, on one XCD
-    const int id = (int)blockIdx.x, row_tile = id / 8 % plan.row_tiles, unit = id / (8 * plan.row_tiles) * 8 + id % 8;
+    // Query heads of one key head that take several units read the same keys: as
+    // workgroups eight apart, on one XCD; as waves (SHARE 1) side by side.
+    int row_tile, unit;
+    if constexpr (SHARE > 1) {
+        const int id = (int)blockIdx.x;
+        row_tile = id / 8 % plan.row_tiles;
+        unit = id / (8 * plan.row_tiles) * 8 + id % 8;
+    } else {
+        const int id = (int)blockIdx.x * kWaves + wave;
+        row_tile = id % plan.row_tiles;
+        unit = id / plan.row_tiles;
+    }
     const int item = unit / a.kv.kv_heads, kv_head = unit % a.kv.kv_heads;
     Item it = {item, 0, 0, 1};
-    if (plan.slots > 0) {
+    if (SHARE > 1 && plan.slots > 0) {
         if (!find_item(a, plan, item, lane, it)) return;
         if (it.chunk == 0 && kv_head == 0 && row_tile == 0 && threadIdx.x == 0)
             plan.joins[it.sequence] = make_int2(item, it.chunks);
@@ -280,7 +313,7 @@ __global__ __launch_bounds__(kThreads, NK <= 2 ? 4 : 2) void attend_kernel(Atten
     const auto place = [&](int page, int key) -> int64_t {
         const int64_t row = ((int64_t)page * a.kv.kv_heads + kv_head) << a.kv.page_shift;
         const int64_t at = (row + (key & ((1 << a.kv.page_shift) - 1))) * dim * 2;
-        return key < span.length && page >= 0 && page < a.kv.pages ? at : -1;
+        return key < span.length && key + 15 >= span.begin && page >= 0 && page < a.kv.pages ? at : -1;
     };
     const int64_t nowhere = (((int64_t)kv_head) << a.kv.page_shift) * dim * 2;  // (page 0: memory of the cache)
 
@@ -329,7 +362,7 @@ __global__ __launch_bounds__(kThreads, NK <= 2 ? 4 : 2) void attend_kernel(Atten
     // One step; MORE: of another one after it, whose keys are loaded when the scores have
     // used the registers, and whose values behind the second product.  (Two copies: a load
     // under a branch would have the wait for this step's values wait for it too.)
-    int tile = tile0 + wave, page[2];
+    int tile = tile0 + (SHARE > 1 ? wave : 0), page[2];
     int64_t at[2];
     const auto step = [&](auto MORE) {
         constexpr bool more = decltype(MORE)::value;
@@ -349,10 +382,10 @@ __global__ __launch_bounds__(kThreads, NK <= 2 ? 4 : 2) void attend_kernel(Atten
         const bool half[2] = {at[0] >= 0, at[1] >= 0};
         const bool whole = key0 >= span.begin && span.length - key0 >= kTile && half[0] && half[1];
         if constexpr (more) {
-            tile += kWaves;
+            tile += SHARE;
             at[0] = place(page[0], kTile * tile), at[1] = place(page[1], kTile * tile + 16);
             load_keys(at);
-            pages_of(min(tile + kWaves, tile1 - 1), page);
+            pages_of(min(tile + SHARE, tile1 - 1), page);
         }
         float x[8];
         if (a.softcap > 0.0f) {
@@ -422,59 +455,87 @@ __global__ __launch_bounds__(kThreads, NK <= 2 ? 4 : 2) void attend_kernel(Atten
         at[0] = place(page[0], kTile * tile), at[1] = place(page[1], kTile * tile + 16);
         load_keys(at);
         load_values(at);
-        pages_of(min(tile + kWaves, tile1 - 1), page);
+        pages_of(min(tile + SHARE, tile1 - 1), page);
 #pragma unroll
         for (int i = 0; i < NK; i++)
             if (c >= rows || (!EXACT && 32 * i + 8 * g >= dim)) q[i] = u32x4{};
-        while (tile + kWaves < tile1) step(std::true_type{});
+        while (tile + SHARE < tile1) step(std::true_type{});
         step(std::false_type{});
     }
 
-    // the waves' sums, rescaled to their common bound, through LDS
     l += __shfl_xor(l, 16);
     l += __shfl_xor(l, 32);
     const float bound = m == ninf ? ninf : base;
-    if (g == 0) lds_m[wave][c] = bound, lds_l[wave][c] = l;
-    __syncthreads();
-    float top = ninf;
-#pragma unroll
-    for (int w = 0; w < kWaves; w++) top = fmaxf(top, lds_m[w][c]);
-    const float keep = __builtin_amdgcn_exp2f(bound - (top == ninf ? 0.0f : top));
-    if (c < rows) {
-#pragma unroll
-        for (int r = 0; r < 4; r++) {  // dims wide * (4 g + r) + i
-            float *const to = lds_o[wave] + c * D::kPitch;
-#pragma unroll
-            for (int i = 0; i < D::kWide0; i++) to[D::kWide0 * (4 * g + r) + i] = keep * o[i][r];
-#pragma unroll
-            for (int i = 0; i < D::kWide1; i++) to[16 * D::kWide0 + D::kWide1 * (4 * g + r) + i] = keep * o[D::kWide0 + i][r];
+    if constexpr (SHARE == 1) {  // the whole sequence: straight from the accumulators
+        if (c >= rows) return;
+        float f = 1.0f, total = l;
+        if (a.sinks != nullptr) {
+            const float sink = a.sinks[head0 + c] * kLog2e, up = fmaxf(sink, bound), at1 = up == ninf ? 0.0f : up;
+            f = __builtin_amdgcn_exp2f(bound - at1);
+            total = l * f + __builtin_amdgcn_exp2f(sink - at1);
         }
-    }
-    __syncthreads();
-    for (int e = (int)threadIdx.x; e < rows * dim; e += kThreads) {
-        const int r = e / dim, d = e - r * dim;
-        float sum = 0.0f, total = 0.0f, most = ninf;
+        const int64_t row = it.sequence * a.out_stride + (head0 + c) * dim;
 #pragma unroll
-        for (int w = 0; w < kWaves; w++) {
-            sum += lds_o[w][r * D::kPitch + d];
-            most = fmaxf(most, lds_m[w][r]);
+        for (int r = 0; r < 4; r++) {
+            const auto put = [&](auto WIDE, int first, int d) {
+                constexpr int wide = decltype(WIDE)::value;
+                if (d >= dim) return;
+                float y[wide];
+#pragma unroll
+                for (int i = 0; i < wide; i++) y[i] = total == 0.0f ? 0.0f : f * o[first + i][r] / total;
+                store_run<wide>(a.out, a.out_type, row + d, y);
+            };
+            put(std::integral_constant<int, D::kWide0>{}, 0, D::kWide0 * (4 * g + r));
+            if constexpr (D::kWide1 > 0)
+                put(std::integral_constant<int, D::kWide1>{}, D::kWide0, 16 * D::kWide0 + D::kWide1 * (4 * g + r));
         }
-        const float at0 = most == ninf ? 0.0f : most;
+        return;
+    } else {
+        // the waves' sums, rescaled to their common bound, through LDS
+        __shared__ __attribute__((aligned(16))) float lds_o[kWaves][kRows * D::kPitch];
+        __shared__ float lds_m[kWaves][kRows], lds_l[kWaves][kRows];
+        if (g == 0) lds_m[wave][c] = bound, lds_l[wave][c] = l;
+        __syncthreads();
+        float top = ninf;
 #pragma unroll
-        for (int w = 0; w < kWaves; w++) total += lds_l[w][r] * __builtin_amdgcn_exp2f(lds_m[w][r] - at0);
-        if (it.chunks > 1) {
-            const int64_t row = (int64_t)item * a.q_heads + head0 + r;
-            plan.part_o[row * dim + d] = sum;
-            if (d == 0) plan.part_ml[row] = make_float2(most, total);
-        } else {
-            if (a.sinks != nullptr) {
-                const float sink = a.sinks[head0 + r] * kLog2e, up = fmaxf(sink, most), at1 = up == ninf ? 0.0f : up;
-                const float f = __builtin_amdgcn_exp2f(at0 - at1);
-                sum *= f;
-                total = total * f + __builtin_amdgcn_exp2f(sink - at1);
+        for (int w = 0; w < kWaves; w++) top = fmaxf(top, lds_m[w][c]);
+        const float keep = __builtin_amdgcn_exp2f(bound - (top == ninf ? 0.0f : top));
+        if (c < rows) {
+#pragma unroll
+            for (int r = 0; r < 4; r++) {  // dims wide * (4 g + r) + i
+                float *const to = lds_o[wave] + c * D::kPitch;
+#pragma unroll
+                for (int i = 0; i < D::kWide0; i++) to[D::kWide0 * (4 * g + r) + i] = keep * o[i][r];
+#pragma unroll
+                for (int i = 0; i < D::kWide1; i++) to[16 * D::kWide0 + D::kWide1 * (4 * g + r) + i] = keep * o[D::kWide0 + i][r];
             }
-            store_element(a.out, a.out_type, it.sequence * a.out_stride + (head0 + r) * dim + d,
-                          total == 0.0f ? 0.0f : sum / total);
+        }
+        __syncthreads();
+        for (int e = (int)threadIdx.x; e < rows * dim; e += kThreads) {
+            const int r = e / dim, d = e - r * dim;
+            float sum = 0.0f, total = 0.0f, most = ninf;
+#pragma unroll
+            for (int w = 0; w < kWaves; w++) {
+                sum += lds_o[w][r * D::kPitch + d];
+                most = fmaxf(most, lds_m[w][r]);
+            }
+            const float at0 = most == ninf ? 0.0f : most;
+#pragma unroll
+            for (int w = 0; w < kWaves; w++) total += lds_l[w][r] * __builtin_amdgcn_exp2f(lds_m[w][r] - at0);
+            if (it.chunks > 1) {
+                const int64_t row = (int64_t)item * a.q_heads + head0 + r;
+                plan.part_o[row * dim + d] = sum;
+                if (d == 0) plan.part_ml[row] = make_float2(most, total);
+            } else {
+                if (a.sinks != nullptr) {
+                    const float sink = a.sinks[head0 + r] * kLog2e, up = fmaxf(sink, most), at1 = up == ninf ? 0.0f : up;
+                    const float f = __builtin_amdgcn_exp2f(at0 - at1);
+                    sum *= f;
+                    total = total * f + __builtin_amdgcn_exp2f(sink - at1);
+                }
+                store_element(a.out, a.out_type, it.sequence * a.out_stride + (head0 + r) * dim + d,
+                              total == 0.0f ? 0.0f : sum / total);
+            }
         }
     }
 }
@@ -550,6 +611,7 @@ AttendPlan make_plan(const KvPages &kv, int sequences, int q_heads, int64_t max_
     if (window > 0 && tiles > window / kTile + 2) tiles = window / kTile + 2;
     p.items = sequences;
     const int64_t per = (int64_t)kv.kv_heads * p.row_tiles;
+    p.share = tiles <= kAloneTiles && sequences * per >= kAloneUnits ? 1 : kWaves;
     if (sequences > kScanMost || tiles <= (sequences * per < kFew ? kWholeFew : kWholeMany)) return p;  // a chunk a sequence
     const int target = sequences < kTargetMost / kTargetEach ? sequences * kTargetEach : kTargetMost;
     const int slots = (int)(per < target ? target / per : 1);
@@ -561,12 +623,16 @@ AttendPlan make_plan(const KvPages &kv, int sequences, int q_heads, int64_t max_
 
 template <int TYPE, int PARTS>
 void launch(int dim, const AttendArgs &a, const AttendPlan &p, unsigned grid, hipStream_t stream) {
-#define GOLLEK_ATTEND(NK)                                                                                               \
-    case NK:                                                                                                            \
-        if (dim == 32 * NK)                                                                                             \
-            hipLaunchKernelGGL((attend_kernel<TYPE, NK, true, PARTS>), dim3(grid), dim3(kThreads), 0, stream, a, p);    \
-        else                                                                                                            \
-            hipLaunchKernelGGL((attend_kernel<TYPE, NK, false, PARTS>), dim3(grid), dim3(kThreads), 0, stream, a, p);   \
+    const auto go = [&](auto kernel) { hipLaunchKernelGGL(kernel, dim3(grid), dim3(kThreads), 0, stream, a, p); };
+#define GOLLEK_ATTEND(NK)                                                      \
+    case NK:                                                                   \
+        if (p.share == 1) {                                                    \
+            if (dim == 32 * NK) go(attend_kernel<TYPE, NK, true, PARTS, 1>);   \
+            else go(attend_kernel<TYPE, NK, false, PARTS, 1>);                 \
+        } else {                                                               \
+            if (dim == 32 * NK) go(attend_kernel<TYPE, NK, true, PARTS, kWaves>); \
+            else go(attend_kernel<TYPE, NK, false, PARTS, kWaves>);            \
+        }                                                                      \
         break
     switch ((dim + 31) / 32) {
         GOLLEK_ATTEND(1);
@@ -604,7 +670,8 @@ hipError_t launch_attend(const AttendArgs &a, uint8_t *workspace, hipStream_t st
     AttendPlan p = make_plan(a.kv, a.sequences, a.q_heads, a.max_pages, a.window);
     (void)lay_out(p, a.kv, a.sequences, a.q_heads, workspace);
     p.q_vec = ((reinterpret_cast<uintptr_t>(a.q) | (uintptr_t)(a.q_stride * 2)) & 15u) == 0;
-    const int64_t units = ((int64_t)p.items * a.kv.kv_heads + 7) / 8 * 8, grid = units * p.row_tiles;
+    const int64_t units = (int64_t)p.items * a.kv.kv_heads;
+    const int64_t grid = p.share == 1 ? (units * p.row_tiles + kWaves - 1) / kWaves : (units + 7) / 8 * 8 * p.row_tiles;
     if (grid > 0x7FFFFFFF) return hipErrorInvalidValue;
     const int dim = a.kv.head_dim;
     if (a.kv.type == kF16) launch<kF16, 2>(dim, a, p, (unsigned)grid, stream);

@@ -943,6 +943,8 @@ class KvCache:
                stream: int = 0) -> None:
         """New tokens' keys (normalised, rotated) and values into their pages, their
         queries (normalised, rotated) to q_out (gollek_hip_kv_append_device)."""
+        if rope is not None and not rope.handle:
+            raise NullPointerError("rotary table")  # a closed one: not the call without rotation
         err = _native.err_buf()
         check(_native.load().gollek_hip_kv_append_device(
             self.handle, None if rope is None else rope.handle, k_ptr, k_stride, v_ptr, v_stride, q_ptr, q_heads,

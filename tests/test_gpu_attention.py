@@ -188,6 +188,34 @@ def test_few_long_among_many(sequences, kv_heads, dim):
     Batch(lengths, 2 * kv_heads, kv_heads, dim, BF16, page=64, seed=sequences).check(F32, rows)
 
 
+@pytest.mark.parametrize("q_heads,kv_heads,dim", [(16, 8, 64), (8, 8, 128), (24, 8, 80), (8, 8, 256), (16, 8, 192), (136, 8, 40),
+                                                  (32, 8, 24), (8, 8, 8)])
+@pytest.mark.parametrize("cache_type,out_type", [(BF16, F32), (F16, BF16), (BF16, F16)])
+def test_many_short_sequences(q_heads, kv_heads, dim, cache_type, out_type):
+    # enough heads of so few tokens that each is a wave's
+    sequences = 260
+    lengths = [(13 * i) % 150 for i in range(sequences)]
+    rows = [0, 1, 2, 5, 11, 12, 23, 100, 101, 258, 259]
+    b = Batch(lengths, q_heads, kv_heads, dim, cache_type, page=32, seed=dim)
+    b.check(out_type, rows)
+    b.check(out_type, rows, sinks=normal(rng(dim), q_heads, sigma=2.0).cuda(), softcap=10.0)
+    b = Batch([7 * x for x in lengths], q_heads, kv_heads, dim, cache_type, page=16, window=100, seed=dim)
+    b.table[11, 2 * 11] = -1
+    b.device().check(out_type, rows)
+
+
+def test_many_short_sequences_in_strided_rows():
+    lengths = [(13 * i) % 90 for i in range(1030)]
+    b = Batch(lengths, 4, 2, 64, BF16, seed=33)
+    for out_type, shift in ((F32, 1), (BF16, 3), (F16, 8)):
+        out = torch.full((1030 * 301 + 8,), float("nan"), dtype=DTYPE[out_type], device="cuda")
+        b.attend(out_type, out=out[shift:], out_stride=301)
+        torch.cuda.synchronize()
+        rows = out[shift:shift + 1030 * 301].view(1030, 301)
+        b.compare(rows[:, :256].reshape(1030, 4, 64), out_type, range(0, 1030, 41))
+        assert torch.isnan(rows[:, 256:]).all() and torch.isnan(out[:shift]).all() and not torch.isnan(rows[:, :256]).any()
+
+
 def test_lengths_past_the_table_and_below_zero():
     b = Batch([64, 64, 64, 64], 4, 2, 64, BF16, seed=18)
     b.lengths = [65, 2**31 - 1, -5, -(2**31)]

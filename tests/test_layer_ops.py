@@ -197,6 +197,17 @@ def test_append_refuses_null(kw):
         append(c, type_id=2)
 
 
+def test_append_refuses_a_closed_table():
+    rope = ops.Rope.__new__(ops.Rope)
+    rope.handle, rope.dims = None, 64
+    with pytest.raises(ops.NullPointerError):
+        append(cache(), rope=rope)
+    closed = cache()
+    closed.close()
+    with pytest.raises(ops.NullPointerError):
+        append(closed)
+
+
 def test_append_and_attend_refuse_a_null_cache():
     lib, e = _native.load(), _native.ErrBuf()
     assert lib.gollek_hip_kv_append_device(None, None, None, 0, None, 0, None, 0, 0, F32, 0, None, None, 0.0, None, None,

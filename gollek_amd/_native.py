@@ -128,6 +128,8 @@ _lib: ctypes.CDLL | None = None
 def load() -> ctypes.CDLL:
     """Load the library and declare every signature; raises if absent."""
     global _lib
+    if _lib is not None:  # (set once, complete: every call of an entry comes here)
+        return _lib
     with _lock:
         if _lib is not None:
             return _lib

@@ -26,11 +26,11 @@
 // (2.04e-3 against 1.65e-3 at 700 tokens) and saves nothing, the matrix cores being idle
 // nine tenths of the time.
 //
-// Bound by bytes: 64 sequences of up to 8192 tokens of 8 heads of 128 217 us (1.37 GB, 6.3
-// TB/s; reads alone outrun a copy's 5.0), one of 131072 of 4 heads 44.0 (268 MB, 6.1
-// TB/s) and 4.8 for the join.  Loads that do not stay in the caches give an eighth of
-// that (plain ones: 246 and 51).  Short sequences are bound by what a CU takes in (60 GB/s)
-// and the chain length, page, keys: 700 tokens 10.4.
+// Bound by bytes: 64 sequences of up to 8192 tokens of 8 heads of 128 219 us (1.37 GB, 6.2
+// TB/s; reads alone outrun a copy's 5.0), one of 131072 of 4 heads 41.2 (268 MB, 6.5
+// TB/s) and 4.8 for the join.  Short sequences are bound by a step's latency and what a CU
+// takes in, a microsecond for the 64 KB of its four waves, whatever the number of steps
+// ahead, waves or dims it is asked for: 700 tokens 10.4.
 //
 // A sequence's tiles are cut into chunks of equal size for workgroups that share the chip
 // evenly whatever the lengths are: every workgroup adds up the batch's tiles, takes the
@@ -52,9 +52,9 @@ typedef float f32x4 __attribute__((ext_vector_type(4)));
 constexpr int kWaves = 4, kThreads = 64 * kWaves;
 constexpr int kTile = 32;           // keys of a step
 constexpr int kRows = 16;           // query heads of a workgroup
-// Tiles of a chunk at least: a step a wave.  (A CU takes in some 60 GB/s, 64 KB a step's
-// round of its four waves, so a short sequence is as fast as it has CUs: 700 tokens of 8
-// heads in chunks of 8 tiles 7.0 us, of 4 6.2, of 2 5.7, to which a join adds 4.3 to 4.5.)
+// Tiles of a chunk at least: a step a wave.  (A short sequence is as fast as it has CUs:
+// 700 tokens of 8 heads in chunks of 8 tiles 7.0 us, of 4 6.2, of 2 5.7, to which a join
+// adds 4.3 to 4.5.)
 constexpr int kLeast = 4;
 // Tables of no more tiles than this are not cut at all, which saves the second launch:
 // with workgroups for fewer than 256 CUs (700 tokens, 22 tiles: 10.5 us whole, 6.2 and 4.3
@@ -217,7 +217,10 @@ __device__ __forceinline__ void store_run(void *p, int type, int64_t i, const fl
     }
 }
 
-// Keys and values are used once a call: loads that do not stay in the caches.
+// Values are used once a call: loads that do not stay in the caches.  Keys are too, but an
+// instruction takes 64 bytes of each of 16 rows, half a line, and the next one the other
+// half: streaming loads fetch it twice (16 sequences of up to 8192, heads of 80: 49 us with
+// both streaming, 37 with values alone, 43 with neither; 64 of heads of 128 219, 219, 242).
 template <class T>
 __device__ __forceinline__ T stream(const T *p) {
     return __builtin_nontemporal_load(p);
@@ -325,7 +328,7 @@ __global__ __launch_bounds__(kThreads, NK <= 2 ? 4 : NK <= 6 ? 2 : 1) void atten
             const uint8_t *const base = static_cast<const uint8_t *>(a.kv.k) + (at[h] < 0 ? nowhere : at[h]);
 #pragma unroll
             for (int i = 0; i < NK; i++)
-                k.word[h][i] = stream(reinterpret_cast<const u32x4 *>(base + (i < NK - 1 ? k_lane + 64 * i : k_last)));
+                k.word[h][i] = *reinterpret_cast<const u32x4 *>(base + (i < NK - 1 ? k_lane + 64 * i : k_last));
         }
     };
     const auto load_values = [&](const int64_t (&at)[2]) {

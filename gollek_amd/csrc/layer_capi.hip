@@ -595,7 +595,8 @@ int32_t gollek_hip_attention_device(const gollek_hip_kv_cache *cache, const void
                     out_type);
     int32_t rc = check_attention(cache, sequences, q_heads, max_pages, err, err_len);
     if (rc != GOLLEK_HIP_OK) return rc;
-    if (!isfinite(scale) || !(softcap >= 0.0f) || !isfinite(softcap) || window < 0)
+    // (the kernel takes scale / softcap and both times log2 e: none may overflow)
+    if (!(fabsf(scale) <= 1e15f) || !(softcap == 0.0f || (softcap >= 1e-15f && softcap <= 1e15f)) || window < 0)
         return fail(GOLLEK_HIP_ERR_ARG, err, err_len, "The attention's scale %g, cap %g or window %lld is out of range",
                     (double)scale, (double)softcap, (long long)window);
     const int64_t dim = cache->pages.head_dim;

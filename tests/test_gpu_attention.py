@@ -216,6 +216,29 @@ def test_many_short_sequences_in_strided_rows():
         assert torch.isnan(rows[:, 256:]).all() and torch.isnan(out[:shift]).all() and not torch.isnan(rows[:, :256]).any()
 
 
+def test_tables_much_wider_than_the_lengths():
+    # cut by the lengths, not by the table
+    for lengths in ([5, 700, 0], [3000], [0, 0, 0, 0], [0], [1, 2, 3]):
+        b = Batch(lengths, 8, 2, 128, BF16, max_pages=5000, seed=34)
+        b.check(F32)
+        b.check(BF16, sinks=normal(rng(35), 8).cuda())
+
+
+def test_one_large_page_a_sequence():
+    b = Batch([65536, 1, 40001], 4, 1, 64, F16, page=65536, seed=36)
+    b.check(F32)
+    Batch([65536, 70, 40001], 4, 1, 64, F16, page=65536, window=50, seed=36).check(F32)
+
+
+@pytest.mark.parametrize("scale,softcap", [(1e15, 1e-15), (1e-15, 1e15), (0.125, 1e15), (0.125, 1e-15)])
+def test_extreme_scales(scale, softcap):
+    # weights alike, or the largest score's alone: nothing overflows on the way
+    b = Batch([40, 300], 4, 2, 64, BF16, seed=37)
+    out = b.attend(F32, scale=scale, softcap=softcap)
+    torch.cuda.synchronize()
+    assert torch.isfinite(out).all()
+
+
 def test_lengths_past_the_table_and_below_zero():
     b = Batch([64, 64, 64, 64], 4, 2, 64, BF16, seed=18)
     b.lengths = [65, 2**31 - 1, -5, -(2**31)]

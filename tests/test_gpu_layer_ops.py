@@ -138,7 +138,7 @@ def test_norm_rows_of_zeros_and_infinities():
     assert abs(y[3, 7].item() - 2.0 / np.sqrt(4.0 / 96 + 1e-6)) < 1e-5 and torch.all(y[3, :7] == 0)
 
 
-@pytest.mark.parametrize("cols", [2880, 77])
+@pytest.mark.parametrize("cols", [2880, 77, 10000, 20001])
 def test_norm_in_place(cols):
     g = rng(20)
     x, r = normal(g, 9, cols).cuda(), normal(g, 9, cols).cuda()
@@ -388,6 +388,26 @@ def test_append_without_queries_rotation_or_fusion():
     run_append(6, 4, 2, 64, F32, BF16, rope=False, seed=51)
     run_append(6, 4, 2, 64, F32, BF16, rope=False, normed=True, fused=False, seed=52)
     run_append(6, 4, 2, 64, F16, BF16, fused=False, seed=53)
+
+
+def test_append_to_strided_queries():
+    g = rng(58)
+    tokens, heads, dim = 5, 4, 64
+    k, v = (torch.zeros(6, 1, 16, dim, dtype=torch.bfloat16, device="cuda") for _ in range(2))
+    cache = ops.KvCache(BF16, ptr(k), ptr(v), 6, 16, 1, dim)
+    src = normal(g, tokens, heads + 2, dim).cuda()
+    at, pages = torch.arange(tokens, dtype=torch.int32).cuda(), torch.arange(5, dtype=torch.int32).cuda()
+    out = torch.full((tokens * 301 + 8,), float("nan"), dtype=torch.bfloat16, device="cuda")
+    rope, angles = table(dim)
+    stride = (heads + 2) * dim
+    cache.append(ptr(src) + heads * dim * 4, ptr(src) + (heads + 1) * dim * 4, F32, tokens, ptr(at), ptr(pages), 5, 1, rope=rope,
+                 k_stride=stride, v_stride=stride, q_ptr=ptr(src), q_heads=heads, q_stride=stride, q_out_ptr=ptr(out) + 6,
+                 q_out_stride=301, stream=stream())
+    torch.cuda.synchronize()
+    rows = out[3:3 + tokens * 301].view(tokens, 301)
+    want, off = ref.rotate(src[:, :heads], at, angles, 1.0, False)
+    close(rows[:, :heads * dim].reshape(tokens, heads, dim), want, off, BF16)
+    assert int(torch.isnan(out).sum()) == out.numel() - tokens * heads * dim
 
 
 @pytest.mark.parametrize("type_id", [F16, BF16])

@@ -229,7 +229,7 @@ def attend(c, **kw):
     dict(sequences=-1), dict(sequences=65536), dict(q_heads=0), dict(q_heads=3), dict(q_heads=65536),
     dict(sequences=65535, q_heads=512), dict(max_pages=0), dict(max_pages=1 << 27), dict(scale=float("nan")),
     dict(scale=float("inf")), dict(softcap=-1.0), dict(softcap=float("nan")), dict(softcap=float("inf")),
-    dict(window=-1), dict(q_stride=255), dict(out_stride=255), dict(q_ptr=BASE + (4 << 20) + 1),
+    dict(scale=2e15), dict(scale=-1e30), dict(softcap=1e-30), dict(softcap=1e20), dict(window=-1), dict(q_stride=255), dict(out_stride=255), dict(q_ptr=BASE + (4 << 20) + 1),
     dict(out_ptr=BASE + (7 << 20) + 2), dict(lengths_ptr=BASE + (5 << 20) + 2), dict(sinks_ptr=BASE + (8 << 20) + 1),
     dict(out_ptr=BASE + (4 << 20), out_type=BF16), dict(out_ptr=BASE + 256), dict(out_ptr=BASE + (1 << 20)),
     dict(out_ptr=BASE + (5 << 20)), dict(out_ptr=BASE + (6 << 20)), dict(sinks_ptr=BASE + (7 << 20)),

@@ -62,11 +62,15 @@ constexpr int kLeast = 4;
 // and 4.0; of 2000, 63 tiles: 36.4, 31.5 and 4.6).
 constexpr int kWholeFew = 24, kWholeMany = 32, kFew = 256;
 // Many units of few tiles take a wave each, which saves their join through LDS and the
-// idle waves (256 sequences in a window of 128, 64 / 8 heads of 64: 17.5 us, by
-// workgroups 20.2; 1000 of up to 60, 16 / 4 of 128: 24.0, 28.5).  From eight tiles on, or
-// with fewer waves than the chip holds, it loses (256 of up to 256, 32 / 8 of 128: 38.4,
-// 33.8; 32 of up to 300: 20.5, 9.1).
-constexpr int kAloneTiles = 6, kAloneUnits = 2048;
+// waves that have no tile: from where workgroups would need more than a round, of `resident`
+// a CU (their registers), up to 6 tiles, or 10 where one is resident.  Measured by
+// workgroups and by waves, us: heads of 128, one tile, 512 units 5.1 and 5.4, 1024 8.1 and
+// 5.6, 2000 13.1 and 7.7; six tiles 1024 15.9 and 15.5, 2000 24.2 and 25.5; heads of 256,
+// one tile, 512 11.4 and 8.6, 2000 43 and 17.7; six 768 28 and 24, 2000 72 and 55; twelve 768
+// 41 and 43.
+constexpr int resident(int head_dim) { return head_dim <= 64 ? 4 : head_dim <= 128 ? 3 : head_dim <= 192 ? 2 : 1; }
+constexpr int alone_tiles(int head_dim) { return resident(head_dim) == 1 ? 10 : 6; }
+constexpr int alone_units(int head_dim, int64_t tiles) { return 256 * (resident(head_dim) + (tiles <= 2 ? 1 : 2)); }
 // Workgroups that a batch is cut into: one for every CU and sequence, up to kTargetMost.
 // The chunks of one sequence are all alike, and one round of them does best (131072 tokens
 // of 4 heads of 128, main kernel and join: 44.1 + 4.8 us, in 512 44.5 + 5.3, in 768 45.1 +
@@ -299,11 +303,9 @@ __global__ __launch_bounds__(kThreads, NK <= 2 ? 4 : NK <= 6 ? 2 : 1) void atten
 
     // where a lane reads in a tile of 16 keys, in bytes: its key's row for K, four
     // rows for V (dims past the head's read its first ones, and are not used)
-    const uint32_t k_lane = (uint32_t)(c * dim + 8 * g) * 2;
     const bool k_rest = !EXACT && 32 * (NK - 1) + 8 * g >= dim;
-    const uint32_t k_last = k_rest ? (uint32_t)(c * dim) * 2 : k_lane + 64 * (NK - 1);
-    const uint32_t v_lane0 = (uint32_t)(4 * g * dim + (D::kWide0 * c < dim ? D::kWide0 * c : 0)) * 2;
-    const uint32_t v_lane1 = (uint32_t)(4 * g * dim + (128 + D::kWide1 * c < dim ? 128 + D::kWide1 * c : 0)) * 2;
+    const uint32_t v_col0 = (uint32_t)(D::kWide0 * c < dim ? D::kWide0 * c : 0) * 2;
+    const uint32_t v_col1 = (uint32_t)(128 + D::kWide1 * c < dim ? 128 + D::kWide1 * c : 0) * 2;
 
     const auto table = reinterpret_cast<const __attribute__((address_space(4))) int32_t *>(
         reinterpret_cast<uintptr_t>(a.page_table + (int64_t)it.sequence * a.max_pages));
@@ -322,37 +324,50 @@ __global__ __launch_bounds__(kThreads, NK <= 2 ? 4 : NK <= 6 ? 2 : 1) void atten
 
     KeyTile<NK> k;
     ValueTile<NK> v;
-    const auto load_keys = [&](const int64_t (&at)[2]) {
+    // The first and last row of a half of a tile that are a sequence's; where there are not
+    // all, the others' lanes read one of these (a page's other rows are no part of the call).
+    const auto rows_of = [&](int key, bool there, int &lo, int &hi) {
+        lo = there ? max(span.begin - key, 0) : 0;
+        hi = there ? min(span.length - key, 16) - 1 : 0;
+    };
+    const auto load_keys = [&](const int64_t (&at)[2], int key) {
 #pragma unroll
         for (int h = 0; h < 2; h++) {
             const uint8_t *const base = static_cast<const uint8_t *>(a.kv.k) + (at[h] < 0 ? nowhere : at[h]);
+            int lo, hi;
+            rows_of(key + 16 * h, at[h] >= 0, lo, hi);
+            const uint32_t row = (uint32_t)(min(max(c, lo), hi) * dim) * 2, off = row + 16 * g;
 #pragma unroll
             for (int i = 0; i < NK; i++)
-                k.word[h][i] = *reinterpret_cast<const u32x4 *>(base + (i < NK - 1 ? k_lane + 64 * i : k_last));
+                k.word[h][i] = *reinterpret_cast<const u32x4 *>(base + (i < NK - 1 || !k_rest ? off + 64 * i : row));
         }
     };
-    const auto load_values = [&](const int64_t (&at)[2]) {
+    const auto load_run = [&](uint32_t *w, const uint8_t *from, auto WIDE) {
+        if constexpr (decltype(WIDE)::value == 8) {
+            const u32x4 x = stream(reinterpret_cast<const u32x4 *>(from));
+            w[0] = x[0], w[1] = x[1], w[2] = x[2], w[3] = x[3];
+        } else if constexpr (decltype(WIDE)::value == 4) {
+            const u32x2 x = stream(reinterpret_cast<const u32x2 *>(from));
+            w[0] = x[0], w[1] = x[1];
+        }
+    };
+    const auto load_values = [&](const int64_t (&at)[2], int key) {
 #pragma unroll
         for (int h = 0; h < 2; h++) {
             const uint8_t *const base = static_cast<const uint8_t *>(a.kv.v) + (at[h] < 0 ? nowhere : at[h]);
+            int lo, hi;
+            rows_of(key + 16 * h, at[h] >= 0, lo, hi);
+            uint32_t row[4];
+#pragma unroll
+            for (int j = 0; j < 4; j++) row[j] = (uint32_t)((4 * g + j) * dim) * 2;
+            if (lo > 0 || hi < 15) {
+#pragma unroll
+                for (int j = 0; j < 4; j++) row[j] = (uint32_t)(min(max(4 * g + j, lo), hi) * dim) * 2;
+            }
 #pragma unroll
             for (int j = 0; j < 4; j++) {
-                uint32_t *const w = v.word[4 * h + j];
-                const uint32_t off = v_lane0 + (uint32_t)(2 * j * dim);
-                if constexpr (D::kWide0 == 8) {
-                    const u32x4 x = stream(reinterpret_cast<const u32x4 *>(base + off));
-                    w[0] = x[0], w[1] = x[1], w[2] = x[2], w[3] = x[3];
-                } else {
-                    const u32x2 x = stream(reinterpret_cast<const u32x2 *>(base + off));
-                    w[0] = x[0], w[1] = x[1];
-                }
-                if constexpr (D::kWide1 == 8) {
-                    const u32x4 x = stream(reinterpret_cast<const u32x4 *>(base + v_lane1 + (uint32_t)(2 * j * dim)));
-                    w[4] = x[0], w[5] = x[1], w[6] = x[2], w[7] = x[3];
-                } else if constexpr (D::kWide1 == 4) {
-                    const u32x2 x = stream(reinterpret_cast<const u32x2 *>(base + v_lane1 + (uint32_t)(2 * j * dim)));
-                    w[4] = x[0], w[5] = x[1];
-                }
+                load_run(v.word[4 * h + j], base + row[j] + v_col0, std::integral_constant<int, D::kWide0>{});
+                load_run(v.word[4 * h + j] + D::kWide0 / 2, base + row[j] + v_col1, std::integral_constant<int, D::kWide1>{});
             }
         }
     };
@@ -387,7 +402,7 @@ __global__ __launch_bounds__(kThreads, NK <= 2 ? 4 : NK <= 6 ? 2 : 1) void atten
         if constexpr (more) {
             tile += SHARE;
             at[0] = place(page[0], kTile * tile), at[1] = place(page[1], kTile * tile + 16);
-            load_keys(at);
+            load_keys(at, kTile * tile);
             pages_of(min(tile + SHARE, tile1 - 1), page);
         }
         float x[8];
@@ -451,13 +466,13 @@ __global__ __launch_bounds__(kThreads, NK <= 2 ? 4 : NK <= 6 ? 2 : 1) void atten
 #pragma unroll
             for (int n = 0; n < PARTS; n++) o[i] = mfma(t, p[n], o[i], type);
         }
-        if constexpr (more) load_values(at);
+        if constexpr (more) load_values(at, kTile * tile);
     };
     if (tile < tile1) {
         pages_of(tile, page);
         at[0] = place(page[0], kTile * tile), at[1] = place(page[1], kTile * tile + 16);
-        load_keys(at);
-        load_values(at);
+        load_keys(at, kTile * tile);
+        load_values(at, kTile * tile);
         pages_of(min(tile + SHARE, tile1 - 1), page);
 #pragma unroll
         for (int i = 0; i < NK; i++)
@@ -614,7 +629,8 @@ AttendPlan make_plan(const KvPages &kv, int sequences, int q_heads, int64_t max_
     if (window > 0 && tiles > window / kTile + 2) tiles = window / kTile + 2;
     p.items = sequences;
     const int64_t per = (int64_t)kv.kv_heads * p.row_tiles;
-    p.share = tiles <= kAloneTiles && sequences * per >= kAloneUnits ? 1 : kWaves;
+    const bool alone = tiles <= alone_tiles(kv.head_dim) && sequences * per >= alone_units(kv.head_dim, tiles);
+    p.share = alone ? 1 : kWaves;
     if (sequences > kScanMost || tiles <= (sequences * per < kFew ? kWholeFew : kWholeMany)) return p;  // a chunk a sequence
     const int target = sequences < kTargetMost / kTargetEach ? sequences * kTargetEach : kTargetMost;
     const int slots = (int)(per < target ? target / per : 1);

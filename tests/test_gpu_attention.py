@@ -204,6 +204,16 @@ def test_many_short_sequences(q_heads, kv_heads, dim, cache_type, out_type):
     b.device().check(out_type, rows)
 
 
+@pytest.mark.parametrize("dim", [64, 128, 192, 256])
+@pytest.mark.parametrize("most", [9, 60, 180, 300, 340])
+def test_short_sequences_around_the_rules(dim, most):
+    # units on both sides of the border between a workgroup and a wave each
+    for sequences in (63, 64, 95, 96, 127, 128, 160, 192):
+        lengths = [(29 * i) % (most + 1) for i in range(sequences)]
+        lengths[-1] = most
+        Batch(lengths, 8, 8, dim, BF16, page=64, seed=dim + sequences).check(BF16, [0, 1, sequences // 2, sequences - 1])
+
+
 def test_many_short_sequences_in_strided_rows():
     lengths = [(13 * i) % 90 for i in range(1030)]
     b = Batch(lengths, 4, 2, 64, BF16, seed=33)

@@ -55,20 +55,27 @@ constexpr int kRows = 16;           // query heads of a workgroup
 // Tiles of a chunk at least: a step a wave.  (A short sequence is as fast as it has CUs:
 // 700 tokens of 8 heads in chunks of 8 tiles 7.0 us, of 4 6.2, of 2 5.7, to which a join
 // adds 4.3 to 4.5.)
-constexpr int kLeast = 4;
-// Tables of no more tiles than this are not cut at all, which saves the second launch:
-// with workgroups for fewer than 256 CUs (700 tokens, 22 tiles: 10.5 us whole, 6.2 and 4.3
-// cut; 1000, 32 tiles: 13.1, 6.2 and 4.4), and with more (32 sequences of 1000: 20.0, 20.5
-// and 4.0; of 2000, 63 tiles: 36.4, 31.5 and 4.6).
-constexpr int kWholeFew = 24, kWholeMany = 32, kFew = 256;
+// Where every CU has a workgroup, kSome: three steps a wave (16 sequences of up to 2048, 8
+// heads of 128, with the join: chunks of 4 23.0 us, 8 20.8, 12 20.4, 16 22.1; heads of 256
+// 53, 41, 39, 39).
+constexpr int kLeast = 4, kSome = 12;
+// Workgroups of the kernel that a CU holds, by the registers of its head size.
+constexpr int resident(int head_dim) { return head_dim <= 64 ? 4 : head_dim <= 128 ? 3 : head_dim <= 192 ? 2 : 1; }
+// Tables of no more tiles than this are not cut at all, which saves the second launch and
+// its wait.  With units (key heads of the batch) for fewer than the 256 CUs, us cut and
+// whole: 8 heads of 64, 24 tiles 8.5 and 7.7, 32 8.4 and 9.1; of 128, 20 9.3 and 9.1, 24
+// 9.3 and 10.1 (but one launch of the caller's less); of 192, 12 10.6 and 9.5, 16 10.7 and
+// 11.3; of 256, 12 11.9 and 11.9.  With more, ragged lengths: 256 heads of 128, 32 23.0 and
+// 17.9, 48 27.0 and 24.6, 96 51.2 and 49.2; of 256, 48 58 and 51 (a single long sequence
+// among them costs a step of 1 to 2 us for every four tiles, hence no further).
+constexpr int whole_few(int head_dim) { return resident(head_dim) == 1 ? 12 : 8 * resident(head_dim); }
+constexpr int kWholeMany = 48, kFew = 256;
 // Many units of few tiles take a wave each, which saves their join through LDS and the
-// waves that have no tile: from where workgroups would need more than a round, of `resident`
-// a CU (their registers), up to 6 tiles, or 10 where one is resident.  Measured by
+// waves that have no tile: from where workgroups would need more than a round, up to 6 tiles, or 10 where one is resident.  Measured by
 // workgroups and by waves, us: heads of 128, one tile, 512 units 5.1 and 5.4, 1024 8.1 and
 // 5.6, 2000 13.1 and 7.7; six tiles 1024 15.9 and 15.5, 2000 24.2 and 25.5; heads of 256,
 // one tile, 512 11.4 and 8.6, 2000 43 and 17.7; six 768 28 and 24, 2000 72 and 55; twelve 768
 // 41 and 43.
-constexpr int resident(int head_dim) { return head_dim <= 64 ? 4 : head_dim <= 128 ? 3 : head_dim <= 192 ? 2 : 1; }
 constexpr int alone_tiles(int head_dim) { return resident(head_dim) == 1 ? 10 : 6; }
 constexpr int alone_units(int head_dim, int64_t tiles) { return 256 * (resident(head_dim) + (tiles <= 2 ? 1 : 2)); }
 // Workgroups that a batch is cut into: one for every CU and sequence, up to kTargetMost.
@@ -84,8 +91,10 @@ constexpr float kLog2e = 1.4426950408889634f;
 
 struct AttendPlan {
     int row_tiles;  // workgroups for the query heads of one key head
-    int slots;      // chunks of a key head that the batch is cut into (0: a chunk a sequence)
-    int items;      // chunks at most
+    bool whole;     // a chunk a sequence
+    int slots;      // chunks of a key head that the batch is cut into
+    int few;        // chunks of a key head that give every CU a workgroup
+    int items;      // chunks at most, and one for every sequence
     int share;      // waves that share a unit (one key head of a chunk, up to kRows query heads)
     bool q_vec;     // queries on 16-byte borders
     // workspace: a chunk's sums, (bound, weight) for each query head, and a sequence's
@@ -148,7 +157,9 @@ __device__ __forceinline__ bool find_item(const AttendArgs &a, const AttendPlan 
         if (s < a.sequences) total += (float)span_of(a, s0 == 0 ? length0 : a.lengths[s]).tiles;
     }
     total = __int_as_float(lane_of(__float_as_int(prefix_sum(total)), 63));
-    const int each = max(kLeast, (int)fminf(total / (float)p.slots * 1.00001f, 1.0e9f) + 1);
+    // (the first bound keeps the chunks within the workspace)
+    const int each = max(max(kLeast, (int)fminf(total / (float)p.slots * 1.00001f, 1.0e9f) + 1),
+                         min(kSome, (int)fminf(total / (float)p.few, 1.0e9f)));
     int before = 0;
     for (int s0 = 0; s0 < a.sequences; s0 += 64) {
         const int s = s0 + lane;
@@ -269,7 +280,7 @@ __global__ __launch_bounds__(kThreads, NK <= 2 ? 4 : NK <= 6 ? 2 : 1) void atten
     }
     const int item = unit / a.kv.kv_heads, kv_head = unit % a.kv.kv_heads;
     Item it = {item, 0, 0, 1};
-    if (SHARE > 1 && plan.slots > 0) {
+    if (SHARE > 1 && !plan.whole) {
         if (!find_item(a, plan, item, lane, it)) return;
         if (it.chunk == 0 && kv_head == 0 && row_tile == 0 && threadIdx.x == 0)
             plan.joins[it.sequence] = make_int2(item, it.chunks);
@@ -627,16 +638,17 @@ AttendPlan make_plan(const KvPages &kv, int sequences, int q_heads, int64_t max_
     p.row_tiles = (q_heads / kv.kv_heads + kRows - 1) / kRows;
     int64_t tiles = ((max_pages << kv.page_shift) + kTile - 1) / kTile;
     if (window > 0 && tiles > window / kTile + 2) tiles = window / kTile + 2;
-    p.items = sequences;
-    const int64_t per = (int64_t)kv.kv_heads * p.row_tiles;
-    const bool alone = tiles <= alone_tiles(kv.head_dim) && sequences * per >= alone_units(kv.head_dim, tiles);
-    p.share = alone ? 1 : kWaves;
-    if (sequences > kScanMost || tiles <= (sequences * per < kFew ? kWholeFew : kWholeMany)) return p;  // a chunk a sequence
-    const int target = sequences < kTargetMost / kTargetEach ? sequences * kTargetEach : kTargetMost;
-    const int slots = (int)(per < target ? target / per : 1);
-    p.slots = slots;
-    const int64_t most = sequences * ((tiles + kLeast - 1) / kLeast);
-    p.items = (int)(most < sequences + slots ? most : sequences + slots);
+    const int64_t per = (int64_t)kv.kv_heads * p.row_tiles, units = sequences * per;
+    p.share = tiles <= alone_tiles(kv.head_dim) && units >= alone_units(kv.head_dim, tiles) ? 1 : kWaves;
+    p.whole = sequences > kScanMost || tiles <= (units < kFew ? whole_few(kv.head_dim) : kWholeMany);
+    // the largest cut, also where this call is not cut: the workspace is asked for by it,
+    // and must not shrink where more sequences fall under another rule
+    const int n = sequences < kScanMost ? sequences : kScanMost;
+    const int target = n < kTargetMost / kTargetEach ? n * kTargetEach : kTargetMost;
+    p.slots = (int)(per < target ? target / per : 1);
+    p.few = (int)(per < kTargetEach ? kTargetEach / per : 1);
+    const int64_t most = n * ((tiles + kLeast - 1) / kLeast);
+    p.items = tiles <= whole_few(kv.head_dim) ? 0 : (int)(most < n + p.slots ? most : n + p.slots);
     return p;
 }
 
@@ -668,19 +680,18 @@ void launch(int dim, const AttendArgs &a, const AttendPlan &p, unsigned grid, hi
 
 // Bytes of the workspace's parts; p's pointers where there is one.
 size_t lay_out(AttendPlan &p, const KvPages &kv, int sequences, int q_heads, uint8_t *workspace) {
-    if (p.slots == 0) return 0;
+    if (p.items == 0) return 0;
     const size_t rows = (size_t)p.items * (size_t)q_heads, o = rows * (size_t)kv.head_dim * sizeof(float);
+    const size_t joins = (size_t)(sequences < kScanMost ? sequences : kScanMost) * sizeof(int2);
     p.part_o = reinterpret_cast<float *>(workspace);
     p.part_ml = reinterpret_cast<float2 *>(workspace + o);
     p.joins = reinterpret_cast<int2 *>(workspace + o + rows * sizeof(float2));
-    return (o + rows * sizeof(float2) + (size_t)sequences * sizeof(int2) + 255) / 256 * 256;
+    return (o + rows * sizeof(float2) + joins + 255) / 256 * 256;
 }
 
 }  // namespace
 
 size_t attend_workspace_bytes(const KvPages &kv, int sequences, int q_heads, int64_t max_pages) {
-    // (past kScanMost nothing is split; the size stays what the batch before needed)
-    if (sequences > kScanMost) sequences = kScanMost;
     AttendPlan p = make_plan(kv, sequences, q_heads, max_pages, 0);
     return lay_out(p, kv, sequences, q_heads, nullptr);
 }
@@ -689,7 +700,7 @@ hipError_t launch_attend(const AttendArgs &a, uint8_t *workspace, hipStream_t st
     AttendPlan p = make_plan(a.kv, a.sequences, a.q_heads, a.max_pages, a.window);
     (void)lay_out(p, a.kv, a.sequences, a.q_heads, workspace);
     p.q_vec = ((reinterpret_cast<uintptr_t>(a.q) | (uintptr_t)(a.q_stride * 2)) & 15u) == 0;
-    const int64_t units = (int64_t)p.items * a.kv.kv_heads;
+    const int64_t units = (int64_t)(p.whole ? a.sequences : p.items) * a.kv.kv_heads;
     const int64_t grid = p.share == 1 ? (units * p.row_tiles + kWaves - 1) / kWaves : (units + 7) / 8 * 8 * p.row_tiles;
     if (grid > 0x7FFFFFFF) return hipErrorInvalidValue;
     const int dim = a.kv.head_dim;
@@ -697,7 +708,7 @@ hipError_t launch_attend(const AttendArgs &a, uint8_t *workspace, hipStream_t st
     else if (a.out_type == kF32) launch<kBF16, 3>(dim, a, p, (unsigned)grid, stream);
     else launch<kBF16, 2>(dim, a, p, (unsigned)grid, stream);
     hipError_t e = hipGetLastError();
-    if (e == hipSuccess && p.slots > 0) {
+    if (e == hipSuccess && !p.whole) {
         const dim3 rows((unsigned)(a.sequences * a.q_heads));
         if (p.slots > 16 * a.sequences || p.slots > 1024) hipLaunchKernelGGL(join_kernel<16>, rows, dim3(1024), 0, stream, a, p);
         else if (p.slots <= 4 * a.sequences && p.slots <= 256) hipLaunchKernelGGL(join_kernel<1>, rows, dim3(64), 0, stream, a, p);

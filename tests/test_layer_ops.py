@@ -265,6 +265,13 @@ def test_attend_workspace():
     for n in (1, 8, 400):
         sizes = [c.attend_workspace_bytes(n, 4, p) for p in (1, 2, 9, 64, 1000, 100000)]
         assert sizes == sorted(sizes)
+    for dim in (8, 64, 128, 192, 256):
+        for page in (16, 64):
+            c = cache(head_dim=dim, page_size=page, v_ptr=BASE + (1 << 24), kv_heads=8)
+            table = [[c.attend_workspace_bytes(n, 16, p) for p in (1, 3, 5, 8, 15, 23, 25, 33, 49, 70, 97, 130, 500, 9000)]
+                     for n in (1, 2, 3, 5, 6, 9, 31, 32, 33, 64, 127, 256, 1023, 1024, 1025, 3000, 65535)]
+            assert all(row == sorted(row) for row in table) and all(list(col) == sorted(col) for col in zip(*table))
+    c = cache()
     assert c.attend_workspace_bytes(1, 3, 4) == -1 and c.attend_workspace_bytes(65536, 4, 4) == -1
 
 

@@ -71,11 +71,11 @@ constexpr int resident(int head_dim) { return head_dim <= 64 ? 4 : head_dim <= 1
 constexpr int whole_few(int head_dim) { return resident(head_dim) == 1 ? 12 : 8 * resident(head_dim); }
 constexpr int kWholeMany = 48, kFew = 256;
 // Many units of few tiles take a wave each, which saves their join through LDS and the
-// waves that have no tile: from where workgroups would need more than a round, up to 6 tiles, or 10 where one is resident.  Measured by
-// workgroups and by waves, us: heads of 128, one tile, 512 units 5.1 and 5.4, 1024 8.1 and
-// 5.6, 2000 13.1 and 7.7; six tiles 1024 15.9 and 15.5, 2000 24.2 and 25.5; heads of 256,
-// one tile, 512 11.4 and 8.6, 2000 43 and 17.7; six 768 28 and 24, 2000 72 and 55; twelve 768
-// 41 and 43.
+// waves that have no tile: from where workgroups would need more than a round, up to 6
+// tiles, or 10 where a CU holds one.  Measured by workgroups and by waves, us: heads of 128,
+// one tile, 512 units 5.1 and 5.4, 1024 8.1 and 5.6, 2000 13.1 and 7.7; six tiles 1024 15.9
+// and 15.5, 2000 24.2 and 25.5; heads of 256, one tile, 512 11.4 and 8.6, 2000 43 and 17.7;
+// six 768 28 and 24, 2000 72 and 55; twelve 768 41 and 43.
 constexpr int alone_tiles(int head_dim) { return resident(head_dim) == 1 ? 10 : 6; }
 constexpr int alone_units(int head_dim, int64_t tiles) { return 256 * (resident(head_dim) + (tiles <= 2 ? 1 : 2)); }
 // Workgroups that a batch is cut into: one for every CU and sequence, up to kTargetMost.
@@ -710,9 +710,16 @@ hipError_t launch_attend(const AttendArgs &a, uint8_t *workspace, hipStream_t st
     hipError_t e = hipGetLastError();
     if (e == hipSuccess && !p.whole) {
         const dim3 rows((unsigned)(a.sequences * a.q_heads));
-        if (p.slots > 16 * a.sequences || p.slots > 1024) hipLaunchKernelGGL(join_kernel<16>, rows, dim3(1024), 0, stream, a, p);
-        else if (p.slots <= 4 * a.sequences && p.slots <= 256) hipLaunchKernelGGL(join_kernel<1>, rows, dim3(64), 0, stream, a, p);
-        else hipLaunchKernelGGL(join_kernel<4>, rows, dim3(256), 0, stream, a, p);
+        // Waves of a row's join by the chunks it has on the average (most rows of a batch
+        // have one, and leave at once), and as many as it may have: 64 sequences of 64 heads
+        // by one wave each 4.9 us, four 8.0, sixteen 26.8; one of 64 chunks by one 5.4, four
+        // 4.8, sixteen 4.9, two of 128 by four 5.7, sixteen 5.0.
+        const auto go = [&](auto kernel, unsigned threads) {
+            hipLaunchKernelGGL(kernel, rows, dim3(threads), 0, stream, a, p);
+        };
+        if (p.slots > 16 * a.sequences || p.slots > 1024) go(join_kernel<16>, 1024);
+        else if (p.slots <= 4 * a.sequences && p.slots <= 256) go(join_kernel<1>, 64);
+        else go(join_kernel<4>, 256);
         e = hipGetLastError();
     }
     return e;

@@ -327,9 +327,10 @@ __global__ __launch_bounds__(kThreads, NK <= 2 ? 4 : NK <= 6 ? 2 : 1) void atten
     };
     // byte offset of 16 keys from `key` on, which lie in `page`; -1 where there is none
     const auto place = [&](int page, int key) -> int64_t {
-        const int64_t row = ((int64_t)page * a.kv.kv_heads + kv_head) << a.kv.page_shift;
+        const bool there = key < span.length && key + 15 >= span.begin && page >= 0 && page < a.kv.pages;
+        const int64_t row = ((int64_t)(there ? page : 0) * a.kv.kv_heads + kv_head) << a.kv.page_shift;
         const int64_t at = (row + (key & ((1 << a.kv.page_shift) - 1))) * dim * 2;
-        return key < span.length && key + 15 >= span.begin && page >= 0 && page < a.kv.pages ? at : -1;
+        return there ? at : -1;
     };
     const int64_t nowhere = (((int64_t)kv_head) << a.kv.page_shift) * dim * 2;  // (page 0: memory of the cache)
 

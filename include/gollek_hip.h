@@ -603,8 +603,8 @@ int32_t gollek_hip_kv_append_device(const gollek_hip_kv_cache *cache, const goll
  * there; a row without any token (or with every s_j -inf) is 0.  Nothing behind a sequence's length or before
  * its window changes a result, whatever it holds.  Several new tokens of one
  * sequence are rows of their own, with equal page_table rows and growing lengths.
- * Results depend in their last bits on the lengths in the batch (they set how the
- * sums are split), not on timing.  sequences and q_heads in [0, 65535] and
+ * Results depend in their last bits on the batch (its rows, lengths and table width set
+ * how the sums are split), not on timing.  sequences and q_heads in [0, 65535] and
  * [1, 65535], sequences * q_heads < 2^24, max_pages as above, scale in [-1e15, 1e15],
  * softcap 0 or in [1e-15, 1e15], window >= 0, workspace (256-byte aligned; calls sharing it must not
  * overlap) of at least gollek_hip_attention_workspace_bytes: else ARG. */

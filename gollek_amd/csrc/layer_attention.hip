@@ -21,10 +21,13 @@
 // row c.  No LDS in the loop; the next keys are loaded as soon as the scores have used the
 // registers, the next values behind the second product.
 //
-// Weights are rounded to the cache's type in PARTS pieces whose sum has 16 or more bits:
-// one piece of bf16 would put an error as large as the output's own rounding beside it
-// (2.04e-3 against 1.65e-3 at 700 tokens) and saves nothing, the matrix cores being idle
-// nine tenths of the time.
+// Weights enter the second product in pieces of the cache's type: three of bf16, together
+// an fp32 number's 24 bits, or two of fp16, 22 bits.  Two pieces of bf16 round four times as
+// many results otherwise than 64 bits do (0.18 % of them at 700 tokens, three 0.04 %, torch
+// in fp32 0.05 %); one puts an error as large as the output's own rounding beside it
+// (2.04e-3 against 1.65e-3).  The third costs nothing where bytes count, 2 % of a short
+// call (700 tokens 10.7 and 10.9 us), and most where 48 heads read the same keys (25.1 and
+// 29.6).
 //
 // Bound by bytes: 64 sequences of up to 8192 tokens of 8 heads of 128 219 us (1.37 GB, 6.2
 // TB/s; reads alone outrun a copy's 5.0), one of 131072 of 4 heads 41.2 (268 MB, 6.5
@@ -252,11 +255,11 @@ struct ValueTile {
 };
 
 // TYPE: of cache and queries.  NK: head_dim / 32, rounded up (EXACT: without a rest).
-// PARTS: the pieces a weight is split into, of 8 (bf16) or 11 (fp16) bits each.
-template <int TYPE, int NK, bool EXACT, int PARTS, int SHARE>
+template <int TYPE, int NK, bool EXACT, int SHARE>
 __global__ __launch_bounds__(kThreads, NK <= 2 ? 4 : NK <= 6 ? 2 : 1) void attend_kernel(AttendArgs a, AttendPlan plan) {
     using D = Dims<NK>;
     constexpr std::integral_constant<int, TYPE> type;
+    constexpr int kParts = TYPE == kBF16 ? 3 : 2;  // pieces of a weight, of 8 (bf16) or 11 (fp16) bits
     // fp16 weights: exp(s - m) times 2^7, so that all but the smallest are normal numbers
     // (2^15 with the slack, below fp16's largest)
     constexpr float kLift = TYPE == kF16 ? 7.0f : 0.0f;
@@ -463,9 +466,9 @@ __global__ __launch_bounds__(kThreads, NK <= 2 ? 4 : NK <= 6 ? 2 : 1) void atten
             x[j] = __builtin_amdgcn_exp2f(x[j] - base);
             l += x[j];
         }
-        u32x4 p[PARTS];
+        u32x4 p[kParts];
 #pragma unroll
-        for (int n = 0; n < PARTS; n++)
+        for (int n = 0; n < kParts; n++)
 #pragma unroll
             for (int j = 0; j < 4; j++) p[n][j] = round_pair<TYPE>(x[2 * j], x[2 * j + 1]);
 #pragma unroll
@@ -476,7 +479,7 @@ __global__ __launch_bounds__(kThreads, NK <= 2 ? 4 : NK <= 6 ? 2 : 1) void atten
                 t[j] = __builtin_amdgcn_perm(v.word[2 * j + 1][i / 2], v.word[2 * j][i / 2],
                                              i % 2 == 0 ? 0x05040100u : 0x07060302u);
 #pragma unroll
-            for (int n = 0; n < PARTS; n++) o[i] = mfma(t, p[n], o[i], type);
+            for (int n = 0; n < kParts; n++) o[i] = mfma(t, p[n], o[i], type);
         }
         if constexpr (more) load_values(at, kTile * tile);
     };
@@ -653,17 +656,17 @@ AttendPlan make_plan(const KvPages &kv, int sequences, int q_heads, int64_t max_
     return p;
 }
 
-template <int TYPE, int PARTS>
+template <int TYPE>
 void launch(int dim, const AttendArgs &a, const AttendPlan &p, unsigned grid, hipStream_t stream) {
     const auto go = [&](auto kernel) { hipLaunchKernelGGL(kernel, dim3(grid), dim3(kThreads), 0, stream, a, p); };
 #define GOLLEK_ATTEND(NK)                                                      \
     case NK:                                                                   \
         if (p.share == 1) {                                                    \
-            if (dim == 32 * NK) go(attend_kernel<TYPE, NK, true, PARTS, 1>);   \
-            else go(attend_kernel<TYPE, NK, false, PARTS, 1>);                 \
+            if (dim == 32 * NK) go(attend_kernel<TYPE, NK, true, 1>);          \
+            else go(attend_kernel<TYPE, NK, false, 1>);                        \
         } else {                                                               \
-            if (dim == 32 * NK) go(attend_kernel<TYPE, NK, true, PARTS, kWaves>); \
-            else go(attend_kernel<TYPE, NK, false, PARTS, kWaves>);            \
+            if (dim == 32 * NK) go(attend_kernel<TYPE, NK, true, kWaves>);    \
+            else go(attend_kernel<TYPE, NK, false, kWaves>);                   \
         }                                                                      \
         break
     switch ((dim + 31) / 32) {
@@ -705,9 +708,8 @@ hipError_t launch_attend(const AttendArgs &a, uint8_t *workspace, hipStream_t st
     const int64_t grid = p.share == 1 ? (units * p.row_tiles + kWaves - 1) / kWaves : (units + 7) / 8 * 8 * p.row_tiles;
     if (grid > 0x7FFFFFFF) return hipErrorInvalidValue;
     const int dim = a.kv.head_dim;
-    if (a.kv.type == kF16) launch<kF16, 2>(dim, a, p, (unsigned)grid, stream);
-    else if (a.out_type == kF32) launch<kBF16, 3>(dim, a, p, (unsigned)grid, stream);
-    else launch<kBF16, 2>(dim, a, p, (unsigned)grid, stream);
+    if (a.kv.type == kF16) launch<kF16>(dim, a, p, (unsigned)grid, stream);
+    else launch<kBF16>(dim, a, p, (unsigned)grid, stream);
     hipError_t e = hipGetLastError();
     if (e == hipSuccess && !p.whole) {
         const dim3 rows((unsigned)(a.sequences * a.q_heads));

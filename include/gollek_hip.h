@@ -603,6 +603,7 @@ int32_t gollek_hip_kv_append_device(const gollek_hip_kv_cache *cache, const goll
  * there; a row without any token (or with every s_j -inf) is 0.  Nothing behind a sequence's length or before
  * its window changes a result, whatever it holds.  Several new tokens of one
  * sequence are rows of their own, with equal page_table rows and growing lengths.
+ * Weights multiply the values with 24 bits (BF16 caches) or 22 (F16).
  * Results depend in their last bits on the batch (its rows, lengths and table width set
  * how the sums are split), not on timing.  sequences and q_heads in [0, 65535] and
  * [1, 65535], sequences * q_heads < 2^24, max_pages as above, scale in [-1e15, 1e15],

@@ -422,17 +422,11 @@ __global__ __launch_bounds__(kThreads, NK <= 2 ? 4 : NK <= 6 ? 2 : 1) void atten
         }
         float x[8];
         if (a.softcap > 0.0f) {
-            if (a.out_type == kF32) {
+            // (1 - 2 / (1 + exp(2 z)) would be off by 2^-21.5 of the cap, whatever the score: at
+            // a cap of 1e6 by all of it.  This one is off by fp32's steps of the score, for 12.3
+            // us in place of 11.6 at 700 tokens, 223.5 in place of 222.3 at 64 of up to 8192.)
 #pragma unroll
-                for (int j = 0; j < 8; j++) x[j] = cap2 * tanhf(turn * s[j >> 2][j & 3]);
-            } else {
-                // 1 - 2 / (1 + exp(2 z)): off by 2^-21.5 of the cap at most, for a cap of 50 a
-                // weight by 2e-5, a 25th of fp16's half step; 8 % of the exact form's instructions
-#pragma unroll
-                for (int j = 0; j < 8; j++)
-                    x[j] = cap2 - 2.0f * cap2 *
-                                      __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(2.0f * kLog2e * turn * s[j >> 2][j & 3]));
-            }
+            for (int j = 0; j < 8; j++) x[j] = cap2 * tanhf(turn * s[j >> 2][j & 3]);
         } else {
 #pragma unroll
             for (int j = 0; j < 8; j++) x[j] = scale2 * s[j >> 2][j & 3];

@@ -76,3 +76,21 @@ def test_weights_keep_fp32(cache_type, out_type, kv_heads):
     # among 60000 results some lie next to a border between two numbers of the type
     b = Batch([8, 5, 7, 8, 6] * 24, 8, kv_heads, 64, cache_type, q_sigma=0.02, seed=50 + kv_heads)
     compare(b, b.attend(out_type), out_type)
+
+
+@pytest.mark.parametrize("softcap", [0.5, 50.0, 1e3, 1e5, 1e8, 1e15])
+@pytest.mark.parametrize("out_type", [F16, BF16, F32])
+@pytest.mark.parametrize("cache_type", [F16, BF16])
+def test_a_cap_of_any_size(cache_type, out_type, softcap):
+    # a cap far above every score is none; a workgroup a head, a wave a head, a chunk of many
+    b = Batch([0, 1, 77, 400, 3000], 8, 2, 128, cache_type, seed=60)
+    compare(b, b.attend(out_type, softcap=softcap), out_type, [1, 2, 3, 4], softcap=softcap)
+    b = Batch([(11 * i) % 50 + 1 for i in range(500)], 8, 4, 64, cache_type, seed=61)
+    compare(b, b.attend(out_type, softcap=softcap), out_type, range(0, 500, 71), softcap=softcap)
+
+
+def test_a_cap_far_above_every_score_changes_nothing():
+    b = Batch([77, 2000], 8, 2, 64, BF16, seed=62)
+    for out_type in (F16, BF16):
+        bits = [b.attend(out_type, softcap=c).float() for c in (0.0, 1e9)]
+        assert torch.allclose(*bits, rtol=2 * torch.finfo(DTYPE[out_type]).eps, atol=1e-6)

@@ -25,9 +25,9 @@
 // an fp32 number's 24 bits, or two of fp16, 22 bits.  Two pieces of bf16 round four times as
 // many results otherwise than 64 bits do (0.18 % of them at 700 tokens, three 0.04 %, torch
 // in fp32 0.05 %); one puts an error as large as the output's own rounding beside it
-// (2.04e-3 against 1.65e-3).  The third costs nothing where bytes count, 2 % of a short
-// call (700 tokens 10.7 and 10.9 us), and most where 48 heads read the same keys (25.1 and
-// 29.6).
+// (2.04e-3 against 1.65e-3).  The third costs nothing where bytes count, 3 % of a short
+// call (700 tokens 10.7 and 11.0 us) and 4 % where 16 heads read the same keys (37.7 and
+// 39.3), as long as the registers of three waves a SIMD suffice for heads of 128.
 //
 // Bound by bytes: 64 sequences of up to 8192 tokens of 8 heads of 128 219 us (1.37 GB, 6.2
 // TB/s; reads alone outrun a copy's 5.0), one of 131072 of 4 heads 41.2 (268 MB, 6.5
@@ -256,7 +256,7 @@ struct ValueTile {
 
 // TYPE: of cache and queries.  NK: head_dim / 32, rounded up (EXACT: without a rest).
 template <int TYPE, int NK, bool EXACT, int SHARE>
-__global__ __launch_bounds__(kThreads, NK <= 2 ? 4 : NK <= 6 ? 2 : 1) void attend_kernel(AttendArgs a, AttendPlan plan) {
+__global__ __launch_bounds__(kThreads, NK <= 2 ? 4 : NK <= 4 ? 3 : NK <= 6 ? 2 : 1) void attend_kernel(AttendArgs a, AttendPlan plan) {
     using D = Dims<NK>;
     constexpr std::integral_constant<int, TYPE> type;
     constexpr int kParts = TYPE == kBF16 ? 3 : 2;  // pieces of a weight, of 8 (bf16) or 11 (fp16) bits

@@ -244,6 +244,26 @@ __device__ __forceinline__ T stream(const T *p) {
     return __builtin_nontemporal_load(p);
 }
 
+// Infinite and NaN values.  A piece of a weight may be 0 or below, so an infinite value comes
+// out of the second product as NaN where its dim's result is infinite.  Where a sum is NaN
+// and its weights' sum is not, the values say what it is: dim d's of keys [first, end) that
+// are not finite, added up (0: all are, and the sum overflowed).
+template <int TYPE>
+__device__ __forceinline__ float not_finite(const AttendArgs &a, int sequence, int kv_head, int first, int end, int d) {
+    const int32_t *const table = a.page_table + (int64_t)sequence * a.max_pages;
+    float sum = 0.0f;
+    for (int key = first; key < end; key++) {
+        const int page = table[key >> a.kv.page_shift];
+        if (page < 0 || page >= a.kv.pages) continue;
+        const int64_t row = (((int64_t)page * a.kv.kv_heads + kv_head) << a.kv.page_shift) + (key & ((1 << a.kv.page_shift) - 1));
+        const float v = load_element(a.kv.v, TYPE, row * a.kv.head_dim + d);
+        if (!(fabsf(v) < __builtin_inff())) sum += v;
+    }
+    return sum;
+}
+// f times a sum; an infinite one stays so where its weights are too small for fp32.
+__device__ __forceinline__ float scaled(float f, float sum) { return fabsf(sum) == __builtin_inff() ? sum : f * sum; }
+
 // The keys or values of one step as they stand in registers.
 template <int NK>
 struct KeyTile {
@@ -502,6 +522,7 @@ __global__ __launch_bounds__(kThreads, NK <= 2 ? 4 : NK <= 4 ? 3 : NK <= 6 ? 2 :
             total = l * f + __builtin_amdgcn_exp2f(sink - at1);
         }
         const int64_t row = it.sequence * a.out_stride + (head0 + c) * dim;
+        bool odd = false;
 #pragma unroll
         for (int r = 0; r < 4; r++) {
             const auto put = [&](auto WIDE, int first, int d) {
@@ -509,12 +530,24 @@ __global__ __launch_bounds__(kThreads, NK <= 2 ? 4 : NK <= 4 ? 3 : NK <= 6 ? 2 :
                 if (d >= dim) return;
                 float y[wide];
 #pragma unroll
-                for (int i = 0; i < wide; i++) y[i] = total == 0.0f ? 0.0f : f * o[first + i][r] / total;
+                for (int i = 0; i < wide; i++) {
+                    y[i] = total == 0.0f ? 0.0f : f * o[first + i][r] / total;
+                    odd |= y[i] != y[i];
+                }
                 store_run<wide>(a.out, a.out_type, row + d, y);
             };
             put(std::integral_constant<int, D::kWide0>{}, 0, D::kWide0 * (4 * g + r));
             if constexpr (D::kWide1 > 0)
                 put(std::integral_constant<int, D::kWide1>{}, D::kWide0, 16 * D::kWide0 + D::kWide1 * (4 * g + r));
+        }
+        if (odd && total == total) {
+#pragma unroll 1
+            for (int e = 0; e < 4 * D::kFragments; e++) {
+                const int d = e < 4 * D::kWide0 ? 4 * D::kWide0 * g + e : 16 * D::kWide0 + 4 * D::kWide1 * g + e - 4 * D::kWide0;
+                if (d >= dim) continue;
+                const float v = not_finite<TYPE>(a, it.sequence, kv_head, span.begin, span.length, d);
+                if (v != 0.0f) store_element(a.out, a.out_type, row + d, v);
+            }
         }
         return;
     } else {
@@ -549,6 +582,11 @@ __global__ __launch_bounds__(kThreads, NK <= 2 ? 4 : NK <= 4 ? 3 : NK <= 6 ? 2 :
             const float at0 = most == ninf ? 0.0f : most;
 #pragma unroll
             for (int w = 0; w < kWaves; w++) total += lds_l[w][r] * __builtin_amdgcn_exp2f(lds_m[w][r] - at0);
+            if (sum != sum && total == total) {
+                const float v = not_finite<TYPE>(a, it.sequence, kv_head, max(span.begin, kTile * tile0),
+                                                 (int)min((int64_t)span.length, (int64_t)kTile * tile1), d);
+                if (v != 0.0f) sum = v;
+            }
             if (it.chunks > 1) {
                 const int64_t row = (int64_t)item * a.q_heads + head0 + r;
                 plan.part_o[row * dim + d] = sum;
@@ -557,7 +595,7 @@ __global__ __launch_bounds__(kThreads, NK <= 2 ? 4 : NK <= 4 ? 3 : NK <= 6 ? 2 :
                 if (a.sinks != nullptr) {
                     const float sink = a.sinks[head0 + r] * kLog2e, up = fmaxf(sink, most), at1 = up == ninf ? 0.0f : up;
                     const float f = __builtin_amdgcn_exp2f(at0 - at1);
-                    sum *= f;
+                    sum = scaled(f, sum);
                     total = total * f + __builtin_amdgcn_exp2f(sink - at1);
                 }
                 store_element(a.out, a.out_type, it.sequence * a.out_stride + (head0 + r) * dim + d,
@@ -616,8 +654,11 @@ __global__ __launch_bounds__(64 * WAVES) void join_kernel(AttendArgs a, AttendPl
         const float *const from = plan.part_o + row0 * dim + d0;
         const int64_t pitch = (int64_t)a.q_heads * dim;
 #pragma unroll 8
-        for (int i = slice; i < chunks; i += slices)
-            o += weight[i] * *reinterpret_cast<const f32x4 *>(from + (int64_t)i * pitch);
+        for (int i = slice; i < chunks; i += slices) {
+            const f32x4 part = *reinterpret_cast<const f32x4 *>(from + (int64_t)i * pitch);
+#pragma unroll
+            for (int j = 0; j < 4; j++) o[j] += scaled(weight[i], part[j]);
+        }
         *reinterpret_cast<f32x4 *>(lds + slice * dim + d0) = o;
     }
     __syncthreads();

@@ -601,7 +601,9 @@ int32_t gollek_hip_kv_append_device(const gollek_hip_kv_cache *cache, const goll
  * (sequences x q_heads x head_dim of out_type).  A length past the table counts as
  * the table's, one below 1 as 0; a token whose page is outside [0, pages) is not
  * there; a row without any token (or with every s_j -inf) is 0.  Nothing behind a sequence's length or before
- * its window changes a result, whatever it holds.  Several new tokens of one
+ * its window changes a result, whatever it holds.  An infinite value among the others
+ * makes its dim's results infinite whatever its weight, a NaN or two infinities of other
+ * signs make them NaN.  Several new tokens of one
  * sequence are rows of their own, with equal page_table rows and growing lengths.
  * Weights multiply the values with 24 bits (BF16 caches) or 22 (F16).
  * Results depend in their last bits on the batch (its rows, lengths and table width set

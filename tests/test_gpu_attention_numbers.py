@@ -94,3 +94,75 @@ def test_a_cap_far_above_every_score_changes_nothing():
     for out_type in (F16, BF16):
         bits = [b.attend(out_type, softcap=c).float() for c in (0.0, 1e9)]
         assert torch.allclose(*bits, rtol=2 * torch.finfo(DTYPE[out_type]).eps, atol=1e-6)
+
+
+INF, NAN = float("inf"), float("nan")
+
+
+def poke(b, s, position, head, dim, value):
+    """A value of sequence s's token at `position`."""
+    b.v[int(b.table[s, position // b.page]), head, position % b.page, dim] = value
+
+
+@pytest.mark.parametrize("lengths,kv_heads,dim,window", [
+    ([1, 40, 700, 90, 33], 2, 128, 0),                        # a workgroup a head
+    ([1, 40, 20000, 90, 9000], 2, 64, 0),                     # cut into chunks, some joined by many
+    ([1, 40, 6000] + [90] * 300, 2, 64, 0),                   # by few
+    ([1, 40, 100, 90, 33] + [60] * 300, 8, 80, 0),            # a wave a head
+    ([1, 40, 100, 90, 33] + [60] * 300, 4, 256, 0),
+    ([1, 40, 3000, 90, 33], 2, 192, 50)])
+@pytest.mark.parametrize("cache_type,out_type", [(F16, F32), (F16, BF16), (BF16, F32), (BF16, F16), (F16, F16)])
+@pytest.mark.parametrize("with_sinks", [False, True])
+def test_infinite_values(lengths, kv_heads, dim, window, cache_type, out_type, with_sinks):
+    # an infinite value makes its dim infinite, also where its weight is tiny; two of other
+    # signs, or a NaN, make it NaN; every other dim, head and sequence stays as it was
+    b = Batch(lengths, 2 * kv_heads, kv_heads, dim, cache_type, window=window, q_sigma=1.0, seed=70)
+    sinks = torch.linspace(-3, 3, 2 * kv_heads).cuda() if with_sinks else None
+    clean = b.device().attend(F32, sinks=sinks).cpu()
+    last = lengths[2] - 1
+    poke(b, 0, 0, 1, 3, INF)           # the only token
+    poke(b, 1, 39, 0, 0, -INF)
+    poke(b, 1, 12, 1, dim - 1, INF)
+    poke(b, 2, last, 0, 5, INF)
+    poke(b, 2, last - 30, 0, 5, INF)   # twice
+    poke(b, 2, last - 7, 0, 6, INF)
+    poke(b, 2, last - 48, 0, 6, -INF)  # both signs
+    poke(b, 2, last - 9, 1, 7, NAN)
+    poke(b, 2, last - 9, 1, 8, NAN)
+    poke(b, 2, last - 20, 1, 8, INF)   # and one with a NaN
+    want = {(0, 1, 3): INF, (1, 0, 0): -INF, (1, 1, dim - 1): INF, (2, 0, 5): INF, (2, 0, 6): NAN, (2, 1, 7): NAN, (2, 1, 8): NAN}
+    out = b.device().attend(out_type, sinks=sinks).cpu().float()
+    for (s, head, d), value in want.items():
+        got = out[s, 2 * head:2 * head + 2, d]
+        assert torch.isnan(got).all() if value != value else (got == value).all(), (s, head, d, got)
+        out[s, 2 * head:2 * head + 2, d] = clean[s, 2 * head:2 * head + 2, d]
+    eps = torch.finfo(DTYPE[out_type]).eps
+    assert torch.allclose(out, clean, rtol=eps, atol=2e-6 if out_type != F16 else 1e-5)
+
+
+@pytest.mark.parametrize("cache_type", [F16, BF16])
+@pytest.mark.parametrize("lengths", [[300], [20000], [300] + [40] * 600])
+def test_infinite_values_of_no_weight_to_speak_of(lengths, cache_type):
+    # their token's weight is e^-200: far below what fp32 holds, and above nothing
+    b = Batch(lengths, 4, 2, 64, cache_type, seed=71)
+    b.q[0].fill_(1.0)
+    for position in range(lengths[0]):
+        b.k[int(b.table[0, position // 16]), :, position % 16] = 0.0
+    for position in (7, lengths[0] - 2):
+        b.k[int(b.table[0, position // 16]), :, position % 16] = -200.0 / 64
+        poke(b, 0, position, 0, 9, -INF)
+    out = b.device().attend(F32, scale=1.0).cpu()
+    assert (out[0, :2, 9] == -INF).all()
+    out[0, :2, 9] = 0.0
+    assert torch.isfinite(out).all()
+
+
+def test_infinite_values_outside_a_window_or_a_length():
+    b = Batch([100, 100, 100], 4, 2, 64, F16, seed=72, window=40)
+    want = b.attend(F32).cpu()
+    inside = torch.zeros(b.v.shape[0], 16, dtype=torch.bool)
+    for s in range(3):
+        for position in range(60, 100):
+            inside[int(b.table[s, position // 16]), position % 16] = True
+    b.v.masked_fill_(~inside[:, None, :, None], INF)
+    assert torch.equal(b.device().attend(F32).cpu(), want)

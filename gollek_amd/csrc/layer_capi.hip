@@ -525,7 +525,7 @@ int32_t gollek_hip_kv_append_device(const gollek_hip_kv_cache *cache, const goll
     for (const Rows &r : in) {
         if (clash(r, tokens, cache->pages.k, cache->bytes) || clash(r, tokens, cache->pages.v, cache->bytes))
             return overlap(r.name, "cache", err, err_len);
-        if (clash(out, r, tokens, r.p == q)) return overlap(out.name, r.name, err, err_len);
+        if (clash(out, r, tokens, &r == &in[2])) return overlap(out.name, r.name, err, err_len);  // (q_out may be q)
     }
     if (clash(out, tokens, cache->pages.k, cache->bytes) || clash(out, tokens, cache->pages.v, cache->bytes))
         return overlap(out.name, "cache", err, err_len);
@@ -627,7 +627,7 @@ int32_t gollek_hip_attention_device(const gollek_hip_kv_cache *cache, const void
                 {"sinks", sinks, q_heads * 4}};
     if (clash(result, in, sequences, false)) return overlap("output", "queries", err, err_len);
     for (const auto &r : read) {
-        if (r.p != q && clash(result, sequences, r.p, r.bytes)) return overlap("output", r.name, err, err_len);
+        if (&r != &read[0] && clash(result, sequences, r.p, r.bytes)) return overlap("output", r.name, err, err_len);
         if (share(r.p, r.bytes, workspace, need)) return overlap("workspace", r.name, err, err_len);
     }
     if (clash(result, sequences, workspace, need)) return overlap("output", "workspace", err, err_len);

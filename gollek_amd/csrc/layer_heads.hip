@@ -97,8 +97,9 @@ __global__ __launch_bounds__(64 * kWaves) void heads_kernel(HeadsArgs a, HeadsPl
     const int lane = (int)threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
     const int64_t unit = (int64_t)blockIdx.x * kWaves + wave;
     const bool in = unit < a.tokens * plan.slices;
+    // (a wave past the last token loads what the first one does, and leaves)
     const int64_t t = in ? unit / plan.slices : 0;
-    const int slice = (int)(unit - t * plan.slices);
+    const int slice = in ? (int)(unit - t * plan.slices) : 0;
     const int kv_heads = CACHE ? a.kv.kv_heads : 0, heads = a.q_heads + 2 * kv_heads;
     const int dim = a.head_dim, dims = a.rope.dims, pairs = dim / 2;
     // everything that waits for nothing is loaded first: a decoded token's call is a chain

@@ -105,9 +105,9 @@ __global__ __launch_bounds__(64 * kWaves) void heads_kernel(HeadsArgs a, HeadsPl
     // everything that waits for nothing is loaded first: a decoded token's call is a chain
     // of loads, position to page to place, and the angles on the way
     const int64_t position = a.positions[t];
-    int64_t sequence = t, page = -1;
+    int64_t sequence = -1, page = -1;
     if constexpr (CACHE) {
-        if (a.sequence != nullptr) sequence = a.sequence[t];
+        sequence = a.sequence != nullptr ? a.sequence[t] : a.first + t;
     }
     // this lane's pairs: p .. p + V - 1; their first and second elements stand at
     // e0 and e1 .. (half), or together from e0 on (interleaved, or behind what turns)
@@ -267,7 +267,6 @@ hipError_t launch(const HeadsArgs &a, hipStream_t stream) {
     const int64_t waves = (int64_t)device_cus() * 16;  // four a SIMD
     p.slices = (int)(a.tokens >= waves ? 1 : (waves + a.tokens - 1) / a.tokens < rounds ? (waves + a.tokens - 1) / a.tokens : rounds);
     const int64_t blocks = (a.tokens * p.slices + kWaves - 1) / kWaves;
-    if (blocks > 0x7FFFFFFF) return hipErrorInvalidValue;
     const auto go = [&](auto kernel) {
         hipLaunchKernelGGL(kernel, dim3((unsigned)blocks), dim3(64 * kWaves), 0, stream, a, p);
         return hipGetLastError();
@@ -280,9 +279,27 @@ hipError_t launch(const HeadsArgs &a, hipStream_t stream) {
 
 }  // namespace
 
-hipError_t launch_heads(const HeadsArgs &a, hipStream_t stream) {
-    if (a.kv.k != nullptr) return a.type == kF32 ? launch<4, 2, true>(a, stream) : launch<2, 2, true>(a, stream);
-    return a.type == kF32 ? launch<4, 4, false>(a, stream) : launch<2, 2, false>(a, stream);
+hipError_t launch_heads(const HeadsArgs &all, hipStream_t stream) {
+    // A grid has at most 2^32 threads in all: more than kMostTokens take several.
+    constexpr int64_t kMostTokens = (int64_t)1 << 25;
+    HeadsArgs a = all;
+    const auto moved = [&](const void *p, int64_t stride, int type) -> const void * {
+        return p == nullptr ? nullptr : static_cast<const uint8_t *>(p) + a.first * stride * (type == kF32 ? 4 : 2);
+    };
+    for (a.first = 0; a.first < all.tokens; a.first += kMostTokens) {
+        a.tokens = all.tokens - a.first < kMostTokens ? all.tokens - a.first : kMostTokens;
+        a.q = moved(all.q, a.q_stride, a.type);
+        a.k = moved(all.k, a.k_stride, a.type);
+        a.v = moved(all.v, a.v_stride, a.type);
+        a.q_out = const_cast<void *>(moved(all.q_out, a.q_out_stride, a.out_type));
+        a.positions = all.positions + a.first;
+        if (all.sequence != nullptr) a.sequence = all.sequence + a.first;
+        const bool wide = a.type == kF32;
+        const hipError_t e = a.kv.k != nullptr ? (wide ? launch<4, 2, true>(a, stream) : launch<2, 2, true>(a, stream))
+                                               : (wide ? launch<4, 4, false>(a, stream) : launch<2, 2, false>(a, stream));
+        if (e != hipSuccess) return e;
+    }
+    return hipSuccess;
 }
 
 }  // namespace gollek

@@ -52,6 +52,7 @@ struct HeadsArgs {
     const int32_t *positions, *sequence, *page_table;
     int64_t sequences, max_pages;
     int64_t tokens;
+    int64_t first;  // the launch's first token's number in the call (sequence nullptr: its sequence)
     int q_heads, head_dim, type, out_type;
 };
 hipError_t launch_heads(const HeadsArgs &a, hipStream_t stream);

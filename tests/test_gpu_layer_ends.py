@@ -4,7 +4,7 @@ import torch
 
 from gollek_amd import tensor_ops as ops
 from tests import layer_ref as ref
-from tests.layer_ref import BF16
+from tests.layer_ref import BF16, F16
 from tests.test_gpu_layer_ops import close, ptr, stream, table
 
 pytestmark = pytest.mark.gpu
@@ -36,3 +36,32 @@ def rope_of_many_tokens(tokens):
 def test_rope_whose_surplus_waves_would_count_past_32_bits():
     # 64 heads a wave: the waves behind the last token would be at head 64 * 2^25
     rope_of_many_tokens((1 << 25) + 1)
+
+
+def test_rope_of_more_tokens_than_one_grid():
+    rope_of_many_tokens((1 << 26) + 5)
+
+
+@pytest.mark.parametrize("numbered", [False, True])
+def test_append_of_more_tokens_than_one_grid(numbered):
+    # a place for a few tokens around the borders of launches; the others' pages are none
+    tokens, page, dim = (1 << 26) + 5, 16, 8
+    chosen = [0, 1, (1 << 25) - 1, 1 << 25, (1 << 25) + 1, (1 << 26) - 1, 1 << 26, tokens - 1]
+    k, v = (torch.full((len(chosen) + 1, 1, page, dim), 9.0, dtype=torch.float16, device="cuda") for _ in range(2))
+    pages = torch.full((tokens,), -1, dtype=torch.int32, device="cuda")
+    at = torch.arange(tokens, device="cuda", dtype=torch.int32) % page
+    sequence = torch.arange(tokens, device="cuda", dtype=torch.int32).flip(0) if numbered else None
+    for i, t in enumerate(chosen):
+        pages[tokens - 1 - t if numbered else t] = i
+    src = (torch.arange(tokens * dim, device="cuda", dtype=torch.int32) * 31 % 2039).to(torch.float16).view(tokens, dim)
+    q_out = torch.full_like(src, float("nan"))
+    cache = ops.KvCache(F16, ptr(k), ptr(v), len(chosen) + 1, page, 1, dim)
+    print(f"[gpu] append {tokens} tokens, numbered={numbered}", flush=True)
+    cache.append(ptr(src), ptr(src), F16, tokens, ptr(at), ptr(pages), tokens, 1, q_ptr=ptr(src), q_heads=1, q_out_ptr=ptr(q_out),
+                 sequence_ptr=ptr(sequence), stream=stream())
+    torch.cuda.synchronize()
+    assert torch.equal(q_out, src)
+    want = torch.full_like(k, 9.0)
+    for i, t in enumerate(chosen):
+        want[i, 0, t % page] = src[t]
+    assert torch.equal(k, want) and torch.equal(v, want)

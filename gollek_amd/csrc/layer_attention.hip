@@ -679,7 +679,6 @@ AttendPlan make_plan(const KvPages &kv, int sequences, int q_heads, int64_t max_
     if (window > 0 && tiles > window / kTile + 2) tiles = window / kTile + 2;
     const int64_t per = (int64_t)kv.kv_heads * p.row_tiles, units = sequences * per;
     p.share = tiles <= alone_tiles(kv.head_dim) && units >= alone_units(kv.head_dim, tiles) ? 1 : kWaves;
-    p.whole = sequences > kScanMost || tiles <= (units < kFew ? whole_few(kv.head_dim) : kWholeMany);
     // the largest cut, also where this call is not cut: the workspace is asked for by it,
     // and must not shrink where more sequences fall under another rule
     const int n = sequences < kScanMost ? sequences : kScanMost;
@@ -687,7 +686,9 @@ AttendPlan make_plan(const KvPages &kv, int sequences, int q_heads, int64_t max_
     p.slots = (int)(per < target ? target / per : 1);
     p.few = (int)(per < kTargetEach ? kTargetEach / per : 1);
     const int64_t most = n * ((tiles + kLeast - 1) / kLeast);
-    p.items = tiles <= whole_few(kv.head_dim) ? 0 : (int)(most < n + p.slots ? most : n + p.slots);
+    // (one slot: no sequence would be cut, its heads are enough)
+    p.items = tiles <= whole_few(kv.head_dim) || p.slots == 1 ? 0 : (int)(most < n + p.slots ? most : n + p.slots);
+    p.whole = sequences > kScanMost || p.slots == 1 || tiles <= (units < kFew ? whole_few(kv.head_dim) : kWholeMany);
     return p;
 }
 
@@ -740,8 +741,12 @@ hipError_t launch_attend(const AttendArgs &a, uint8_t *workspace, hipStream_t st
     (void)lay_out(p, a.kv, a.sequences, a.q_heads, workspace);
     p.q_vec = ((reinterpret_cast<uintptr_t>(a.q) | (uintptr_t)(a.q_stride * 2)) & 15u) == 0;
     const int64_t units = (int64_t)(p.whole ? a.sequences : p.items) * a.kv.kv_heads;
-    const int64_t grid = p.share == 1 ? (units * p.row_tiles + kWaves - 1) / kWaves : (units + 7) / 8 * 8 * p.row_tiles;
-    if (grid > 0x7FFFFFFF) return hipErrorInvalidValue;
+    // (below 2^24 workgroups, a grid's 2^32 threads: there are fewer rows than that, an uncut
+    // unit has one at least, 17 where there are row tiles, and a cut batch has at most 1024 + 1536
+    // items of 768 heads)
+    const int64_t grid = p.share == 1        ? (units * p.row_tiles + kWaves - 1) / kWaves
+                         : p.row_tiles == 1 ? units
+                                            : (units + 7) / 8 * 8 * p.row_tiles;
     const int dim = a.kv.head_dim;
     if (a.kv.type == kF16) launch<kF16>(dim, a, p, (unsigned)grid, stream);
     else launch<kBF16>(dim, a, p, (unsigned)grid, stream);

@@ -1,4 +1,4 @@
-"""Norms, rotary positions and appends at the ends of their ranges, on the GPU."""
+"""Norms, rotary positions, appends and attention at the ends of their ranges, on the GPU."""
 import pytest
 import torch
 
@@ -65,3 +65,24 @@ def test_append_of_more_tokens_than_one_grid(numbered):
     for i, t in enumerate(chosen):
         want[i, 0, t % page] = src[t]
     assert torch.equal(k, want) and torch.equal(v, want)
+
+
+@pytest.mark.parametrize("sequences,heads,max_pages", [(256, 65535, 200), (4095, 4097, 20), (255, 65535, 1)])
+def test_attention_of_almost_2_to_24_rows(sequences, heads, max_pages):
+    # one token each: its value, whatever the score
+    page, dim = 16, 8
+    k = torch.ones(3, heads, page, dim, dtype=torch.float16, device="cuda")
+    v = torch.randn(3, heads, page, dim, dtype=torch.float16, device="cuda")
+    q = torch.ones(sequences, heads, dim, dtype=torch.float16, device="cuda")
+    pages = torch.full((sequences, max_pages), -1, dtype=torch.int32, device="cuda")
+    pages[:, 0] = torch.arange(sequences, device="cuda") % 3
+    lengths = torch.ones(sequences, dtype=torch.int32, device="cuda")
+    out = torch.full_like(q, float("nan"))
+    cache = ops.KvCache(F16, ptr(k), ptr(v), 3, page, heads, dim)
+    need = cache.attend_workspace_bytes(sequences, heads, max_pages)
+    ws = torch.zeros(max(need, 256), dtype=torch.uint8, device="cuda")
+    print(f"[gpu] attend {sequences} x {heads}, table of {max_pages}, workspace {need}", flush=True)
+    cache.attend(ptr(q), sequences, heads, ptr(lengths), ptr(pages), max_pages, ptr(out), F16, scale=1.0, ws_ptr=ptr(ws),
+                 ws_bytes=need, stream=stream())
+    torch.cuda.synchronize()
+    assert torch.equal(out, v[pages[:, 0].long(), :, 0])

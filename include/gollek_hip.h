@@ -503,8 +503,10 @@ int32_t gollek_hip_next_token(gollek_hip_weight *lm_head, const float *x, int64_
  * bias 0; hidden or y may be NULL (not both).  rows up to 2^31 - 1, cols in
  * [1, 65536], a finite scale, eps >= 0 and finite: else ARG.  hidden may be x or the
  * residual itself, y may be x or the residual (the same address, type size and
- * stride).  A row of zeros with eps 0 divides 0 by 0 (NaN); squares are fp32's, so
- * rows of magnitudes past 1e18 overflow.
+ * stride).  The sum of a row's squares is fp32's: it has to stay below 3.4e38, a root
+ * mean square below 1.8e19 / sqrt(cols) (2.8e17 at 4096, 7.2e16 at 65536), else the
+ * norm is 0.  With eps 0 a row of zeros divides 0 by 0 (NaN), and so small a row that
+ * its squares are 0 (elements below 1e-23) divides by 0 (infinities).
  * The host form takes packed rows and copies them up (synchronous). */
 int32_t gollek_hip_norm(const void *x, int32_t x_type, int64_t rows, int64_t cols, const float *post_weight,
                         const float *gate, float scale, const void *residual, void *hidden, int32_t hidden_type,

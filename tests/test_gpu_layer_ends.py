@@ -4,8 +4,8 @@ import torch
 
 from gollek_amd import tensor_ops as ops
 from tests import layer_ref as ref
-from tests.layer_ref import BF16, F16
-from tests.test_gpu_layer_ops import close, ptr, stream, table
+from tests.layer_ref import BF16, F16, F32
+from tests.test_gpu_layer_ops import close, ptr, run_norm, stream, table
 
 pytestmark = pytest.mark.gpu
 
@@ -86,3 +86,15 @@ def test_attention_of_almost_2_to_24_rows(sequences, heads, max_pages):
                  ws_bytes=need, stream=stream())
     torch.cuda.synchronize()
     assert torch.equal(out, v[pages[:, 0].long(), :, 0])
+
+
+@pytest.mark.parametrize("cols,sigma", [(64, 1.5e18), (4096, 2.6e17), (8000, 1.9e17), (65536, 7e16)])
+@pytest.mark.parametrize("post", [False, True])
+def test_norm_of_rows_near_the_largest(cols, sigma, post):
+    # root mean squares a little below 1.8e19 / sqrt(cols) (64: a third below, rows of so few vary)
+    run_norm(5, cols, F32, F32, F32, sigma=sigma, post=post, seed=80)
+
+
+@pytest.mark.parametrize("sigma", [1e-15, 1e-18])
+def test_norm_of_small_rows_without_eps(sigma):
+    run_norm(5, 1000, F32, F32, F32, sigma=sigma, residual=False, eps=0.0, seed=81)

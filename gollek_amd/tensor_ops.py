@@ -864,7 +864,9 @@ def rope_frequencies(dims: int, *, base: float = 10000.0, scaling: int = ROPE_NO
 
 
 class Rope:
-    """A model's rotary table on the current device (gollek_hip_rope)."""
+    """A model's rotary table on the current device (gollek_hip_rope).  Keep it as long as
+    the model: it must outlive its calls and the captured graphs that hold one, and must
+    not be closed (or collected) while a stream is captured."""
 
     def __init__(self, dims: int, *, layout: int = ROPE_HALF, base: float = 10000.0, scaling: int = ROPE_NONE,
                  factor: float = 1.0, original_context: float = 0.0, low: float = 0.0, high: float = 0.0,
@@ -915,7 +917,7 @@ class Rope:
 class KvCache:
     """A paged cache of keys and values in the caller's device memory
     (gollek_hip_kv_cache): k and v (pages, kv_heads, page_size, head_dim) of F16 or
-    BF16, which must outlive it."""
+    BF16, which must outlive it and the captured graphs that hold a call on it."""
 
     def __init__(self, type_id: int, k_ptr: int, v_ptr: int, pages: int, page_size: int, kv_heads: int, head_dim: int):
         err = _native.ErrBuf()

@@ -528,7 +528,9 @@ int32_t gollek_hip_norm_device(const void *x, int32_t x_type, int64_t rows, int6
                                   * than `high` times, mixed by a ramp over the pairs between; magnitude 0.1 ln(factor) + 1 */
 #define GOLLEK_HIP_ROPE_LLAMA3 3 /* the same borders, mixed by the number of turns; magnitude 1 */
 
-/* Opaque table of a model's rotary frequencies, on the device that was current. */
+/* Opaque table of a model's rotary frequencies, on the device that was current.  It
+ * must outlive every call that takes it, and every captured graph that holds one: a
+ * replay reads the table again. */
 typedef struct gollek_hip_rope gollek_hip_rope;
 
 /* Frequencies (radians a position, dims / 2 floats) and magnitude (one float) that
@@ -546,7 +548,7 @@ int32_t gollek_hip_rope_frequencies(int64_t dims, float base, int32_t scaling, f
 gollek_hip_rope *gollek_hip_rope_create(int32_t layout, int64_t dims, float base, int32_t scaling, float factor,
                                         float original_context, float low, float high, float magnitude,
                                         const float *factors, char *err, size_t err_len);
-/* Waits for the device's work first.  NULL is a no-op. */
+/* Waits for the device's work first, so not while a stream is captured.  NULL is a no-op. */
 void gollek_hip_rope_free(gollek_hip_rope *rope);
 
 /* out = x (tokens x heads x head_dim) with every head's first dims elements rotated
@@ -568,7 +570,8 @@ typedef struct gollek_hip_kv_cache gollek_hip_kv_cache;
  * else ARG; another type -> UNSUPPORTED.  NULL on failure. */
 gollek_hip_kv_cache *gollek_hip_kv_cache_wrap_device(int32_t type, void *k, void *v, int64_t pages, int64_t page_size,
                                                      int64_t kv_heads, int64_t head_dim, char *err, size_t err_len);
-/* Frees the handle, not the arrays.  NULL is a no-op. */
+/* Frees the handle, not the arrays, which calls and captured graphs go on using.  NULL is
+ * a no-op. */
 void gollek_hip_kv_cache_free(gollek_hip_kv_cache *cache);
 
 /* Appends new tokens to a cache, and makes their queries ready for it:

@@ -329,7 +329,12 @@ void gollek_hip_rope_free(gollek_hip_rope *r) {
     if (r == nullptr) return;
     {
         const DeviceGuard device(r->device);
-        (void)hipFree(r->turns);  // (hipFree waits for the device)
+        // (the table of a handle that the garbage collector closes while some stream is
+        // captured: an ordinary hipFree would break that capture)
+        hipStreamCaptureMode mode = hipStreamCaptureModeRelaxed;
+        const bool relaxed = hipThreadExchangeStreamCaptureMode(&mode) == hipSuccess;
+        (void)hipFree(r->turns);  // (waits for the device)
+        if (relaxed) (void)hipThreadExchangeStreamCaptureMode(&mode);
     }
     delete r;
 }

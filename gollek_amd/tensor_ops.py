@@ -865,8 +865,7 @@ def rope_frequencies(dims: int, *, base: float = 10000.0, scaling: int = ROPE_NO
 
 class Rope:
     """A model's rotary table on the current device (gollek_hip_rope).  Keep it as long as
-    the model: it must outlive its calls and the captured graphs that hold one, and must
-    not be closed (or collected) while a stream is captured."""
+    the model: it must outlive its calls and the captured graphs that hold one."""
 
     def __init__(self, dims: int, *, layout: int = ROPE_HALF, base: float = 10000.0, scaling: int = ROPE_NONE,
                  factor: float = 1.0, original_context: float = 0.0, low: float = 0.0, high: float = 0.0,

@@ -548,7 +548,7 @@ int32_t gollek_hip_rope_frequencies(int64_t dims, float base, int32_t scaling, f
 gollek_hip_rope *gollek_hip_rope_create(int32_t layout, int64_t dims, float base, int32_t scaling, float factor,
                                         float original_context, float low, float high, float magnitude,
                                         const float *factors, char *err, size_t err_len);
-/* Waits for the device's work first, so not while a stream is captured.  NULL is a no-op. */
+/* Waits for the device's work first; captures that go on are left alone.  NULL is a no-op. */
 void gollek_hip_rope_free(gollek_hip_rope *rope);
 
 /* out = x (tokens x heads x head_dim) with every head's first dims elements rotated

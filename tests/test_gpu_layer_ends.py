@@ -98,3 +98,24 @@ def test_norm_of_rows_near_the_largest(cols, sigma, post):
 @pytest.mark.parametrize("sigma", [1e-15, 1e-18])
 def test_norm_of_small_rows_without_eps(sigma):
     run_norm(5, 1000, F32, F32, F32, sigma=sigma, residual=False, eps=0.0, seed=81)
+
+
+def test_a_table_closed_while_a_stream_is_captured():
+    # as the garbage collector may: the capture goes on, with the table that it holds
+    rope, _ = table(64)
+    other, _ = table(64, base=5000.0)
+    x = torch.randn(4, 2, 64, device="cuda")
+    at = torch.arange(4, dtype=torch.int32, device="cuda")
+    want, out = torch.empty_like(x), torch.zeros_like(x)
+    rope.apply_device(ptr(x), F32, 4, 2, 64, ptr(at), ptr(want), stream=stream())
+    torch.cuda.synchronize()
+    side, graph = torch.cuda.Stream(), torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph, stream=side):
+        rope.apply_device(ptr(x), F32, 4, 2, 64, ptr(at), ptr(out), stream=side.cuda_stream)
+        other.close()
+        twice = out * 2
+    for _ in range(3):
+        out.zero_()
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(out, want) and torch.equal(twice, 2 * want)

@@ -261,6 +261,12 @@ __device__ __forceinline__ float not_finite(const AttendArgs &a, int sequence, i
     }
     return sum;
 }
+// A head's sink in powers of two.  One past fp32 there stands for the largest score: it takes
+// all weight, and its own stays a number.
+__device__ __forceinline__ float sink_of(const AttendArgs &a, int64_t head) {
+    const float sink = a.sinks[head] * kLog2e;
+    return sink > 3e38f ? 3e38f : sink;
+}
 // f times a sum; an infinite one stays so where its weights are too small for fp32.
 __device__ __forceinline__ float scaled(float f, float sum) { return fabsf(sum) == __builtin_inff() ? sum : f * sum; }
 
@@ -517,7 +523,7 @@ __global__ __launch_bounds__(kThreads, NK <= 2 ? 4 : NK <= 4 ? 3 : NK <= 6 ? 2 :
         if (c >= rows) return;
         float f = 1.0f, total = l;
         if (a.sinks != nullptr) {
-            const float sink = a.sinks[head0 + c] * kLog2e, up = fmaxf(sink, bound), at1 = up == ninf ? 0.0f : up;
+            const float sink = sink_of(a, head0 + c), up = fmaxf(sink, bound), at1 = up == ninf ? 0.0f : up;
             f = __builtin_amdgcn_exp2f(bound - at1);
             total = l * f + __builtin_amdgcn_exp2f(sink - at1);
         }
@@ -593,7 +599,7 @@ __global__ __launch_bounds__(kThreads, NK <= 2 ? 4 : NK <= 4 ? 3 : NK <= 6 ? 2 :
                 if (d == 0) plan.part_ml[row] = make_float2(most, total);
             } else {
                 if (a.sinks != nullptr) {
-                    const float sink = a.sinks[head0 + r] * kLog2e, up = fmaxf(sink, most), at1 = up == ninf ? 0.0f : up;
+                    const float sink = sink_of(a, head0 + r), up = fmaxf(sink, most), at1 = up == ninf ? 0.0f : up;
                     const float f = __builtin_amdgcn_exp2f(at0 - at1);
                     sum = scaled(f, sum);
                     total = total * f + __builtin_amdgcn_exp2f(sink - at1);
@@ -619,7 +625,7 @@ __global__ __launch_bounds__(64 * WAVES) void join_kernel(AttendArgs a, AttendPl
     const int64_t row0 = (int64_t)join.x * a.q_heads + head;
     const int chunks = join.y;
     if (chunks <= 1) return;
-    const float sink = a.sinks != nullptr ? a.sinks[head] * kLog2e : ninf;
+    const float sink = a.sinks != nullptr ? sink_of(a, head) : ninf;
     float2 ml[kEach];
     float most = sink;
 #pragma unroll

@@ -166,3 +166,20 @@ def test_infinite_values_outside_a_window_or_a_length():
             inside[int(b.table[s, position // 16]), position % 16] = True
     b.v.masked_fill_(~inside[:, None, :, None], INF)
     assert torch.equal(b.device().attend(F32).cpu(), want)
+
+
+@pytest.mark.parametrize("lengths", [[0, 1, 77, 400], [0, 1, 77, 9000], [5, 60] * 300])
+def test_sinks_at_the_ends(lengths):
+    # a sink past every score takes all weight, one at the lowest value none, and a NaN is its head's
+    b = Batch(lengths, 8, 4, 64, BF16, seed=63)
+    most = torch.finfo(torch.float32).max
+    sinks = torch.tensor([most, 3e38, INF, -most, -INF, NAN, 0.5, -3e38]).cuda()
+    out, plain = b.attend(F32, sinks=sinks).cpu(), b.attend(F32).cpu()
+    assert not out[:, :3].any()
+    assert torch.equal(out[:, [3, 4, 7]], plain[:, [3, 4, 7]])
+    some = [i for i, n in enumerate(lengths) if n > 0]
+    assert torch.isnan(out[some, 5]).all()
+    for s in range(4):
+        if lengths[s]:
+            want, off = definition(b.q[s], *rows_of(b, s), ref.softmax_scale(64), 0.0, torch.full((8,), 0.5))
+            between(out[s, 6], want[6], off[6], F32, f"sequence {s}")

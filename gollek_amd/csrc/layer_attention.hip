@@ -286,9 +286,10 @@ __global__ __launch_bounds__(kThreads, NK <= 2 ? 4 : NK <= 4 ? 3 : NK <= 6 ? 2 :
     using D = Dims<NK>;
     constexpr std::integral_constant<int, TYPE> type;
     constexpr int kParts = TYPE == kBF16 ? 3 : 2;  // pieces of a weight, of 8 (bf16) or 11 (fp16) bits
-    // fp16 weights: exp(s - m) times 2^7, so that all but the smallest are normal numbers
-    // (2^15 with the slack, below fp16's largest)
-    constexpr float kLift = TYPE == kF16 ? 7.0f : 0.0f;
+    // Weights are exp(s - m) times 2^kLift.  fp16: 2^7, so that all but the smallest are normal
+    // numbers (2^15 with the slack, below fp16's largest).  bf16: 2^-kSlack, so that none passes
+    // 1 and a value near fp32's largest stays finite times it.
+    constexpr float kLift = TYPE == kF16 ? 7.0f : -kSlack;
     const float ninf = -__builtin_inff();
 
     const int lane = (int)threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);

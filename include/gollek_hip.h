@@ -610,7 +610,8 @@ int32_t gollek_hip_kv_append_device(const gollek_hip_kv_cache *cache, const goll
  * makes its dim's results infinite whatever its weight, a NaN or two infinities of other
  * signs make them NaN.  Several new tokens of one
  * sequence are rows of their own, with equal page_table rows and growing lengths.
- * Weights multiply the values with 24 bits (BF16 caches) or 22 (F16).
+ * Weights multiply the values with 24 bits (BF16 caches) or 22 (F16); scores and sums are
+ * fp32's: scores past 2.3e38 and values that add up past 3.4e38 overflow.
  * Results depend in their last bits on the batch (its rows, lengths and table width set
  * how the sums are split), not on timing.  sequences and q_heads in [0, 65535] and
  * [1, 65535], sequences * q_heads < 2^24, max_pages as above, scale in [-1e15, 1e15],

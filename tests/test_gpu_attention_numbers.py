@@ -183,3 +183,16 @@ def test_sinks_at_the_ends(lengths):
         if lengths[s]:
             want, off = definition(b.q[s], *rows_of(b, s), ref.softmax_scale(64), 0.0, torch.full((8,), 0.5))
             between(out[s, 6], want[6], off[6], F32, f"sequence {s}")
+
+
+def test_large_values_under_growing_scores():
+    # a score up to 2^8 above those before it: its weight and bf16's largest values stay in range
+    b = Batch([1000], 2, 1, 64, BF16, seed=64)
+    b.q.fill_(1.0)
+    b.v.fill_(1.0)
+    for position in range(1000):
+        b.k[int(b.table[0, position // 16]), 0, position % 16] = 0.0 if position % 640 < 600 else 5.0 / 64
+        if position % 640 == 639:
+            b.v[int(b.table[0, position // 16]), 0, position % 16] = 3e36 * torch.linspace(-1, 1, 64)
+    b.device()
+    compare(b, b.attend(F32, scale=1.0), F32, scale=1.0)

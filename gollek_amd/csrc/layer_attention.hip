@@ -72,6 +72,8 @@ constexpr int resident(int head_dim) { return head_dim <= 64 ? 4 : head_dim <= 1
 // 17.9, 48 27.0 and 24.6, 96 51.2 and 49.2; of 256, 48 58 and 51 (a single long sequence
 // among them costs a step of 1 to 2 us for every four tiles, hence no further).
 constexpr int whole_few(int head_dim) { return resident(head_dim) == 1 ? 12 : 8 * resident(head_dim); }
+// (256 here and below is an MI355X's CUs as a number, not asked of the device: a workspace's
+// size must not change between the call that asks for it and the one that uses it.)
 constexpr int kWholeMany = 48, kFew = 256;
 // Many units of few tiles take a wave each, which saves their join through LDS and the
 // waves that have no tile: from where workgroups would need more than a round, up to 6

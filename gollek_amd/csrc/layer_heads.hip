@@ -5,7 +5,10 @@
 // first `dims` elements turns by the token's position:
 //   (a, b) <- magnitude * (a cos t - b sin t, b cos t + a sin t),  t = position * f_i.
 // The angle is position * turns_i in 64 bits with its whole revolutions taken off:
-// fp32 would be off by 2^-24 of the position, 0.006 revolutions at 100000.
+// fp32 would be off by 2^-24 of the position, 0.006 revolutions at 100000.  What is left, at
+// most half a revolution, is rounded to fp32 for the sine and cosine: 2^-26 of a revolution,
+// 2^-23.3 radians, about a step of the largest sine; fp32 results of random heads are 3.4e-8 off
+// in place of 2.9e-8 with the angle in 64 bits to the end.
 //
 // A wave works on heads of one token.  Its lanes compute one sine and cosine each (all
 // heads of a token have the same angles) and share them through LDS; then a group of

@@ -196,3 +196,18 @@ def test_large_values_under_growing_scores():
             b.v[int(b.table[0, position // 16]), 0, position % 16] = 3e36 * torch.linspace(-1, 1, 64)
     b.device()
     compare(b, b.attend(F32, scale=1.0), F32, scale=1.0)
+
+
+@pytest.mark.parametrize("lengths,some", [([3000], True), ([900] * 5, False)])
+def test_a_workspace_one_byte_short_is_refused(lengths, some):
+    # tables of up to 32 tiles of 32 tokens (heads of 64, few of them) are not cut and need none: 900
+    # tokens' 57 pages are 29 tiles
+    b = Batch(lengths, 4, 2, 64, BF16, seed=65)
+    assert (b.need > 0) == some
+    if some:
+        b.need -= 1
+        with pytest.raises(ops.IllegalArgumentError, match="Workspace"):
+            b.attend(F32)
+        b.need += 1
+    compare(b, b.attend(F32), F32)
+    assert torch.all(b.ws[b.need:] == 0xFF)

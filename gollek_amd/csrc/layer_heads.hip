@@ -6,9 +6,9 @@
 //   (a, b) <- magnitude * (a cos t - b sin t, b cos t + a sin t),  t = position * f_i.
 // The angle is position * turns_i in 64 bits with its whole revolutions taken off:
 // fp32 would be off by 2^-24 of the position, 0.006 revolutions at 100000.  What is left, at
-// most half a revolution, is rounded to fp32 for the sine and cosine: 2^-26 of a revolution,
-// 2^-23.3 radians, about a step of the largest sine; fp32 results of random heads are 3.4e-8 off
-// in place of 2.9e-8 with the angle in 64 bits to the end.
+// most half a revolution, goes to sine and cosine as an fp32 number and what that lost: in one
+// number sines next to half a revolution would be off by 2^-23.3, and random heads by 3.4e-8 in
+// place of 2.9e-8.
 //
 // A wave works on heads of one token.  Its lanes compute one sine and cosine each (all
 // heads of a token have the same angles) and share them through LDS; then a group of
@@ -166,10 +166,11 @@ __global__ __launch_bounds__(64 * kWaves) void heads_kernel(HeadsArgs a, HeadsPl
 #pragma unroll
     for (int n = 0; n < 2; n++) {
         if (lane + 64 * n >= dims / 2) continue;
-        const double turn = (double)position * angle[n];
+        const double turn = (double)position * angle[n], part = turn - rint(turn);
+        const float near = (float)part, rest = (float)(2.0 * M_PI * (part - (double)near));
         float s, c;
-        sincospif(2.0f * (float)(turn - rint(turn)), &s, &c);
-        turns[wave][lane + 64 * n] = make_float2(a.rope.magnitude * c, a.rope.magnitude * s);
+        sincospif(2.0f * near, &s, &c);
+        turns[wave][lane + 64 * n] = make_float2(a.rope.magnitude * fmaf(-s, rest, c), a.rope.magnitude * fmaf(c, rest, s));
     }
     __syncthreads();
     if (!in || padding) return;

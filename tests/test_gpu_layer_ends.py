@@ -1,4 +1,5 @@
 """Norms, rotary positions, appends and attention at the ends of their ranges, on the GPU."""
+import numpy as np
 import pytest
 import torch
 
@@ -119,3 +120,22 @@ def test_a_table_closed_while_a_stream_is_captured():
         graph.replay()
         torch.cuda.synchronize()
         assert torch.equal(out, want) and torch.equal(twice, 2 * want)
+
+
+@pytest.mark.parametrize("first", [0, 100000])
+def test_rope_sines_next_to_half_a_revolution(first):
+    # (0, 1) becomes (-sin, cos): each off by no more than 8 half steps of itself (sine and cosine 4
+    # ulp, and a product), small ones too, besides what position * frequency is off by in 64 bits:
+    # three roundings of the angle in revolutions, 2^-53 each
+    rope, angles = table(128)
+    tokens = 4096
+    at = first + torch.arange(tokens, dtype=torch.int32)
+    x = torch.cat([torch.zeros(tokens, 64), torch.ones(tokens, 64)], 1).cuda()
+    out = torch.empty_like(x)
+    rope.apply_device(ptr(x), F32, tokens, 1, 128, ptr(at.cuda()), ptr(out), stream=stream())
+    torch.cuda.synchronize()
+    t = at.numpy()[:, None].astype(np.longdouble) * (np.longdouble(10000) ** (-2 * np.arange(64, dtype=np.longdouble) / 128))
+    want = torch.from_numpy(np.concatenate([-np.sin(t), np.cos(t)], 1).astype(np.float64))
+    off = 8 * ref.STEP * want.abs() + 4 * 2.0**-53 * torch.from_numpy(np.concatenate([t, t], 1).astype(np.float64)) + 1e-30
+    bad = (out.cpu().double() - want).abs() > off
+    assert not bad.any(), (int(bad.sum()), want[bad][:4], out.cpu()[bad][:4])

@@ -248,20 +248,57 @@ __device__ __forceinline__ T stream(const T *p) {
 
 // Infinite and NaN values.  A piece of a weight may be 0 or below, so an infinite value comes
 // out of the second product as NaN where its dim's result is infinite.  Where a sum is NaN
-// and its weights' sum is not, the values say what it is: dim d's of keys [first, end) that
-// are not finite, added up (0: all are, and the sum overflowed).
+// and its weights' sum is not, the wave that ends it reads the values once more, and they say
+// what it is (64 sequences of up to 8192 with an infinity each 410 us in place of 230, one of
+// 131072 190 in place of 54; nothing else takes longer).
+//
+// Of keys first .. end - 1, by a wave: three bits (+infinity, -infinity, NaN among the values)
+// for each of the dims 8 piece .. 8 piece + 7 of a lane; piece is its number within `across`,
+// the power of two from head_dim / 8 on, and the other lanes take other keys.
 template <int TYPE>
-__device__ __forceinline__ float not_finite(const AttendArgs &a, int sequence, int kv_head, int first, int end, int d) {
+__device__ __forceinline__ uint32_t odd_values(const AttendArgs &a, int sequence, int kv_head, int first, int end, int lane,
+                                               int across) {
+    constexpr uint32_t kExponent = TYPE == kBF16 ? 0x7F80u : 0x7C00u;
     const int32_t *const table = a.page_table + (int64_t)sequence * a.max_pages;
-    float sum = 0.0f;
-    for (int key = first; key < end; key++) {
-        const int page = table[key >> a.kv.page_shift];
-        if (page < 0 || page >= a.kv.pages) continue;
-        const int64_t row = (((int64_t)page * a.kv.kv_heads + kv_head) << a.kv.page_shift) + (key & ((1 << a.kv.page_shift) - 1));
-        const float v = load_element(a.kv.v, TYPE, row * a.kv.head_dim + d);
-        if (!(fabsf(v) < __builtin_inff())) sum += v;
+    const int piece = lane & (across - 1), stripes = 64 / across;
+    const bool mine = 8 * piece < a.kv.head_dim;
+    uint32_t bits = 0;
+    constexpr int kAhead = 8;  // keys of a lane in flight
+    for (int64_t key0 = first; key0 < end; key0 += kAhead * stripes) {
+        int64_t key[kAhead];
+        int page[kAhead];
+        u32x4 x[kAhead];
+#pragma unroll
+        for (int n = 0; n < kAhead; n++) {
+            key[n] = min(key0 + n * stripes + lane / across, (int64_t)end - 1);  // (the last one again: no harm)
+            page[n] = table[key[n] >> a.kv.page_shift];
+        }
+#pragma unroll
+        for (int n = 0; n < kAhead; n++) {
+            if (page[n] < 0 || page[n] >= a.kv.pages) page[n] = -1;
+            const int64_t row = (((int64_t)max(page[n], 0) * a.kv.kv_heads + kv_head) << a.kv.page_shift) +
+                                (key[n] & ((1 << a.kv.page_shift) - 1));
+            x[n] = *reinterpret_cast<const u32x4 *>(static_cast<const uint16_t *>(a.kv.v) + row * a.kv.head_dim +
+                                                    (mine ? 8 * piece : 0));
+        }
+#pragma unroll
+        for (int n = 0; n < kAhead; n++)
+#pragma unroll
+            for (int j = 0; j < 8; j++) {
+                const uint32_t h = x[n][j >> 1] >> (16 * (j & 1)) & 0xFFFFu;
+                const uint32_t kind = (h & 0x7FFFu) > kExponent ? 4u : h >> 15 != 0 ? 2u : 1u;
+                if (page[n] >= 0 && mine && (h & kExponent) == kExponent) bits |= kind << (3 * j);
+            }
     }
-    return sum;
+    for (int m = across; m < 64; m <<= 1) bits |= (uint32_t)__shfl_xor((int)bits, m);
+    return bits;
+}
+__device__ __forceinline__ int piece_lanes(int dim) { return dim <= 8 ? 1 : 1 << (32 - __builtin_clz((unsigned)(dim / 8 - 1))); }
+// Dim d's bits of those, for every lane of the wave (which all call it).
+__device__ __forceinline__ uint32_t odd_kind(uint32_t bits, int d) { return (uint32_t)__shfl((int)bits, d >> 3) >> (3 * (d & 7)) & 7u; }
+// The sum that those bits of a dim stand for; `sum` where they are none.
+__device__ __forceinline__ float odd_sum(uint32_t kind, float sum) {
+    return kind == 0 ? sum : kind == 1 ? __builtin_inff() : kind == 2 ? -__builtin_inff() : __builtin_nanf("");
 }
 // A head's sink in powers of two.  One past fp32 there stands for the largest score: it takes
 // all weight, and its own stays a number.
@@ -523,9 +560,8 @@ __global__ __launch_bounds__(kThreads, NK <= 2 ? 4 : NK <= 4 ? 3 : NK <= 6 ? 2 :
     l += __shfl_xor(l, 32);
     const float bound = m == ninf ? ninf : base;
     if constexpr (SHARE == 1) {  // the whole sequence: straight from the accumulators
-        if (c >= rows) return;
         float f = 1.0f, total = l;
-        if (a.sinks != nullptr) {
+        if (a.sinks != nullptr && c < rows) {
             const float sink = sink_of(a, head0 + c), up = fmaxf(sink, bound), at1 = up == ninf ? 0.0f : up;
             f = __builtin_amdgcn_exp2f(bound - at1);
             total = l * f + __builtin_amdgcn_exp2f(sink - at1);
@@ -536,7 +572,7 @@ __global__ __launch_bounds__(kThreads, NK <= 2 ? 4 : NK <= 4 ? 3 : NK <= 6 ? 2 :
         for (int r = 0; r < 4; r++) {
             const auto put = [&](auto WIDE, int first, int d) {
                 constexpr int wide = decltype(WIDE)::value;
-                if (d >= dim) return;
+                if (d >= dim || c >= rows) return;
                 float y[wide];
 #pragma unroll
                 for (int i = 0; i < wide; i++) {
@@ -549,13 +585,14 @@ __global__ __launch_bounds__(kThreads, NK <= 2 ? 4 : NK <= 4 ? 3 : NK <= 6 ? 2 :
             if constexpr (D::kWide1 > 0)
                 put(std::integral_constant<int, D::kWide1>{}, D::kWide0, 16 * D::kWide0 + D::kWide1 * (4 * g + r));
         }
-        if (odd && total == total) {
+        odd = odd && total == total;
+        if (__any(odd)) {
+            const uint32_t bits = odd_values<TYPE>(a, it.sequence, kv_head, span.begin, span.length, lane, piece_lanes(dim));
 #pragma unroll 1
             for (int e = 0; e < 4 * D::kFragments; e++) {
                 const int d = e < 4 * D::kWide0 ? 4 * D::kWide0 * g + e : 16 * D::kWide0 + 4 * D::kWide1 * g + e - 4 * D::kWide0;
-                if (d >= dim) continue;
-                const float v = not_finite<TYPE>(a, it.sequence, kv_head, span.begin, span.length, d);
-                if (v != 0.0f) store_element(a.out, a.out_type, row + d, v);
+                const uint32_t kind = odd_kind(bits, d < dim ? d : 0);
+                if (odd && d < dim && kind != 0) store_element(a.out, a.out_type, row + d, odd_sum(kind, 0.0f));
             }
         }
         return;
@@ -580,7 +617,9 @@ __global__ __launch_bounds__(kThreads, NK <= 2 ? 4 : NK <= 4 ? 3 : NK <= 6 ? 2 :
             }
         }
         __syncthreads();
-        for (int e = (int)threadIdx.x; e < rows * dim; e += kThreads) {
+        // the sum of element e (kind: what its values' bits say), left where it goes; whether it
+        // is NaN over weights that are numbers
+        const auto finish = [&](int e, uint32_t kind) -> bool {
             const int r = e / dim, d = e - r * dim;
             float sum = 0.0f, total = 0.0f, most = ninf;
 #pragma unroll
@@ -591,11 +630,8 @@ __global__ __launch_bounds__(kThreads, NK <= 2 ? 4 : NK <= 4 ? 3 : NK <= 6 ? 2 :
             const float at0 = most == ninf ? 0.0f : most;
 #pragma unroll
             for (int w = 0; w < kWaves; w++) total += lds_l[w][r] * __builtin_amdgcn_exp2f(lds_m[w][r] - at0);
-            if (sum != sum && total == total) {
-                const float v = not_finite<TYPE>(a, it.sequence, kv_head, max(span.begin, kTile * tile0),
-                                                 (int)min((int64_t)span.length, (int64_t)kTile * tile1), d);
-                if (v != 0.0f) sum = v;
-            }
+            sum = odd_sum(kind, sum);
+            const bool odd = sum != sum && total == total;
             if (it.chunks > 1) {
                 const int64_t row = (int64_t)item * a.q_heads + head0 + r;
                 plan.part_o[row * dim + d] = sum;
@@ -609,6 +645,18 @@ __global__ __launch_bounds__(kThreads, NK <= 2 ? 4 : NK <= 4 ? 3 : NK <= 6 ? 2 :
                 }
                 store_element(a.out, a.out_type, it.sequence * a.out_stride + (head0 + r) * dim + d,
                               total == 0.0f ? 0.0f : sum / total);
+            }
+            return odd;
+        };
+        bool odd = false;
+        for (int e = (int)threadIdx.x; e < rows * dim; e += kThreads) odd |= finish(e, 0);
+        if (__any(odd)) {
+            const uint32_t bits =
+                odd_values<TYPE>(a, it.sequence, kv_head, max(span.begin, kTile * tile0),
+                                 (int)min((int64_t)span.length, (int64_t)kTile * tile1), lane, piece_lanes(dim));
+            for (int e0 = 64 * wave; e0 < rows * dim; e0 += kThreads) {
+                const uint32_t kind = odd_kind(bits, (e0 + lane) % dim);
+                if (e0 + lane < rows * dim && kind != 0) (void)finish(e0 + lane, kind);
             }
         }
     }

@@ -30,10 +30,10 @@
 // 39.3), as long as the registers of three waves a SIMD suffice for heads of 128.
 //
 // Bound by bytes: 64 sequences of up to 8192 tokens of 8 heads of 128 219 us (1.37 GB, 6.2
-// TB/s; reads alone outrun a copy's 5.0), one of 131072 of 4 heads 41.2 (268 MB, 6.5
-// TB/s) and 4.8 for the join.  Short sequences are bound by a step's latency and what a CU
+// TB/s; reads alone outrun a copy's 5.0), one of 131072 of 4 heads 41.6 (268 MB, 6.5
+// TB/s) and 5.0 for the join.  Short sequences are bound by a step's latency and what a CU
 // takes in, a microsecond for the 64 KB of its four waves, whatever the number of steps
-// ahead, waves or dims it is asked for: 700 tokens 10.4.
+// ahead, waves or dims it is asked for: 700 tokens 10.6.
 //
 // A sequence's tiles are cut into chunks of equal size for workgroups that share the chip
 // evenly whatever the lengths are: every workgroup adds up the batch's tiles, takes the
